@@ -38,7 +38,7 @@ enum {
   SPK_ERR_ARG = -5        /* any other invalid argument */
 };
 
-enum { SPK_F32 = 0, SPK_F16 = 1 };
+enum { SPK_F32 = 0, SPK_F16 = 1, SPK_BF16 = 2 };
 
 /* Message for the last non-zero status returned on this thread. */
 const char* spk_last_error(void);
@@ -466,6 +466,116 @@ int spk_matvec_f16_rows(const uint16_t* W, const uint16_t* X, int64_t ldx, uint1
  * fp16; workspace 16); workspace of spk_chunk_prefill_ordered_workspace_size(). */
 size_t spk_chunk_prefill_ordered_workspace_size(int32_t num_heads, int32_t total_tokens);
 int spk_chunk_prefill_ordered(const SpkChunkArgs* args, spk_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * A serving step over a paged key/value cache (no reference counterpart: the
+ * reference decodes one sequence, its positions in consecutive rows).  The
+ * new tokens of all sequences are packed along the token axis: sequence s
+ * owns rows [cu_seqlens[s], cu_seqlens[s+1]).  One token per sequence is a
+ * decode step, the last accepted token and n drafted ones a verification,
+ * thousands a chunk of a prompt; a step may mix them.
+ *
+ * The cache is a pool of num_pages pages of page_size tokens; position p of
+ * sequence s lies in page block_table[s][p / page_size].  Strides are in
+ * elements and the same for K and V, so a pool may be laid out
+ * [page][token][head][dim] or [page][head][token][dim], and one
+ * attention layer's [max_seq][K 2x256 | V 2x256] rows of the session are a
+ * pool of one page.  context_lens[s] counts the tokens of s after the step:
+ * its new tokens are the last cu_seqlens[s+1] - cu_seqlens[s] of them.
+ *
+ * The three tables are device memory and may change between replays of a
+ * captured call.  What they hold is brought into the buffers: offsets into
+ * [0, total_tokens], lengths into [0, max_pages * page_size]; a page id
+ * outside [0, num_pages) stands for no page (its tokens are neither stored
+ * nor attended).  Rows past cu_seqlens[num_seqs] are left as they were.
+ * k_cache, v_cache and all row strides of q, k, v, gate and out: 16-byte
+ * aligned (strides multiples of 8 elements).
+ * ---------------------------------------------------------------------- */
+typedef struct SpkPagedCache {
+  int32_t dtype;             /* SPK_F16 or SPK_BF16: the cache, q, k, v, gate, out, weights */
+  int32_t num_kv_heads;
+  int32_t head_dim;          /* 64, 128 or 256 */
+  int32_t page_size;         /* any > 0 */
+  int32_t num_pages;
+  int32_t max_pages;         /* entries of a block_table row that may be read */
+  int32_t num_seqs;
+  int32_t total_tokens;      /* rows of q, k, v, out */
+  void* k_cache;
+  void* v_cache;
+  int64_t page_stride, token_stride, head_stride;
+  const int32_t* block_table;
+  int64_t table_stride;      /* entries between rows */
+  const int32_t* cu_seqlens;
+  const int32_t* context_lens;
+} SpkPagedCache;
+
+/* Rotary positions with several axes, and the store into the pages.  Every
+ * q and k head of a token is normalised where a weight is given (RMSNorm over
+ * head_dim, weights applied as 1 + w, as rms_norm_per_head.comp), and its
+ * first rot_dim dimensions are rotated: pair i of the rot_dim / 2 pairs turns
+ * by the angle of row positions[pair_axis[i]][token] of the table rope
+ * [rope_rows][rot_dim], (cos, sin) per pair (rope_apply.comp's table;
+ * positions outside it take its first or last row).  Text has one axis, or
+ * equal positions on all; images and videos have time, height and width.
+ * q_out receives the queries (it may be q), the pages the keys and values.
+ * fp32 throughout, one rounding at the end (rope_apply.comp's separate
+ * dispatches round after the norm as well). */
+enum { SPK_ROPE_HALVES = 0 /* pairs (i, i + rot_dim/2) */, SPK_ROPE_ADJACENT = 1 /* pairs (2i, 2i + 1) */ };
+typedef struct SpkMropeArgs {
+  SpkPagedCache cache;
+  int32_t num_q_heads;
+  int32_t rot_dim;             /* multiple of 16, <= head_dim */
+  int32_t pairing;
+  int32_t num_axes;            /* 1 .. 4 */
+  const uint8_t* pair_axis;    /* HOST, [rot_dim / 2], each < num_axes */
+  const int32_t* positions;    /* [num_axes][positions_stride] */
+  int64_t positions_stride;
+  const float* rope;
+  int32_t rope_rows;
+  float eps;                   /* 0 => 1e-6 */
+  const void* q;               int64_t q_token_stride, q_head_stride;
+  const void* k;               int64_t k_token_stride, k_head_stride;
+  const void* v;               int64_t v_token_stride, v_head_stride;
+  const void* q_norm_w;        /* nullable, [head_dim] */
+  const void* k_norm_w;        /* nullable, [head_dim] */
+  void* q_out;                 int64_t out_token_stride, out_head_stride;
+} SpkMropeArgs;
+int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
+
+/* Attention of every sequence's new tokens over its pages (which hold their
+ * keys and values already).  The query at position p sees the keys 0 .. p, or
+ * with window > 0 the last `window` of them; query head h reads KV head
+ * h / (num_q_heads / num_kv_heads).  out = softmax(scale q.K^T) V, times
+ * sigmoid(gate) where a gate is given (sigmoid_gate.comp); lse (nullable,
+ * [total_tokens][num_q_heads]) = log sum exp of the scaled scores.  A row that
+ * sees nothing that weighs (a position before the first, bad pages, every
+ * score -inf) is zero with lse -inf; keys and values that a row does not see
+ * cannot reach it, whatever they hold.
+ * max_query_len and max_context_len: host bounds of the sequences' lengths;
+ * they choose the kernels and the split of the keys, not the result, which
+ * follows the device's lengths.
+ * workspace: 256-byte aligned, spk_paged_attention_workspace_size() bytes,
+ * contents ignored (may be 0 bytes: then NULL is fine).  Calls that overlap on
+ * one workspace race.
+ * Numerics: products of 16-bit values accumulate in fp32, softmax statistics
+ * in fp32; the weights are rounded to the 16-bit type before the product with
+ * V (they enter the sum of weights unrounded), out is rounded once. */
+typedef struct SpkPagedAttnArgs {
+  SpkPagedCache cache;
+  int32_t num_q_heads;
+  int32_t max_query_len;
+  int32_t max_context_len;
+  int32_t window;              /* 0: all */
+  float scale;                 /* 0 => 1/sqrt(head_dim) */
+  const void* q;               int64_t q_token_stride, q_head_stride;
+  const void* gate;            int64_t gate_token_stride, gate_head_stride;
+  void* out;                   int64_t out_token_stride, out_head_stride;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} SpkPagedAttnArgs;
+size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* args);
+int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Diagnostics (no reference counterpart).

@@ -65,6 +65,10 @@ SIGNATURES = {
     "spk_matvec_f16_rows": (C.c_int, [_p, _p, _i64, _p, _i64, _p, _i32, _i32, _i32, _p]),
     "spk_chunk_prefill_ordered_workspace_size": (_sz, [_i32, _i32]),
     "spk_chunk_prefill_ordered": (C.c_int, [_p, _p]),
+    # a serving step over a paged cache
+    "spk_mrope_append": (C.c_int, [_p, _p]),
+    "spk_paged_attention_workspace_size": (_sz, [_p]),
+    "spk_paged_attention": (C.c_int, [_p, _p]),
 }
 
 
@@ -112,12 +116,42 @@ class SpkAttnArgs(C.Structure):
                 ("workspace_bytes", _sz)]
 
 
+class SpkPagedCache(C.Structure):
+    _fields_ = [("dtype", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("page_size", _i32),
+                ("num_pages", _i32), ("max_pages", _i32), ("num_seqs", _i32), ("total_tokens", _i32),
+                ("k_cache", _p), ("v_cache", _p),
+                ("page_stride", _i64), ("token_stride", _i64), ("head_stride", _i64),
+                ("block_table", _p), ("table_stride", _i64), ("cu_seqlens", _p), ("context_lens", _p)]
+
+
+class SpkMropeArgs(C.Structure):
+    _fields_ = [("cache", SpkPagedCache), ("num_q_heads", _i32), ("rot_dim", _i32), ("pairing", _i32),
+                ("num_axes", _i32), ("pair_axis", C.c_char_p), ("positions", _p), ("positions_stride", _i64),
+                ("rope", _p), ("rope_rows", _i32), ("eps", _f32),
+                ("q", _p), ("q_token_stride", _i64), ("q_head_stride", _i64),
+                ("k", _p), ("k_token_stride", _i64), ("k_head_stride", _i64),
+                ("v", _p), ("v_token_stride", _i64), ("v_head_stride", _i64),
+                ("q_norm_w", _p), ("k_norm_w", _p),
+                ("q_out", _p), ("out_token_stride", _i64), ("out_head_stride", _i64)]
+
+
+class SpkPagedAttnArgs(C.Structure):
+    _fields_ = [("cache", SpkPagedCache), ("num_q_heads", _i32), ("max_query_len", _i32),
+                ("max_context_len", _i32), ("window", _i32), ("scale", _f32),
+                ("q", _p), ("q_token_stride", _i64), ("q_head_stride", _i64),
+                ("gate", _p), ("gate_token_stride", _i64), ("gate_head_stride", _i64),
+                ("out", _p), ("out_token_stride", _i64), ("out_head_stride", _i64),
+                ("lse", _p), ("workspace", _p), ("workspace_bytes", _sz)]
+
+
 class SpkMatvecDesc(C.Structure):
     _fields_ = [("W", _p), ("x", _p), ("y", _p), ("out_dim", _i32), ("in_dim", _i32)]
 
 
 SPK_F32 = 0
 SPK_F16 = 1
+SPK_BF16 = 2
+SPK_ROPE_HALVES, SPK_ROPE_ADJACENT = 0, 1
 
 _LIB = None
 

@@ -13,7 +13,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import SpkChunkArgs, SpkDecodeArgs, SpkMatvecDesc, check, lib
+from ._lib import (SpkChunkArgs, SpkDecodeArgs, SpkMatvecDesc, SpkMropeArgs, SpkPagedAttnArgs, SpkPagedCache,
+                   check, lib)
 
 KEY_DIM = 128
 VALUE_DIM = 128
@@ -279,3 +280,167 @@ def lm_head_argmax(W: torch.Tensor, x: torch.Tensor, logits: Optional[torch.Tens
                                    _ptr(workspace), workspace.numel() * workspace.element_size(),
                                    _stream()), "spk_lm_head_argmax")
     return out
+
+
+# ----------------------------------------------------------------------------
+# a serving step over a paged cache
+# ----------------------------------------------------------------------------
+_HALF = {torch.float16: _lib.SPK_F16, torch.bfloat16: _lib.SPK_BF16}
+_PAIRINGS = {"halves": _lib.SPK_ROPE_HALVES, "adjacent": _lib.SPK_ROPE_ADJACENT}
+
+
+def _on(what: str, name: str, t: torch.Tensor, dev, dtype, shape=None) -> None:
+    if t.device != dev or t.dtype != dtype:
+        raise _lib.SpockError(f"{what}: {name} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise _lib.SpockError(f"{what}: {name} shape {tuple(t.shape)} != {shape}")
+
+
+def _rows(what: str, name: str, t: torch.Tensor, dev, dtype, shape) -> None:
+    """A [tokens][heads][dim] view: any strides of the first two dimensions."""
+    _on(what, name, t, dev, dtype, shape)
+    if t.stride(2) != 1:
+        raise _lib.SpockError(f"{what}: the last dimension of {name} must be contiguous")
+
+
+def _paged_cache(what: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                 cu_seqlens: torch.Tensor, context_lens: torch.Tensor) -> SpkPagedCache:
+    dev = q.device
+    if dev.type != "cuda":
+        raise _lib.SpockError(f"{what}: expected device tensors")
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise _lib.SpockError(f"{what}: q must be [tokens][heads][dim] and the caches [pages][page_size][kv_heads][dim], "
+                              f"got {tuple(q.shape)} and {tuple(k_cache.shape)}")
+    if q.dtype not in _HALF:
+        raise _lib.SpockError(f"{what}: q must be float16 or bfloat16, got {q.dtype}")
+    pages, page_size, kv_heads, dim = k_cache.shape
+    if q.shape[2] != dim:
+        raise _lib.SpockError(f"{what}: q has head_dim {q.shape[2]}, the cache {dim}")
+    _on(what, "k_cache", k_cache, dev, q.dtype)
+    _on(what, "v_cache", v_cache, dev, q.dtype, (pages, page_size, kv_heads, dim))
+    strides = k_cache.stride()
+    if v_cache.stride() != strides or strides[3] != 1:
+        raise _lib.SpockError(f"{what}: k_cache and v_cache need equal strides and a contiguous last dimension, "
+                              f"got {strides} and {v_cache.stride()}")
+    seqs = context_lens.numel()
+    _on(what, "block_table", block_table, dev, torch.int32)
+    _on(what, "cu_seqlens", cu_seqlens, dev, torch.int32, (seqs + 1,))
+    _on(what, "context_lens", context_lens, dev, torch.int32, (seqs,))
+    if block_table.dim() != 2 or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise _lib.SpockError(f"{what}: block_table must be [{seqs}][max_pages] with contiguous rows, "
+                              f"got {tuple(block_table.shape)}")
+    if not (cu_seqlens.is_contiguous() and context_lens.is_contiguous()):
+        raise _lib.SpockError(f"{what}: cu_seqlens and context_lens must be contiguous")
+    return SpkPagedCache(_HALF[q.dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, q.shape[0],
+                         k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2],
+                         block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), context_lens.data_ptr())
+
+
+def _call(fn, a, dev, what: str) -> None:
+    """fn(a) on the current stream of the tensors' device, which is made current for the launch."""
+    if torch.cuda.current_device() == dev.index:
+        check(fn(C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+
+
+def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor,
+                 pair_axis: Sequence[int], k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                 cu_seqlens: torch.Tensor, context_lens: torch.Tensor, q_norm_weight: Optional[torch.Tensor] = None,
+                 k_norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, pairing: str = "halves",
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions with several axes, and the store into the pages (spk_mrope_append).
+
+    q [T][Hq][D], k, v [T][Hkv][D] (float16 or bfloat16, any token and head strides); positions [axes][T] int32;
+    rope [rows][rot_dim] float32, (cos, sin) per pair; pair_axis: the axis of each of the rot_dim / 2 pairs (host);
+    caches [pages][page_size][Hkv][D] (any page, token and head strides, the same for both); block_table
+    [S][max_pages], cu_seqlens [S+1], context_lens [S] int32 on the device.  q and k are normalised first where a
+    norm weight [D] is given (RMSNorm, 1 + w).  Writes the new tokens' keys and values into the caches and returns
+    the queries (in `out`, which may be q; rows past cu_seqlens[S] are not written).
+    """
+    what = "mrope_append"
+    cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
+    T, heads, D = q.shape
+    dev, kv = q.device, cache.num_kv_heads
+    _rows(what, "q", q, dev, q.dtype, (T, heads, D))
+    _rows(what, "k", k, dev, q.dtype, (T, kv, D))
+    _rows(what, "v", v, dev, q.dtype, (T, kv, D))
+    try:
+        axes = bytes(list(pair_axis))
+    except (TypeError, ValueError):
+        raise _lib.SpockError(f"{what}: pair_axis must be a sequence of axis numbers, got {pair_axis!r}") from None
+    _on(what, "rope", rope, dev, torch.float32, (rope.shape[0], 2 * len(axes)))
+    if not rope.is_contiguous():
+        raise _lib.SpockError(f"{what}: rope must be contiguous")
+    _on(what, "positions", positions, dev, torch.int32, (positions.shape[0], T))
+    if T > 1 and positions.stride(1) != 1:
+        raise _lib.SpockError(f"{what}: positions must have contiguous rows")
+    for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
+        if w is not None:
+            _on(what, name, _dev(w), dev, q.dtype, (D,))
+    if pairing not in _PAIRINGS:
+        raise _lib.SpockError(f"{what}: pairing must be one of {sorted(_PAIRINGS)}, got {pairing!r}")
+    if out is None:
+        out = torch.empty((T, heads, D), dtype=q.dtype, device=dev)
+    else:
+        _rows(what, "out", out, dev, q.dtype, (T, heads, D))
+    a = SpkMropeArgs(cache, heads, 2 * len(axes), _PAIRINGS[pairing], positions.shape[0], axes, positions.data_ptr(),
+                     positions.stride(0), rope.data_ptr(), rope.shape[0], eps,
+                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                     v.data_ptr(), v.stride(0), v.stride(1), _ptr(q_norm_weight), _ptr(k_norm_weight),
+                     out.data_ptr(), out.stride(0), out.stride(1))
+    _call(lib().spk_mrope_append, a, dev, "spk_mrope_append")
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    cu_seqlens: torch.Tensor, context_lens: torch.Tensor, max_query_len: int, max_context_len: int,
+                    scale: float = 0.0, window: int = 0, gate: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, return_lse: bool = False, lse: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None):
+    """Attention of each sequence's new tokens over its pages (spk_paged_attention).
+
+    q [T][Hq][D]; caches, tables and lengths as in mrope_append; max_query_len, max_context_len: host bounds of the
+    sequences' lengths; scale 0 = 1/sqrt(D); window > 0: only the last `window` positions are seen; gate [T][Hq][D]:
+    the output is multiplied by sigmoid(gate).  Returns out [T][Hq][D], or (out, lse [T][Hq] float32) with return_lse
+    or an lse buffer.  Rows past cu_seqlens[S] are not written.
+    """
+    what = "paged_attention"
+    cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
+    dev, shape = q.device, tuple(q.shape)
+    _rows(what, "q", q, dev, q.dtype, shape)
+    if gate is not None:
+        _rows(what, "gate", gate, dev, q.dtype, shape)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    else:
+        _rows(what, "out", out, dev, q.dtype, shape)
+    if lse is not None:
+        _on(what, "lse", _dev(lse), dev, torch.float32, shape[:2])
+    elif return_lse:
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+    a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale,
+                         q.data_ptr(), q.stride(0), q.stride(1), _ptr(gate), 0, 0,
+                         out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), None, 0)
+    if gate is not None:
+        a.gate_token_stride, a.gate_head_stride = gate.stride(0), gate.stride(1)
+    need = lib().spk_paged_attention_workspace_size(C.byref(a))
+    if need:
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.device != dev:
+            raise _lib.SpockError(f"{what}: workspace must be on {dev}, got {workspace.device}")
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call(lib().spk_paged_attention, a, dev, "spk_paged_attention")
+    return out if lse is None else (out, lse)
+
+
+def paged_attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
+                                    max_pages: int, num_seqs: int, max_query_len: int, max_context_len: int,
+                                    window: int = 0) -> int:
+    """Bytes of paged_attention's workspace for these sizes, for callers that keep one."""
+    cache = SpkPagedCache(_lib.SPK_F16, kv_heads, head_dim, page_size, 1, max_pages, num_seqs, tokens, 16, 16, 0, 0, 0,
+                          16, max_pages, 16, 16)
+    a = SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window)
+    return int(lib().spk_paged_attention_workspace_size(C.byref(a)))
