@@ -577,6 +577,56 @@ typedef struct SpkPagedAttnArgs {
 size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* args);
 int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
 
+/* Verification of drafted tokens.  The rows of a step are packed as above:
+ * tokens[t] was the model's input at row t, target row t its distribution of
+ * the token that follows, so the drafts of a sequence that owns rows
+ * [a, b) are tokens[a+1 .. b-1].  Draft row t (nullable) is the distribution
+ * that tokens[t+1] was drawn from; without it the drafter's choice counts as
+ * certain (probability 1).  From the first row on, draft d at row t is
+ * accepted while u_accept[t] * draft(d) < target(d); the first row that
+ * refuses its draft draws from max(target - draft, 0) (without draft rows:
+ * from target without d; from target itself where that leaves nothing), and
+ * after n acceptances the last row draws from target: the smallest token x
+ * with C(x) > u_sample[s] * C(vocab - 1), C the running sum.
+ * SPK_VERIFY_LOGITS: rows are logits, distributions softmax(row /
+ * temperature[s]) (NULL: 1); temperature <= 0 (or NaN) is greedy: a draft is
+ * accepted when it is the row's largest logit, lowest index first (NaN never
+ * is), and that token is the one drawn.  SPK_VERIFY_PROBS: rows are
+ * probabilities (temperature must be NULL).
+ * out_tokens[t] = the token emitted after row t: the accepted drafts, then the
+ * drawn token, then -1.  accepted[s] = accepted drafts.  logprobs (nullable):
+ * log target(out_tokens[t]) (greedy: at temperature 1), 0 where -1.
+ * context_out (nullable, with context_lens; may be the same buffer):
+ * context_lens[s] less the refused drafts, the cache's length before the drawn
+ * token is fed.  A drawn row without a distribution (NaN, no mass) emits -1.
+ * Tokens outside [0, vocab) are refused; a sequence without rows only gets
+ * accepted[s] = 0 and its context.  Comparisons and running sums are fp64.
+ * workspace: 256-byte aligned, contents ignored; overlapping calls race on it. */
+enum { SPK_VERIFY_LOGITS = 0, SPK_VERIFY_PROBS = 1 };
+typedef struct SpkVerifyArgs {
+  int32_t kind;
+  int32_t dtype;               /* SPK_F32, SPK_F16 or SPK_BF16: target and draft */
+  int32_t vocab;
+  int32_t num_seqs;
+  int32_t total_tokens;
+  const int32_t* cu_seqlens;   /* [num_seqs + 1] */
+  const int32_t* tokens;       /* [total_tokens] */
+  const void* target;          int64_t target_stride;  /* elements between rows */
+  const void* draft;           int64_t draft_stride;
+  const float* temperature;    /* nullable, [num_seqs] */
+  const float* u_accept;       /* [total_tokens], in [0, 1) */
+  const float* u_sample;       /* [num_seqs], in [0, 1) */
+  int32_t* out_tokens;         /* [total_tokens] */
+  int32_t* accepted;           /* [num_seqs] */
+  float* logprobs;             /* nullable, [total_tokens] */
+  const int32_t* context_lens; /* nullable, [num_seqs] */
+  int32_t* context_out;
+  void* workspace;
+  size_t workspace_bytes;
+} SpkVerifyArgs;
+size_t spk_verify_drafts_workspace_size(int32_t vocab, int32_t num_seqs, int32_t total_tokens);
+int spk_verify_drafts(const SpkVerifyArgs* args, spk_stream_t stream);
+
 /* ------------------------------------------------------------------------
  * Diagnostics (no reference counterpart).
  * ---------------------------------------------------------------------- */

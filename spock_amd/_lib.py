@@ -69,6 +69,8 @@ SIGNATURES = {
     "spk_mrope_append": (C.c_int, [_p, _p]),
     "spk_paged_attention_workspace_size": (_sz, [_p]),
     "spk_paged_attention": (C.c_int, [_p, _p]),
+    "spk_verify_drafts_workspace_size": (_sz, [_i32, _i32, _i32]),
+    "spk_verify_drafts": (C.c_int, [_p, _p]),
 }
 
 
@@ -144,6 +146,14 @@ class SpkPagedAttnArgs(C.Structure):
                 ("lse", _p), ("workspace", _p), ("workspace_bytes", _sz)]
 
 
+class SpkVerifyArgs(C.Structure):
+    _fields_ = [("kind", _i32), ("dtype", _i32), ("vocab", _i32), ("num_seqs", _i32), ("total_tokens", _i32),
+                ("cu_seqlens", _p), ("tokens", _p), ("target", _p), ("target_stride", _i64), ("draft", _p),
+                ("draft_stride", _i64), ("temperature", _p), ("u_accept", _p), ("u_sample", _p), ("out_tokens", _p),
+                ("accepted", _p), ("logprobs", _p), ("context_lens", _p), ("context_out", _p),
+                ("workspace", _p), ("workspace_bytes", _sz)]
+
+
 class SpkMatvecDesc(C.Structure):
     _fields_ = [("W", _p), ("x", _p), ("y", _p), ("out_dim", _i32), ("in_dim", _i32)]
 
@@ -152,6 +162,7 @@ SPK_F32 = 0
 SPK_F16 = 1
 SPK_BF16 = 2
 SPK_ROPE_HALVES, SPK_ROPE_ADJACENT = 0, 1
+SPK_VERIFY_LOGITS, SPK_VERIFY_PROBS = 0, 1
 
 _LIB = None
 

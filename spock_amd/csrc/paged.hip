@@ -85,19 +85,6 @@ struct Mrope {
   uint8_t axis[128];
 };
 
-// The sequence of token t: how many sequences end at or before it.  One load
-// per lane and ballot for 64 sequences; every lane returns the same.
-__device__ __forceinline__ int seq_of_token(const Cache& c, int t, int lane) {
-  int s = 0;
-  for (int s0 = 0; s0 < c.num_seqs; s0 += 64) {
-    const bool ended = s0 + lane < c.num_seqs && c.cu[s0 + lane + 1] <= t;
-    const int n = __popcll(__ballot(ended));
-    s += n;
-    if (n < 64) break;
-  }
-  return s;
-}
-
 // One wave per token.  D / 16 lanes hold a head, 16 elements each: chunks of 8
 // that rotate together (HALVES: chunk j and j + rot/16; ADJACENT: the pairs
 // lie inside a chunk), so the angles of a lane are the same for every head of
@@ -108,7 +95,7 @@ __global__ __launch_bounds__(256) void mrope_append_kernel(Mrope a) {
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.c.total_tokens) return;
-  const int s = seq_of_token(a.c, t, lane);
+  const int s = spk_paged::seq_of_token(a.c.cu, a.c.num_seqs, t, lane);
   if (s >= a.c.num_seqs) return;
   const Seq sq = spk_paged::seq_at(a.c, s);
   if (t < sq.first || t >= sq.first + sq.n) return;
@@ -555,7 +542,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a, int tile_rows) 
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int token = (int)(at / a.heads), head = (int)(at - (int64_t)token * a.heads);
   if (token >= a.c.total_tokens) return;
-  const int s = seq_of_token(a.c, token, lane);
+  const int s = spk_paged::seq_of_token(a.c.cu, a.c.num_seqs, token, lane);
   if (s >= a.c.num_seqs) return;
   const Seq sq = spk_paged::seq_at(a.c, s);
   if (token < sq.first || token >= sq.first + sq.n) return;

@@ -77,4 +77,19 @@ SPK_HD void visible(const Seq& s, int32_t i, int32_t window, int32_t* lo, int32_
   *lo = window > 0 && *hi > window ? *hi - window : 0;
 }
 
+#if defined(__HIPCC__)
+// The sequence of row t: how many sequences end at or before it.  One load
+// per lane and a ballot for 64 sequences; every lane returns the same.
+__device__ __forceinline__ int seq_of_token(const int32_t* cu, int num_seqs, int t, int lane) {
+  int s = 0;
+  for (int s0 = 0; s0 < num_seqs; s0 += 64) {
+    const bool ended = s0 + lane < num_seqs && cu[s0 + lane + 1] <= t;
+    const int n = __popcll(__ballot(ended));
+    s += n;
+    if (n < 64) break;
+  }
+  return s;
+}
+#endif
+
 }  // namespace spk_paged

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import (SpkChunkArgs, SpkDecodeArgs, SpkMatvecDesc, SpkMropeArgs, SpkPagedAttnArgs, SpkPagedCache,
-                   check, lib)
+                   SpkVerifyArgs, check, lib)
 
 KEY_DIM = 128
 VALUE_DIM = 128
@@ -444,3 +444,71 @@ def paged_attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head
                           16, max_pages, 16, 16)
     a = SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window)
     return int(lib().spk_paged_attention_workspace_size(C.byref(a)))
+
+
+_ROWS = {**_HALF, torch.float32: _lib.SPK_F32}
+_KINDS = {"logits": _lib.SPK_VERIFY_LOGITS, "probs": _lib.SPK_VERIFY_PROBS}
+
+
+def verify_workspace_bytes(vocab: int, num_seqs: int, tokens: int) -> int:
+    return int(lib().spk_verify_drafts_workspace_size(vocab, num_seqs, tokens))
+
+
+def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.Tensor, u_accept: torch.Tensor,
+                  u_sample: torch.Tensor, draft: Optional[torch.Tensor] = None, kind: str = "logits",
+                  temperature: Optional[torch.Tensor] = None, context_lens: Optional[torch.Tensor] = None,
+                  out_tokens: Optional[torch.Tensor] = None, accepted: Optional[torch.Tensor] = None,
+                  logprobs: Optional[torch.Tensor] = None, context_out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None):
+    """Accepts or refuses drafted tokens and draws the next one (spk_verify_drafts).
+
+    target [T][vocab] (float16, bfloat16 or float32): row t is the distribution of the token after row t, as logits or
+    as probabilities (`kind`); tokens [T] int32: the input token of every row; cu_seqlens [S+1] int32: the rows of each
+    sequence, the last accepted token's first; draft [T][vocab]: the rows that the drafts were drawn from, None for a
+    drafter that is certain; temperature [S] float32 (logits; None = 1, 0 = greedy); u_accept [T], u_sample [S] float32
+    in [0, 1).  Returns (out_tokens [T] int32, accepted [S] int32, logprobs [T] float32, context_out [S] int32 or None
+    without context_lens).  Rows past cu_seqlens[S] are not written.
+    """
+    what = "verify_drafts"
+    dev = target.device
+    if dev.type != "cuda":
+        raise _lib.SpockError(f"{what}: expected device tensors")
+    if target.dim() != 2 or target.dtype not in _ROWS or (target.shape[1] > 1 and target.numel() and target.stride(1) != 1):
+        raise _lib.SpockError(f"{what}: target must be [rows][vocab] float16, bfloat16 or float32 with contiguous rows, "
+                              f"got {tuple(target.shape)} {target.dtype}")
+    if kind not in _KINDS:
+        raise _lib.SpockError(f"{what}: kind must be one of {sorted(_KINDS)}, got {kind!r}")
+    T, vocab = target.shape
+    seqs = u_sample.numel()
+    if draft is not None:
+        _on(what, "draft", draft, dev, target.dtype, (T, vocab))
+        if vocab > 1 and T and draft.stride(1) != 1:
+            raise _lib.SpockError(f"{what}: draft must have contiguous rows")
+    for name, t, dtype, shape in (("tokens", tokens, torch.int32, (T,)), ("cu_seqlens", cu_seqlens, torch.int32, (seqs + 1,)),
+                                  ("u_accept", u_accept, torch.float32, (T,)), ("u_sample", u_sample, torch.float32, (seqs,)),
+                                  ("temperature", temperature, torch.float32, (seqs,)),
+                                  ("context_lens", context_lens, torch.int32, (seqs,)),
+                                  ("out_tokens", out_tokens, torch.int32, (T,)), ("accepted", accepted, torch.int32, (seqs,)),
+                                  ("logprobs", logprobs, torch.float32, (T,)), ("context_out", context_out, torch.int32, (seqs,))):
+        if t is not None:
+            _on(what, name, _dev(t), dev, dtype, shape)
+    if out_tokens is None:
+        out_tokens = torch.empty(T, dtype=torch.int32, device=dev)
+    if accepted is None:
+        accepted = torch.empty(seqs, dtype=torch.int32, device=dev)
+    if logprobs is None:
+        logprobs = torch.empty(T, dtype=torch.float32, device=dev)
+    if context_out is None and context_lens is not None:
+        context_out = torch.empty(seqs, dtype=torch.int32, device=dev)
+    need = lib().spk_verify_drafts_workspace_size(vocab, seqs, T)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev:
+        raise _lib.SpockError(f"{what}: workspace must be on {dev}, got {workspace.device}")
+    a = SpkVerifyArgs(_KINDS[kind], _ROWS[target.dtype], vocab, seqs, T, cu_seqlens.data_ptr(), tokens.data_ptr(),
+                      target.data_ptr(), target.stride(0) if T > 1 else vocab, _ptr(draft),
+                      0 if draft is None else draft.stride(0) if T > 1 else vocab, _ptr(temperature), u_accept.data_ptr(),
+                      u_sample.data_ptr(), out_tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(),
+                      _ptr(context_lens), _ptr(context_out), workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _call(lib().spk_verify_drafts, a, dev, "spk_verify_drafts")
+    return out_tokens, accepted, logprobs, context_out

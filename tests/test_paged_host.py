@@ -188,3 +188,28 @@ def test_host_tensors_are_refused():
     q, c, i = z(1, 4, 64, dtype=torch.float16), z(2, 16, 2, 64, dtype=torch.float16), z(2, dtype=torch.int32)
     with pytest.raises(_lib.SpockError, match="device tensors"):
         ops.paged_attention(q, c, c, z(1, 2, dtype=torch.int32), i, i[:1], 1, 32)
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(kind=2), -5), (dict(dtype=3), -5), (dict(vocab=0), -2), (dict(vocab=2 ** 31 - 1), -2), (dict(num_seqs=-1), -2),
+    (dict(total_tokens=65536), -2), (dict(num_seqs=65536), -2), (dict(kind=1, temperature=256), -5), (dict(context_out=256), -1),
+    (dict(cu_seqlens=None), -1), (dict(accepted=None), -1), (dict(tokens=None), -1), (dict(target=None), -1),
+    (dict(u_accept=None), -1), (dict(u_sample=None), -1), (dict(out_tokens=None), -1), (dict(target_stride=99), -2),
+    (dict(draft=256, draft_stride=99), -2), (dict(target=257), -4), (dict(draft=257, draft_stride=100), -4),
+    (dict(out_tokens=256, tokens=256), -5), (dict(workspace=None), -1), (dict(workspace_bytes=8), -5), (dict(workspace=264), -5)])
+def test_verify_refusals(over, code):
+    from spock_amd import _lib
+    lib = _lib.lib()
+    assert lib.spk_verify_drafts(None, None) == -1
+    a = _lib.SpkVerifyArgs(0, _lib.SPK_F16, 100, 2, 6, 256, 256, 256, 100, None, 0, None, 256, 256, 512, 256, None, None, None, 256, 1 << 20)
+    for k, v in over.items():
+        setattr(a, k, v)
+    assert lib.spk_verify_drafts(C.byref(a), None) == code, lib.spk_last_error()
+
+
+def test_verify_nothing_to_do():
+    from spock_amd import _lib
+    a = _lib.SpkVerifyArgs(0, _lib.SPK_F16, 100, 0, 0)
+    assert _lib.lib().spk_verify_drafts(C.byref(a), None) == 0
+    assert _lib.lib().spk_verify_drafts_workspace_size(100, 0, 4) == 0
+    assert C.sizeof(_lib.SpkVerifyArgs) == 152 and _lib.SpkVerifyArgs.workspace.offset == 136
