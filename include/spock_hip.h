@@ -566,7 +566,7 @@ typedef struct SpkPagedAttnArgs {
   int32_t max_query_len;
   int32_t max_context_len;
   int32_t window;              /* 0: all */
-  float scale;                 /* 0 => 1/sqrt(head_dim) */
+  float scale;                 /* > 0; 0 => 1/sqrt(head_dim) */
   const void* q;               int64_t q_token_stride, q_head_stride;
   const void* gate;            int64_t gate_token_stride, gate_head_stride;
   void* out;                   int64_t out_token_stride, out_head_stride;

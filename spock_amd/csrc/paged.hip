@@ -20,6 +20,7 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 // The two 16-bit types: conversions (round to nearest even) and products.
 template <bool BF>
@@ -43,8 +44,16 @@ struct Half<false> {
   static __device__ __forceinline__ bool odd(uint32_t u) {
     return (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
   }
+  // the two with such values as zeros
+  static __device__ __forceinline__ uint32_t finite(uint32_t u) {
+    return ((u & 0x7c00u) == 0x7c00u ? 0u : u & 0xffffu) | ((u & 0x7c000000u) == 0x7c000000u ? 0u : u & 0xffff0000u);
+  }
   static __device__ __forceinline__ floatx4 mfma16(uint4 a, uint4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+  }
+  static __device__ __forceinline__ floatx16 mfma32(uint4 a, uint4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
                                                   0, 0);
   }
 };
@@ -62,8 +71,15 @@ struct Half<true> {
   static __device__ __forceinline__ bool odd(uint32_t u) {
     return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
   }
+  static __device__ __forceinline__ uint32_t finite(uint32_t u) {
+    return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u);
+  }
   static __device__ __forceinline__ floatx4 mfma16(uint4 a, uint4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0,
+                                                   0);
+  }
+  static __device__ __forceinline__ floatx16 mfma32(uint4 a, uint4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0,
                                                    0);
   }
 };
@@ -194,7 +210,10 @@ struct Attn {
   float* lse;
   float* part;  // [splits][total_tokens * heads][D + 2] where splits > 1
   int64_t qt, qh, gt, gh, ot, oh;
-  int32_t heads, kv_heads, group, window, splits, chunk, one_tile;
+  int32_t heads, kv_heads, group, window, one_tile;
+  // key ranges of a tile and the least keys of one: [0] sequences of few rows, [1] of many
+  int32_t splits[2], chunk[2], tile_rows[2];
+  int32_t many;      // a sequence has many rows from this on
   float scale_log2;  // scale * log2(e)
 };
 
@@ -205,19 +224,21 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // Keys in one range of a tile that sees [lo, hi): the plan's, or more where
 // the lengths pass the host's bound.
-__device__ __forceinline__ int range_keys(const Attn& a, int lo, int hi) {
-  const int span = max(hi - (lo & ~31), 0);
-  return max(a.chunk, (int)((((int64_t)span + a.splits - 1) / a.splits + 127) & ~127));
+__device__ __forceinline__ int range_keys(const Attn& a, int kind, int lo, int hi) {
+  const int span = max(hi - (lo & ~31), 0), splits = a.splits[kind];
+  return max(a.chunk[kind], (int)((((int64_t)span + splits - 1) / splits + 127) & ~127));
 }
 
-// Tile `at` of the step's row tiles (n * group rows of a sequence, `rows` to a
-// tile, sequences in order): its sequence and its index there.  false past
-// the last.
-__device__ __forceinline__ bool find_tile(const Attn& a, int rows, int at, int lane, int* seq, int* tile) {
+// Tile `at` of the row tiles of the sequences of few (kind 0) or many (1) rows
+// (n * group rows of a sequence, `rows` to a tile, sequences in order): its
+// sequence and its index there.  false past the last.
+__device__ __forceinline__ bool find_tile(const Attn& a, int kind, int rows, int at, int lane, int* seq, int* tile) {
   for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64) {
     int mine = 0;
-    if (s0 + lane < a.c.num_seqs)
-      mine = (spk_paged::make_seq(a.c, a.c.cu[s0 + lane], a.c.cu[s0 + lane + 1], 0).n * a.group + rows - 1) / rows;
+    if (s0 + lane < a.c.num_seqs) {
+      const int n = spk_paged::make_seq(a.c, a.c.cu[s0 + lane], a.c.cu[s0 + lane + 1], 0).n * a.group;
+      if ((n >= a.many) == (kind == 1)) mine = (n + rows - 1) / rows;
+    }
     int sum = mine;  // inclusive scan
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -284,7 +305,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
   const int ln = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, kvh = blockIdx.y;
   int seq = blockIdx.z, tile = 0;
-  if (!a.one_tile && !find_tile(a, 16 * MT, blockIdx.z, lane, &seq, &tile)) return;
+  if (!a.one_tile && !find_tile(a, 0, 16 * MT, blockIdx.z, lane, &seq, &tile)) return;
   const Seq sq = spk_paged::seq_at(a.c, seq);
   const int rows = sq.n * a.group;
   const int r0 = tile * 16 * MT;
@@ -293,10 +314,10 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
   int lo, hi, lo_all, hi_all;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
   spk_paged::visible(sq, (min(r0 + 16 * MT, rows) - 1) / a.group, a.window, &lo_all, &hi);
-  const int keys = range_keys(a, lo, hi);
+  const int keys = range_keys(a, 0, lo, hi);
   const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
   const int end = begin + min(keys, hi - begin);
-  if (begin >= end && a.splits > 1) return;
+  if (begin >= end && a.splits[0] > 1) return;
 
   // this lane's row of each 16-row tile
   uint4 q[MT][DC];
@@ -399,7 +420,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
       float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = s[mt][i >> 2][i & 3] * a.scale_log2;
+        x[i] = s[mt][i >> 2][i & 3];
         if (!full) {
           const int kl = 16 * (i >> 2) + 4 * g + (i & 3);
           const bool see = (valid >> kl & 1u) && k0 + kl >= row_lo[mt] && k0 + kl < row_hi[mt];
@@ -409,6 +430,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
       float top = x[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
+      top *= a.scale_log2;
       if (__any(top > m[mt] + kBehind)) {
         top = fmaxf(top, spk::lane_xor16(top));
         top = fmaxf(top, spk::lane_xor32(top));
@@ -425,7 +447,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = exp2_fast(x[i] - base[mt] + H::kShift);
+        x[i] = exp2_fast(__builtin_fmaf(x[i], a.scale_log2, H::kShift - base[mt]));
         l[mt] += x[i];
       }
       p[mt] = make_uint4(H::pack(x[0], x[1]), H::pack(x[2], x[3]), H::pack(x[4], x[5]), H::pack(x[6], x[7]));
@@ -513,7 +535,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
           o[2] += f[w] * x.z;
           o[3] += f[w] * x.w;
         }
-        if (a.splits == 1) {
+        if (a.splits[0] == 1) {
 #pragma unroll
           for (int n = 0; n < 4; ++n) o[n] *= inv;
           store_out<BF, 4>(a, token, head, d, o);
@@ -523,7 +545,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
         }
       }
       if ((threadIdx.x & 15) == 0) {
-        if (a.splits > 1) {
+        if (a.splits[0] > 1) {
           part[0] = top;
           part[1] = sum;
         } else if (a.lse) {
@@ -534,9 +556,320 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
   }
 }
 
+// Many rows per sequence and KV head: a workgroup of 8 waves takes 256 of the
+// n * group rows, 32 to a wave, and walks the keys in tiles of KT that all
+// waves share in LDS, the next tile loading while this one is used.
+//
+// Scores are again S^T = K Q^T (32x32x16): a lane holds 16 keys' scores of one
+// row, and its weights are the B operand of O^T += V^T P^T as they are (lane
+// half h supplies keys 4h..4h+3 and 8+4h..+3 of each 16).  Both A operands are
+// one 16-byte LDS read of a lane.  K rows lie as in memory, their 16-byte
+// pieces exchanged by the row number so that 16 rows' pieces are in different
+// banks.  V is turned on the way in: a thread takes 8 keys' pieces of 4
+// dimensions and writes 4 dimensions' pieces of 8 keys, in fragment order; the
+// dimension of row m of output tile 4 u + e is 4 (m + 32 u) + e, which makes
+// these writes (and a lane's output) contiguous.
+template <int D, bool BF>
+__global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
+  using H = Half<BF>;
+  constexpr int KT = D == 256 ? 64 : 128;  // keys of a tile
+  constexpr int KS = D / 16;               // contraction steps of the scores
+  constexpr int QR = D == 256 ? 14 : KS;   // of the queries' pieces in registers, the rest in LDS
+  constexpr int DT = D / 32;               // output tiles
+  constexpr int CH = D / 8;                // 16-byte pieces of a row
+  constexpr int RPW = 64 / CH;             // rows of K in one wave-wide load
+  constexpr int KL = KT / 8 / RPW;         // such loads of a wave per tile
+  constexpr int RS = 32 / RPW;             // distance of its rows: load x of 32 keys holds rows x, x + RS, ...
+  constexpr int LG = D / 4;                // lanes that cover a row of V (8 bytes each)
+  constexpr int GW = 64 / LG;              // groups of 8 keys of a wave
+  constexpr int VW = KT / 8 / GW;          // waves that load V
+  constexpr int U = KT / 64;               // lookups of a lane per tile
+  // two tiles, as separate arrays: a load into one is then known not to touch the other
+  __shared__ __align__(16) uint4 k0s[KT * CH / 64 * 65], k1s[KT * CH / 64 * 65], v0s[KT * CH], v1s[KT * CH];
+  __shared__ __align__(16) uint4 qs[KS > QR ? (KS - QR) * 512 : 1];
+  __shared__ uint32_t odd_of[3][KT / 32];  // keys of a tile with values that are not finite (tile number % 3)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.y, split = blockIdx.x;
+  int seq, tile;
+  if (!find_tile(a, 1, 256, blockIdx.z, lane, &seq, &tile)) return;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const Seq sq = spk_paged::seq_at(a.c, seq);
+  const int rows = sq.n * a.group;
+  const int r0 = tile * 256, r1 = min(r0 + 256, rows);
+  int lo, hi, lo_all, hi_all;
+  spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
+  spk_paged::visible(sq, (r1 - 1) / a.group, a.window, &lo_all, &hi);
+  const int keys = range_keys(a, 1, lo, hi);
+  const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
+  const int end = begin + min(keys, hi - begin);
+  if (begin >= end && a.splits[1] > 1) return;
+
+  const int r = min(r0 + 32 * wave + ln, rows - 1);
+  const int ri = r / a.group, head = kvh * a.group + r - ri * a.group, token = sq.first + ri;
+  int row_lo, row_hi, wave_lo, wave_hi, wave_lo_all, wave_hi_all;
+  spk_paged::visible(sq, ri, a.window, &row_lo, &row_hi);
+  spk_paged::visible(sq, min(r0 + 32 * wave, rows - 1) / a.group, a.window, &wave_lo, &wave_hi_all);
+  spk_paged::visible(sq, min(r0 + 32 * wave + 31, rows - 1) / a.group, a.window, &wave_lo_all, &wave_hi);
+  uint4 q[QR];
+  {
+    const uint16_t* src = a.q + token * a.qt + head * a.qh + 8 * h;
+#pragma unroll
+    for (int c = 0; c < QR; ++c) q[c] = *reinterpret_cast<const uint4*>(src + 16 * c);
+#pragma unroll
+    for (int c = QR; c < KS; ++c) qs[(c - QR) * 512 + tid] = *reinterpret_cast<const uint4*>(src + 16 * c);
+  }
+  floatx16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
+  const uint16_t* kbase = a.k + kvh * a.c.head_stride;
+  const uint16_t* vbase = a.v + kvh * a.c.head_stride;
+
+  // key k0 + 64 u + lane of the tile that is loaded next
+  int64_t off[U];
+  unsigned long long valid[U];
+  auto look_up = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = k0 + 64 * u + lane;
+      off[u] = -1;
+      if (key >= lo && key < end) off[u] = spk_paged::offset_in(a.c, table[spk_paged::divide(a.c.div, (uint32_t)key)], key);
+      valid[u] = __ballot(off[u] >= 0);
+      if (off[u] < 0) off[u] = 0;
+    }
+  };
+  auto offset = [&](int kl) -> int64_t {  // of key kl of the tile, from its lane
+    int64_t o = off[0];
+    if constexpr (U == 2) o = kl & 64 ? off[1] : off[0];
+    return __shfl(o, kl & 63);
+  };
+  auto scalar_offset = [&](int kl) -> int64_t {  // the same for a key that the whole wave asks for
+    return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)off[0], kl) |
+           (int64_t)__builtin_amdgcn_readlane((int)(off[0] >> 32), kl) << 32;
+  };
+  uint2 vr[8];
+  const int vg = GW == 1 ? wave : wave * GW + lane / LG, dc = lane % LG;  // V: group of 8 keys, piece of 4 dimensions
+  auto load_k = [&](uint4* ks) {
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int x = wave * KL + i;
+      const int row = x % RS + 32 * (x / RS);
+      int64_t at;
+      if constexpr (RPW == 2)
+        at = h ? scalar_offset(row + RS) : scalar_offset(row);
+      else
+        at = offset(row + RS * (lane / CH));
+      const uint16_t* src = kbase + at + 8 * (lane % CH);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (__attribute__((address_space(3))) void*)&ks[x * 65], 16, 0, 0);
+    }
+  };
+  const int kread = (ln % RS) * 65 + (ln / RS) * CH + h;  // of this lane's row and half in the 32 keys' loads
+  auto v_key = [&](int kk) { return 16 * (vg >> 1) + 8 * (kk >> 2) + 4 * (vg & 1) + (kk & 3); };
+  auto load_v = [&]() {
+    if (VW == 8 || wave < VW) {
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        int64_t at;
+        if constexpr (GW == 1)
+          at = scalar_offset(v_key(kk));
+        else
+          at = offset(v_key(kk));
+        vr[kk] = *reinterpret_cast<const uint2*>(vbase + at + 4 * dc);
+      }
+    }
+  };
+  // Some row of the workgroup does not see the whole tile at k0.  Then a value
+  // that is not finite must not meet the zero weight of a row that does not
+  // see it: such elements are stored as zeros, and added row by row.
+  auto partial = [&](int k0) {
+    bool all = k0 >= lo_all && k0 + KT <= min(hi_all, end);
+#pragma unroll
+    for (int u = 0; u < U; ++u) all = all && valid[u] == ~0ull;
+    return !all;
+  };
+  auto store_v = [&](uint4* vs, int k0, int third) {
+    if (VW < 8 && wave >= VW) return;
+    if (partial(k0)) {
+      uint32_t odd = 0;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const int kl = v_key(kk);
+        const bool has = (U == 2 && (kl & 64) ? valid[U - 1] : valid[0]) >> (kl & 63) & 1ull;
+        if (!has) vr[kk] = make_uint2(0, 0);
+        if (H::odd(vr[kk].x) || H::odd(vr[kk].y)) odd |= 1u << kk;
+        vr[kk] = make_uint2(H::finite(vr[kk].x), H::finite(vr[kk].y));
+      }
+      while (odd) {
+        const int kl = v_key(__ffs(odd) - 1);
+        odd &= odd - 1;
+        atomicOr(&odd_of[third][kl >> 5], 1u << (kl & 31));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint4 f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        (&f.x)[w] = __builtin_amdgcn_perm((&vr[2 * w + 1].x)[e >> 1], (&vr[2 * w].x)[e >> 1],
+                                          e & 1 ? 0x07060302u : 0x05040100u);
+      const int t = D >= 128 ? e + 4 * (dc / 32) : e >> 1, row = D >= 128 ? dc % 32 : dc + 16 * (e & 1);
+      vs[((vg >> 1) * DT + t) * 64 + row + 32 * (vg & 1)] = f;
+    }
+  };
+  auto dim_of = [&](int t, int row) { return D >= 128 ? 4 * (row + 32 * (t >> 2)) + (t & 3) : 4 * (row & 15) + 2 * t + (row >> 4); };
+
+  if (tid < 3 * (KT / 32)) odd_of[tid / (KT / 32)][tid % (KT / 32)] = 0;
+  int third = 0;
+  unsigned long long now[U];
+  bool part = true;
+  auto step = [&](int k0, uint4* ks, uint4* vs, uint4* ks_next, uint4* vs_next) __attribute__((always_inline)) {
+    const bool more = k0 + KT < end;
+    const int after = third == 2 ? 0 : third + 1;
+    part = partial(k0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = valid[u];
+    if (tid < KT / 32) odd_of[after == 2 ? 0 : after + 1][tid] = 0;  // the tile before this one's
+    if (more) {
+      look_up(k0 + KT);
+      load_k(ks_next);
+    }
+#pragma unroll 1
+    for (int j = 0; j < KT / 32; ++j) {
+      const int kj = k0 + 32 * j;
+      if (j == KT / 32 - 1 && more) load_v();
+      if (kj >= min(wave_hi, end) || kj + 32 <= wave_lo) continue;
+      const uint32_t has = (uint32_t)((U == 2 && j > 1 ? now[U - 1] : now[0]) >> (32 * (j & 1)));
+      const bool full = has == 0xffffffffu && kj >= wave_lo_all && kj + 32 <= wave_hi_all;
+      floatx16 s;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < KS; ++c) s = H::mfma32(ks[j * RS * 65 + kread + 2 * c], c < QR ? q[c] : qs[(c - QR) * 512 + tid], s);
+      if (!full) {
+        // bit n: this row sees key n of the 32; shifted so that a lane's keys are at constant places
+        const int first = min(max(row_lo - kj, 0), 31), last = min(max(row_hi - kj, 0), 32);
+        uint32_t see = row_lo - kj > 31 || last == 0 ? 0u : has & (0xffffffffu << first) & (0xffffffffu >> (32 - last));
+        see >>= 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[i] : -INFINITY;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top *= a.scale_log2;
+      if (__any(top > m + kBehind)) {
+        top = fmaxf(top, spk::lane_xor32(top));
+        const float next = fmaxf(m, top);
+        const float nb = next == -INFINITY ? 0.0f : next;
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nb);
+        m = next;
+        base = nb;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[t] *= f;
+      }
+      uint4 p[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = exp2_fast(__builtin_fmaf(s[i], a.scale_log2, H::kShift - base));
+        l += s[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        p[i] = make_uint4(H::pack(s[8 * i], s[8 * i + 1]), H::pack(s[8 * i + 2], s[8 * i + 3]),
+                          H::pack(s[8 * i + 4], s[8 * i + 5]), H::pack(s[8 * i + 6], s[8 * i + 7]));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[t] = H::mfma32(vs[((2 * j + i) * DT + t) * 64 + lane], p[i], acc[t]);
+      if (part) {
+        uint32_t odd = __builtin_amdgcn_readfirstlane(odd_of[third][j]);
+        while (odd) {
+          const int kl = __ffs(odd) - 1;
+          odd &= odd - 1;
+          const uint16_t* row = vbase + spk_paged::offset_of(a.c, seq, kj + kl);
+          const uint4 quad = kl & 16 ? p[1] : p[0];
+          uint32_t pair = kl & 8 ? (kl & 2 ? quad.w : quad.z) : (kl & 2 ? quad.y : quad.x);
+          pair = __shfl((int)pair, ln + 32 * ((kl >> 2) & 1));
+          const float weight = H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
+          if (kj + kl >= row_lo && kj + kl < row_hi) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const uint16_t x = row[dim_of(t, 8 * (i >> 2) + 4 * h + (i & 3))];
+                if (H::odd(x)) acc[t][i] += weight * H::widen(x);
+                __builtin_amdgcn_sched_barrier(0);  // one at a time: this path takes no registers from the others
+              }
+          }
+        }
+      }
+    }
+    if (more) {
+      store_v(vs_next, k0 + KT, after);
+    }
+    third = after;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the keys' loads into LDS
+    __syncthreads();
+  };
+  if (begin < end) {
+    look_up(begin);
+    load_k(k0s);
+    load_v();
+    __syncthreads();
+    store_v(v0s, begin, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int k0 = begin; k0 < end; k0 += 2 * KT) {
+      step(k0, k0s, v0s, k1s, v1s);
+      if (k0 + KT >= end) break;
+      step(k0 + KT, k1s, v1s, k0s, v0s);
+    }
+  }
+
+  l += spk::lane_xor32(l);
+  if (r0 + 32 * wave + ln >= rows) return;
+  const int64_t at = (int64_t)token * a.heads + head;
+  if (a.splits[1] > 1) {
+    float* part = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
+    if (h == 0) {
+      part[0] = m;
+      part[1] = l;
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[2 + dim_of(t, 8 * (i >> 2) + 4 * h + (i & 3))] = acc[t][i];
+    return;
+  }
+  if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m - H::kShift + __builtin_amdgcn_logf(l)) * kLn2;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if constexpr (D >= 128) {
+#pragma unroll
+    for (int u = 0; u < DT / 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float o[4] = {acc[4 * u][i] * inv, acc[4 * u + 1][i] * inv, acc[4 * u + 2][i] * inv, acc[4 * u + 3][i] * inv};
+        store_out<BF, 4>(a, token, head, dim_of(4 * u, 8 * (i >> 2) + 4 * h + (i & 3)), o);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // rows m and m + 16 hold dimensions 4 (m % 16) + 2 t + 0 and 1
+      const float o[4] = {acc[0][i] * inv, acc[0][i + 8] * inv, acc[1][i] * inv, acc[1][i + 8] * inv};
+      store_out<BF, 4>(a, token, head, dim_of(0, 8 * (i >> 2) + 4 * h + (i & 3)), o);
+    }
+  }
+}
+
 // Joins the key ranges of a row: one wave per (token, head).
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void paged_join_kernel(Attn a, int tile_rows) {
+__global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
   constexpr int N = D / 64 >= 2 ? D / 64 : 1;
   const int lane = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -548,12 +881,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a, int tile_rows) 
   if (token < sq.first || token >= sq.first + sq.n) return;
   // the ranges that the row's tile had
   const int rows = sq.n * a.group, r = (token - sq.first) * a.group + head % a.group;
+  const int kind = rows >= a.many, tile_rows = a.tile_rows[kind];
+  if (a.splits[kind] == 1) return;
   const int r0 = r / tile_rows * tile_rows;
   int lo, hi, x;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
   spk_paged::visible(sq, (min(r0 + tile_rows, rows) - 1) / a.group, a.window, &x, &hi);
   const int span = hi - (lo & ~31);
-  const int keys = range_keys(a, lo, hi);
+  const int keys = range_keys(a, kind, lo, hi);
   const int n = span <= 0 ? 0 : (int)(((int64_t)span + keys - 1) / keys);
   const int64_t step = (int64_t)a.c.total_tokens * a.heads * (D + 2);
   const float* part = a.part + at * (D + 2);
@@ -628,28 +963,42 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
   return SPK_OK;
 }
 
-// How a call's rows and keys are dealt: rows per tile, tiles, key ranges.
+// How a call's rows and keys are dealt to the two kernels.
 struct Plan {
-  int mt, tiles, one_tile, splits, chunk;
+  int mt, one_tile, many;
+  int tiles[2], splits[2], chunk[2], tile_rows[2];
 };
 
-Plan plan_rows(const SpkPagedAttnArgs& p) {
+Plan plan_of(const SpkPagedAttnArgs& p) {
   const SpkPagedCache& c = p.cache;
   const int group = p.num_q_heads / c.num_kv_heads;
-  const int64_t longest = (int64_t)std::min(p.max_query_len, c.total_tokens) * group;
+  const int64_t tokens = std::min(p.max_query_len, c.total_tokens);
+  const int64_t longest = tokens * group, all = (int64_t)c.total_tokens * group;
   Plan r;
-  r.mt = longest <= 16 ? 1 : 2;
-  r.one_tile = longest <= 16 * r.mt;
-  r.tiles = r.one_tile ? c.num_seqs
-                       : (int)std::min<int64_t>((int64_t)c.total_tokens * group / (16 * r.mt) + c.num_seqs, INT32_MAX);
+  r.many = 65;
+  const bool any_many = longest >= r.many;
+  const int64_t few = std::min<int64_t>(longest, r.many - 1);
+  r.mt = few <= 16 ? 1 : 2;
+  r.tile_rows[0] = 16 * r.mt;
+  r.tile_rows[1] = 256;
+  r.one_tile = !any_many && few <= r.tile_rows[0];
+  // sequences of few rows: all of them, unless the longest takes every row
+  r.tiles[0] = r.one_tile ? c.num_seqs
+               : any_many && c.num_seqs == 1
+                   ? 0
+                   : (int)std::min<int64_t>(all / r.tile_rows[0] + c.num_seqs, INT32_MAX);
+  r.tiles[1] = any_many ? (int)std::min<int64_t>(all / 256 + std::min<int64_t>(c.num_seqs, all / r.many), INT32_MAX) : 0;
   int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
-  if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + std::min(p.max_query_len, c.total_tokens) + 31);
-  const int64_t groups = (int64_t)r.tiles * c.num_kv_heads;
-  const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(groups, 1));
-  const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);
-  const int64_t per = (steps + want - 1) / want;
-  r.chunk = (int)(128 * per);
-  r.splits = (int)((steps + per - 1) / per);
+  if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
+  for (int kind = 0; kind < 2; ++kind) {
+    const int64_t groups = (int64_t)r.tiles[kind] * c.num_kv_heads;
+    const int64_t want = std::max<int64_t>(1, (kind ? 256 : 1024) / std::max<int64_t>(groups, 1));
+    const int64_t least = kind ? 4 : 1;  // steps of 128 keys
+    const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);
+    const int64_t per = std::max(least, (steps + want - 1) / want);
+    r.chunk[kind] = (int)(128 * per);
+    r.splits[kind] = r.tiles[kind] ? (int)((steps + per - 1) / per) : 1;
+  }
   return r;
 }
 
@@ -659,6 +1008,8 @@ int check_attn(const SpkPagedAttnArgs* p, Cache* c) {
   if (p->num_q_heads <= 0 || p->num_q_heads % p->cache.num_kv_heads)
     return spk::fail(SPK_ERR_SHAPE, "spk_paged_attention: %d query heads over %d KV heads", p->num_q_heads,
                      p->cache.num_kv_heads);
+  if (!(p->scale >= 0.0f) || p->scale > 1e30f)
+    return spk::fail(SPK_ERR_ARG, "spk_paged_attention: scale %g (positive, or 0 for 1/sqrt(head_dim))", (double)p->scale);
   if (p->max_query_len < 0 || p->max_context_len < 0 || p->window < 0)
     return spk::fail(SPK_ERR_SHAPE, "spk_paged_attention: max_query_len %d max_context_len %d window %d",
                      p->max_query_len, p->max_context_len, p->window);
@@ -668,21 +1019,24 @@ int check_attn(const SpkPagedAttnArgs* p, Cache* c) {
 }
 
 size_t workspace_of(const SpkPagedAttnArgs& p) {
-  const Plan r = plan_rows(p);
-  if (r.splits <= 1) return 0;
-  return (size_t)r.splits * p.cache.total_tokens * p.num_q_heads * (p.cache.head_dim + 2) * sizeof(float);
+  const Plan r = plan_of(p);
+  const int splits = std::max(r.splits[0], r.splits[1]);
+  if (splits <= 1) return 0;
+  return (size_t)splits * p.cache.total_tokens * p.num_q_heads * (p.cache.head_dim + 2) * sizeof(float);
 }
 
 template <int D, bool BF>
 void launch_attn(const Attn& a, const Plan& r, hipStream_t s) {
-  const dim3 grid(r.splits, a.kv_heads, r.tiles);
-  if (r.mt == 1)
+  const dim3 grid(r.splits[0], a.kv_heads, r.tiles[0]);
+  if (r.tiles[0] && r.mt == 1)
     hipLaunchKernelGGL((paged_rows_kernel<D, 1, BF>), grid, dim3(256), 0, s, a);
-  else
+  else if (r.tiles[0])
     hipLaunchKernelGGL((paged_rows_kernel<D, 2, BF>), grid, dim3(256), 0, s, a);
-  if (r.splits > 1) {
+  if (r.tiles[1])
+    hipLaunchKernelGGL((paged_tiles_kernel<D, BF>), dim3(r.splits[1], a.kv_heads, r.tiles[1]), dim3(512), 0, s, a);
+  if (r.splits[0] > 1 || r.splits[1] > 1) {
     const int64_t rows = (int64_t)a.c.total_tokens * a.heads;
-    hipLaunchKernelGGL((paged_join_kernel<D, BF>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, 16 * r.mt);
+    hipLaunchKernelGGL((paged_join_kernel<D, BF>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
   }
 }
 
@@ -781,13 +1135,14 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
       !strides_ok(p->q_token_stride, p->q_head_stride) || !strides_ok(p->out_token_stride, p->out_head_stride) ||
       (p->gate && !strides_ok(p->gate_token_stride, p->gate_head_stride)))
     return spk::fail(SPK_ERR_ALIGN, "%s: q, gate and out and their strides must be 16-byte aligned", who);
-  const Plan r = plan_rows(*p);
+  const Plan r = plan_of(*p);
   const size_t need = workspace_of(*p);
   if (need && (!p->workspace || p->workspace_bytes < need || !spk::aligned(p->workspace, 256)))
     return spk::fail(p->workspace ? SPK_ERR_ARG : SPK_ERR_NULL, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)",
                      who, p->workspace ? p->workspace_bytes : (size_t)0, need);
-  if (c.num_kv_heads > 65535 || r.tiles > 65535)
-    return spk::fail(SPK_ERR_SHAPE, "%s: %d KV heads, %d row tiles (65535 at most)", who, c.num_kv_heads, r.tiles);
+  if (c.num_kv_heads > 65535 || r.tiles[0] > 65535 || r.tiles[1] > 65535)
+    return spk::fail(SPK_ERR_SHAPE, "%s: %d KV heads, %d row tiles (65535 at most)", who, c.num_kv_heads,
+                     std::max(r.tiles[0], r.tiles[1]));
   a.q = static_cast<const uint16_t*>(p->q);
   a.k = static_cast<const uint16_t*>(c.k_cache);
   a.v = static_cast<const uint16_t*>(c.v_cache);
@@ -805,9 +1160,13 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
   a.kv_heads = c.num_kv_heads;
   a.group = p->num_q_heads / c.num_kv_heads;
   a.window = p->window;
-  a.splits = r.splits;
-  a.chunk = r.chunk;
+  for (int kind = 0; kind < 2; ++kind) {
+    a.splits[kind] = r.splits[kind];
+    a.chunk[kind] = r.chunk[kind];
+    a.tile_rows[kind] = r.tile_rows[kind];
+  }
   a.one_tile = r.one_tile;
+  a.many = r.many;
   const float scale = p->scale != 0.0f ? p->scale : 1.0f / std::sqrt((float)c.head_dim);
   a.scale_log2 = scale * 1.44269504088896341f;
   hipStream_t s = spk::to_hip(stream);
