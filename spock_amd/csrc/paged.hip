@@ -208,12 +208,14 @@ struct Attn {
   const uint16_t *q, *k, *v, *gate;
   uint16_t* out;
   float* lse;
-  float* part;  // [splits][total_tokens * heads][D + 2] where splits > 1
+  float* shared;  // few rows: [shares][share_rows][D + 2], of the shares that are not alone
+  float* part;    // many rows: [splits][total_tokens * heads][D + 2] where splits > 1
   int64_t qt, qh, gt, gh, ot, oh;
-  int32_t heads, kv_heads, group, window, one_tile;
-  // key ranges of a tile and the least keys of one: [0] sequences of few rows, [1] of many
-  int32_t splits[2], chunk[2], tile_rows[2];
-  int32_t many;      // a sequence has many rows from this on
+  int32_t heads, kv_heads, group, window;
+  int32_t many;                // a sequence has many rows from this on
+  int32_t shares, share_rows;  // few rows: workgroups, and rows of one
+  int32_t alone;               // few rows: no ranges
+  int32_t splits, chunk;       // many rows: key ranges of a tile and the least keys of one
   float scale_log2;  // scale * log2(e)
 };
 
@@ -222,39 +224,209 @@ constexpr float kBehind = 8.0f;  // binades that the running maximum may lag
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Keys in one range of a tile that sees [lo, hi): the plan's, or more where
-// the lengths pass the host's bound.
-__device__ __forceinline__ int range_keys(const Attn& a, int kind, int lo, int hi) {
-  const int span = max(hi - (lo & ~31), 0), splits = a.splits[kind];
-  return max(a.chunk[kind], (int)((((int64_t)span + splits - 1) / splits + 127) & ~127));
+// A load of what is read once.
+__device__ __forceinline__ uint4 load_once(const uint16_t* p) {
+  typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)));
 }
 
-// Tile `at` of the row tiles of the sequences of few (kind 0) or many (1) rows
-// (n * group rows of a sequence, `rows` to a tile, sequences in order): its
-// sequence and its index there.  false past the last.
-__device__ __forceinline__ bool find_tile(const Attn& a, int kind, int rows, int at, int lane, int* seq, int* tile) {
+// The work of the sequences of few rows, dealt to the workgroups of a launch:
+// each takes the rows of one sequence, tile of rows and KV head over one range
+// of its keys.  The ranges' length follows from the lengths on the device, so
+// that they fill the launch once and are nearly equal: with pieces = (sequence,
+// tile, head) the number of shares for ranges of c keys is the sum of
+// ceil(keys / c) over the pieces, and c the smallest tried with no more shares
+// than workgroups.  Every workgroup finds c and its share by itself.
+struct Share {
+  int seq, tile, kvh;
+  int range, ranges, keys;  // this one of the piece's, and the keys of each
+  int lo;                   // where the first range begins
+  int first;                // the piece's first share
+};
+
+struct Load {
+  int tiles, span;  // tiles of rows, keys that they see
+};
+
+// Of sequence s; nothing past the last.  No branch before the loads: those of
+// several sequences are under way together.
+__device__ __forceinline__ Load load_of(const Attn& a, int s) {
+  const Seq sq = spk_paged::seq_at(a.c, min(s, a.c.num_seqs - 1));
+  const int rows = s < a.c.num_seqs ? sq.n * a.group : 0;
+  int lo, hi, x;
+  spk_paged::visible(sq, 0, a.window, &lo, &x);
+  spk_paged::visible(sq, sq.n - 1, a.window, &x, &hi);
+  const bool few = rows > 0 && rows < a.many;
+  return {few ? (rows + a.share_rows - 1) / a.share_rows : 0, few ? max(hi - (lo & ~31), 1) : 0};
+}
+
+__device__ __forceinline__ int ranges_of(const Load& l, int c) { return (l.span - 1) / c + (l.span > 0); }
+
+// Sum over the wave, in every lane; and the inclusive running sum.  Lane swaps
+// and DPP moves: an LDS permute is ten times as long, and every workgroup
+// stands still for these.
+__device__ __forceinline__ int wave_sum(int v) {
+  v += (int)spk::lane_xor32_u((uint32_t)v);
+  v += (int)spk::lane_xor16_u((uint32_t)v);
+  v += (int)spk::row_ror_u<8>((uint32_t)v);
+  v += (int)spk::row_ror_u<4>((uint32_t)v);
+  v += (int)spk::row_ror_u<2>((uint32_t)v);
+  v += (int)spk::row_ror_u<1>((uint32_t)v);
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += spk::lane_xor32(v);
+  v += spk::lane_xor16(v);
+  v += __uint_as_float(spk::row_ror_u<8>(__float_as_uint(v)));
+  v += __uint_as_float(spk::row_ror_u<4>(__float_as_uint(v)));
+  v += __uint_as_float(spk::row_ror_u<2>(__float_as_uint(v)));
+  v += __uint_as_float(spk::row_ror_u<1>(__float_as_uint(v)));
+  return v;
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15 of a row to the next row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 to the upper half
+  return v;
+}
+
+// The share numbered `at`, or (seq >= 0) the first of the piece (seq, tile, kvh).  false: there is none.
+__device__ __forceinline__ bool find_share(const Attn& a, int at, int seq, int tile, int kvh, int lane, Share* out) {
+  constexpr int N = 4;  // sequences of a lane at a time
+  Load mine[N];
+  long long keys = 0;
+  int pieces = 0, low = 0, high = 0;  // keys = high * 2^16 + low
+  for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64 * N)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      mine[j] = load_of(a, s0 + N * lane + j);
+      keys += (long long)mine[j].tiles * mine[j].span;
+      pieces += mine[j].tiles;
+    }
+  low = (int)(keys & 0xffff);
+  high = (int)(keys >> 16);
+  keys = (((long long)__builtin_amdgcn_readfirstlane(wave_sum(high)) << 16) + __builtin_amdgcn_readfirstlane(wave_sum(low))) *
+         a.kv_heads;
+  pieces = __builtin_amdgcn_readfirstlane(wave_sum(pieces)) * a.kv_heads;
+  if (pieces == 0) return false;
+  // enough for any lengths: each piece's last range may be short
+  auto whole = [](long long k) { return (int)((min(k, (long long)INT32_MAX - 128) + 127) & ~127ll); };
+  int c = INT32_MAX;
+  if (!a.alone) {
+    const int room = max(a.shares - pieces, 1);
+    c = __builtin_amdgcn_readfirstlane(whole((keys + room - 1) / room));
+  }
+  if (!a.alone && a.c.num_seqs <= 64 * N) {
+    for (int t = __builtin_amdgcn_readfirstlane(whole((keys + a.shares - 1) / a.shares)); t < c; t += max(128, (t >> 4) & ~127)) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) n += mine[j].tiles * ranges_of(mine[j], t);
+      if (__builtin_amdgcn_readfirstlane(wave_sum(n)) * a.kv_heads <= a.shares) c = t;
+    }
+  }
+  int before = 0;
+  for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64 * N) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (a.c.num_seqs > 64 * N) mine[j] = load_of(a, s0 + N * lane + j);
+      n += mine[j].tiles * a.kv_heads * ranges_of(mine[j], c);
+    }
+    const int sum = wave_scan(n), total = __builtin_amdgcn_readlane(sum, 63);
+    if (seq >= 0 ? seq < s0 + 64 * N : at < before + total) {
+      // the lane that holds it, then the one of its sequences
+      const int l = __builtin_amdgcn_readfirstlane(seq >= 0 ? (seq - s0) / N : __popcll(__ballot(before + sum <= at)));
+      int first = before + sum - n;
+      Load found{0, 0};
+      int s = -1;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int count = mine[j].tiles * a.kv_heads * ranges_of(mine[j], c);
+        const bool here = seq >= 0 ? s0 + N * lane + j == seq : at >= first && at < first + count;
+        if (s < 0) {
+          if (here) {
+            s = s0 + N * lane + j;
+            found = mine[j];
+          } else {
+            first += count;
+          }
+        }
+      }
+      s = __builtin_amdgcn_readlane(s, l);
+      first = __builtin_amdgcn_readlane(first, l);
+      found.tiles = __builtin_amdgcn_readlane(found.tiles, l);
+      found.span = __builtin_amdgcn_readlane(found.span, l);
+      if (s < 0 || found.tiles == 0) return false;
+      out->seq = s;
+      out->ranges = ranges_of(found, c);
+      out->keys = (((found.span + out->ranges - 1) / out->ranges) + 127) & ~127;
+      if (seq >= 0) {
+        out->tile = tile;
+        out->kvh = kvh;
+        out->range = 0;
+      } else {
+        const int rest = at - first, piece = rest / out->ranges;
+        out->range = rest - piece * out->ranges;
+        out->tile = piece / a.kv_heads;
+        out->kvh = piece - out->tile * a.kv_heads;
+      }
+      out->first = first + (out->tile * a.kv_heads + out->kvh) * out->ranges;
+      int x;
+      spk_paged::visible(spk_paged::seq_at(a.c, out->seq), 0, a.window, &out->lo, &x);
+      out->lo &= ~31;
+      return true;
+    }
+    before += total;
+  }
+  return false;
+}
+
+// Keys in one range of a tile of many rows that sees [lo, hi): the plan's, or
+// more where the lengths pass the host's bound.
+__device__ __forceinline__ int range_keys(const Attn& a, int lo, int hi) {
+  const int span = max(hi - (lo & ~31), 0);
+  return max(a.chunk, (int)((((int64_t)span + a.splits - 1) / a.splits + 127) & ~127));
+}
+
+// Bit n: a row that sees keys [lo, hi) sees key k0 + n, where `has` says that
+// the key exists.
+__device__ __forceinline__ uint32_t seen(uint32_t has, int k0, int lo, int hi) {
+  const int first = lo - k0, last = hi - k0;
+  if (first > 31 || last <= 0) return 0;
+  return has & (0xffffffffu << max(first, 0)) & (0xffffffffu >> (32 - min(last, 32)));
+}
+
+// Tile `at` of the row tiles of the sequences of many rows (n * group rows of a
+// sequence, `rows` to a tile, sequences in order): its sequence and its index
+// there.  false past the last.
+__device__ __forceinline__ bool find_tile(const Attn& a, int rows, int at, int lane, int* seq, int* tile) {
   for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64) {
     int mine = 0;
     if (s0 + lane < a.c.num_seqs) {
       const int n = spk_paged::make_seq(a.c, a.c.cu[s0 + lane], a.c.cu[s0 + lane + 1], 0).n * a.group;
-      if ((n >= a.many) == (kind == 1)) mine = (n + rows - 1) / rows;
+      if (n >= a.many) mine = (n + rows - 1) / rows;
     }
-    int sum = mine;  // inclusive scan
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(sum, d);
-      if (lane >= d) sum += o;
-    }
-    const int total = __shfl(sum, 63);
+    const int sum = wave_scan(mine), total = __builtin_amdgcn_readlane(sum, 63);
     if (at < total) {
       const int l = __popcll(__ballot(sum <= at));
       *seq = s0 + l;
-      *tile = at - (__shfl(sum, l) - __shfl(mine, l));
+      *tile = at - __builtin_amdgcn_readlane(sum - mine, l);
       return true;
     }
     at -= total;
   }
   return false;
+}
+
+// 16 lanes' 8-byte pieces of 4 rows (4 lanes a row) turned: lane l of the 16
+// gets column l's four.
+__device__ __forceinline__ uint2 transposed(const uint2* p) {
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
 }
 
 // out (gated, rounded) of 4-aligned elements d .. d + N of a row.
@@ -279,11 +451,13 @@ __device__ __forceinline__ void store_out(const Attn& a, int token, int head, in
         make_uint2(Half<BF>::pack(x[i], x[i + 1]), Half<BF>::pack(x[i + 2], x[i + 3]));
 }
 
-// Few rows per sequence and KV head.  A workgroup takes 16 * MT of the
+// Few rows per sequence and KV head.  A workgroup takes 16 of the
 // n * group rows and a range of the keys; each of its 4 waves takes every
 // fourth step of 32 keys by itself, straight from memory into registers (the
 // rows share each K and V element, nothing is staged), and the waves' softmax
-// states are joined in LDS at the end.
+// states are joined in LDS at the end.  The next step's keys are loaded into
+// the registers that the scores have used, its values into those that the
+// output has: every wave has 16 to 32 KiB in flight all the time.
 //
 // Scores are formed transposed, S^T = K Q^T (16x16x32), so that a lane holds
 // 8 keys' scores of one row: the running maximum and sum need no exchange
@@ -291,99 +465,176 @@ __device__ __forceinline__ void store_out(const Attn& a, int token, int head, in
 // directly the B operand of O^T += V^T P^T.  The order of the 32 keys in that
 // product is free: lane group g supplies keys 4g..4g+3 and 16+4g..+3, which are the
 // ones its scores are.  V's A operand (8 keys of one dimension) is made from
-// 16-byte row pieces by pairing halfwords of two keys.
-template <int D, int MT, bool BF>
-__global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
+// 16-byte row pieces by pairing halfwords of two keys.  A weight enters as
+// two 16-bit parts (value and remainder): the kernel waits for memory, and the
+// second product keeps a few heavy keys' rounding out of the result.
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
   using H = Half<BF>;
   constexpr int DC = D / 32;             // contraction steps of the scores
   constexpr int EV = D >= 128 ? 8 : 4;   // elements of V in one load
   constexpr int NH = D / (16 * EV);      // loads that cover a row
   constexpr int LD = D + 4;              // padded rows of the joint
+  constexpr bool QL = D == 256;          // the queries lie in LDS, in fragment order
   __shared__ __align__(16) float joint[4][16][LD];
   __shared__ float stat[4][16][2];
+  __shared__ __align__(16) uint4 qs[QL ? DC * 64 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int ln = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, kvh = blockIdx.y;
-  int seq = blockIdx.z, tile = 0;
-  if (!a.one_tile && !find_tile(a, 0, 16 * MT, blockIdx.z, lane, &seq, &tile)) return;
+  Share sh;
+  if (!find_share(a, blockIdx.x, -1, 0, 0, lane, &sh)) return;
+  const int seq = sh.seq, kvh = sh.kvh;
   const Seq sq = spk_paged::seq_at(a.c, seq);
   const int rows = sq.n * a.group;
-  const int r0 = tile * 16 * MT;
-  if (r0 >= rows) return;
-  // keys that any row of the tile sees, and those that all see
+  const int r0 = sh.tile * 16;
+  // keys of the range that any row of the tile sees, and those that all see
   int lo, hi, lo_all, hi_all;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
-  spk_paged::visible(sq, (min(r0 + 16 * MT, rows) - 1) / a.group, a.window, &lo_all, &hi);
-  const int keys = range_keys(a, 0, lo, hi);
-  const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
-  const int end = begin + min(keys, hi - begin);
-  if (begin >= end && a.splits[0] > 1) return;
+  spk_paged::visible(sq, (min(r0 + 16, rows) - 1) / a.group, a.window, &lo_all, &hi);
+  const int begin = (int)min((int64_t)sh.lo + (int64_t)sh.range * sh.keys, (int64_t)hi);
+  const int end = begin + min(sh.keys, hi - begin);
 
-  // this lane's row of each 16-row tile
-  uint4 q[MT][DC];
-  int row_lo[MT], row_hi[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = min(r0 + 16 * mt + ln, rows - 1);
-    const int i = r / a.group;
-    spk_paged::visible(sq, i, a.window, &row_lo[mt], &row_hi[mt]);
-    const uint16_t* src = a.q + (sq.first + i) * a.qt + (kvh * a.group + r - i * a.group) * a.qh;
-#pragma unroll
-    for (int c = 0; c < DC; ++c) q[mt][c] = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * g);
-  }
-  float m[MT], base[MT], l[MT];
-  floatx4 acc[MT][NH][EV];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = -INFINITY;
-    base[mt] = 0.0f;
-    l[mt] = 0.0f;
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int e = 0; e < EV; ++e) acc[mt][h][e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
   const uint16_t* kbase = a.k + kvh * a.c.head_stride;
   const uint16_t* vbase = a.v + kvh * a.c.head_stride;
-
-  for (int k0 = begin + 32 * wave; k0 < end; k0 += 128) {
-    // lane l looks up key k0 + l % 32; keys outside the range or without a
-    // page read the pool's first row and are masked
+  // lane l asks for key k0 + l % 32; keys outside the range or without a page
+  // read the pool's first row and are masked.  A step's page ids are loaded two
+  // steps ahead, before the next step's keys, so that no wait for them is a
+  // wait for keys or values still on their way.
+  auto load_page = [&](int k0) {
     const int key = k0 + (lane & 31);
-    int64_t off = -1;
-    if (key >= lo && key < end) off = spk_paged::offset_in(a.c, table[spk_paged::divide(a.c.div, (uint32_t)key)], key);
-    const uint32_t valid = (uint32_t)__ballot(off >= 0);
+    return key >= lo && key < end ? table[spk_paged::divide(a.c.div, (uint32_t)key)] : -1;
+  };
+  int64_t off = 0;
+  uint32_t valid = 0;
+  auto look_up = [&](int k0, int page) {
+    off = spk_paged::offset_in(a.c, page, k0 + (lane & 31));
+    valid = (uint32_t)__ballot(off >= 0);
     if (off < 0) off = 0;
-    const bool full = valid == 0xffffffffu && k0 >= lo_all && k0 + 32 <= hi_all;
-    uint4 v[8][NH];
+  };
+  // lane l of a wave as the compiler cannot know it: the lanes asked for below
+  // are then formed where they are used, not held in registers throughout
+  auto here = [&]() {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  uint4 kf[2][DC], v[8][NH];
+  auto load_k = [&]() {
+    const int x = here();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint16_t* p = kbase + (__shfl(off, 16 * t + (x & 15)) + 8 * (x >> 4));
+#pragma unroll
+      for (int c = 0; c < DC; ++c) kf[t][c] = *reinterpret_cast<const uint4*>(p + 32 * c);
+    }
+  };
+  auto load_v = [&]() {
+    const int x = here();
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
-      const int64_t at = __shfl(off, 16 * (kk >> 2) + 4 * g + (kk & 3));
+      const uint16_t* p = vbase + (__shfl(off, 16 * (kk >> 2) + 4 * (x >> 4) + (kk & 3)) + EV * (x & 15));
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        const uint16_t* p = vbase + at + 16 * EV * h + EV * ln;
         if constexpr (EV == 8) {
-          v[kk][h] = *reinterpret_cast<const uint4*>(p);
+          v[kk][h] = load_once(p + 16 * EV * h);
         } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(p);
+          const uint2 w = *reinterpret_cast<const uint2*>(p + 16 * EV * h);
           v[kk][h] = make_uint4(w.x, w.y, 0, 0);
         }
       }
     }
-    floatx4 s[MT][2];
+  };
+
+  int k0 = begin + 32 * wave;
+  int page = -1;  // of the step after the one that is loaded
+  if (k0 < end) {
+    const int first = load_page(k0);
+    page = load_page(k0 + 128);
+    look_up(k0, first);
+    load_k();
+    load_v();
+  }
+  const int r = min(r0 + ln, rows - 1);  // this lane's row
+  uint4 q[DC];
+  int row_lo, row_hi;
+  {
+    const int i = r / a.group;
+    spk_paged::visible(sq, i, a.window, &row_lo, &row_hi);
+    const uint16_t* src = a.q + (sq.first + i) * a.qt + (kvh * a.group + r - i * a.group) * a.qh + 8 * g;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t* p = kbase + __shfl(off, 16 * t + ln) + 8 * g;
-      uint4 kf[DC];
+    for (int c = 0; c < DC; ++c) {
+      if constexpr (!QL)
+        q[c] = *reinterpret_cast<const uint4*>(src + 32 * c);
+      else if (c % 4 == wave)
+        qs[c * 64 + lane] = *reinterpret_cast<const uint4*>(src + 32 * c);
+    }
+  }
+  if constexpr (QL) __syncthreads();
+  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  floatx4 acc[NH][EV];
 #pragma unroll
-      for (int c = 0; c < DC; ++c) kf[c] = *reinterpret_cast<const uint4*>(p + 32 * c);
+  for (int h = 0; h < NH; ++h)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        s[mt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int e = 0; e < EV; ++e) acc[h][e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (; k0 < end; k0 += 128) {
+    const bool full = valid == 0xffffffffu && k0 >= lo_all && k0 + 32 <= hi_all;
+    const uint32_t has = valid;
+    const bool more = k0 + 128 < end;
+    floatx4 s0 = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
-        for (int c = 0; c < DC; ++c) s[mt][t] = H::mfma16(kf[c], q[mt][c], s[mt][t]);
-      }
+    for (int c = 0; c < DC; ++c) {
+      const uint4 qf = QL ? qs[c * 64 + lane] : q[c];
+      s0 = H::mfma16(kf[0][c], qf, s0);
+      s1 = H::mfma16(kf[1][c], qf, s1);
+    }
+    if (more) {
+      look_up(k0 + 128, page);
+      page = load_page(k0 + 256);
+      load_k();
+    }
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = s0[i];
+      w[4 + i] = s1[i];
+    }
+    if (!full) {
+      const uint32_t see = seen(has, k0, row_lo, row_hi) >> (4 * g);  // a lane's keys at constant places
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = see >> (16 * (i >> 2) + (i & 3)) & 1u ? w[i] : -INFINITY;
+    }
+    float top = w[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, w[i]);
+    top *= a.scale_log2;
+    if (__any(top > m + kBehind)) {
+      top = fmaxf(top, spk::lane_xor16(top));
+      top = fmaxf(top, spk::lane_xor32(top));
+      const float now = fmaxf(m, top);
+      const float nb = now == -INFINITY ? 0.0f : now;
+      const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nb);
+      m = now;
+      base = nb;
+      l *= f;
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < EV; ++e) acc[h][e] *= f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = exp2_fast(__builtin_fmaf(w[i], a.scale_log2, H::kShift - base));
+      l += w[i];
+    }
+    uint4 p0, p1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = H::pack(w[2 * i], w[2 * i + 1]);
+      const float2_t x = H::unpack(u);
+      (&p0.x)[i] = u;
+      (&p1.x)[i] = H::pack(w[2 * i] - x.x, w[2 * i + 1] - x.y);
     }
     uint32_t odd_keys = 0;
     if (!full) {
@@ -393,18 +644,18 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
       uint32_t mine = 0;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        const bool has = (valid >> (16 * (kk >> 2) + 4 * g + (kk & 3))) & 1u;
+        const int kl = 16 * (kk >> 2) + 4 * g + (kk & 3);
         bool odd = false;
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
-          if (!has) v[kk][h] = make_uint4(0, 0, 0, 0);
+          if (!(has >> kl & 1u)) v[kk][h] = make_uint4(0, 0, 0, 0);
           odd = odd || H::odd(v[kk][h].x) || H::odd(v[kk][h].y) || H::odd(v[kk][h].z) || H::odd(v[kk][h].w);
         }
         const unsigned long long b = __ballot(odd);
 #pragma unroll
         for (int gg = 0; gg < 4; ++gg)
           if ((b >> (16 * gg)) & 0xffffull) odd_keys |= 1u << (16 * (kk >> 2) + 4 * gg + (kk & 3));
-        mine |= (odd_keys >> (16 * (kk >> 2) + 4 * g + (kk & 3)) & 1u) << kk;
+        mine |= (odd_keys >> kl & 1u) << kk;
       }
       if (odd_keys) {
 #pragma unroll
@@ -414,44 +665,6 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
             if (mine >> kk & 1u) v[kk][h] = make_uint4(0, 0, 0, 0);
       }
     }
-    uint4 p[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = s[mt][i >> 2][i & 3];
-        if (!full) {
-          const int kl = 16 * (i >> 2) + 4 * g + (i & 3);
-          const bool see = (valid >> kl & 1u) && k0 + kl >= row_lo[mt] && k0 + kl < row_hi[mt];
-          x[i] = see ? x[i] : -INFINITY;
-        }
-      }
-      float top = x[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-      top *= a.scale_log2;
-      if (__any(top > m[mt] + kBehind)) {
-        top = fmaxf(top, spk::lane_xor16(top));
-        top = fmaxf(top, spk::lane_xor32(top));
-        const float now = fmaxf(m[mt], top);
-        const float nb = now == -INFINITY ? 0.0f : now;
-        const float f = m[mt] == -INFINITY ? 0.0f : exp2_fast(m[mt] - nb);
-        m[mt] = now;
-        base[mt] = nb;
-        l[mt] = l[mt] * f;
-#pragma unroll
-        for (int h = 0; h < NH; ++h)
-#pragma unroll
-          for (int e = 0; e < EV; ++e) acc[mt][h][e] *= f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = exp2_fast(__builtin_fmaf(x[i], a.scale_log2, H::kShift - base[mt]));
-        l[mt] += x[i];
-      }
-      p[mt] = make_uint4(H::pack(x[0], x[1]), H::pack(x[2], x[3]), H::pack(x[4], x[5]), H::pack(x[6], x[7]));
-    }
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -459,100 +672,414 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(Attn a) {
         // element e of the 8 keys' pieces
         uint4 f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-          (&f.x)[w] = __builtin_amdgcn_perm((&v[2 * w + 1][h].x)[e >> 1], (&v[2 * w][h].x)[e >> 1],
+        for (int i = 0; i < 4; ++i)
+          (&f.x)[i] = __builtin_amdgcn_perm((&v[2 * i + 1][h].x)[e >> 1], (&v[2 * i][h].x)[e >> 1],
                                             e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt][h][e] = H::mfma16(f, p[mt], acc[mt][h][e]);
+        acc[h][e] = H::mfma16(f, p0, acc[h][e]);
+        acc[h][e] = H::mfma16(f, p1, acc[h][e]);
       }
+    if (more) load_v();
     while (odd_keys) {
       const int kl = __ffs(odd_keys) - 1;
       odd_keys &= odd_keys - 1;
-      const uint16_t* vr = vbase + __shfl(off, kl);
+      const uint16_t* vr = vbase + max(spk_paged::offset_of(a.c, seq, k0 + kl), (int64_t)0);
+      float weight = 0.0f;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        uint32_t pair = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (w == 2 * (kl >> 4) + ((kl & 3) >> 1)) pair = (&p[mt].x)[w];
+      for (int part = 0; part < 2; ++part) {
+        const uint4 quad = part ? p1 : p0;
+        uint32_t pair = kl & 16 ? (kl & 2 ? quad.w : quad.z) : (kl & 2 ? quad.y : quad.x);
         pair = __shfl((int)pair, ln + 16 * ((kl >> 2) & 3));
-        const float weight = H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
-        if (k0 + kl >= row_lo[mt] && k0 + kl < row_hi[mt]) {
+        weight += H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
+      }
+      if (k0 + kl >= row_lo && k0 + kl < row_hi) {
 #pragma unroll
-          for (int h = 0; h < NH; ++h)
+        for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int e = 0; e < EV; ++e)
+          for (int e = 0; e < EV; ++e)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                acc[mt][h][e][i] += weight * H::widen(vr[16 * EV * h + EV * (4 * g + i) + e]);
-        }
+            for (int i = 0; i < 4; ++i) {
+              acc[h][e][i] += weight * H::widen(vr[16 * EV * h + EV * (4 * g + i) + e]);
+              __builtin_amdgcn_sched_barrier(0);  // one at a time: this path takes no registers from the others
+            }
       }
     }
   }
 
-  // join the waves, one 16-row tile at a time
+  // join the waves
+  l += spk::lane_xor16(l);
+  l += spk::lane_xor32(l);
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    l[mt] += spk::lane_xor16(l[mt]);
-    l[mt] += spk::lane_xor32(l[mt]);
-    if (mt) __syncthreads();
+  for (int h = 0; h < NH; ++h)
 #pragma unroll
-    for (int h = 0; h < NH; ++h)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int e = 0; e < EV; e += 4)
+        *reinterpret_cast<float4*>(&joint[wave][ln][16 * EV * h + EV * (4 * g + i) + e]) =
+            make_float4(acc[h][e][i], acc[h][e + 1][i], acc[h][e + 2][i], acc[h][e + 3][i]);
+  if (g == 0) {
+    stat[wave][ln][0] = m;
+    stat[wave][ln][1] = l;
+  }
+  __syncthreads();
+  const int row = threadIdx.x >> 4, rj = r0 + row;
+  if (rj >= rows) return;
+  float top = -INFINITY, sum = 0.0f, f[4];
 #pragma unroll
-        for (int e = 0; e < EV; e += 4)
-          *reinterpret_cast<float4*>(&joint[wave][ln][16 * EV * h + EV * (4 * g + i) + e]) =
-              make_float4(acc[mt][h][e][i], acc[mt][h][e + 1][i], acc[mt][h][e + 2][i], acc[mt][h][e + 3][i]);
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][row][0]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = top == -INFINITY ? 1.0f : exp2_fast(stat[w][row][0] - top);
+    sum += f[w] * stat[w][row][1];
+  }
+  const int i = rj / a.group, token = sq.first + i, head = kvh * a.group + rj - i * a.group;
+  const int64_t at = (int64_t)token * a.heads + head;
+  float* part = a.shared + ((int64_t)blockIdx.x * 16 + row) * (D + 2);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    const int d = 64 * c + 4 * (threadIdx.x & 15);
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(&joint[w][row][d]);
+      o[0] += f[w] * x.x;
+      o[1] += f[w] * x.y;
+      o[2] += f[w] * x.z;
+      o[3] += f[w] * x.w;
+    }
+    if (sh.ranges == 1) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) o[n] *= inv;
+      store_out<BF, 4>(a, token, head, d, o);
+    } else {
+      *reinterpret_cast<float2*>(part + 2 + d) = make_float2(o[0], o[1]);
+      *reinterpret_cast<float2*>(part + 4 + d) = make_float2(o[2], o[3]);
+    }
+  }
+  if ((threadIdx.x & 15) == 0) {
+    if (sh.ranges > 1) {
+      part[0] = top;
+      part[1] = sum;
+    } else if (a.lse) {
+      a.lse[at] = sum == 0.0f ? -INFINITY : (top - H::kShift + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+  }
+}
+
+// A middle number of rows per sequence and KV head (17 .. 64: a few drafted
+// tokens): too many for the registers of one wave beside the keys on their
+// way, too few to be bound by anything but memory.  A workgroup takes 64 rows,
+// 16 to each of its 4 waves, and all waves read every step of 32 keys from
+// LDS, which holds four steps: loads go straight into LDS, three steps ahead.
+// The waves have their own rows, so nothing is joined.
+//
+// The arithmetic is paged_rows_kernel's.  Rows lie in LDS as in memory, one
+// load's 1 KiB (rows x, x + RS, ...) apart by 16 bytes more for the keys, whose
+// rows 0..7 are read side by side, and by 32 for the values, which are read
+// by the transposing load: 16 lanes take 4 keys' pieces of 16 dimensions and
+// get 4 keys of a dimension each.
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
+  using H = Half<BF>;
+  constexpr int DC = D / 32;      // contraction steps of the scores
+  constexpr int DT = D / 16;      // output tiles
+  constexpr int CH = D / 8;       // 16-byte pieces of a row
+  constexpr int RPW = 64 / CH;    // rows of one load
+  constexpr int RS = 32 / RPW;    // loads of 32 keys, and the distance of a load's rows
+  constexpr int LW = RS / 4;      // loads of a wave
+  // four steps, as separate arrays: a load into one is then known not to touch the others
+  __shared__ __align__(16) uint4 ka[RS * 65], kb[RS * 65], kc[RS * 65], kd[RS * 65];
+  __shared__ __align__(16) uint4 va[RS * 66], vb[RS * 66], vc[RS * 66], vd[RS * 66];
+  __shared__ __align__(16) uint32_t there[4][4];  // per step and wave: its rows' keys that exist
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 15, g = lane >> 4;
+  Share sh;
+  if (!find_share(a, blockIdx.x, -1, 0, 0, lane, &sh)) return;
+  const int seq = sh.seq, kvh = sh.kvh;
+  const Seq sq = spk_paged::seq_at(a.c, seq);
+  const int rows = sq.n * a.group;
+  const int r0 = sh.tile * 64;
+  int lo, hi, lo_all, hi_all, x;
+  spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
+  spk_paged::visible(sq, (min(r0 + 64, rows) - 1) / a.group, a.window, &x, &hi);
+  const int begin = (int)min((int64_t)sh.lo + (int64_t)sh.range * sh.keys, (int64_t)hi);
+  const int end = begin + min(sh.keys, hi - begin);
+
+  // the row of this lane; the keys that all rows of the wave see
+  const int r = min(r0 + 16 * wave + ln, rows - 1);
+  const int ri = r / a.group, token = sq.first + ri, head = kvh * a.group + r - ri * a.group;
+  int row_lo, row_hi;
+  spk_paged::visible(sq, ri, a.window, &row_lo, &row_hi);
+  spk_paged::visible(sq, min(r0 + 16 * wave, rows - 1) / a.group, a.window, &x, &hi_all);
+  spk_paged::visible(sq, min(r0 + 16 * wave + 15, rows - 1) / a.group, a.window, &lo_all, &x);
+  const bool idle = r0 + 16 * wave >= rows;
+  uint4 q[DC];
+  {
+    const uint16_t* src = a.q + token * a.qt + head * a.qh + 8 * g;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) q[c] = *reinterpret_cast<const uint4*>(src + 32 * c);
+  }
+  // the keys of a wave's loads are the wave's: their page ids are scalar loads,
+  // and the vector memory counter counts the keys and values alone
+  typedef const __attribute__((address_space(4))) int32_t* Table;
+  const Table table = (Table)(a.c.table + (int64_t)seq * a.c.table_stride);
+  const uint16_t* kbase = a.k + kvh * a.c.head_stride + 8 * (lane % CH);
+  const uint16_t* vbase = a.v + kvh * a.c.head_stride + 8 * (lane % CH);
+  // A wave's loads hold RPW groups of LW consecutive keys; where the page size is
+  // a multiple of LW (and a step begins at one of 32), a group has one page.
+  const bool grouped = a.c.page_size % LW == 0;
+  int page[RPW][LW];  // of the step that is loaded next
+  auto look_up = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < RPW; ++j) {
+      const int key = k0 + wave * LW + RS * j;
+      if (grouped) {
+        page[j][0] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(key, lo), end - 1))];
+#pragma unroll
+        for (int i = 1; i < LW; ++i) page[j][i] = page[j][0];
+      } else {
+#pragma unroll
+        for (int i = 0; i < LW; ++i)
+          page[j][i] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(key + i, lo), end - 1))];
+      }
+    }
+  };
+  auto load = [&](int k0, uint4* ks, uint4* vs, int stage) __attribute__((always_inline)) {
+    uint32_t mine = 0;
+    int64_t at[LW];
+#pragma unroll
+    for (int i = 0; i < LW; ++i) at[i] = 0;  // a key without a place reads the pool's first row and is masked
+#pragma unroll
+    for (int j = 0; j < RPW; ++j) {
+      const int first = wave * LW + RS * j;
+      const bool here = lane / CH == j;
+      if (grouped && k0 + first >= lo && k0 + first + LW <= end) {
+        const int64_t o = spk_paged::offset_in(a.c, page[j][0], k0 + first);
+        if (o >= 0) {
+          mine |= ((1u << LW) - 1) << first;
+#pragma unroll
+          for (int i = 0; i < LW; ++i) at[i] = here ? o + i * a.c.token_stride : at[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+          const int key = k0 + first + i;
+          const int64_t o = key >= lo && key < end ? spk_paged::offset_in(a.c, page[j][i], key) : -1;
+          mine |= o >= 0 ? 1u << (first + i) : 0u;
+          at[i] = here && o >= 0 ? o : at[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < LW; ++i) {
+      const int first = wave * LW + i;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kbase + at[i]),
+                                       (__attribute__((address_space(3))) void*)&ks[first * 65], 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vbase + at[i]),
+                                       (__attribute__((address_space(3))) void*)&vs[first * 66], 16, 0, 0);
+    }
+    if (lane == 0) there[stage][wave] = mine;
+    look_up(k0 + 32);
+  };
+  floatx4 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  constexpr int K16 = CH * 16 / RS;                       // 16 rows on, in 16-byte pieces
+  const int kread = (ln % RS) * 65 + (ln / RS) * CH + g;  // + 4 c
+  const int vrow = 4 * g + (ln >> 2);                     // of the transposing load
+  const int vread = (vrow % RS) * 132 + (vrow / RS) * 2 * CH + (ln & 3);  // in 8-byte pieces, + 4 t
+
+  auto step = [&](int k0, const uint4* ks, const uint4* vs, int stage, uint4* ks_next, uint4* vs_next)
+                  __attribute__((always_inline)) {
+    // this step's loads are older than those of the two steps after it; with
+    // the barrier every wave's have arrived, and every wave has done with the
+    // step before, whose place the next loads take
+    if constexpr (LW == 4)
+      asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
+    else if constexpr (LW == 2)
+      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load(k0 + 96, ks_next, vs_next, (stage + 3) & 3);
+    if (idle) return;
+    const uint4 four = *reinterpret_cast<const uint4*>(&there[stage][0]);
+    const uint32_t has = __builtin_amdgcn_readfirstlane(four.x | four.y | four.z | four.w);
+    const bool full = has == 0xffffffffu && k0 >= lo_all && k0 + 32 <= min(hi_all, end);
+    floatx4 s0 = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+    uint4 kf[2][DC];
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      kf[0][c] = ks[kread + 4 * c];
+      kf[1][c] = ks[kread + K16 + 4 * c];
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all reads under way before the first product waits for one
+#pragma unroll
+    for (int c = 0; c < DC; ++c) {
+      s0 = H::mfma16(kf[0][c], q[c], s0);
+      s1 = H::mfma16(kf[1][c], q[c], s1);
+    }
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = s0[i];
+      w[4 + i] = s1[i];
+    }
+    if (!full) {
+      const uint32_t see = seen(has, k0, row_lo, row_hi) >> (4 * g);  // a lane's keys at constant places
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = see >> (16 * (i >> 2) + (i & 3)) & 1u ? w[i] : -INFINITY;
+    }
+    float top = w[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, w[i]);
+    top *= a.scale_log2;
+    if (__any(top > m + kBehind)) {
+      top = fmaxf(top, spk::lane_xor16(top));
+      top = fmaxf(top, spk::lane_xor32(top));
+      const float now = fmaxf(m, top);
+      const float nb = now == -INFINITY ? 0.0f : now;
+      const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nb);
+      m = now;
+      base = nb;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc[t] *= f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = exp2_fast(__builtin_fmaf(w[i], a.scale_log2, H::kShift - base));
+      l += w[i];
+    }
+    uint4 p0, p1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = H::pack(w[2 * i], w[2 * i + 1]);
+      const float2_t v = H::unpack(u);
+      (&p0.x)[i] = u;
+      (&p1.x)[i] = H::pack(w[2 * i] - v.x, w[2 * i + 1] - v.y);
+    }
+    auto values = [&](int t) {  // 8 keys of dimension 16 t + ln
+      const auto* at = reinterpret_cast<const uint2*>(vs) + vread + 4 * t;
+      const uint2 u = transposed(at), v = transposed(at + 2 * K16);
+      return make_uint4(u.x, u.y, v.x, v.y);
+    };
+    if (full) {
+      constexpr int A = 4;  // tiles whose values are read ahead
+      uint4 f[A];
+#pragma unroll
+      for (int t = 0; t < A; ++t) f[t] = values(t);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const uint4 u = f[t % A];
+        if (t + A < DT) f[t % A] = values(t + A);
+        __builtin_amdgcn_sched_barrier(0);
+        acc[t] = H::mfma16(u, p0, acc[t]);
+        acc[t] = H::mfma16(u, p1, acc[t]);
+      }
+      return;
+    }
+    // as in paged_rows_kernel: no value that is not finite meets a zero weight
+    const uint32_t mine = has >> (4 * g);
+    uint32_t keep[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t two = mine >> (16 * (i >> 1) + 2 * (i & 1));
+      keep[i] = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+    }
+    uint32_t odd = 0;  // bit i: of this lane's keys 2 i and 2 i + 1
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      uint4 f = values(t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = (&f.x)[i] & keep[i];
+        if (H::odd(u)) odd |= 1u << i;
+        (&f.x)[i] = H::finite(u);
+      }
+      acc[t] = H::mfma16(f, p0, acc[t]);
+      acc[t] = H::mfma16(f, p1, acc[t]);
+    }
+    uint32_t odd_keys = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned long long b = __ballot(odd >> i & 1u);
+#pragma unroll
+      for (int gg = 0; gg < 4; ++gg)
+        if ((b >> (16 * gg)) & 0xffffull) odd_keys |= 3u << (16 * (i >> 1) + 4 * gg + 2 * (i & 1));
+    }
+    while (odd_keys) {
+      const int kl = __ffs(odd_keys) - 1;
+      odd_keys &= odd_keys - 1;
+      if (!(has >> kl & 1u)) continue;
+      const uint16_t* row = a.v + kvh * a.c.head_stride + spk_paged::offset_of(a.c, seq, k0 + kl);
+      float weight = 0.0f;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const uint4 quad = part ? p1 : p0;
+        uint32_t pair = kl & 16 ? (kl & 2 ? quad.w : quad.z) : (kl & 2 ? quad.y : quad.x);
+        pair = __shfl((int)pair, ln + 16 * ((kl >> 2) & 3));
+        weight += H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
+      }
+      if (k0 + kl >= row_lo && k0 + kl < row_hi) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint16_t u = row[16 * t + 4 * g + i];
+            if (H::odd(u)) acc[t][i] += weight * H::widen(u);
+            __builtin_amdgcn_sched_barrier(0);  // one at a time: this path takes no registers from the others
+          }
+      }
+    }
+  };
+  if (begin < end) {
+    look_up(begin);
+    load(begin, ka, va, 0);
+    load(begin + 32, kb, vb, 1);
+    load(begin + 64, kc, vc, 2);
+    // the queries have arrived: from here on only loads into LDS are under way,
+    // and a wait for one step's need not be a wait for all
+#pragma unroll
+    for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(q[c].x), "+v"(q[c].y), "+v"(q[c].z), "+v"(q[c].w));
+    for (int k0 = begin;;) {
+      step(k0, ka, va, 0, kd, vd);
+      if ((k0 += 32) >= end) break;
+      step(k0, kb, vb, 1, ka, va);
+      if ((k0 += 32) >= end) break;
+      step(k0, kc, vc, 2, kb, vb);
+      if ((k0 += 32) >= end) break;
+      step(k0, kd, vd, 3, kc, vc);
+      if ((k0 += 32) >= end) break;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
+  }
+
+  l += spk::lane_xor16(l);
+  l += spk::lane_xor32(l);
+  if (r0 + 16 * wave + ln >= rows) return;
+  const int64_t at = (int64_t)token * a.heads + head;
+  if (sh.ranges > 1) {
+    float* part = a.shared + ((int64_t)blockIdx.x * 64 + 16 * wave + ln) * (D + 2);
     if (g == 0) {
-      stat[wave][ln][0] = m[mt];
-      stat[wave][ln][1] = l[mt];
+      part[0] = m;
+      part[1] = l;
     }
-    __syncthreads();
-    const int row = threadIdx.x >> 4, r = r0 + 16 * mt + row;
-    if (r < rows) {
-      float top = -INFINITY, sum = 0.0f, f[4];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][row][0]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        f[w] = top == -INFINITY ? 1.0f : exp2_fast(stat[w][row][0] - top);
-        sum += f[w] * stat[w][row][1];
-      }
-      const int i = r / a.group, token = sq.first + i, head = kvh * a.group + r - i * a.group;
-      const int64_t at = (int64_t)token * a.heads + head;
-      float* part = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const int d = 64 * c + 4 * (threadIdx.x & 15);
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(&joint[w][row][d]);
-          o[0] += f[w] * x.x;
-          o[1] += f[w] * x.y;
-          o[2] += f[w] * x.z;
-          o[3] += f[w] * x.w;
-        }
-        if (a.splits[0] == 1) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) o[n] *= inv;
-          store_out<BF, 4>(a, token, head, d, o);
-        } else {
-          *reinterpret_cast<float2*>(part + 2 + d) = make_float2(o[0], o[1]);
-          *reinterpret_cast<float2*>(part + 4 + d) = make_float2(o[2], o[3]);
-        }
-      }
-      if ((threadIdx.x & 15) == 0) {
-        if (a.splits[0] > 1) {
-          part[0] = top;
-          part[1] = sum;
-        } else if (a.lse) {
-          a.lse[at] = sum == 0.0f ? -INFINITY : (top - H::kShift + __builtin_amdgcn_logf(sum)) * kLn2;
-        }
-      }
+    for (int t = 0; t < DT; ++t) {
+      *reinterpret_cast<float2*>(part + 2 + 16 * t + 4 * g) = make_float2(acc[t][0], acc[t][1]);
+      *reinterpret_cast<float2*>(part + 4 + 16 * t + 4 * g) = make_float2(acc[t][2], acc[t][3]);
     }
+    return;
+  }
+  if (a.lse && g == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m - H::kShift + __builtin_amdgcn_logf(l)) * kLn2;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int t = 0; t < DT; ++t) {
+    const float o[4] = {acc[t][0] * inv, acc[t][1] * inv, acc[t][2] * inv, acc[t][3] * inv};
+    store_out<BF, 4>(a, token, head, 16 * t + 4 * g, o);
   }
 }
 
@@ -592,7 +1119,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   const int ln = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.y, split = blockIdx.x;
   int seq, tile;
-  if (!find_tile(a, 1, 256, blockIdx.z, lane, &seq, &tile)) return;
+  if (!find_tile(a, 256, blockIdx.z, lane, &seq, &tile)) return;
   seq = __builtin_amdgcn_readfirstlane(seq);
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Seq sq = spk_paged::seq_at(a.c, seq);
@@ -601,10 +1128,10 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   int lo, hi, lo_all, hi_all;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
   spk_paged::visible(sq, (r1 - 1) / a.group, a.window, &lo_all, &hi);
-  const int keys = range_keys(a, 1, lo, hi);
+  const int keys = range_keys(a, lo, hi);
   const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
   const int end = begin + min(keys, hi - begin);
-  if (begin >= end && a.splits[1] > 1) return;
+  if (begin >= end && a.splits > 1) return;
 
   const int r = min(r0 + 32 * wave + ln, rows - 1);
   const int ri = r / a.group, head = kvh * a.group + r - ri * a.group, token = sq.first + ri;
@@ -752,10 +1279,8 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
 #pragma unroll
       for (int c = 0; c < KS; ++c) s = H::mfma32(ks[j * RS * 65 + kread + 2 * c], c < QR ? q[c] : qs[(c - QR) * 512 + tid], s);
       if (!full) {
-        // bit n: this row sees key n of the 32; shifted so that a lane's keys are at constant places
-        const int first = min(max(row_lo - kj, 0), 31), last = min(max(row_hi - kj, 0), 32);
-        uint32_t see = row_lo - kj > 31 || last == 0 ? 0u : has & (0xffffffffu << first) & (0xffffffffu >> (32 - last));
-        see >>= 4 * h;
+        uint32_t see = seen(has, kj, row_lo, row_hi);
+        see >>= 4 * h;  // a lane's keys at constant places
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[i] : -INFINITY;
       }
@@ -836,7 +1361,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   l += spk::lane_xor32(l);
   if (r0 + 32 * wave + ln >= rows) return;
   const int64_t at = (int64_t)token * a.heads + head;
-  if (a.splits[1] > 1) {
+  if (a.splits > 1) {
     float* part = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
     if (h == 0) {
       part[0] = m;
@@ -867,12 +1392,30 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   }
 }
 
-// Joins the key ranges of a row: one wave per (token, head).
-template <int D, bool BF>
+// Joins the key ranges of a row: 256 / LANES rows to a workgroup, for many rows
+// of few ranges 64 lanes to each, for few rows of many ranges all 256.  The
+// ranges' maxima and sums are read by the lanes side by side; D / 4 lanes add
+// a range's output, the other lanes take other ranges, and LDS joins them.
+template <int D, int LANES, bool BF>
 __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
-  constexpr int N = D / 64 >= 2 ? D / 64 : 1;
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int L = D / 4 < LANES ? D / 4 : LANES, W = LANES / L;  // lanes of a range, ranges at a time
+  constexpr int ROWS = 256 / LANES;
+  __shared__ float weights[ROWS][LANES];
+  __shared__ float reds[ROWS][4];
+  __shared__ float4 all[ROWS][W][L];
+  const int lane = threadIdx.x & 63, tid = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  float* weight = weights[mine];
+  float* red = reds[mine];
+  auto together = [&]() {  // a row of 64 lanes is one wave
+    if constexpr (LANES == 256) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  };
+  const int64_t at = (int64_t)blockIdx.x * ROWS + mine;
   const int token = (int)(at / a.heads), head = (int)(at - (int64_t)token * a.heads);
   if (token >= a.c.total_tokens) return;
   const int s = spk_paged::seq_of_token(a.c.cu, a.c.num_seqs, token, lane);
@@ -880,40 +1423,97 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
   const Seq sq = spk_paged::seq_at(a.c, s);
   if (token < sq.first || token >= sq.first + sq.n) return;
   // the ranges that the row's tile had
-  const int rows = sq.n * a.group, r = (token - sq.first) * a.group + head % a.group;
-  const int kind = rows >= a.many, tile_rows = a.tile_rows[kind];
-  if (a.splits[kind] == 1) return;
-  const int r0 = r / tile_rows * tile_rows;
-  int lo, hi, x;
-  spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
-  spk_paged::visible(sq, (min(r0 + tile_rows, rows) - 1) / a.group, a.window, &x, &hi);
-  const int span = hi - (lo & ~31);
-  const int keys = range_keys(a, kind, lo, hi);
-  const int n = span <= 0 ? 0 : (int)(((int64_t)span + keys - 1) / keys);
-  const int64_t step = (int64_t)a.c.total_tokens * a.heads * (D + 2);
-  const float* part = a.part + at * (D + 2);
-  float top = -INFINITY, sum = 0.0f, o[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.0f;
-  for (int j = 0; j < n; ++j) top = fmaxf(top, part[j * step]);
-  for (int j = 0; j < n; ++j) {
-    const float f = top == -INFINITY ? 1.0f : exp2_fast(part[j * step] - top);
-    sum += f * part[j * step + 1];
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] += f * part[j * step + 2 + N * lane + i];
+  const int rows = sq.n * a.group, kvh = head / a.group, r = (token - sq.first) * a.group + head - kvh * a.group;
+  int n;
+  int64_t step;
+  const float* part;
+  if (rows < a.many) {
+    Share sh;
+    if (!find_share(a, 0, s, r / a.share_rows, kvh, lane, &sh) || sh.ranges == 1) return;
+    n = sh.ranges;
+    step = (int64_t)a.share_rows * (D + 2);
+    part = a.shared + sh.first * step + r % a.share_rows * (D + 2);
+  } else {
+    if (a.splits == 1) return;
+    const int r0 = r & ~255;
+    int lo, hi, x;
+    spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
+    spk_paged::visible(sq, (min(r0 + 256, rows) - 1) / a.group, a.window, &x, &hi);
+    const int span = hi - (lo & ~31), keys = range_keys(a, lo, hi);
+    n = span <= 0 ? 0 : (int)(((int64_t)span + keys - 1) / keys);
+    step = (int64_t)a.c.total_tokens * a.heads * (D + 2);
+    part = a.part + at * (D + 2);
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* out = a.out + token * a.ot + head * a.oh + N * lane;
+
+  float top = -INFINITY;
+  for (int j = tid; j < n; j += LANES) top = fmaxf(top, part[j * step]);
+  top = spk::wave_max(top);
+  if constexpr (LANES == 256) {
+    if (lane == 0) red[tid >> 6] = top;
+    together();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+  constexpr int E = D / (4 * L);  // groups of four elements of a lane
+  float sum = 0.0f;
+  float4 o[E];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float y = o[i] * inv;
-    if (a.gate) {
-      const float v = Half<BF>::widen(a.gate[token * a.gt + head * a.gh + N * lane + i]);
-      y = y / (1.0f + exp2_fast(v * -1.44269504f));
+  for (int e = 0; e < E; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int j0 = 0; j0 < n; j0 += LANES) {
+    together();
+    if (j0 + tid < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(part + (j0 + tid) * step);
+      const float f = top == -INFINITY ? 1.0f : exp2_fast(ml.x - top);
+      weight[tid] = f;
+      sum += f * ml.y;
     }
-    out[i] = Half<BF>::one(y);
+    together();
+    const int m = min(LANES, n - j0);
+#pragma unroll 4
+    for (int j = tid / L; j < m; j += W) {
+      const float f = weight[j];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float* p = part + (j0 + j) * step + 2 + 4 * (tid % L + L * e);
+        const float2 u = *reinterpret_cast<const float2*>(p), v = *reinterpret_cast<const float2*>(p + 2);
+        o[e].x += f * u.x;
+        o[e].y += f * u.y;
+        o[e].z += f * v.x;
+        o[e].w += f * v.y;
+      }
+    }
   }
-  if (lane == 0 && a.lse)
+  sum = wave_sum(sum);
+  if constexpr (LANES == 256) {
+    together();
+    if (lane == 0) red[tid >> 6] = sum;
+  }
+  if constexpr (W > 1) {
+    all[mine][tid / L][tid % L] = o[0];
+    together();
+    if (tid < L) {
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        const float4 u = all[mine][w][tid];
+        o[0].x += u.x;
+        o[0].y += u.y;
+        o[0].z += u.z;
+        o[0].w += u.w;
+      }
+    }
+  }
+  if constexpr (LANES == 256) {
+    if constexpr (W == 1) together();
+    sum = (red[0] + red[1]) + (red[2] + red[3]);
+  }
+  if (tid < L) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float y[4] = {o[e].x * inv, o[e].y * inv, o[e].z * inv, o[e].w * inv};
+      store_out<BF, 4>(a, token, head, 4 * (tid + L * e), y);
+    }
+  }
+  if (tid == 0 && a.lse)
     a.lse[at] = sum == 0.0f ? -INFINITY : (top - Half<BF>::kShift + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
@@ -935,7 +1535,7 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
       p.total_tokens < 0)
     return spk::fail(SPK_ERR_SHAPE, "%s: kv_heads %d page_size %d num_pages %d max_pages %d num_seqs %d total_tokens %d",
                      who, p.num_kv_heads, p.page_size, p.num_pages, p.max_pages, p.num_seqs, p.total_tokens);
-  if ((int64_t)p.max_pages * p.page_size > INT32_MAX - 64)
+  if ((int64_t)p.max_pages * p.page_size > INT32_MAX - 4096)
     return spk::fail(SPK_ERR_SHAPE, "%s: max_pages %d of %d tokens pass 2^31 positions", who, p.max_pages, p.page_size);
   if (p.num_seqs && p.total_tokens) {
     if (!p.k_cache || !p.v_cache || !p.block_table || !p.cu_seqlens || !p.context_lens)
@@ -963,10 +1563,10 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
   return SPK_OK;
 }
 
-// How a call's rows and keys are dealt to the two kernels.
+// How a call's rows and keys are dealt to the kernels.
 struct Plan {
-  int mt, one_tile, many;
-  int tiles[2], splits[2], chunk[2], tile_rows[2];
+  int many, shares, share_rows, tiles, splits, chunk;
+  bool join;
 };
 
 Plan plan_of(const SpkPagedAttnArgs& p) {
@@ -975,30 +1575,33 @@ Plan plan_of(const SpkPagedAttnArgs& p) {
   const int64_t tokens = std::min(p.max_query_len, c.total_tokens);
   const int64_t longest = tokens * group, all = (int64_t)c.total_tokens * group;
   Plan r;
-  r.many = 65;
-  const bool any_many = longest >= r.many;
-  const int64_t few = std::min<int64_t>(longest, r.many - 1);
-  r.mt = few <= 16 ? 1 : 2;
-  r.tile_rows[0] = 16 * r.mt;
-  r.tile_rows[1] = 256;
-  r.one_tile = !any_many && few <= r.tile_rows[0];
-  // sequences of few rows: all of them, unless the longest takes every row
-  r.tiles[0] = r.one_tile ? c.num_seqs
-               : any_many && c.num_seqs == 1
-                   ? 0
-                   : (int)std::min<int64_t>(all / r.tile_rows[0] + c.num_seqs, INT32_MAX);
-  r.tiles[1] = any_many ? (int)std::min<int64_t>(all / 256 + std::min<int64_t>(c.num_seqs, all / r.many), INT32_MAX) : 0;
+  // a call of one sequence that may have many rows goes to their kernel
+  // whatever it has; one that has none to the others
+  const bool any_many = longest > 64;
+  r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : 65;
+  const int64_t few = std::min<int64_t>(longest, 64);
+  r.share_rows = few <= 16 ? 16 : 64;
   int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
   if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
-  for (int kind = 0; kind < 2; ++kind) {
-    const int64_t groups = (int64_t)r.tiles[kind] * c.num_kv_heads;
-    const int64_t want = std::max<int64_t>(1, (kind ? 256 : 1024) / std::max<int64_t>(groups, 1));
-    const int64_t least = kind ? 4 : 1;  // steps of 128 keys
-    const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);
-    const int64_t per = std::max(least, (steps + want - 1) / want);
-    r.chunk[kind] = (int)(128 * per);
-    r.splits[kind] = r.tiles[kind] ? (int)((steps + per - 1) / per) : 1;
-  }
+  const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
+
+  // sequences of few rows: all of them, unless the one there is has many.  As
+  // many workgroups as the chip holds at once (2 to a CU; 4 with heads of 64,
+  // 1 where 64 rows' keys of 256 dimensions fill the LDS), more only where the
+  // pieces alone are more, and no more than ranges of 128 keys.
+  const int64_t pieces = any_many && c.num_seqs == 1 ? 0 : (all / r.share_rows + c.num_seqs) * c.num_kv_heads;
+  const int64_t slots = c.head_dim == 64 ? 1024 : c.head_dim == 256 && r.share_rows == 64 ? 256 : 512;
+  r.shares = (int)std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)),
+                                    INT32_MAX);
+
+  // sequences of many rows: a workgroup to a CU, ranges of at least 512 keys
+  r.tiles = any_many ? (int)std::min<int64_t>(all / 256 + std::min<int64_t>(c.num_seqs, all / 65 + 1), INT32_MAX) : 0;
+  const int64_t groups = std::max<int64_t>(1, (int64_t)r.tiles * c.num_kv_heads);
+  const int64_t ranges = std::max<int64_t>(1, 256 / groups);
+  const int64_t per = std::max<int64_t>(4, (steps + ranges - 1) / ranges);
+  r.chunk = (int)(128 * per);
+  r.splits = r.tiles ? (int)((steps + per - 1) / per) : 1;
+  r.join = r.splits > 1 || (r.shares && steps > 1);
   return r;
 }
 
@@ -1018,26 +1621,32 @@ int check_attn(const SpkPagedAttnArgs* p, Cache* c) {
   return SPK_OK;
 }
 
-size_t workspace_of(const SpkPagedAttnArgs& p) {
-  const Plan r = plan_of(p);
-  const int splits = std::max(r.splits[0], r.splits[1]);
-  if (splits <= 1) return 0;
-  return (size_t)splits * p.cache.total_tokens * p.num_q_heads * (p.cache.head_dim + 2) * sizeof(float);
+size_t shared_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
+  const size_t n = (size_t)r.shares * r.share_rows * (p.cache.head_dim + 2) * sizeof(float);
+  return r.join ? (n + 255) & ~(size_t)255 : 0;
+}
+
+size_t workspace_of(const SpkPagedAttnArgs& p, const Plan& r) {
+  const size_t part = r.splits <= 1 ? 0
+                                    : (size_t)r.splits * p.cache.total_tokens * p.num_q_heads *
+                                          (p.cache.head_dim + 2) * sizeof(float);
+  return shared_bytes(p, r) + part;
 }
 
 template <int D, bool BF>
 void launch_attn(const Attn& a, const Plan& r, hipStream_t s) {
-  const dim3 grid(r.splits[0], a.kv_heads, r.tiles[0]);
-  if (r.tiles[0] && r.mt == 1)
-    hipLaunchKernelGGL((paged_rows_kernel<D, 1, BF>), grid, dim3(256), 0, s, a);
-  else if (r.tiles[0])
-    hipLaunchKernelGGL((paged_rows_kernel<D, 2, BF>), grid, dim3(256), 0, s, a);
-  if (r.tiles[1])
-    hipLaunchKernelGGL((paged_tiles_kernel<D, BF>), dim3(r.splits[1], a.kv_heads, r.tiles[1]), dim3(512), 0, s, a);
-  if (r.splits[0] > 1 || r.splits[1] > 1) {
-    const int64_t rows = (int64_t)a.c.total_tokens * a.heads;
-    hipLaunchKernelGGL((paged_join_kernel<D, BF>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-  }
+  if (r.shares && r.share_rows == 16)
+    hipLaunchKernelGGL((paged_rows_kernel<D, BF>), dim3(r.shares), dim3(256), 0, s, a);
+  else if (r.shares)
+    hipLaunchKernelGGL((paged_mid_kernel<D, BF>), dim3(r.shares), dim3(256), 0, s, a);
+  if (r.tiles)
+    hipLaunchKernelGGL((paged_tiles_kernel<D, BF>), dim3(r.splits, a.kv_heads, r.tiles), dim3(512), 0, s, a);
+  if (!r.join) return;
+  const int64_t rows = (int64_t)a.c.total_tokens * a.heads;
+  if (rows >= 1024)
+    hipLaunchKernelGGL((paged_join_kernel<D, 64, BF>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((paged_join_kernel<D, 256, BF>), dim3((unsigned)rows), dim3(256), 0, s, a);
 }
 
 template <int D, bool BF>
@@ -1121,7 +1730,7 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
 extern "C" size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* p) {
   Cache c;
   if (check_attn(p, &c) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
-  return workspace_of(*p);
+  return workspace_of(*p, plan_of(*p));
 }
 
 extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t stream) {
@@ -1136,20 +1745,20 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
       (p->gate && !strides_ok(p->gate_token_stride, p->gate_head_stride)))
     return spk::fail(SPK_ERR_ALIGN, "%s: q, gate and out and their strides must be 16-byte aligned", who);
   const Plan r = plan_of(*p);
-  const size_t need = workspace_of(*p);
+  const size_t need = workspace_of(*p, r);
   if (need && (!p->workspace || p->workspace_bytes < need || !spk::aligned(p->workspace, 256)))
     return spk::fail(p->workspace ? SPK_ERR_ARG : SPK_ERR_NULL, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)",
                      who, p->workspace ? p->workspace_bytes : (size_t)0, need);
-  if (c.num_kv_heads > 65535 || r.tiles[0] > 65535 || r.tiles[1] > 65535)
-    return spk::fail(SPK_ERR_SHAPE, "%s: %d KV heads, %d row tiles (65535 at most)", who, c.num_kv_heads,
-                     std::max(r.tiles[0], r.tiles[1]));
+  if (c.num_kv_heads > 65535 || r.tiles > 65535)
+    return spk::fail(SPK_ERR_SHAPE, "%s: %d KV heads, %d row tiles (65535 at most)", who, c.num_kv_heads, r.tiles);
   a.q = static_cast<const uint16_t*>(p->q);
   a.k = static_cast<const uint16_t*>(c.k_cache);
   a.v = static_cast<const uint16_t*>(c.v_cache);
   a.gate = static_cast<const uint16_t*>(p->gate);
   a.out = static_cast<uint16_t*>(p->out);
   a.lse = p->lse;
-  a.part = static_cast<float*>(p->workspace);
+  a.shared = static_cast<float*>(p->workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + shared_bytes(*p, r));
   a.qt = p->q_token_stride;
   a.qh = p->q_head_stride;
   a.gt = p->gate_token_stride;
@@ -1160,13 +1769,12 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
   a.kv_heads = c.num_kv_heads;
   a.group = p->num_q_heads / c.num_kv_heads;
   a.window = p->window;
-  for (int kind = 0; kind < 2; ++kind) {
-    a.splits[kind] = r.splits[kind];
-    a.chunk[kind] = r.chunk[kind];
-    a.tile_rows[kind] = r.tile_rows[kind];
-  }
-  a.one_tile = r.one_tile;
   a.many = r.many;
+  a.shares = r.shares;
+  a.share_rows = r.share_rows;
+  a.alone = !r.join;
+  a.splits = r.splits;
+  a.chunk = r.chunk;
   const float scale = p->scale != 0.0f ? p->scale : 1.0f / std::sqrt((float)c.head_dim);
   a.scale_log2 = scale * 1.44269504088896341f;
   hipStream_t s = spk::to_hip(stream);

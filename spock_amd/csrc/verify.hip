@@ -12,11 +12,13 @@
 //      the token in it.
 // The outcome hangs on comparisons, so whatever enters one is fp64: products
 // u q(d) of two values, the exponentials of the drawn row and the running sums.
-// The rows' sums of exponentials are fp32 exponentials with an exact argument
-// (two-float product with log2(e) / T), added in fp64.
+// The rows' sums of exponentials are fp32 exponentials, each off by a few units
+// in the last place but none in common (log2(e) / T enters as two floats), in
+// fp64 sums of eight.
 #include <algorithm>
 
 #include "capi_common.hpp"
+#include "numerics.hpp"
 #include "paged.hpp"
 
 namespace {
@@ -43,21 +45,18 @@ struct Stat {
   double sum;
 };
 
-constexpr int kPiece = 4096;  // vocabulary entries of a residual piece
-
-template <class T>
-__device__ __forceinline__ float value(const T* p, int64_t i) {
-  return (float)p[i];
-}
+constexpr int kPiece = 4096;    // vocabulary entries of a residual piece
+constexpr int kMaxParts = 64;   // of a row's statistics: one for each lane
 
 __device__ __forceinline__ bool better(float m, int a, float om, int oa) {
   return om > m || (om == m && (uint32_t)oa < (uint32_t)a);  // -1 is the largest index
 }
 
-// log2(e) / T as two floats; greedy rows count at T = 1.
+// log2(e) / T, also as two floats; greedy rows count at T = 1.  The second is
+// larger than 0, so that a logit of -inf stays one.
 struct Heat {
-  float c, lo, least;  // least: differences below it weigh nothing
-  double inv;
+  float c, lo;
+  double scale;
   bool greedy;
 };
 __device__ __forceinline__ Heat heat_of(const Verify& a, int s) {
@@ -65,12 +64,28 @@ __device__ __forceinline__ Heat heat_of(const Verify& a, int s) {
   Heat h;
   h.greedy = !(t > 0.0f);
   if (h.greedy) t = 1.0f;
-  const double c = 1.4426950408889634 / fmax((double)t, 1e-30);
-  h.c = (float)c;
-  h.lo = (float)(c - (double)h.c);
-  h.least = -200.0f / h.c;
-  h.inv = (double)t;
+  h.scale = 1.4426950408889634 / fmax((double)t, 1e-30);
+  h.c = __uint_as_float(__float_as_uint((float)h.scale) - 1);
+  h.lo = (float)(h.scale - (double)h.c);
   return h;
+}
+
+// 2^x, x <= 0 or NaN: 2^k e^(r ln 2), |r| <= 1/2, the exponential's series to
+// the tenth power (2e-13 relative).
+__device__ __forceinline__ double exp2_f64(double x) {
+  const double k = __builtin_rint(x), t = (x - k) * 0.6931471805599453;
+  double p = 1.0 / 3628800;
+  p = __builtin_fma(p, t, 1.0 / 362880);
+  p = __builtin_fma(p, t, 1.0 / 40320);
+  p = __builtin_fma(p, t, 1.0 / 5040);
+  p = __builtin_fma(p, t, 1.0 / 720);
+  p = __builtin_fma(p, t, 1.0 / 120);
+  p = __builtin_fma(p, t, 1.0 / 24);
+  p = __builtin_fma(p, t, 1.0 / 6);
+  p = __builtin_fma(p, t, 0.5);
+  p = __builtin_fma(p, t, 1.0);
+  p = __builtin_fma(p, t, 1.0);
+  return x < -1000.0 ? 0.0 : __builtin_ldexp(p, (int)k);
 }
 
 // grid (parts, total_tokens, sides); block 256
@@ -91,29 +106,32 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(Verify a) {
   float m = -INFINITY;
   int arg = -1;
   double sum = 0.0;
-  auto take = [&](const float* x, int count, int first) {
+  auto shrink = [&](float from, float to) {  // of a sum whose maximum was `from`
+    const float d = from - to;
+    return (double)__builtin_amdgcn_exp2f(__builtin_fmaf(d, heat.lo, d * heat.c));
+  };
+  auto take = [&](const float* x, int count, int first) __attribute__((always_inline)) {
     float top = x[0];
+#pragma unroll
     for (int i = 1; i < count; ++i) top = fmaxf(top, x[i]);
     if (top > m) {
-      const float d = m - top;
-      if (m != -INFINITY) sum *= (double)__builtin_amdgcn_exp2f(d < heat.least ? -200.0f : d * heat.c);
+      if (m != -INFINITY) sum *= shrink(m, top);
       m = top;
+#pragma unroll
       for (int i = count - 1; i >= 0; --i)
         if (x[i] == top) arg = first + i;
     }
     const float base = m == -INFINITY ? 0.0f : m;
     float part = 0.0f;
+#pragma unroll
     for (int i = 0; i < count; ++i) {
-      float d = x[i] - base;
-      d = d < heat.least ? heat.least : d;
-      const float k = __builtin_rintf(d * heat.c);
-      const float r = __builtin_fmaf(d, heat.lo, __builtin_fmaf(d, heat.c, -k));
-      part += __builtin_ldexpf(__builtin_amdgcn_exp2f(r), (int)k);
+      const float d = x[i] - base;
+      part += __builtin_amdgcn_exp2f(__builtin_fmaf(d, heat.lo, d * heat.c));
     }
     sum += (double)part;
   };
   if ((int)threadIdx.x < head) {
-    const float x[1] = {value(row, threadIdx.x)};
+    const float x[1] = {(float)row[threadIdx.x]};
     take(x, 1, c0 + threadIdx.x);
   }
   for (int v = threadIdx.x; v < vecs; v += 256) {
@@ -126,20 +144,17 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(Verify a) {
     take(x, VE, c0 + head + v * VE);
   }
   if ((int)threadIdx.x < tail) {
-    const float x[1] = {value(row, n - tail + threadIdx.x)};
+    const float x[1] = {(float)row[n - tail + threadIdx.x]};
     take(x, 1, c0 + n - tail + threadIdx.x);
   }
 
   auto join = [&](float om, int oa, double os) {
-    if (om > m) {
-      const float d = m - om;
-      sum = (m == -INFINITY ? sum : sum * (double)__builtin_amdgcn_exp2f(d < heat.least ? -200.0f : d * heat.c)) + os;
-    } else if (m > om) {
-      const float d = om - m;
-      sum += om == -INFINITY ? os : os * (double)__builtin_amdgcn_exp2f(d < heat.least ? -200.0f : d * heat.c);
-    } else {
+    if (om > m)
+      sum = (m == -INFINITY ? sum : sum * shrink(m, om)) + os;
+    else if (m > om)
+      sum += om == -INFINITY ? os : os * shrink(om, m);
+    else
       sum += os;
-    }
     if (better(m, arg, om, oa)) arg = oa;
     m = fmaxf(m, om);
   };
@@ -156,43 +171,43 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(Verify a) {
 // The statistics of a row from its parts; every lane of the wave returns them.
 __device__ __forceinline__ Stat row_stat(const Verify& a, const Heat& heat, int side, int t, int lane) {
   Stat r{-INFINITY, -1, 0.0};
-  const Stat* p = a.stats + ((int64_t)side * a.total + t) * a.parts;
-  float m = -INFINITY;
-  for (int j = lane; j < a.parts; j += 64) m = fmaxf(m, p[j].max);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-  double sum = 0.0;
-  int arg = -1;
-  for (int j = lane; j < a.parts; j += 64) {
-    const Stat x = p[j];
-    sum += x.max == -INFINITY || x.max == m ? x.sum : x.sum * exp(((double)x.max - (double)m) / heat.inv);
-    if (x.max == m && (uint32_t)x.arg < (uint32_t)arg) arg = x.arg;
-  }
+  if (lane < a.parts) r = a.stats[((int64_t)side * a.total + t) * a.parts + lane];
+  const float m = spk::wave_max(r.max);
+  double sum = r.max == -INFINITY || r.max == m ? r.sum : r.sum * exp2_f64(((double)r.max - (double)m) * heat.scale);
+  uint32_t arg = r.max == m ? (uint32_t)r.arg : ~0u;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     sum += __shfl_xor(sum, d);
-    const int o = __shfl_xor(arg, d);
-    if ((uint32_t)o < (uint32_t)arg) arg = o;
+    arg = min(arg, (uint32_t)__shfl_xor((int)arg, d));
   }
-  r.max = m;
-  r.arg = arg;
-  r.sum = sum;
-  return r;
+  return {m, (int)arg, sum};
 }
 
-// The probability of entry i of a row.
+// A row's distribution: entries count as 2^((x - max) scale) / sum of logits, as
+// they are of probabilities.
 template <class T>
-__device__ __forceinline__ double prob(const Verify& a, const T* row, int64_t i, const Stat& st, const Heat& heat) {
-  const double x = (double)(float)row[i];
-  return a.probs ? x : exp((x - (double)st.max) / heat.inv) / st.sum;
-}
-
-// Log of it, without the exponential's underflow.
-template <class T>
-__device__ __forceinline__ float log_prob(const Verify& a, const T* row, int64_t i, const Stat& st, const Heat& heat) {
-  const double x = (double)(float)row[i];
-  return (float)(a.probs ? log(x) : (x - (double)st.max) / heat.inv - log(st.sum));
-}
+struct Dist {
+  const T* row;
+  double max, scale, inv, log_sum;
+  bool probs;
+  __device__ __forceinline__ void set(const Verify& a, const T* r, const Stat& st, const Heat& heat) {
+    row = r;
+    probs = a.probs;
+    max = (double)st.max;
+    scale = heat.scale;
+    inv = 1.0 / st.sum;
+    log_sum = st.sum;
+  }
+  __device__ __forceinline__ double of(float x) const {
+    return probs ? (double)x : exp2_f64(((double)x - max) * scale) * inv;
+  }
+  __device__ __forceinline__ double at(int64_t i) const { return of((float)row[i]); }
+  // without the exponential's underflow
+  __device__ __forceinline__ float log_at(int64_t i) const {
+    const double x = (double)(float)row[i];
+    return (float)(probs ? log(x) : (x - max) * scale * 0.6931471805599453 - log(log_sum));
+  }
+};
 
 struct Span {
   int first, rows;
@@ -208,27 +223,38 @@ __device__ __forceinline__ int draft_of(const Verify& a, int row) {
   return (uint32_t)d < (uint32_t)a.vocab ? d : INT32_MAX;
 }
 
-// What row `t` leaves for token i: the residual where a draft `d` was refused
+// What a row leaves for token i: the residual where a draft `d` was refused
 // there (d < 0: the row itself).
 template <class T>
 struct Rest {
-  const T *p, *q;
-  Stat ps, qs;
-  Heat heat;
+  Dist<T> p, q;
+  bool drafted;  // q is there
   int d;
-  __device__ __forceinline__ void at(const Verify& a, int i, double* rest, double* base) const {
-    const double x = prob(a, p, i, ps, heat);
-    *base = x;
+  __device__ __forceinline__ void of(int i, float x, float y, double* rest, double* base) const {
+    const double u = p.of(x);
+    *base = u;
     if (d < 0) {
-      *rest = x;
-    } else if (q) {
-      const double y = x - prob(a, q, i, qs, heat);
-      *rest = y > 0.0 || y != y ? y : 0.0;
+      *rest = u;
+    } else if (drafted) {
+      const double v = u - q.of(y);
+      *rest = v > 0.0 || v != v ? v : 0.0;
     } else {
-      *rest = i == d ? 0.0 : x;
+      *rest = i == d ? 0.0 : u;
     }
   }
 };
+
+template <class T>
+__device__ __forceinline__ Rest<T> rest_of(const Verify& a, const Heat& heat, int row, bool refused, int lane) {
+  Rest<T> r;
+  r.drafted = refused && a.draft;
+  r.p.set(a, static_cast<const T*>(a.target) + row * a.target_stride,
+          a.probs ? Stat{} : row_stat(a, heat, 0, row, lane), heat);
+  r.q.set(a, r.drafted ? static_cast<const T*>(a.draft) + row * a.draft_stride : nullptr,
+          r.drafted && !a.probs ? row_stat(a, heat, 1, row, lane) : Stat{}, heat);
+  r.d = refused ? draft_of(a, row) : -1;
+  return r;
+}
 
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
@@ -255,44 +281,51 @@ __global__ __launch_bounds__(256) void verify_accept_kernel(Verify a) {
     return;
   }
   const Heat heat = heat_of(a, s);
+  if (heat.greedy && !lead) return;
   if (threadIdx.x == 0) stop_at = sp.rows - 1;
   __syncthreads();
   for (int i = wave; i < sp.rows - 1; i += 4) {
     const int t = sp.first + i, d = a.tokens[t + 1];
     bool yes = (uint32_t)d < (uint32_t)a.vocab;
     if (yes) {
-      const T* p = static_cast<const T*>(a.target) + t * a.target_stride;
-      const T* q = static_cast<const T*>(a.draft) + t * a.draft_stride;
       const Stat ps = a.probs ? Stat{} : row_stat(a, heat, 0, t, lane);
       if (heat.greedy) {
         yes = ps.arg == d;
       } else {
-        const Stat qs = a.probs || !a.draft ? Stat{} : row_stat(a, heat, 1, t, lane);
-        const double qd = a.draft ? prob(a, q, d, qs, heat) : 1.0;
-        yes = (double)a.u_accept[t] * qd < prob(a, p, d, ps, heat);
+        Dist<T> p, q;
+        p.set(a, static_cast<const T*>(a.target) + t * a.target_stride, ps, heat);
+        double qd = 1.0;
+        if (a.draft) {
+          q.set(a, static_cast<const T*>(a.draft) + t * a.draft_stride, a.probs ? Stat{} : row_stat(a, heat, 1, t, lane),
+                heat);
+          qd = q.at(d);
+        }
+        yes = (double)a.u_accept[t] * qd < p.at(d);
       }
     }
     if (!yes && lane == 0) atomicMin(&stop_at, i);
   }
   __syncthreads();
   const int stop = stop_at, row = sp.first + stop;
-  const T* p = static_cast<const T*>(a.target) + row * a.target_stride;
-  const Stat ps = a.probs ? Stat{} : row_stat(a, heat, 0, row, lane);
 
   if (lead) {
     for (int i = wave; i < sp.rows; i += 4) {
       const int t = sp.first + i;
-      if (i < stop) {
-        const int d = a.tokens[t + 1];
-        const Stat st = a.probs || !a.logprobs ? Stat{} : row_stat(a, heat, 0, t, lane);
-        if (lane == 0) {
-          a.out[t] = d;
-          if (a.logprobs) a.logprobs[t] = log_prob(a, static_cast<const T*>(a.target) + t * a.target_stride, d, st, heat);
+      if (i == stop && !heat.greedy) continue;  // drawn by the next launch
+      int token = i < stop ? a.tokens[t + 1] : -1;
+      float logp = 0.0f;
+      if (i <= stop) {
+        const Stat st = a.probs ? Stat{} : row_stat(a, heat, 0, t, lane);
+        if (i == stop) token = st.arg;
+        if (token >= 0 && a.logprobs) {
+          Dist<T> p;
+          p.set(a, static_cast<const T*>(a.target) + t * a.target_stride, st, heat);
+          logp = p.log_at(token);
         }
-      } else if (lane == 0 && (i > stop || heat.greedy)) {
-        const bool here = i == stop && ps.arg >= 0;
-        a.out[t] = here ? ps.arg : -1;
-        if (a.logprobs) a.logprobs[t] = here ? log_prob(a, p, ps.arg, ps, heat) : 0.0f;
+      }
+      if (lane == 0) {
+        a.out[t] = token;
+        if (a.logprobs) a.logprobs[t] = logp;
       }
     }
     if (threadIdx.x == 0) {
@@ -302,19 +335,13 @@ __global__ __launch_bounds__(256) void verify_accept_kernel(Verify a) {
   }
   if (heat.greedy) return;
 
-  Rest<T> rest;
-  const bool refused = stop < sp.rows - 1;
-  rest.p = p;
-  rest.ps = ps;
-  rest.q = refused && a.draft ? static_cast<const T*>(a.draft) + row * a.draft_stride : nullptr;
-  rest.qs = rest.q && !a.probs ? row_stat(a, heat, 1, row, lane) : Stat{};
-  rest.heat = heat;
-  rest.d = refused ? draft_of(a, row) : -1;
+  const Rest<T> rest = rest_of<T>(a, heat, row, stop < sp.rows - 1, lane);
   double left = 0.0, all = 0.0;
   const int end = min(a.vocab, (int)(blockIdx.x + 1) * kPiece);
+#pragma unroll 4
   for (int i = blockIdx.x * kPiece + threadIdx.x; i < end; i += 256) {
     double x, y;
-    rest.at(a, i, &x, &y);
+    rest.of(i, (float)rest.p.row[i], rest.drafted ? (float)rest.q.row[i] : 0.0f, &x, &y);
     left += x;
     all += y;
   }
@@ -327,98 +354,115 @@ __global__ __launch_bounds__(256) void verify_accept_kernel(Verify a) {
   }
 }
 
-// The first index i of 0 .. n-1 whose running sum from `before` on passes x,
-// else the last with weight, else -1; `next`: the running sum before it.
-// value(i) is asked by one wave, 64 at a time, in order.
-template <class F>
-__device__ __forceinline__ int first_past(int n, double before, double x, int lane, F value, double* next) {
-  int last = -1;
-  double last_sum = before;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const double v = i0 + lane < n ? value(i0 + lane) : 0.0;
-    double sum = v;
+// Inclusive running sum over the workgroup's 256 threads.
+__device__ __forceinline__ double block_scan(double v, double* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double o = __shfl_up(sum, d);
-      if (lane >= d) sum += o;
-    }
-    const unsigned long long past = __ballot(i0 + lane < n && before + sum > x);
-    const unsigned long long some = __ballot(v > 0.0);
-    const double prior = before + (sum - v);
-    if (past) {
-      const int l = __ffsll(past) - 1;
-      *next = __shfl(prior, l);
-      return i0 + l;
-    }
-    if (some) {
-      const int l = 63 - __clzll(some);
-      last = i0 + l;
-      last_sum = __shfl(prior, l);
-    }
-    before += __shfl(sum, 63);
+  for (int d = 1; d < 64; d <<= 1) {
+    const double o = __shfl_up(v, d);
+    if (lane >= d) v += o;
   }
-  *next = last_sum;
-  return last;
+  __syncthreads();
+  if (lane == 63) red[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += red[w];
+  return v;
 }
 
-// grid (num_seqs); block 64
+// grid (num_seqs); block 256.  The piece in which the running sum passes
+// u * total, then 16 consecutive entries of it to a thread, then the entry.  Where
+// rounding leaves the last sum short, the last entry with weight.
 template <class T>
-__global__ __launch_bounds__(64) void verify_draw_kernel(Verify a) {
-  const int s = blockIdx.x, lane = threadIdx.x;
+__global__ __launch_bounds__(256) void verify_draw_kernel(Verify a) {
+  __shared__ double red[4];
+  __shared__ double before_at;
+  __shared__ int found, last, token_at;
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const Span sp = span_of(a, s);
   if (sp.rows == 0) return;
   const Heat heat = heat_of(a, s);
   if (heat.greedy) return;
-  const int stop = min(max(a.accepted[s], 0), sp.rows - 1), row = sp.first + stop;
-  const bool refused = stop < sp.rows - 1;
-  Rest<T> rest;
-  rest.p = static_cast<const T*>(a.target) + row * a.target_stride;
-  rest.ps = a.probs ? Stat{} : row_stat(a, heat, 0, row, lane);
-  rest.q = refused && a.draft ? static_cast<const T*>(a.draft) + row * a.draft_stride : nullptr;
-  rest.qs = rest.q && !a.probs ? row_stat(a, heat, 1, row, lane) : Stat{};
-  rest.heat = heat;
-  rest.d = refused ? draft_of(a, row) : -1;
   const double* m = a.mass + (int64_t)s * a.pieces * 2;
-  double total = 0.0, base = 0.0;
-  for (int i = lane; i < a.pieces; i += 64) {
-    total += m[2 * i];
+  double left = 0.0, base = 0.0;
+  for (int i = tid; i < a.pieces; i += 256) {
+    left += m[2 * i];
     base += m[2 * i + 1];
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    total += __shfl_xor(total, d);
-    base += __shfl_xor(base, d);
+  const int stop = min(max(a.accepted[s], 0), sp.rows - 1), row = sp.first + stop;
+  const Rest<T> rest = rest_of<T>(a, heat, row, stop < sp.rows - 1, lane);
+  left = block_sum(left, red);
+  base = block_sum(base, red);
+  const bool itself = !(left > 0.0);  // nothing left: the row itself
+  const double total = itself ? base : left, x = (double)a.u_sample[s] * total;
+  if (tid == 0) {
+    found = INT32_MAX;
+    last = -1;
+    token_at = -1;
+    before_at = 0.0;
   }
-  const int which = total > 0.0 ? 0 : 1;  // nothing left: the row itself
-  if (which) total = base;
-  int token = -1;
+  __syncthreads();
   if (total > 0.0) {
-    const double x = (double)a.u_sample[s] * total;
-    double before;
-    const int piece = first_past(a.pieces, 0.0, x, lane, [&](int i) { return m[2 * i + which]; }, &before);
-    if (piece >= 0) {
-      const int i0 = piece * kPiece, n = min(kPiece, a.vocab - i0);
-      const int i = first_past(n, before, x, lane,
-                               [&](int j) {
-                                 double r, b;
-                                 rest.at(a, i0 + j, &r, &b);
-                                 return which ? b : r;
-                               },
-                               &before);
-      token = i < 0 ? -1 : i0 + i;
+    // the first piece past x: found by its index, and the running sum before it
+    double before = 0.0;
+    for (int i0 = 0; i0 < a.pieces; i0 += 256) {
+      const int i = i0 + tid;
+      const double v = i < a.pieces ? m[2 * i + itself] : 0.0, sum = before + block_scan(v, red);
+      if (i < a.pieces && sum > x) atomicMin(&found, i);
+      if (v > 0.0) atomicMax(&last, i);
+      __syncthreads();
+      const int here = found != INT32_MAX ? found : last;
+      if (i == here) before_at = sum - v;
+      before += red[0] + red[1] + red[2] + red[3];
+      if (found != INT32_MAX) break;
+      __syncthreads();
     }
+    __syncthreads();
+    const int piece = found != INT32_MAX ? found : last;
+    const double from = before_at;
+    __syncthreads();
+    if (tid == 0) {
+      found = INT32_MAX;
+      last = -1;
+    }
+    constexpr int N = kPiece / 256;
+    const int i0 = piece * kPiece + N * tid;
+    double v[N], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      v[j] = 0.0;
+      if (i0 + j < a.vocab) {
+        double r, b;
+        rest.of(i0 + j, (float)rest.p.row[i0 + j], rest.drafted ? (float)rest.q.row[i0 + j] : 0.0f, &r, &b);
+        v[j] = itself ? b : r;
+      }
+      sum += v[j];
+    }
+    double run = from + block_scan(sum, red) - sum;
+    int first = INT32_MAX, some = -1;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      run += v[j];
+      if (i0 + j < a.vocab && run > x) first = min(first, i0 + j);
+      if (v[j] > 0.0) some = i0 + j;
+    }
+    if (first != INT32_MAX) atomicMin(&found, first);
+    if (some >= 0) atomicMax(&last, some);
+    __syncthreads();
+    if (tid == 0) token_at = found != INT32_MAX ? found : last;
+    __syncthreads();
   }
-  if (lane == 0) {
+  if (tid == 0) {
+    const int token = token_at;
     a.out[row] = token;
-    if (a.logprobs) a.logprobs[row] = token < 0 ? 0.0f : log_prob(a, rest.p, token, rest.ps, heat);
+    if (a.logprobs) a.logprobs[row] = token < 0 ? 0.0f : rest.p.log_at(token);
   }
 }
 
 // Parts of a row's statistics: enough workgroups to fill the chip (2,048),
-// pieces of at least 2,048 entries.
+// parts of at least 2,048 entries, and a lane for each.
 int parts_of(int vocab, int rows) {
   const int64_t want = std::max<int64_t>(1, 2048 / std::max(1, rows));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (vocab + 2047) / 2048));
+  return (int)std::min<int64_t>(kMaxParts, std::max<int64_t>(1, std::min<int64_t>(want, ((int64_t)vocab + 2047) / 2048)));
 }
 
 int pieces_of(int vocab) { return (vocab + kPiece - 1) / kPiece; }
@@ -428,7 +472,7 @@ void launch(const Verify& a, hipStream_t s) {
   if (!a.probs)
     hipLaunchKernelGGL(verify_stats_kernel<T>, dim3(a.parts, a.total, a.draft ? 2 : 1), dim3(256), 0, s, a);
   hipLaunchKernelGGL(verify_accept_kernel<T>, dim3(a.pieces, a.num_seqs), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(verify_draw_kernel<T>, dim3(a.num_seqs), dim3(64), 0, s, a);
+  hipLaunchKernelGGL(verify_draw_kernel<T>, dim3(a.num_seqs), dim3(256), 0, s, a);
 }
 
 }  // namespace

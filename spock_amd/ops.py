@@ -289,60 +289,75 @@ _HALF = {torch.float16: _lib.SPK_F16, torch.bfloat16: _lib.SPK_BF16}
 _PAIRINGS = {"halves": _lib.SPK_ROPE_HALVES, "adjacent": _lib.SPK_ROPE_ADJACENT}
 
 
-def _on(what: str, name: str, t: torch.Tensor, dev, dtype, shape=None) -> None:
-    if t.device != dev or t.dtype != dtype:
-        raise _lib.SpockError(f"{what}: {name} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise _lib.SpockError(f"{what}: {name} shape {tuple(t.shape)} != {shape}")
+def _on(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape=None) -> None:
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise _lib.SpockError(f"{what}: {name} must be {dtype} on cuda:{dev}, got {t.dtype} on {t.device}")
+    if shape is not None and t.shape != shape:
+        raise _lib.SpockError(f"{what}: {name} shape {tuple(t.shape)} != {tuple(shape)}")
 
 
-def _rows(what: str, name: str, t: torch.Tensor, dev, dtype, shape) -> None:
-    """A [tokens][heads][dim] view: any strides of the first two dimensions."""
+def _flat(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape) -> None:
     _on(what, name, t, dev, dtype, shape)
-    if t.stride(2) != 1:
+    if not t.is_contiguous():
+        raise _lib.SpockError(f"{what}: {name} must be contiguous")
+
+
+def _rows(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape):
+    """Strides of a [tokens][heads][dim] view: any of the first two dimensions."""
+    _on(what, name, t, dev, dtype, shape)
+    strides = t.stride()
+    if strides[2] != 1:
         raise _lib.SpockError(f"{what}: the last dimension of {name} must be contiguous")
+    return strides
+
+
+def _device(what: str, t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise _lib.SpockError(f"{what}: expected device tensors")
+    return t.get_device()
 
 
 def _paged_cache(what: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                  cu_seqlens: torch.Tensor, context_lens: torch.Tensor) -> SpkPagedCache:
-    dev = q.device
-    if dev.type != "cuda":
-        raise _lib.SpockError(f"{what}: expected device tensors")
+    dev, dtype = _device(what, q), q.dtype
     if q.dim() != 3 or k_cache.dim() != 4:
         raise _lib.SpockError(f"{what}: q must be [tokens][heads][dim] and the caches [pages][page_size][kv_heads][dim], "
                               f"got {tuple(q.shape)} and {tuple(k_cache.shape)}")
-    if q.dtype not in _HALF:
-        raise _lib.SpockError(f"{what}: q must be float16 or bfloat16, got {q.dtype}")
-    pages, page_size, kv_heads, dim = k_cache.shape
-    if q.shape[2] != dim:
-        raise _lib.SpockError(f"{what}: q has head_dim {q.shape[2]}, the cache {dim}")
-    _on(what, "k_cache", k_cache, dev, q.dtype)
-    _on(what, "v_cache", v_cache, dev, q.dtype, (pages, page_size, kv_heads, dim))
+    if dtype not in _HALF:
+        raise _lib.SpockError(f"{what}: q must be float16 or bfloat16, got {dtype}")
+    shape = k_cache.shape
+    pages, page_size, kv_heads, dim = shape
+    tokens, _, q_dim = q.shape
+    if q_dim != dim:
+        raise _lib.SpockError(f"{what}: q has head_dim {q_dim}, the cache {dim}")
+    _on(what, "k_cache", k_cache, dev, dtype)
+    _on(what, "v_cache", v_cache, dev, dtype, shape)
     strides = k_cache.stride()
     if v_cache.stride() != strides or strides[3] != 1:
         raise _lib.SpockError(f"{what}: k_cache and v_cache need equal strides and a contiguous last dimension, "
                               f"got {strides} and {v_cache.stride()}")
     seqs = context_lens.numel()
     _on(what, "block_table", block_table, dev, torch.int32)
-    _on(what, "cu_seqlens", cu_seqlens, dev, torch.int32, (seqs + 1,))
-    _on(what, "context_lens", context_lens, dev, torch.int32, (seqs,))
+    _flat(what, "cu_seqlens", cu_seqlens, dev, torch.int32, (seqs + 1,))
+    _flat(what, "context_lens", context_lens, dev, torch.int32, (seqs,))
     if block_table.dim() != 2 or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise _lib.SpockError(f"{what}: block_table must be [{seqs}][max_pages] with contiguous rows, "
                               f"got {tuple(block_table.shape)}")
-    if not (cu_seqlens.is_contiguous() and context_lens.is_contiguous()):
-        raise _lib.SpockError(f"{what}: cu_seqlens and context_lens must be contiguous")
-    return SpkPagedCache(_HALF[q.dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, q.shape[0],
+    return SpkPagedCache(_HALF[dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, tokens,
                          k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2],
                          block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), context_lens.data_ptr())
 
 
-def _call(fn, a, dev, what: str) -> None:
-    """fn(a) on the current stream of the tensors' device, which is made current for the launch."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+def _call(fn, a, dev: int, what: str) -> None:
+    """fn(a) on the current stream of the tensors' device, which is made current for the launch.  (The raw handle of
+    the stream costs a tenth of the torch.cuda.Stream object around it, 2 us of a 20 us call.)"""
+    if torch.cuda.current_device() == dev:
+        rc = fn(C.byref(a), torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            check(fn(C.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+            rc = fn(C.byref(a), torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
 
 
 def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor,
@@ -361,36 +376,36 @@ def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     """
     what = "mrope_append"
     cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
-    T, heads, D = q.shape
-    dev, kv = q.device, cache.num_kv_heads
-    _rows(what, "q", q, dev, q.dtype, (T, heads, D))
-    _rows(what, "k", k, dev, q.dtype, (T, kv, D))
-    _rows(what, "v", v, dev, q.dtype, (T, kv, D))
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    T, heads, D = shape
+    kv_shape = (T, cache.num_kv_heads, D)
+    qs = _rows(what, "q", q, dev, dtype, shape)
+    ks = _rows(what, "k", k, dev, dtype, kv_shape)
+    vs = _rows(what, "v", v, dev, dtype, kv_shape)
     try:
         axes = bytes(list(pair_axis))
     except (TypeError, ValueError):
         raise _lib.SpockError(f"{what}: pair_axis must be a sequence of axis numbers, got {pair_axis!r}") from None
-    _on(what, "rope", rope, dev, torch.float32, (rope.shape[0], 2 * len(axes)))
-    if not rope.is_contiguous():
-        raise _lib.SpockError(f"{what}: rope must be contiguous")
-    _on(what, "positions", positions, dev, torch.int32, (positions.shape[0], T))
+    rot = 2 * len(axes)
+    rows = rope.shape[0]
+    _flat(what, "rope", rope, dev, torch.float32, (rows, rot))
+    num_axes = positions.shape[0]
+    _on(what, "positions", positions, dev, torch.int32, (num_axes, T))
     if T > 1 and positions.stride(1) != 1:
         raise _lib.SpockError(f"{what}: positions must have contiguous rows")
-    for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
-        if w is not None:
-            _on(what, name, _dev(w), dev, q.dtype, (D,))
+    if q_norm_weight is not None:
+        _flat(what, "q_norm_weight", q_norm_weight, dev, dtype, (D,))
+    if k_norm_weight is not None:
+        _flat(what, "k_norm_weight", k_norm_weight, dev, dtype, (D,))
     if pairing not in _PAIRINGS:
         raise _lib.SpockError(f"{what}: pairing must be one of {sorted(_PAIRINGS)}, got {pairing!r}")
     if out is None:
-        out = torch.empty((T, heads, D), dtype=q.dtype, device=dev)
-    else:
-        _rows(what, "out", out, dev, q.dtype, (T, heads, D))
-    a = SpkMropeArgs(cache, heads, 2 * len(axes), _PAIRINGS[pairing], positions.shape[0], axes, positions.data_ptr(),
-                     positions.stride(0), rope.data_ptr(), rope.shape[0], eps,
-                     q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                     v.data_ptr(), v.stride(0), v.stride(1), _ptr(q_norm_weight), _ptr(k_norm_weight),
-                     out.data_ptr(), out.stride(0), out.stride(1))
-    _call(lib().spk_mrope_append, a, dev, "spk_mrope_append")
+        out = q.new_empty(shape)
+    outs = _rows(what, "out", out, dev, dtype, shape)
+    a = SpkMropeArgs(cache, heads, rot, _PAIRINGS[pairing], num_axes, axes, positions.data_ptr(), positions.stride(0),
+                     rope.data_ptr(), rows, eps, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+                     v.data_ptr(), vs[0], vs[1], _ptr(q_norm_weight), _ptr(k_norm_weight), out.data_ptr(), outs[0], outs[1])
+    _call(lib().spk_mrope_append, a, dev, what)
     return out
 
 
@@ -408,31 +423,26 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """
     what = "paged_attention"
     cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
-    dev, shape = q.device, tuple(q.shape)
-    _rows(what, "q", q, dev, q.dtype, shape)
-    if gate is not None:
-        _rows(what, "gate", gate, dev, q.dtype, shape)
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    qs = _rows(what, "q", q, dev, dtype, shape)
+    gs = (0, 0) if gate is None else _rows(what, "gate", gate, dev, dtype, shape)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-    else:
-        _rows(what, "out", out, dev, q.dtype, shape)
+        out = q.new_empty(shape)
+    outs = _rows(what, "out", out, dev, dtype, shape)
     if lse is not None:
-        _on(what, "lse", _dev(lse), dev, torch.float32, shape[:2])
+        _flat(what, "lse", lse, dev, torch.float32, shape[:2])
     elif return_lse:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
-    a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale,
-                         q.data_ptr(), q.stride(0), q.stride(1), _ptr(gate), 0, 0,
-                         out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse), None, 0)
-    if gate is not None:
-        a.gate_token_stride, a.gate_head_stride = gate.stride(0), gate.stride(1)
+        lse = q.new_empty(shape[:2], dtype=torch.float32)
+    a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale, q.data_ptr(), qs[0], qs[1],
+                         _ptr(gate), gs[0], gs[1], out.data_ptr(), outs[0], outs[1], _ptr(lse), None, 0)
     need = lib().spk_paged_attention_workspace_size(C.byref(a))
     if need:
         if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.device != dev:
-            raise _lib.SpockError(f"{what}: workspace must be on {dev}, got {workspace.device}")
+            workspace = q.new_empty(need, dtype=torch.uint8)
+        elif workspace.get_device() != dev:
+            raise _lib.SpockError(f"{what}: workspace must be on cuda:{dev}, got {workspace.device}")
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(lib().spk_paged_attention, a, dev, "spk_paged_attention")
+    _call(lib().spk_paged_attention, a, dev, what)
     return out if lse is None else (out, lse)
 
 
@@ -470,45 +480,51 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     without context_lens).  Rows past cu_seqlens[S] are not written.
     """
     what = "verify_drafts"
-    dev = target.device
-    if dev.type != "cuda":
-        raise _lib.SpockError(f"{what}: expected device tensors")
+    dev = _device(what, target)
     if target.dim() != 2 or target.dtype not in _ROWS or (target.shape[1] > 1 and target.numel() and target.stride(1) != 1):
         raise _lib.SpockError(f"{what}: target must be [rows][vocab] float16, bfloat16 or float32 with contiguous rows, "
                               f"got {tuple(target.shape)} {target.dtype}")
     if kind not in _KINDS:
         raise _lib.SpockError(f"{what}: kind must be one of {sorted(_KINDS)}, got {kind!r}")
     T, vocab = target.shape
-    seqs = u_sample.numel()
+    rows, seqs = (T,), (u_sample.numel(),)
+    S = seqs[0]
+    stride, draft_stride = (target.stride(0) if T > 1 else vocab), 0
     if draft is not None:
         _on(what, "draft", draft, dev, target.dtype, (T, vocab))
         if vocab > 1 and T and draft.stride(1) != 1:
             raise _lib.SpockError(f"{what}: draft must have contiguous rows")
-    for name, t, dtype, shape in (("tokens", tokens, torch.int32, (T,)), ("cu_seqlens", cu_seqlens, torch.int32, (seqs + 1,)),
-                                  ("u_accept", u_accept, torch.float32, (T,)), ("u_sample", u_sample, torch.float32, (seqs,)),
-                                  ("temperature", temperature, torch.float32, (seqs,)),
-                                  ("context_lens", context_lens, torch.int32, (seqs,)),
-                                  ("out_tokens", out_tokens, torch.int32, (T,)), ("accepted", accepted, torch.int32, (seqs,)),
-                                  ("logprobs", logprobs, torch.float32, (T,)), ("context_out", context_out, torch.int32, (seqs,))):
-        if t is not None:
-            _on(what, name, _dev(t), dev, dtype, shape)
+        draft_stride = draft.stride(0) if T > 1 else vocab
+    i32, f32 = torch.int32, torch.float32
+    _flat(what, "tokens", tokens, dev, i32, rows)
+    _flat(what, "cu_seqlens", cu_seqlens, dev, i32, (S + 1,))
+    _flat(what, "u_accept", u_accept, dev, f32, rows)
+    _flat(what, "u_sample", u_sample, dev, f32, seqs)
+    if temperature is not None:
+        _flat(what, "temperature", temperature, dev, f32, seqs)
+    if context_lens is not None:
+        _flat(what, "context_lens", context_lens, dev, i32, seqs)
+        if context_out is None:
+            context_out = torch.empty(seqs, dtype=i32, device=target.device)
+    if context_out is not None:
+        _flat(what, "context_out", context_out, dev, i32, seqs)
     if out_tokens is None:
-        out_tokens = torch.empty(T, dtype=torch.int32, device=dev)
+        out_tokens = torch.empty(rows, dtype=i32, device=target.device)
     if accepted is None:
-        accepted = torch.empty(seqs, dtype=torch.int32, device=dev)
+        accepted = torch.empty(seqs, dtype=i32, device=target.device)
     if logprobs is None:
-        logprobs = torch.empty(T, dtype=torch.float32, device=dev)
-    if context_out is None and context_lens is not None:
-        context_out = torch.empty(seqs, dtype=torch.int32, device=dev)
-    need = lib().spk_verify_drafts_workspace_size(vocab, seqs, T)
+        logprobs = torch.empty(rows, dtype=f32, device=target.device)
+    _flat(what, "out_tokens", out_tokens, dev, i32, rows)
+    _flat(what, "accepted", accepted, dev, i32, seqs)
+    _flat(what, "logprobs", logprobs, dev, f32, rows)
+    need = lib().spk_verify_drafts_workspace_size(vocab, S, T)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev:
-        raise _lib.SpockError(f"{what}: workspace must be on {dev}, got {workspace.device}")
-    a = SpkVerifyArgs(_KINDS[kind], _ROWS[target.dtype], vocab, seqs, T, cu_seqlens.data_ptr(), tokens.data_ptr(),
-                      target.data_ptr(), target.stride(0) if T > 1 else vocab, _ptr(draft),
-                      0 if draft is None else draft.stride(0) if T > 1 else vocab, _ptr(temperature), u_accept.data_ptr(),
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=target.device)
+    elif workspace.get_device() != dev:
+        raise _lib.SpockError(f"{what}: workspace must be on cuda:{dev}, got {workspace.device}")
+    a = SpkVerifyArgs(_KINDS[kind], _ROWS[target.dtype], vocab, S, T, cu_seqlens.data_ptr(), tokens.data_ptr(),
+                      target.data_ptr(), stride, _ptr(draft), draft_stride, _ptr(temperature), u_accept.data_ptr(),
                       u_sample.data_ptr(), out_tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(),
                       _ptr(context_lens), _ptr(context_out), workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    _call(lib().spk_verify_drafts, a, dev, "spk_verify_drafts")
+    _call(lib().spk_verify_drafts, a, dev, what)
     return out_tokens, accepted, logprobs, context_out
