@@ -770,7 +770,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
 // tokens): too many for the registers of one wave beside the keys on their
 // way, too few to be bound by anything but memory.  A workgroup takes 64 rows,
 // 16 to each of its 4 waves, and all waves read every step of 32 keys from
-// LDS, which holds four steps: loads go straight into LDS, three steps ahead.
+// LDS.  A wave loads its part of a step's keys and values two steps ahead, into
+// registers, two steps lie in LDS, and two workgroups share a CU.
 // The waves have their own rows, so nothing is joined.
 //
 // The arithmetic is paged_rows_kernel's.  Rows lie in LDS as in memory, one
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
 // by the transposing load: 16 lanes take 4 keys' pieces of 16 dimensions and
 // get 4 keys of a dimension each.
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
+__global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   using H = Half<BF>;
   constexpr int DC = D / 32;      // contraction steps of the scores
   constexpr int DT = D / 16;      // output tiles
@@ -787,10 +788,8 @@ __global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
   constexpr int RPW = 64 / CH;    // rows of one load
   constexpr int RS = 32 / RPW;    // loads of 32 keys, and the distance of a load's rows
   constexpr int LW = RS / 4;      // loads of a wave
-  // four steps, as separate arrays: a load into one is then known not to touch the others
-  __shared__ __align__(16) uint4 ka[RS * 65], kb[RS * 65], kc[RS * 65], kd[RS * 65];
-  __shared__ __align__(16) uint4 va[RS * 66], vb[RS * 66], vc[RS * 66], vd[RS * 66];
-  __shared__ __align__(16) uint32_t there[4][4];  // per step and wave: its rows' keys that exist
+  __shared__ __align__(16) uint4 kss[2][RS * 65], vss[2][RS * 66];
+  __shared__ __align__(16) uint32_t there[2][4];  // per step and wave: its rows' keys that exist
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 15, g = lane >> 4;
   Share sh;
@@ -819,67 +818,42 @@ __global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
 #pragma unroll
     for (int c = 0; c < DC; ++c) q[c] = *reinterpret_cast<const uint4*>(src + 32 * c);
   }
-  // the keys of a wave's loads are the wave's: their page ids are scalar loads,
-  // and the vector memory counter counts the keys and values alone
-  typedef const __attribute__((address_space(4))) int32_t* Table;
-  const Table table = (Table)(a.c.table + (int64_t)seq * a.c.table_stride);
-  const uint16_t* kbase = a.k + kvh * a.c.head_stride + 8 * (lane % CH);
-  const uint16_t* vbase = a.v + kvh * a.c.head_stride + 8 * (lane % CH);
-  // A wave's loads hold RPW groups of LW consecutive keys; where the page size is
-  // a multiple of LW (and a step begins at one of 32), a group has one page.
-  const bool grouped = a.c.page_size % LW == 0;
-  int page[RPW][LW];  // of the step that is loaded next
-  auto look_up = [&](int k0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < RPW; ++j) {
-      const int key = k0 + wave * LW + RS * j;
-      if (grouped) {
-        page[j][0] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(key, lo), end - 1))];
-#pragma unroll
-        for (int i = 1; i < LW; ++i) page[j][i] = page[j][0];
-      } else {
-#pragma unroll
-        for (int i = 0; i < LW; ++i)
-          page[j][i] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(key + i, lo), end - 1))];
-      }
-    }
+  const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
+  const uint16_t* kbase = a.k + kvh * a.c.head_stride;
+  const uint16_t* vbase = a.v + kvh * a.c.head_stride;
+  // A wave's part of a step, on its way, and the page ids of the one that
+  // takes its place two steps on: vector loads return in order, so an id
+  // is asked for before everything that may still be under way when it is used.
+  struct Part {
+    uint4 k[LW], v[LW];
+    int page[LW];
+    uint32_t mine;  // its keys that exist
   };
-  auto load = [&](int k0, uint4* ks, uint4* vs, int stage) __attribute__((always_inline)) {
-    uint32_t mine = 0;
+  const int own = wave * LW + RS * (lane / CH);  // this lane's first row of a step
+  auto look_up = [&](int k0, Part& p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LW; ++i)
+      p.page[i] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + own + i, lo), end - 1))];
+  };
+  auto load = [&](int k0, Part& p) __attribute__((always_inline)) {
+    p.mine = 0;
     int64_t at[LW];
 #pragma unroll
-    for (int i = 0; i < LW; ++i) at[i] = 0;  // a key without a place reads the pool's first row and is masked
+    for (int i = 0; i < LW; ++i) {
+      const int key = k0 + own + i;
+      const int64_t o = spk_paged::offset_in(a.c, p.page[i], key);
+      const bool there = key >= lo && key < end && o >= 0;
+      at[i] = there ? o : 0;  // a key without a place reads the pool's first row and is masked
+      const unsigned long long b = __ballot(there);
 #pragma unroll
-    for (int j = 0; j < RPW; ++j) {
-      const int first = wave * LW + RS * j;
-      const bool here = lane / CH == j;
-      if (grouped && k0 + first >= lo && k0 + first + LW <= end) {
-        const int64_t o = spk_paged::offset_in(a.c, page[j][0], k0 + first);
-        if (o >= 0) {
-          mine |= ((1u << LW) - 1) << first;
-#pragma unroll
-          for (int i = 0; i < LW; ++i) at[i] = here ? o + i * a.c.token_stride : at[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < LW; ++i) {
-          const int key = k0 + first + i;
-          const int64_t o = key >= lo && key < end ? spk_paged::offset_in(a.c, page[j][i], key) : -1;
-          mine |= o >= 0 ? 1u << (first + i) : 0u;
-          at[i] = here && o >= 0 ? o : at[i];
-        }
-      }
+      for (int j = 0; j < RPW; ++j) p.mine |= (uint32_t)(b >> (CH * j) & 1) << (wave * LW + i + RS * j);
     }
+    look_up(k0 + 64, p);
 #pragma unroll
     for (int i = 0; i < LW; ++i) {
-      const int first = wave * LW + i;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kbase + at[i]),
-                                       (__attribute__((address_space(3))) void*)&ks[first * 65], 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vbase + at[i]),
-                                       (__attribute__((address_space(3))) void*)&vs[first * 66], 16, 0, 0);
+      p.k[i] = load_once(kbase + (at[i] + 8 * (lane % CH)));
+      p.v[i] = load_once(vbase + (at[i] + 8 * (lane % CH)));
     }
-    if (lane == 0) there[stage][wave] = mine;
-    look_up(k0 + 32);
   };
   floatx4 acc[DT];
 #pragma unroll
@@ -890,36 +864,43 @@ __global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
   const int vrow = 4 * g + (ln >> 2);                     // of the transposing load
   const int vread = (vrow % RS) * 132 + (vrow / RS) * 2 * CH + (ln & 3);  // in 8-byte pieces, + 4 t
 
-  auto step = [&](int k0, const uint4* ks, const uint4* vs, int stage, uint4* ks_next, uint4* vs_next)
-                  __attribute__((always_inline)) {
-    // this step's loads are older than those of the two steps after it; with
-    // the barrier every wave's have arrived, and every wave has done with the
-    // step before, whose place the next loads take
-    if constexpr (LW == 4)
-      asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)" ::: "memory");
-    else if constexpr (LW == 2)
-      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+  auto step = [&](int k0, int buf, Part& p) __attribute__((always_inline)) {
+    uint4* ks = kss[buf];
+    uint4* vs = vss[buf];
+#pragma unroll
+    for (int i = 0; i < LW; ++i) {
+      ks[(wave * LW + i) * 65 + lane] = p.k[i];
+      vs[(wave * LW + i) * 66 + lane] = p.v[i];
+    }
+    if (lane == 0) there[buf][wave] = p.mine;
+    load(k0 + 64, p);
+    // every wave's part is there, and every wave has done with the step before
+    // the last, whose place this one's took
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    load(k0 + 96, ks_next, vs_next, (stage + 3) & 3);
-    if (idle) return;
-    const uint4 four = *reinterpret_cast<const uint4*>(&there[stage][0]);
+    if (idle || k0 >= end) return;
+    const uint4 four = *reinterpret_cast<const uint4*>(&there[buf][0]);
     const uint32_t has = __builtin_amdgcn_readfirstlane(four.x | four.y | four.z | four.w);
     const bool full = has == 0xffffffffu && k0 >= lo_all && k0 + 32 <= min(hi_all, end);
     floatx4 s0 = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
-    uint4 kf[2][DC];
+    constexpr int KA = DC < 4 ? DC : 4;  // pieces of the keys that are read ahead
+    uint4 kf[2][KA];
 #pragma unroll
-    for (int c = 0; c < DC; ++c) {
+    for (int c = 0; c < KA; ++c) {
       kf[0][c] = ks[kread + 4 * c];
       kf[1][c] = ks[kread + K16 + 4 * c];
     }
-    __builtin_amdgcn_sched_barrier(0);  // all reads under way before the first product waits for one
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
-      s0 = H::mfma16(kf[0][c], q[c], s0);
-      s1 = H::mfma16(kf[1][c], q[c], s1);
+      const uint4 u = kf[0][c % KA], v = kf[1][c % KA];
+      if (c + KA < DC) {
+        kf[0][c % KA] = ks[kread + 4 * (c + KA)];
+        kf[1][c % KA] = ks[kread + K16 + 4 * (c + KA)];
+      }
+      __builtin_amdgcn_sched_barrier(0);  // the reads go out before the products that wait for earlier ones
+      s0 = H::mfma16(u, q[c], s0);
+      s1 = H::mfma16(v, q[c], s1);
     }
     float w[8];
 #pragma unroll
@@ -966,42 +947,31 @@ __global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
       const uint2 u = transposed(at), v = transposed(at + 2 * K16);
       return make_uint4(u.x, u.y, v.x, v.y);
     };
-    if (full) {
-      constexpr int A = 4;  // tiles whose values are read ahead
-      uint4 f[A];
-#pragma unroll
-      for (int t = 0; t < A; ++t) f[t] = values(t);
-#pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const uint4 u = f[t % A];
-        if (t + A < DT) f[t % A] = values(t + A);
-        __builtin_amdgcn_sched_barrier(0);
-        acc[t] = H::mfma16(u, p0, acc[t]);
-        acc[t] = H::mfma16(u, p1, acc[t]);
-      }
-      return;
-    }
     // as in paged_rows_kernel: no value that is not finite meets a zero weight
-    const uint32_t mine = has >> (4 * g);
-    uint32_t keep[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t two = mine >> (16 * (i >> 1) + 2 * (i & 1));
-      keep[i] = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-    }
+    const uint32_t exists = has >> (4 * g);
     uint32_t odd = 0;  // bit i: of this lane's keys 2 i and 2 i + 1
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-      uint4 f = values(t);
+    auto clean = [&](uint4& f) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t u = (&f.x)[i] & keep[i];
+        const uint32_t two = exists >> (16 * (i >> 1) + 2 * (i & 1));
+        const uint32_t u = (&f.x)[i] & ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
         if (H::odd(u)) odd |= 1u << i;
         (&f.x)[i] = H::finite(u);
       }
-      acc[t] = H::mfma16(f, p0, acc[t]);
-      acc[t] = H::mfma16(f, p1, acc[t]);
+    };
+    constexpr int A = 4;  // tiles whose values are read ahead
+    uint4 f[A];
+#pragma unroll
+    for (int t = 0; t < A; ++t) f[t] = values(t);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      uint4 u = f[t % A];
+      if (t + A < DT) f[t % A] = values(t + A);
+      if (!full) clean(u);
+      acc[t] = H::mfma16(u, p0, acc[t]);
+      acc[t] = H::mfma16(u, p1, acc[t]);
     }
+    if (full) return;
     uint32_t odd_keys = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1036,25 +1006,17 @@ __global__ __launch_bounds__(256) void paged_mid_kernel(Attn a) {
     }
   };
   if (begin < end) {
-    look_up(begin);
-    load(begin, ka, va, 0);
-    load(begin + 32, kb, vb, 1);
-    load(begin + 64, kc, vc, 2);
-    // the queries have arrived: from here on only loads into LDS are under way,
-    // and a wait for one step's need not be a wait for all
-#pragma unroll
-    for (int c = 0; c < DC; ++c) asm volatile("" : "+v"(q[c].x), "+v"(q[c].y), "+v"(q[c].z), "+v"(q[c].w));
-    for (int k0 = begin;;) {
-      step(k0, ka, va, 0, kd, vd);
-      if ((k0 += 32) >= end) break;
-      step(k0, kb, vb, 1, ka, va);
-      if ((k0 += 32) >= end) break;
-      step(k0, kc, vc, 2, kb, vb);
-      if ((k0 += 32) >= end) break;
-      step(k0, kd, vd, 3, kc, vc);
-      if ((k0 += 32) >= end) break;
+    Part pa, pb;
+    look_up(begin, pa);
+    look_up(begin + 32, pb);
+    load(begin, pa);
+    load(begin + 32, pb);
+    // the second step may lie past the end and is empty then: with a way out
+    // between the two, the wait for the older part would be one for both
+    for (int k0 = begin; k0 < end; k0 += 64) {
+      step(k0, 0, pa);
+      step(k0 + 32, 1, pb);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
   }
 
   l += spk::lane_xor16(l);
@@ -1544,6 +1506,9 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
         p.page_stride < 0 || p.page_stride % 8)
       return spk::fail(SPK_ERR_ALIGN, "%s: the cache and its strides (page %lld token %lld head %lld) must be 16-byte aligned",
                        who, (long long)p.page_stride, (long long)p.token_stride, (long long)p.head_stride);
+    if (p.page_stride > UINT32_MAX || p.token_stride > UINT32_MAX)
+      return spk::fail(SPK_ERR_SHAPE, "%s: page_stride %lld, token_stride %lld (below 2^32)", who,
+                       (long long)p.page_stride, (long long)p.token_stride);
     if (p.table_stride < p.max_pages && p.num_seqs > 1)
       return spk::fail(SPK_ERR_SHAPE, "%s: table_stride %lld < max_pages %d", who, (long long)p.table_stride, p.max_pages);
   }
@@ -1551,8 +1516,8 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
   c->cu = p.cu_seqlens;
   c->ctx = p.context_lens;
   c->table_stride = p.table_stride;
-  c->page_stride = p.page_stride;
-  c->token_stride = p.token_stride;
+  c->page_stride = (uint32_t)p.page_stride;
+  c->token_stride = (uint32_t)p.token_stride;
   c->head_stride = p.head_stride;
   c->num_seqs = p.num_seqs;
   c->total_tokens = p.total_tokens;
@@ -1586,11 +1551,11 @@ Plan plan_of(const SpkPagedAttnArgs& p) {
   const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
 
   // sequences of few rows: all of them, unless the one there is has many.  As
-  // many workgroups as the chip holds at once (2 to a CU; 4 with heads of 64,
-  // 1 where 64 rows' keys of 256 dimensions fill the LDS), more only where the
-  // pieces alone are more, and no more than ranges of 128 keys.
+  // many workgroups as the chip holds at once (2 to a CU; 4 with heads of 64),
+  // more only where the pieces alone are more, and no more than ranges of 128
+  // keys.
   const int64_t pieces = any_many && c.num_seqs == 1 ? 0 : (all / r.share_rows + c.num_seqs) * c.num_kv_heads;
-  const int64_t slots = c.head_dim == 64 ? 1024 : c.head_dim == 256 && r.share_rows == 64 ? 256 : 512;
+  const int64_t slots = c.head_dim == 64 ? 1024 : 512;
   r.shares = (int)std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)),
                                     INT32_MAX);
 

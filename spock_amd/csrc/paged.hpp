@@ -14,9 +14,10 @@
 
 namespace spk_paged {
 
-// p / d for 0 <= p < 2^31 as one 64-bit product and a shift: with
-// 2^(s-1) < d <= 2^s and mul = floor(2^(31+s) / d) + 1 the product is at most
-// p (d / 2^(31+s)) < 1 / d too large, which never reaches the next integer.
+// p / d for 0 <= p < 2^31 as the high half of a 32-bit product and a shift:
+// with 2^(s-1) < d <= 2^s and mul = floor(2^(31+s) / d) + 1 the product p mul /
+// 2^(31+s) is at most p / 2^(31+s) < 1 / d too large, which never reaches the
+// next integer.
 struct PageDiv {
   uint32_t mul, shift;
 };
@@ -24,17 +25,18 @@ struct PageDiv {
 SPK_HD PageDiv page_div(uint32_t d) {
   uint32_t s = 0;
   while ((uint64_t(1) << s) < d) ++s;
-  return {(uint32_t)((uint64_t(1) << (31 + s)) / d + 1), 31 + s};
+  return {(uint32_t)((uint64_t(1) << (31 + s)) / d + 1), s};
 }
 
-SPK_HD uint32_t divide(PageDiv v, uint32_t p) { return (uint32_t)(((uint64_t)p * v.mul) >> v.shift); }
+SPK_HD uint32_t divide(PageDiv v, uint32_t p) { return (uint32_t)(((uint64_t)(2 * p) * v.mul) >> 32) >> v.shift; }
 
 struct Cache {
   const int32_t* table;  // [num_seqs][table_stride]
   const int32_t* cu;     // [num_seqs + 1]
   const int32_t* ctx;    // [num_seqs]
   int64_t table_stride;
-  int64_t page_stride, token_stride, head_stride;  // elements
+  int64_t head_stride;                  // elements, as all strides
+  uint32_t page_stride, token_stride;
   int32_t num_seqs, total_tokens, page_size, num_pages, max_pages;
   PageDiv div;
 };
@@ -61,7 +63,7 @@ SPK_HD Seq seq_at(const Cache& c, int32_t s) { return make_seq(c, c.cu[s], c.cu[
 SPK_HD int64_t offset_in(const Cache& c, int32_t page, int32_t pos) {
   if ((uint32_t)page >= (uint32_t)c.num_pages) return -1;
   const int32_t at = pos - (int32_t)(divide(c.div, (uint32_t)pos) * (uint32_t)c.page_size);
-  return (int64_t)page * c.page_stride + (int64_t)at * c.token_stride;
+  return (int64_t)((uint64_t)(uint32_t)page * c.page_stride + (uint64_t)(uint32_t)at * c.token_stride);
 }
 
 SPK_HD int64_t offset_of(const Cache& c, int32_t s, int32_t pos) {

@@ -21,8 +21,8 @@ int first_wrong_quotient(uint32_t d, const uint32_t* p, int n) {
 // the slots of every position of every sequence: how many lie outside a pool of `elements`, how many have a page
 void walk(const int32_t* table, long stride, const int32_t* cu, const int32_t* ctx, int seqs, int total, int page_size,
           int pages, int max_pages, long page_stride, long token_stride, long elements, long row, long* out) {
-  Cache c{table, cu, ctx, stride, page_stride, token_stride, 0, seqs, total, page_size, pages, max_pages,
-          page_div(page_size)};
+  Cache c{table, cu, ctx, stride, 0, (uint32_t)page_stride, (uint32_t)token_stride, seqs, total, page_size, pages,
+          max_pages, page_div(page_size)};
   out[0] = out[1] = out[2] = out[3] = 0;
   for (int s = 0; s < seqs; ++s) {
     const Seq q = seq_at(c, s);
@@ -109,7 +109,7 @@ BAD_CACHE = [(dict(dtype=0), -5), (dict(dtype=3), -5), (dict(head_dim=96), -2), 
              (dict(total_tokens=-1), -2), (dict(max_pages=2 ** 27), -2), (dict(k_cache=None), -1),
              (dict(v_cache=None), -1), (dict(block_table=None), -1), (dict(cu_seqlens=None), -1),
              (dict(context_lens=None), -1), (dict(k_cache=264), -4), (dict(token_stride=100), -4),
-             (dict(head_stride=-64), -4), (dict(page_stride=2047), -4), (dict(num_seqs=2, table_stride=3), -2)]
+             (dict(head_stride=-64), -4), (dict(page_stride=2047), -4), (dict(page_stride=2 ** 32), -2), (dict(token_stride=2 ** 32), -2), (dict(num_seqs=2, table_stride=3), -2)]
 
 
 @pytest.mark.parametrize("over,code", BAD_CACHE)
