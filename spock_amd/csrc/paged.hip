@@ -1046,42 +1046,42 @@ __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
 }
 
 // Many rows per sequence and KV head: a workgroup of 8 waves takes 256 of the
-// n * group rows, 32 to a wave, and walks the keys in tiles of KT that all
-// waves share in LDS, the next tile loading while this one is used.
+// n * group rows, 32 to a wave, and walks the keys in tiles of KT (16 KiB of
+// keys) that all waves share in LDS, the next tile loading while this one is
+// used.
 //
 // Scores are again S^T = K Q^T (32x32x16): a lane holds 16 keys' scores of one
 // row, and its weights are the B operand of O^T += V^T P^T as they are (lane
 // half h supplies keys 4h..4h+3 and 8+4h..+3 of each 16).  Both A operands are
-// one 16-byte LDS read of a lane.  K rows lie as in memory, their 16-byte
-// pieces exchanged by the row number so that 16 rows' pieces are in different
-// banks.  V is turned on the way in: a thread takes 8 keys' pieces of 4
-// dimensions and writes 4 dimensions' pieces of 8 keys, in fragment order; the
-// dimension of row m of output tile 4 u + e is 4 (m + 32 u) + e, which makes
-// these writes (and a lane's output) contiguous.
+// one 16-byte LDS read of a lane; a read feeds one product, and both pipes are
+// full at the same time, 32 clocks of a SIMD each.  K rows lie as in memory,
+// one load's 1 KiB (rows x, x + RS, ...) apart by 16 bytes more, so that rows
+// read side by side are in different banks.  V is turned on the way in: a
+// thread takes 2 dimensions of 8 keys and writes 8 keys of each, in fragment
+// order; the dimension of row m of output tile 2 u + e is 2 (m + 32 u) + e,
+// which makes these writes (and a lane's output) contiguous.
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   using H = Half<BF>;
-  constexpr int KT = D == 256 ? 64 : 128;  // keys of a tile
+  constexpr int KT = 8192 / D;             // keys of a tile
   constexpr int KS = D / 16;               // contraction steps of the scores
   constexpr int QR = D == 256 ? 14 : KS;   // of the queries' pieces in registers, the rest in LDS
   constexpr int DT = D / 32;               // output tiles
   constexpr int CH = D / 8;                // 16-byte pieces of a row
-  constexpr int RPW = 64 / CH;             // rows of K in one wave-wide load
-  constexpr int KL = KT / 8 / RPW;         // such loads of a wave per tile
+  constexpr int RPW = 64 / CH;             // rows of K in one wave-wide load, of which a wave has two
   constexpr int RS = 32 / RPW;             // distance of its rows: load x of 32 keys holds rows x, x + RS, ...
-  constexpr int LG = D / 4;                // lanes that cover a row of V (8 bytes each)
-  constexpr int GW = 64 / LG;              // groups of 8 keys of a wave
-  constexpr int VW = KT / 8 / GW;          // waves that load V
-  constexpr int U = KT / 64;               // lookups of a lane per tile
+  constexpr int LG = D / 2;                // threads that cover a row of V
+  constexpr int U = KT > 64 ? 2 : 1;       // lookups of a lane per tile
   // two tiles, as separate arrays: a load into one is then known not to touch the other
-  __shared__ __align__(16) uint4 k0s[KT * CH / 64 * 65], k1s[KT * CH / 64 * 65], v0s[KT * CH], v1s[KT * CH];
+  __shared__ __align__(16) uint4 k0s[16 * 65], k1s[16 * 65], v0s[1024], v1s[1024];
   __shared__ __align__(16) uint4 qs[KS > QR ? (KS - QR) * 512 : 1];
   __shared__ uint32_t odd_of[3][KT / 32];  // keys of a tile with values that are not finite (tile number % 3)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.y, split = blockIdx.x;
   int seq, tile;
-  if (!find_tile(a, 256, blockIdx.z, lane, &seq, &tile)) return;
+  // the last tiles, which see the most keys, first
+  if (!find_tile(a, 256, gridDim.z - 1 - blockIdx.z, lane, &seq, &tile)) return;
   seq = __builtin_amdgcn_readfirstlane(seq);
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Seq sq = spk_paged::seq_at(a.c, seq);
@@ -1096,14 +1096,15 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   if (begin >= end && a.splits > 1) return;
 
   const int r = min(r0 + 32 * wave + ln, rows - 1);
-  const int ri = r / a.group, head = kvh * a.group + r - ri * a.group, token = sq.first + ri;
   int row_lo, row_hi, wave_lo, wave_hi, wave_lo_all, wave_hi_all;
-  spk_paged::visible(sq, ri, a.window, &row_lo, &row_hi);
+  spk_paged::visible(sq, r / a.group, a.window, &row_lo, &row_hi);
   spk_paged::visible(sq, min(r0 + 32 * wave, rows - 1) / a.group, a.window, &wave_lo, &wave_hi_all);
   spk_paged::visible(sq, min(r0 + 32 * wave + 31, rows - 1) / a.group, a.window, &wave_lo_all, &wave_hi);
+  wave_hi = min(wave_hi, end);
   uint4 q[QR];
   {
-    const uint16_t* src = a.q + token * a.qt + head * a.qh + 8 * h;
+    const int i = r / a.group;
+    const uint16_t* src = a.q + (sq.first + i) * a.qt + (kvh * a.group + r - i * a.group) * a.qh + 8 * h;
 #pragma unroll
     for (int c = 0; c < QR; ++c) q[c] = *reinterpret_cast<const uint4*>(src + 16 * c);
 #pragma unroll
@@ -1114,22 +1115,30 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-  float m = -INFINITY, base = 0.0f, l = 0.0f;
+  float m = -INFINITY, shift = H::kShift, l = 0.0f;  // shift: less the maximum that the weights are relative to
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
   const uint16_t* kbase = a.k + kvh * a.c.head_stride;
   const uint16_t* vbase = a.v + kvh * a.c.head_stride;
 
-  // key k0 + 64 u + lane of the tile that is loaded next
+  // Key k0 + 64 u + lane (32 keys: lane % 32) of the tile that is loaded next; its
+  // page id was asked for a tile earlier.
+  const int klane = KT == 32 ? ln : lane;
+  int page[U];
   int64_t off[U];
   unsigned long long valid[U];
+  auto ask = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      page[u] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + 64 * u + klane, lo), end - 1))];
+  };
   auto look_up = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int key = k0 + 64 * u + lane;
-      off[u] = -1;
-      if (key >= lo && key < end) off[u] = spk_paged::offset_in(a.c, table[spk_paged::divide(a.c.div, (uint32_t)key)], key);
-      valid[u] = __ballot(off[u] >= 0);
-      if (off[u] < 0) off[u] = 0;
+      const int key = k0 + 64 * u + klane;
+      off[u] = spk_paged::offset_in(a.c, page[u], key);
+      const bool there = key >= lo && key < end && off[u] >= 0;
+      valid[u] = __ballot(there);
+      off[u] = there ? off[u] : 0;
     }
   };
   auto offset = [&](int kl) -> int64_t {  // of key kl of the tile, from its lane
@@ -1141,36 +1150,34 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
     return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)off[0], kl) |
            (int64_t)__builtin_amdgcn_readlane((int)(off[0] >> 32), kl) << 32;
   };
-  uint2 vr[8];
-  const int vg = GW == 1 ? wave : wave * GW + lane / LG, dc = lane % LG;  // V: group of 8 keys, piece of 4 dimensions
   auto load_k = [&](uint4* ks) {
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      const int x = wave * KL + i;
-      const int row = x % RS + 32 * (x / RS);
+    for (int i = 0; i < 2; ++i) {
+      const int x = wave * 2 + i, row = x % RS + 32 * (x / RS);
       int64_t at;
       if constexpr (RPW == 2)
         at = h ? scalar_offset(row + RS) : scalar_offset(row);
       else
         at = offset(row + RS * (lane / CH));
-      const uint16_t* src = kbase + at + 8 * (lane % CH);
+      const uint16_t* src = kbase + (at + 8 * (lane % CH));
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                        (__attribute__((address_space(3))) void*)&ks[x * 65], 16, 0, 0);
     }
   };
   const int kread = (ln % RS) * 65 + (ln / RS) * CH + h;  // of this lane's row and half in the 32 keys' loads
+  // V: this thread's group of 8 keys, and its piece of 2 dimensions
+  const int vg = LG >= 64 ? wave / (LG / 64) : tid / LG, dc = tid % LG;
+  uint32_t vr[8];
   auto v_key = [&](int kk) { return 16 * (vg >> 1) + 8 * (kk >> 2) + 4 * (vg & 1) + (kk & 3); };
   auto load_v = [&]() {
-    if (VW == 8 || wave < VW) {
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        int64_t at;
-        if constexpr (GW == 1)
-          at = scalar_offset(v_key(kk));
-        else
-          at = offset(v_key(kk));
-        vr[kk] = *reinterpret_cast<const uint2*>(vbase + at + 4 * dc);
-      }
+    for (int kk = 0; kk < 8; ++kk) {
+      int64_t at;
+      if constexpr (LG >= 64)
+        at = scalar_offset(v_key(kk));
+      else
+        at = offset(v_key(kk));
+      vr[kk] = *reinterpret_cast<const uint32_t*>(vbase + (at + 2 * dc));
     }
   };
   // Some row of the workgroup does not see the whole tile at k0.  Then a value
@@ -1183,16 +1190,15 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
     return !all;
   };
   auto store_v = [&](uint4* vs, int k0, int third) {
-    if (VW < 8 && wave >= VW) return;
     if (partial(k0)) {
       uint32_t odd = 0;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         const int kl = v_key(kk);
         const bool has = (U == 2 && (kl & 64) ? valid[U - 1] : valid[0]) >> (kl & 63) & 1ull;
-        if (!has) vr[kk] = make_uint2(0, 0);
-        if (H::odd(vr[kk].x) || H::odd(vr[kk].y)) odd |= 1u << kk;
-        vr[kk] = make_uint2(H::finite(vr[kk].x), H::finite(vr[kk].y));
+        if (!has) vr[kk] = 0;
+        if (H::odd(vr[kk])) odd |= 1u << kk;
+        vr[kk] = H::finite(vr[kk]);
       }
       while (odd) {
         const int kl = v_key(__ffs(odd) - 1);
@@ -1201,38 +1207,36 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
       uint4 f;
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        (&f.x)[w] = __builtin_amdgcn_perm((&vr[2 * w + 1].x)[e >> 1], (&vr[2 * w].x)[e >> 1],
-                                          e & 1 ? 0x07060302u : 0x05040100u);
-      const int t = D >= 128 ? e + 4 * (dc / 32) : e >> 1, row = D >= 128 ? dc % 32 : dc + 16 * (e & 1);
-      vs[((vg >> 1) * DT + t) * 64 + row + 32 * (vg & 1)] = f;
+        (&f.x)[w] = __builtin_amdgcn_perm(vr[2 * w + 1], vr[2 * w], e & 1 ? 0x07060302u : 0x05040100u);
+      vs[((vg >> 1) * DT + e + 2 * (dc / 32)) * 64 + dc % 32 + 32 * (vg & 1)] = f;
     }
   };
-  auto dim_of = [&](int t, int row) { return D >= 128 ? 4 * (row + 32 * (t >> 2)) + (t & 3) : 4 * (row & 15) + 2 * t + (row >> 4); };
+  auto dim_of = [&](int t, int row) { return 2 * (row + 32 * (t >> 1)) + (t & 1); };
 
   if (tid < 3 * (KT / 32)) odd_of[tid / (KT / 32)][tid % (KT / 32)] = 0;
   int third = 0;
-  unsigned long long now[U];
-  bool part = true;
   auto step = [&](int k0, uint4* ks, uint4* vs, uint4* ks_next, uint4* vs_next) __attribute__((always_inline)) {
     const bool more = k0 + KT < end;
     const int after = third == 2 ? 0 : third + 1;
-    part = partial(k0);
+    const bool part = partial(k0);
+    unsigned long long now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = valid[u];
     if (tid < KT / 32) odd_of[after == 2 ? 0 : after + 1][tid] = 0;  // the tile before this one's
     if (more) {
       look_up(k0 + KT);
+      ask(k0 + 2 * KT);
       load_k(ks_next);
+      load_v();
     }
 #pragma unroll 1
     for (int j = 0; j < KT / 32; ++j) {
       const int kj = k0 + 32 * j;
-      if (j == KT / 32 - 1 && more) load_v();
-      if (kj >= min(wave_hi, end) || kj + 32 <= wave_lo) continue;
+      if (kj >= wave_hi || kj + 32 <= wave_lo) continue;
       const uint32_t has = (uint32_t)((U == 2 && j > 1 ? now[U - 1] : now[0]) >> (32 * (j & 1)));
       const bool full = has == 0xffffffffu && kj >= wave_lo_all && kj + 32 <= wave_hi_all;
       floatx16 s;
@@ -1241,8 +1245,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
 #pragma unroll
       for (int c = 0; c < KS; ++c) s = H::mfma32(ks[j * RS * 65 + kread + 2 * c], c < QR ? q[c] : qs[(c - QR) * 512 + tid], s);
       if (!full) {
-        uint32_t see = seen(has, kj, row_lo, row_hi);
-        see >>= 4 * h;  // a lane's keys at constant places
+        const uint32_t see = seen(has, kj, row_lo, row_hi) >> (4 * h);  // a lane's keys at constant places
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[i] : -INFINITY;
       }
@@ -1253,10 +1256,9 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       if (__any(top > m + kBehind)) {
         top = fmaxf(top, spk::lane_xor32(top));
         const float next = fmaxf(m, top);
-        const float nb = next == -INFINITY ? 0.0f : next;
-        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nb);
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next);
         m = next;
-        base = nb;
+        shift = H::kShift - (next == -INFINITY ? 0.0f : next);
         l *= f;
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[t] *= f;
@@ -1264,7 +1266,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       uint4 p[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[i] = exp2_fast(__builtin_fmaf(s[i], a.scale_log2, H::kShift - base));
+        s[i] = exp2_fast(__builtin_fmaf(s[i], a.scale_log2, shift));
         l += s[i];
       }
 #pragma unroll
@@ -1280,9 +1282,9 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
         while (odd) {
           const int kl = __ffs(odd) - 1;
           odd &= odd - 1;
-          const uint16_t* row = vbase + spk_paged::offset_of(a.c, seq, kj + kl);
-          const uint4 quad = kl & 16 ? p[1] : p[0];
-          uint32_t pair = kl & 8 ? (kl & 2 ? quad.w : quad.z) : (kl & 2 ? quad.y : quad.x);
+          const uint16_t* row = vbase + max(spk_paged::offset_of(a.c, seq, kj + kl), (int64_t)0);
+          uint32_t pair = kl & 16 ? (kl & 8 ? (kl & 2 ? p[1].w : p[1].z) : (kl & 2 ? p[1].y : p[1].x))
+                                  : (kl & 8 ? (kl & 2 ? p[0].w : p[0].z) : (kl & 2 ? p[0].y : p[0].x));
           pair = __shfl((int)pair, ln + 32 * ((kl >> 2) & 1));
           const float weight = H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
           if (kj + kl >= row_lo && kj + kl < row_hi) {
@@ -1298,15 +1300,15 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
         }
       }
     }
-    if (more) {
-      store_v(vs_next, k0 + KT, after);
-    }
+    if (more) store_v(vs_next, k0 + KT, after);
     third = after;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the keys' loads into LDS
     __syncthreads();
   };
   if (begin < end) {
+    ask(begin);
     look_up(begin);
+    ask(begin + KT);
     load_k(k0s);
     load_v();
     __syncthreads();
@@ -1322,36 +1324,33 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
 
   l += spk::lane_xor32(l);
   if (r0 + 32 * wave + ln >= rows) return;
+  const int ri = r / a.group, head = kvh * a.group + r - ri * a.group, token = sq.first + ri;
   const int64_t at = (int64_t)token * a.heads + head;
-  if (a.splits > 1) {
-    float* part = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
-    if (h == 0) {
+  float* part = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
+  if (h == 0) {
+    if (a.splits > 1) {
       part[0] = m;
       part[1] = l;
+    } else if (a.lse) {
+      a.lse[at] = l == 0.0f ? -INFINITY : (m - H::kShift + __builtin_amdgcn_logf(l)) * kLn2;
     }
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) part[2 + dim_of(t, 8 * (i >> 2) + 4 * h + (i & 3))] = acc[t][i];
-    return;
   }
-  if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m - H::kShift + __builtin_amdgcn_logf(l)) * kLn2;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if constexpr (D >= 128) {
+  const float inv = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int u = 0; u < DT / 4; ++u)
+  for (int u = 0; u < DT / 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float o[4] = {acc[4 * u][i] * inv, acc[4 * u + 1][i] * inv, acc[4 * u + 2][i] * inv, acc[4 * u + 3][i] * inv};
-        store_out<BF, 4>(a, token, head, dim_of(4 * u, 8 * (i >> 2) + 4 * h + (i & 3)), o);
+    for (int i = 0; i < 4; ++i) {
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = acc[2 * u + (j & 1)][4 * i + (j >> 1)] * inv;
+      const int d = dim_of(2 * u, 8 * i + 4 * h);
+      if (a.splits > 1) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) *reinterpret_cast<float2*>(part + 2 + d + j) = make_float2(o[j], o[j + 1]);
+      } else {
+        store_out<BF, 8>(a, token, head, d, o);
       }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {  // rows m and m + 16 hold dimensions 4 (m % 16) + 2 t + 0 and 1
-      const float o[4] = {acc[0][i] * inv, acc[0][i + 8] * inv, acc[1][i] * inv, acc[1][i + 8] * inv};
-      store_out<BF, 4>(a, token, head, dim_of(0, 8 * (i >> 2) + 4 * h + (i & 3)), o);
     }
-  }
 }
 
 // Joins the key ranges of a row: 256 / LANES rows to a workgroup, for many rows
