@@ -216,6 +216,7 @@ struct Attn {
   int32_t shares, share_rows;  // few rows: workgroups, and rows of one
   int32_t alone;               // few rows: no ranges
   int32_t splits, chunk;       // many rows: key ranges of a tile and the least keys of one
+  int32_t join_few;            // the join has [num_seqs][kv_heads][64] rows, for sequences of few; else [total_tokens][heads]
   float scale_log2;  // scale * log2(e)
 };
 
@@ -1045,19 +1046,39 @@ __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   }
 }
 
+// use(c, read(c)) for c below N, with the reads AHEAD of their use, or as the
+// compiler has them.
+template <int N, int AHEAD, typename Read, typename Use>
+__device__ __forceinline__ void in_turn(Read read, Use use) {
+  if constexpr (AHEAD == 0) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) use(c, read(c));
+  } else {
+    uint4 f[N];
+#pragma unroll
+    for (int c = 0; c < (AHEAD < N ? AHEAD : N); ++c) f[c] = read(c);
+    __builtin_amdgcn_sched_barrier(6);  // only scalar and vector arithmetic may move past it
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (c + AHEAD < N) f[c + AHEAD] = read(c + AHEAD);
+      use(c, f[c]);
+      __builtin_amdgcn_sched_barrier(6);
+    }
+  }
+}
+
 // Many rows per sequence and KV head: a workgroup of 8 waves takes 256 of the
 // n * group rows, 32 to a wave, and walks the keys in tiles of KT (16 KiB of
-// keys) that all waves share in LDS, the next tile loading while this one is
-// used.
+// keys) that all waves share in LDS.  Loads go straight into LDS, the keys' two
+// tiles ahead and the values' three: a tile takes less time than a load.
 //
 // Scores are again S^T = K Q^T (32x32x16): a lane holds 16 keys' scores of one
 // row, and its weights are the B operand of O^T += V^T P^T as they are (lane
 // half h supplies keys 4h..4h+3 and 8+4h..+3 of each 16).  Both A operands are
-// one 16-byte LDS read of a lane; a read feeds one product, and both pipes are
-// full at the same time, 32 clocks of a SIMD each.  K rows lie as in memory,
-// one load's 1 KiB (rows x, x + RS, ...) apart by 16 bytes more, so that rows
-// read side by side are in different banks.  V is turned on the way in: a
-// thread takes 2 dimensions of 8 keys and writes 8 keys of each, in fragment
+// one 16-byte LDS read of a lane.  K rows lie as in memory, one load's 1 KiB
+// (rows x, x + RS, ...) apart by 16 bytes more, so that rows read side by side
+// are in different banks.  V is turned in LDS a tile before it is used: a
+// thread reads 2 dimensions of 8 keys and writes 8 keys of each, in fragment
 // order; the dimension of row m of output tile 2 u + e is 2 (m + 32 u) + e,
 // which makes these writes (and a lane's output) contiguous.
 template <int D, bool BF>
@@ -1072,8 +1093,13 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   constexpr int RS = 32 / RPW;             // distance of its rows: load x of 32 keys holds rows x, x + RS, ...
   constexpr int LG = D / 2;                // threads that cover a row of V
   constexpr int U = KT > 64 ? 2 : 1;       // lookups of a lane per tile
-  // two tiles, as separate arrays: a load into one is then known not to touch the other
-  __shared__ __align__(16) uint4 k0s[16 * 65], k1s[16 * 65], v0s[1024], v1s[1024];
+  // LDS reads ahead of the matrix instruction that uses them.  Heads of 256 have
+  // no registers left for it: 2 ahead spills and takes 356 us for 347, while with
+  // heads of 128, 4 ahead take 207 us for 217.
+  constexpr int AHEAD = D == 256 ? 0 : 4;
+  // keys, values as they come: three tiles, as separate arrays: a load into one is then known not to touch the others
+  __shared__ __align__(16) uint4 ka[16 * 65], kb[16 * 65], kc[16 * 65], ra[1024], rb[1024], rc[1024];
+  __shared__ __align__(16) uint4 vss[2 * 1024];  // values turned: two tiles
   __shared__ __align__(16) uint4 qs[KS > QR ? (KS - QR) * 512 : 1];
   __shared__ uint32_t odd_of[3][KT / 32];  // keys of a tile with values that are not finite (tile number % 3)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1117,16 +1143,15 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
   float m = -INFINITY, shift = H::kShift, l = 0.0f;  // shift: less the maximum that the weights are relative to
   const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
-  const uint16_t* kbase = a.k + kvh * a.c.head_stride;
   const uint16_t* vbase = a.v + kvh * a.c.head_stride;
 
-  // Key k0 + 64 u + lane (32 keys: lane % 32) of the tile that is loaded next; its
-  // page id was asked for a tile earlier.
+  // Key k0 + 64 u + lane (32 keys: lane % 32) of the tile whose values are loaded
+  // next; its page id was asked for a tile earlier.
   const int klane = KT == 32 ? ln : lane;
   int page[U];
   int64_t off[U];
   unsigned long long valid[U];
-  auto ask = [&](int k0) {
+  auto ask = [&](int k0, int (&page)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       page[u] = table[spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + 64 * u + klane, lo), end - 1))];
@@ -1138,64 +1163,58 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       off[u] = spk_paged::offset_in(a.c, page[u], key);
       const bool there = key >= lo && key < end && off[u] >= 0;
       valid[u] = __ballot(there);
-      off[u] = there ? off[u] : 0;
+      off[u] = there ? off[u] : 0;  // a key without a place reads the pool's first row and is masked
     }
   };
-  auto offset = [&](int kl) -> int64_t {  // of key kl of the tile, from its lane
-    int64_t o = off[0];
-    if constexpr (U == 2) o = kl & 64 ? off[1] : off[0];
-    return __shfl(o, kl & 63);
-  };
-  auto scalar_offset = [&](int kl) -> int64_t {  // the same for a key that the whole wave asks for
-    return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)off[0], kl) |
-           (int64_t)__builtin_amdgcn_readlane((int)(off[0] >> 32), kl) << 32;
-  };
-  auto load_k = [&](uint4* ks) {
+  // a wave's two loads of a tile, its rows at `off`, into `to`, loads `apart`
+  auto load = [&](const uint16_t* from, uint4* to, int apart) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int x = wave * 2 + i, row = x % RS + 32 * (x / RS);
       int64_t at;
-      if constexpr (RPW == 2)
-        at = h ? scalar_offset(row + RS) : scalar_offset(row);
-      else
-        at = offset(row + RS * (lane / CH));
-      const uint16_t* src = kbase + (at + 8 * (lane % CH));
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)&ks[x * 65], 16, 0, 0);
+      if constexpr (RPW == 2) {
+        const int64_t first = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)off[0], row) |
+                              (int64_t)__builtin_amdgcn_readlane((int)(off[0] >> 32), row) << 32;
+        const int64_t second = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)off[0], row + RS) |
+                               (int64_t)__builtin_amdgcn_readlane((int)(off[0] >> 32), row + RS) << 32;
+        at = h ? second : first;
+      } else {
+        const int kl = row + RS * (lane / CH);
+        int64_t o = off[0];
+        if constexpr (U == 2) o = row & 64 ? off[1] : off[0];
+        at = __shfl(o, kl & 63);
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (at + 8 * (lane % CH))),
+                                       (__attribute__((address_space(3))) void*)&to[x * apart], 16, 0, 0);
     }
   };
   const int kread = (ln % RS) * 65 + (ln / RS) * CH + h;  // of this lane's row and half in the 32 keys' loads
-  // V: this thread's group of 8 keys, and its piece of 2 dimensions
-  const int vg = LG >= 64 ? wave / (LG / 64) : tid / LG, dc = tid % LG;
-  uint32_t vr[8];
-  auto v_key = [&](int kk) { return 16 * (vg >> 1) + 8 * (kk >> 2) + 4 * (vg & 1) + (kk & 3); };
-  auto load_v = [&]() {
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      int64_t at;
-      if constexpr (LG >= 64)
-        at = scalar_offset(v_key(kk));
-      else
-        at = offset(v_key(kk));
-      vr[kk] = *reinterpret_cast<const uint32_t*>(vbase + (at + 2 * dc));
-    }
-  };
   // Some row of the workgroup does not see the whole tile at k0.  Then a value
   // that is not finite must not meet the zero weight of a row that does not
-  // see it: such elements are stored as zeros, and added row by row.
-  auto partial = [&](int k0) {
+  // see it: such elements are turned into zeros, and added row by row.
+  auto partial = [&](int k0, const unsigned long long (&exist)[U]) {
     bool all = k0 >= lo_all && k0 + KT <= min(hi_all, end);
 #pragma unroll
-    for (int u = 0; u < U; ++u) all = all && valid[u] == ~0ull;
+    for (int u = 0; u < U; ++u) all = all && exist[u] == ~0ull;
     return !all;
   };
-  auto store_v = [&](uint4* vs, int k0, int third) {
-    if (partial(k0)) {
+  // V: this thread's group of 8 keys, and its piece of 2 dimensions
+  const int vg = LG >= 64 ? wave / (LG / 64) : tid / LG, dc = tid % LG;
+  auto v_key = [&](int kk) { return 16 * (vg >> 1) + 8 * (kk >> 2) + 4 * (vg & 1) + (kk & 3); };
+  auto turn = [&](const uint4* raw, uint4* vs, bool part, const unsigned long long (&exist)[U], uint32_t* odd_keys)
+                  __attribute__((always_inline)) {
+    uint32_t vr[8];
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      const int kl = v_key(kk), x = kl % RS + RS * (kl / 32);
+      vr[kk] = reinterpret_cast<const uint32_t*>(raw)[(x * 64 + (kl % 32) / RS * CH) * 4 + dc];
+    }
+    if (part) {
       uint32_t odd = 0;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         const int kl = v_key(kk);
-        const bool has = (U == 2 && (kl & 64) ? valid[U - 1] : valid[0]) >> (kl & 63) & 1ull;
+        const bool has = (U == 2 && (kl & 64) ? exist[U - 1] : exist[0]) >> (kl & 63) & 1ull;
         if (!has) vr[kk] = 0;
         if (H::odd(vr[kk])) odd |= 1u << kk;
         vr[kk] = H::finite(vr[kk]);
@@ -1203,7 +1222,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       while (odd) {
         const int kl = v_key(__ffs(odd) - 1);
         odd &= odd - 1;
-        atomicOr(&odd_of[third][kl >> 5], 1u << (kl & 31));
+        atomicOr(&odd_keys[kl >> 5], 1u << (kl & 31));
       }
     }
 #pragma unroll
@@ -1218,32 +1237,36 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   auto dim_of = [&](int t, int row) { return 2 * (row + 32 * (t >> 1)) + (t & 1); };
 
   if (tid < 3 * (KT / 32)) odd_of[tid / (KT / 32)][tid % (KT / 32)] = 0;
-  int third = 0;
-  auto step = [&](int k0, uint4* ks, uint4* vs, uint4* ks_next, uint4* vs_next) __attribute__((always_inline)) {
-    const bool more = k0 + KT < end;
-    const int after = third == 2 ? 0 : third + 1;
-    const bool part = partial(k0);
-    unsigned long long now[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) now[u] = valid[u];
-    if (tid < KT / 32) odd_of[after == 2 ? 0 : after + 1][tid] = 0;  // the tile before this one's
-    if (more) {
-      look_up(k0 + KT);
-      ask(k0 + 2 * KT);
-      load_k(ks_next);
-      load_v();
-    }
+  // the keys that exist of this tile and the two after it
+  unsigned long long now[U], next[U], second[U];
+  auto meet = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // Tile number n at k0 (n % 3 = third, n % 2 = vs' half): loads the keys of tile
+  // n + 2 and the values of tile n + 3, uses tile n, turns the values of n + 1.
+  auto step = [&](int k0, int third, int parity, const uint4* ks, uint4* ks_load, const uint4* raw, uint4* raw_load)
+                  __attribute__((always_inline)) {
+    int asked[U];
+    ask(k0 + 4 * KT, asked);
+    load(a.k + kvh * a.c.head_stride, ks_load, 65);  // at the offsets that the step before found
+    look_up(k0 + 3 * KT);
+    load(vbase, raw_load, 64);
+    const uint4* vs = &vss[parity * 1024];
+    if (tid < KT / 32) odd_of[third == 0 ? 2 : third - 1][tid] = 0;  // the tile before this one's
+    const bool part = partial(k0, now);
 #pragma unroll 1
     for (int j = 0; j < KT / 32; ++j) {
       const int kj = k0 + 32 * j;
-      if (kj >= wave_hi || kj + 32 <= wave_lo) continue;
+      if (kj >= wave_hi || kj + 32 <= wave_lo) continue;  // also past the end
       const uint32_t has = (uint32_t)((U == 2 && j > 1 ? now[U - 1] : now[0]) >> (32 * (j & 1)));
       const bool full = has == 0xffffffffu && kj >= wave_lo_all && kj + 32 <= wave_hi_all;
       floatx16 s;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < KS; ++c) s = H::mfma32(ks[j * RS * 65 + kread + 2 * c], c < QR ? q[c] : qs[(c - QR) * 512 + tid], s);
+      in_turn<KS, AHEAD>([&](int c) { return ks[j * RS * 65 + kread + 2 * c]; },
+                         [&](int c, uint4 k) { s = H::mfma32(k, c < QR ? q[c] : qs[(c - QR) * 512 + tid], s); });
       if (!full) {
         const uint32_t see = seen(has, kj, row_lo, row_hi) >> (4 * h);  // a lane's keys at constant places
 #pragma unroll
@@ -1273,10 +1296,8 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       for (int i = 0; i < 2; ++i)
         p[i] = make_uint4(H::pack(s[8 * i], s[8 * i + 1]), H::pack(s[8 * i + 2], s[8 * i + 3]),
                           H::pack(s[8 * i + 4], s[8 * i + 5]), H::pack(s[8 * i + 6], s[8 * i + 7]));
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int t = 0; t < DT; ++t) acc[t] = H::mfma32(vs[((2 * j + i) * DT + t) * 64 + lane], p[i], acc[t]);
+      in_turn<2 * DT, AHEAD>([&](int c) { return vs[(2 * j * DT + c) * 64 + lane]; },
+                             [&](int c, uint4 v) { acc[c % DT] = H::mfma32(v, p[c / DT], acc[c % DT]); });
       if (part) {
         uint32_t odd = __builtin_amdgcn_readfirstlane(odd_of[third][j]);
         while (odd) {
@@ -1300,26 +1321,52 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
         }
       }
     }
-    if (more) store_v(vs_next, k0 + KT, after);
-    third = after;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the keys' loads into LDS
-    __syncthreads();
+    turn(raw, &vss[(parity ^ 1) * 1024], partial(k0 + KT, next), next, odd_of[third == 2 ? 0 : third + 1]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      now[u] = next[u];
+      next[u] = second[u];
+      second[u] = valid[u];
+    }
+    // all but this step's own four loads have arrived
+#pragma unroll
+    for (int u = 0; u < U; ++u) page[u] = asked[u];
+    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    meet();
   };
   if (begin < end) {
-    ask(begin);
+    const uint16_t* kbase = a.k + kvh * a.c.head_stride;
+    ask(begin, page);
     look_up(begin);
-    ask(begin + KT);
-    load_k(k0s);
-    load_v();
-    __syncthreads();
-    store_v(v0s, begin, 0);
+    ask(begin + KT, page);
+    load(kbase, ka, 65);
+    load(vbase, ra, 64);
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = valid[u];
+    look_up(begin + KT);
+    ask(begin + 2 * KT, page);
+    load(kbase, kb, 65);
+    load(vbase, rb, 64);
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = valid[u];
+    look_up(begin + 2 * KT);
+    ask(begin + 3 * KT, page);
+    load(vbase, rc, 64);
+#pragma unroll
+    for (int u = 0; u < U; ++u) second[u] = valid[u];
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int k0 = begin; k0 < end; k0 += 2 * KT) {
-      step(k0, k0s, v0s, k1s, v1s);
-      if (k0 + KT >= end) break;
-      step(k0 + KT, k1s, v1s, k0s, v0s);
+    meet();
+    turn(ra, vss, partial(begin, now), now, odd_of[0]);
+    meet();
+    // steps past the end are empty: with a way out between the steps, what is
+    // under way would not be known where they meet
+    int parity = 0;
+    for (int k0 = begin; k0 < end; k0 += 3 * KT, parity ^= 1) {
+      step(k0, 0, parity, ka, kc, rb, ra);
+      step(k0 + KT, 1, parity ^ 1, kb, ka, rc, rb);
+      step(k0 + 2 * KT, 2, parity, kc, kb, ra, rc);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
   }
 
   l += spk::lane_xor32(l);
@@ -1376,15 +1423,32 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
   };
-  const int64_t at = (int64_t)blockIdx.x * ROWS + mine;
-  const int token = (int)(at / a.heads), head = (int)(at - (int64_t)token * a.heads);
-  if (token >= a.c.total_tokens) return;
-  const int s = spk_paged::seq_of_token(a.c.cu, a.c.num_seqs, token, lane);
-  if (s >= a.c.num_seqs) return;
-  const Seq sq = spk_paged::seq_at(a.c, s);
-  if (token < sq.first || token >= sq.first + sq.n) return;
+  int64_t at = (int64_t)blockIdx.x * ROWS + mine;
+  int s, token, head, kvh, r;
+  Seq sq;
+  if (a.join_few) {
+    r = (int)(at & 63);
+    s = (int)((at >> 6) / a.kv_heads);
+    kvh = (int)(at >> 6) - s * a.kv_heads;
+    if (s >= a.c.num_seqs) return;
+    sq = spk_paged::seq_at(a.c, s);
+    if (r >= sq.n * a.group || sq.n * a.group >= a.many) return;
+    token = sq.first + r / a.group;
+    head = kvh * a.group + r % a.group;
+    at = (int64_t)token * a.heads + head;
+  } else {
+    token = (int)(at / a.heads);
+    head = (int)(at - (int64_t)token * a.heads);
+    if (token >= a.c.total_tokens) return;
+    s = spk_paged::seq_of_token(a.c.cu, a.c.num_seqs, token, lane);
+    if (s >= a.c.num_seqs) return;
+    sq = spk_paged::seq_at(a.c, s);
+    if (token < sq.first || token >= sq.first + sq.n) return;
+    kvh = head / a.group;
+    r = (token - sq.first) * a.group + head - kvh * a.group;
+  }
   // the ranges that the row's tile had
-  const int rows = sq.n * a.group, kvh = head / a.group, r = (token - sq.first) * a.group + head - kvh * a.group;
+  const int rows = sq.n * a.group;
   int n;
   int64_t step;
   const float* part;
@@ -1530,7 +1594,8 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
 // How a call's rows and keys are dealt to the kernels.
 struct Plan {
   int many, shares, share_rows, tiles, splits, chunk;
-  bool join;
+  bool join, join_few;
+  int64_t join_rows;
 };
 
 Plan plan_of(const SpkPagedAttnArgs& p) {
@@ -1553,19 +1618,32 @@ Plan plan_of(const SpkPagedAttnArgs& p) {
   // many workgroups as the chip holds at once (2 to a CU; 4 with heads of 64),
   // more only where the pieces alone are more, and no more than ranges of 128
   // keys.
-  const int64_t pieces = any_many && c.num_seqs == 1 ? 0 : (all / r.share_rows + c.num_seqs) * c.num_kv_heads;
+  // Next to many rows a sequence of few is one piece; else the bound may be low.
+  const int64_t pieces = !any_many ? (all / r.share_rows + c.num_seqs) * c.num_kv_heads
+                         : c.num_seqs > 1 ? std::min<int64_t>(c.num_seqs, all) * c.num_kv_heads : 0;
   const int64_t slots = c.head_dim == 64 ? 1024 : 512;
   r.shares = (int)std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)),
                                     INT32_MAX);
 
-  // sequences of many rows: a workgroup to a CU, ranges of at least 512 keys
-  r.tiles = any_many ? (int)std::min<int64_t>(all / 256 + std::min<int64_t>(c.num_seqs, all / 65 + 1), INT32_MAX) : 0;
+  // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
+  // the number of ranges that takes the fewest rounds of 256 workgroups times
+  // steps in each; a range's share of the join costs as much as some 4 steps
+  // (2048 tokens after 4096 in 64 workgroups: 347 us in 3 ranges, 322 in 4, where 4 fill the chip).
+  const int64_t seqs = std::min<int64_t>(c.num_seqs, all / 65 + 1);
+  r.tiles = any_many ? (int)std::min<int64_t>((all + 255 * seqs) / 256, INT32_MAX) : 0;
   const int64_t groups = std::max<int64_t>(1, (int64_t)r.tiles * c.num_kv_heads);
-  const int64_t ranges = std::max<int64_t>(1, 256 / groups);
-  const int64_t per = std::max<int64_t>(4, (steps + ranges - 1) / ranges);
+  int64_t per = steps, least = (groups + 255) / 256 * steps;
+  for (int64_t n = 2; n <= std::min<int64_t>(512 / groups + 1, steps / 4); ++n) {
+    const int64_t in = (steps + n - 1) / n, cost = (groups * n + 255) / 256 * (in + 4);
+    if (cost < least) per = in, least = cost;
+  }
   r.chunk = (int)(128 * per);
   r.splits = r.tiles ? (int)((steps + per - 1) / per) : 1;
   r.join = r.splits > 1 || (r.shares && steps > 1);
+  // rows to join: all tokens', or of each sequence those that few can be
+  const int64_t every = (int64_t)c.total_tokens * p.num_q_heads, of_few = (int64_t)c.num_seqs * c.num_kv_heads * 64;
+  r.join_few = any_many && r.splits == 1 && of_few < every;
+  r.join_rows = r.join_few ? of_few : every;
   return r;
 }
 
@@ -1606,7 +1684,7 @@ void launch_attn(const Attn& a, const Plan& r, hipStream_t s) {
   if (r.tiles)
     hipLaunchKernelGGL((paged_tiles_kernel<D, BF>), dim3(r.splits, a.kv_heads, r.tiles), dim3(512), 0, s, a);
   if (!r.join) return;
-  const int64_t rows = (int64_t)a.c.total_tokens * a.heads;
+  const int64_t rows = r.join_rows;
   if (rows >= 1024)
     hipLaunchKernelGGL((paged_join_kernel<D, 64, BF>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
   else
@@ -1739,6 +1817,7 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
   a.alone = !r.join;
   a.splits = r.splits;
   a.chunk = r.chunk;
+  a.join_few = r.join_few;
   const float scale = p->scale != 0.0f ? p->scale : 1.0f / std::sqrt((float)c.head_dim);
   a.scale_log2 = scale * 1.44269504088896341f;
   hipStream_t s = spk::to_hip(stream);
