@@ -284,6 +284,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += __uint_as_float(spk::row_ror_u<1>(__float_as_uint(v)));
   return v;
 }
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, (int)spk::lane_xor32_u((uint32_t)v));
+  v = max(v, (int)spk::lane_xor16_u((uint32_t)v));
+  v = max(v, (int)spk::row_ror_u<8>((uint32_t)v));
+  v = max(v, (int)spk::row_ror_u<4>((uint32_t)v));
+  v = max(v, (int)spk::row_ror_u<2>((uint32_t)v));
+  return max(v, (int)spk::row_ror_u<1>((uint32_t)v));
+}
 __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
@@ -400,26 +408,83 @@ __device__ __forceinline__ uint32_t seen(uint32_t has, int k0, int lo, int hi) {
   return has & (0xffffffffu << max(first, 0)) & (0xffffffffu >> (32 - min(last, 32)));
 }
 
-// Tile `at` of the row tiles of the sequences of many rows (n * group rows of a
-// sequence, `rows` to a tile, sequences in order): its sequence and its index
-// there.  false past the last.
-__device__ __forceinline__ bool find_tile(const Attn& a, int rows, int at, int lane, int* seq, int* tile) {
-  for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64) {
-    int mine = 0;
-    if (s0 + lane < a.c.num_seqs) {
-      const int n = spk_paged::make_seq(a.c, a.c.cu[s0 + lane], a.c.cu[s0 + lane + 1], 0).n * a.group;
-      if (n >= a.many) mine = (n + rows - 1) / rows;
+// Tile `at` of the tiles of 256 of the n * group rows of the sequences of many:
+// its sequence and its index there.  false past the last of them.  Those that
+// see the most keys come first, to within 128 keys, so that the last that
+// workgroups take are short (six prompts of 16 heads over 4: TILES us, SEQUENCE
+// us with the last sequence's last tile first).
+__device__ __forceinline__ bool find_tile(const Attn& a, int at, int last, int lane, int* seq, int* tile) {
+  constexpr int N = 4;  // sequences of a lane
+  if (a.c.num_seqs > 64 * N) {  // more than are looked at together: by sequence, the last tiles first
+    at = last - at;
+    for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64) {
+      int mine = 0;
+      if (s0 + lane < a.c.num_seqs) {
+        const int n = spk_paged::make_seq(a.c, a.c.cu[s0 + lane], a.c.cu[s0 + lane + 1], 0).n * a.group;
+        if (n >= a.many) mine = (n + 255) / 256;
+      }
+      const int sum = wave_scan(mine), total = __builtin_amdgcn_readlane(sum, 63);
+      if (at < total) {
+        const int l = __popcll(__ballot(sum <= at));
+        *seq = s0 + l;
+        *tile = at - __builtin_amdgcn_readlane(sum - mine, l);
+        return true;
+      }
+      at -= total;
     }
-    const int sum = wave_scan(mine), total = __builtin_amdgcn_readlane(sum, 63);
-    if (at < total) {
-      const int l = __popcll(__ballot(sum <= at));
-      *seq = s0 + l;
-      *tile = at - __builtin_amdgcn_readlane(sum - mine, l);
-      return true;
-    }
-    at -= total;
+    return false;
   }
-  return false;
+  Seq sq[N];
+  int tiles[N], total = 0, top = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) sq[j] = spk_paged::seq_at(a.c, min(N * lane + j, a.c.num_seqs - 1));
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int rows = N * lane + j < a.c.num_seqs ? sq[j].n * a.group : 0;
+    tiles[j] = rows >= a.many ? (rows + 255) / 256 : 0;
+    if (tiles[j] == 0) sq[j] = {0, 0, 0};  // no tokens: past() is 0
+    total += tiles[j];
+    top = max(top, sq[j].ctx);
+  }
+  if (at >= __builtin_amdgcn_readfirstlane(wave_sum(total))) return false;
+  // tiles of the lane's sequence j that see past key 128 * level; all for -1
+  auto past = [&](int j, int level) {
+    const int64_t d = 128ll * level - sq[j].ctx + sq[j].n;  // its tokens that do not
+    return level < 0 || d <= 0 ? tiles[j] : d >= sq[j].n ? 0 : tiles[j] - ((int)d * a.group >> 8);
+  };
+  int low = -1, high = __builtin_amdgcn_readfirstlane(wave_max(top)) / 128 + 1;
+  int before = 0;  // tiles past high
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += past(j, mid);
+    n = __builtin_amdgcn_readfirstlane(wave_sum(n));
+    if (n > at) {
+      low = mid;
+    } else {
+      high = mid;
+      before = n;
+    }
+  }
+  at -= before;
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) n += past(j, low) - past(j, high);
+  const int sum = wave_scan(n), l = __popcll(__ballot(sum <= at));
+  int first = sum - n, found = -1, its = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int m = past(j, low) - past(j, high);
+    if (found < 0 && at < first + m) {
+      found = N * lane + j;
+      its = tiles[j] - 1 - past(j, high) - (at - first);
+    }
+    first += m;
+  }
+  *seq = __builtin_amdgcn_readlane(found, l);
+  *tile = __builtin_amdgcn_readlane(its, l);
+  return true;
 }
 
 // 16 lanes' 8-byte pieces of 4 rows (4 lanes a row) turned: lane l of the 16
@@ -1093,6 +1158,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   constexpr int RS = 32 / RPW;             // distance of its rows: load x of 32 keys holds rows x, x + RS, ...
   constexpr int LG = D / 2;                // threads that cover a row of V
   constexpr int U = KT > 64 ? 2 : 1;       // lookups of a lane per tile
+  constexpr int NB = D == 256 ? 1 : 2;     // blocks of 32 keys at a time
   // LDS reads ahead of the matrix instruction that uses them.  Heads of 256 have
   // no registers left for it: 2 ahead spills and takes 356 us for 347, while with
   // heads of 128, 4 ahead take 207 us for 217.
@@ -1106,8 +1172,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   const int ln = lane & 31, h = lane >> 5;
   const int kvh = blockIdx.y, split = blockIdx.x;
   int seq, tile;
-  // the last tiles, which see the most keys, first
-  if (!find_tile(a, 256, gridDim.z - 1 - blockIdx.z, lane, &seq, &tile)) return;
+  if (!find_tile(a, blockIdx.z, gridDim.z - 1, lane, &seq, &tile)) return;
   seq = __builtin_amdgcn_readfirstlane(seq);
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Seq sq = spk_paged::seq_at(a.c, seq);
@@ -1166,8 +1231,9 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
       off[u] = there ? off[u] : 0;  // a key without a place reads the pool's first row and is masked
     }
   };
-  // a wave's two loads of a tile, its rows at `off`, into `to`, loads `apart`
-  auto load = [&](const uint16_t* from, uint4* to, int apart) __attribute__((always_inline)) {
+  // a wave's two loads of a tile, its rows at `off`, into `to`, loads `apart`;
+  // lane l brings piece l % CH ^ other of its row
+  auto load = [&](const uint16_t* from, uint4* to, int apart, int other) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int x = wave * 2 + i, row = x % RS + 32 * (x / RS);
@@ -1184,11 +1250,17 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
         if constexpr (U == 2) o = row & 64 ? off[1] : off[0];
         at = __shfl(o, kl & 63);
       }
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (at + 8 * (lane % CH))),
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (at + 8 * (lane % CH ^ other))),
                                        (__attribute__((address_space(3))) void*)&to[x * apart], 16, 0, 0);
     }
   };
+  // Rows that share a load have their halves exchanged in turn, so that 16 rows
+  // read side by side are in different banks: of heads of 128 every other row,
+  // of 64 every other two.
+  auto swapped = [](int row) { return CH == 16 ? 8 * (row & 1) : CH == 8 ? 4 * (row >> 1 & 1) : 0; };
+  const int kload = swapped(lane / CH), kswap = swapped(ln / RS);
   const int kread = (ln % RS) * 65 + (ln / RS) * CH + h;  // of this lane's row and half in the 32 keys' loads
+  const int klow = kread + kswap, khigh = kread - kswap;  // its first and its second half's pieces
   // Some row of the workgroup does not see the whole tile at k0.  Then a value
   // that is not finite must not meet the zero weight of a row that does not
   // see it: such elements are turned into zeros, and added row by row.
@@ -1250,31 +1322,39 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
                   __attribute__((always_inline)) {
     int asked[U];
     ask(k0 + 4 * KT, asked);
-    load(a.k + kvh * a.c.head_stride, ks_load, 65);  // at the offsets that the step before found
+    load(a.k + kvh * a.c.head_stride, ks_load, 65, kload);  // at the offsets that the step before found
     look_up(k0 + 3 * KT);
-    load(vbase, raw_load, 64);
+    load(vbase, raw_load, 64, 0);
     const uint4* vs = &vss[parity * 1024];
     if (tid < KT / 32) odd_of[third == 0 ? 2 : third - 1][tid] = 0;  // the tile before this one's
     const bool part = partial(k0, now);
 #pragma unroll 1
-    for (int j = 0; j < KT / 32; ++j) {
+    for (int j = 0; j < KT / 32; j += NB) {
       const int kj = k0 + 32 * j;
-      if (kj >= wave_hi || kj + 32 <= wave_lo) continue;  // also past the end
-      const uint32_t has = (uint32_t)((U == 2 && j > 1 ? now[U - 1] : now[0]) >> (32 * (j & 1)));
-      const bool full = has == 0xffffffffu && kj >= wave_lo_all && kj + 32 <= wave_hi_all;
-      floatx16 s;
+      if (kj >= wave_hi || kj + 32 * NB <= wave_lo) continue;  // also past the end
+      floatx16 s[NB];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-      in_turn<KS, AHEAD>([&](int c) { return ks[j * RS * 65 + kread + 2 * c]; },
-                         [&](int c, uint4 k) { s = H::mfma32(k, c < QR ? q[c] : qs[(c - QR) * 512 + tid], s); });
-      if (!full) {
-        const uint32_t see = seen(has, kj, row_lo, row_hi) >> (4 * h);  // a lane's keys at constant places
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+      in_turn<NB * KS, AHEAD>([&](int x) { return ks[(j + x % NB) * RS * 65 + (x / NB < KS / 2 ? klow : khigh) + 2 * (x / NB)]; }, [&](int x, uint4 k) {
+        const int c = x / NB;
+        s[x % NB] = H::mfma32(k, c < QR ? q[c] : qs[(c - QR) * 512 + tid], s[x % NB]);
+      });
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int kb = kj + 32 * b;
+        const uint32_t has = (uint32_t)((U == 2 && j > 1 ? now[U - 1] : now[0]) >> (32 * ((j + b) & 1)));
+        if (has == 0xffffffffu && kb >= wave_lo_all && kb + 32 <= wave_hi_all) continue;
+        const uint32_t see = seen(has, kb, row_lo, row_hi) >> (4 * h);  // a lane's keys at constant places
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[b][i] : -INFINITY;
       }
-      float top = s[0];
+      float top = s[0][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
       top *= a.scale_log2;
       if (__any(top > m + kBehind)) {
         top = fmaxf(top, spk::lane_xor32(top));
@@ -1286,37 +1366,50 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[t] *= f;
       }
-      uint4 p[2];
+      // the weights of 16 keys while the product of the 16 before them runs
+      uint4 p[2 * NB];
+      auto weigh = [&](int i, int e0, int e1) __attribute__((always_inline)) {
+        floatx16& x = s[i >> 1];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = exp2_fast(__builtin_fmaf(s[i], a.scale_log2, shift));
-        l += s[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        p[i] = make_uint4(H::pack(s[8 * i], s[8 * i + 1]), H::pack(s[8 * i + 2], s[8 * i + 3]),
-                          H::pack(s[8 * i + 4], s[8 * i + 5]), H::pack(s[8 * i + 6], s[8 * i + 7]));
-      in_turn<2 * DT, AHEAD>([&](int c) { return vs[(2 * j * DT + c) * 64 + lane]; },
-                             [&](int c, uint4 v) { acc[c % DT] = H::mfma32(v, p[c / DT], acc[c % DT]); });
+        for (int e = 8 * (i & 1) + e0; e < 8 * (i & 1) + e1; ++e) {
+          x[e] = exp2_fast(__builtin_fmaf(x[e], a.scale_log2, shift));
+          l += x[e];
+        }
+        if (e1 == 8) {
+          const int f = 8 * (i & 1);
+          p[i] = make_uint4(H::pack(x[f], x[f + 1]), H::pack(x[f + 2], x[f + 3]), H::pack(x[f + 4], x[f + 5]),
+                            H::pack(x[f + 6], x[f + 7]));
+        }
+      };
+      weigh(0, 0, 8);
+      in_turn<2 * NB * DT, AHEAD>([&](int c) { return vs[(2 * j * DT + c) * 64 + lane]; }, [&](int c, uint4 v) {
+        const int i = c / DT, t = c % DT;
+        acc[t] = H::mfma32(v, p[i], acc[t]);
+        if (i + 1 < 2 * NB) weigh(i + 1, 8 * t / DT, 8 * (t + 1) / DT);
+      });
       if (part) {
-        uint32_t odd = __builtin_amdgcn_readfirstlane(odd_of[third][j]);
-        while (odd) {
-          const int kl = __ffs(odd) - 1;
-          odd &= odd - 1;
-          const uint16_t* row = vbase + max(spk_paged::offset_of(a.c, seq, kj + kl), (int64_t)0);
-          uint32_t pair = kl & 16 ? (kl & 8 ? (kl & 2 ? p[1].w : p[1].z) : (kl & 2 ? p[1].y : p[1].x))
-                                  : (kl & 8 ? (kl & 2 ? p[0].w : p[0].z) : (kl & 2 ? p[0].y : p[0].x));
-          pair = __shfl((int)pair, ln + 32 * ((kl >> 2) & 1));
-          const float weight = H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
-          if (kj + kl >= row_lo && kj + kl < row_hi) {
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+        for (int b = 0; b < NB; ++b) {
+          uint32_t odd = __builtin_amdgcn_readfirstlane(odd_of[third][j + b]);
+          while (odd) {
+            const int kl = __ffs(odd) - 1, key = kj + 32 * b + kl;
+            odd &= odd - 1;
+            const uint16_t* row = vbase + max(spk_paged::offset_of(a.c, seq, key), (int64_t)0);
+            const uint4 p0 = p[2 * b], p1 = p[2 * b + 1];
+            uint32_t pair = kl & 16 ? (kl & 8 ? (kl & 2 ? p1.w : p1.z) : (kl & 2 ? p1.y : p1.x))
+                                    : (kl & 8 ? (kl & 2 ? p0.w : p0.z) : (kl & 2 ? p0.y : p0.x));
+            pair = __shfl((int)pair, ln + 32 * ((kl >> 2) & 1));
+            const float weight = H::widen((uint16_t)(kl & 1 ? pair >> 16 : pair));
+            if (key >= row_lo && key < row_hi) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const uint16_t x = row[dim_of(t, 8 * (i >> 2) + 4 * h + (i & 3))];
-                if (H::odd(x)) acc[t][i] += weight * H::widen(x);
-                __builtin_amdgcn_sched_barrier(0);  // one at a time: this path takes no registers from the others
-              }
+              for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const uint16_t x = row[dim_of(t, 8 * (i >> 2) + 4 * h + (i & 3))];
+                  if (H::odd(x)) acc[t][i] += weight * H::widen(x);
+                  __builtin_amdgcn_sched_barrier(0);  // one at a time: this path takes no registers from the others
+                }
+            }
           }
         }
       }
@@ -1339,19 +1432,19 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
     ask(begin, page);
     look_up(begin);
     ask(begin + KT, page);
-    load(kbase, ka, 65);
-    load(vbase, ra, 64);
+    load(kbase, ka, 65, kload);
+    load(vbase, ra, 64, 0);
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = valid[u];
     look_up(begin + KT);
     ask(begin + 2 * KT, page);
-    load(kbase, kb, 65);
-    load(vbase, rb, 64);
+    load(kbase, kb, 65, kload);
+    load(vbase, rb, 64, 0);
 #pragma unroll
     for (int u = 0; u < U; ++u) next[u] = valid[u];
     look_up(begin + 2 * KT);
     ask(begin + 3 * KT, page);
-    load(vbase, rc, 64);
+    load(vbase, rc, 64, 0);
 #pragma unroll
     for (int u = 0; u < U; ++u) second[u] = valid[u];
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
