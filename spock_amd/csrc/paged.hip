@@ -411,8 +411,8 @@ __device__ __forceinline__ uint32_t seen(uint32_t has, int k0, int lo, int hi) {
 // Tile `at` of the tiles of 256 of the n * group rows of the sequences of many:
 // its sequence and its index there.  false past the last of them.  Those that
 // see the most keys come first, to within 128 keys, so that the last that
-// workgroups take are short (six prompts of 16 heads over 4: TILES us, SEQUENCE
-// us with the last sequence's last tile first).
+// workgroups take are short (six prompts of 16 heads over 4: 180 us, 185 with
+// the last sequence's last tile first).
 __device__ __forceinline__ bool find_tile(const Attn& a, int at, int last, int lane, int* seq, int* tile) {
   constexpr int N = 4;  // sequences of a lane
   if (a.c.num_seqs > 64 * N) {  // more than are looked at together: by sequence, the last tiles first
@@ -1170,7 +1170,10 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   __shared__ uint32_t odd_of[3][KT / 32];  // keys of a tile with values that are not finite (tile number % 3)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, h = lane >> 5;
-  const int kvh = blockIdx.y, split = blockIdx.x;
+  // Workgroups go to the 8 XCDs in turn.  Every 8 tiles another range goes to an
+  // XCD, or one has all the short last ranges (2048 tokens after 4096: 335 us ->
+  // 316; with another at every tile, which shares fewer keys in an L2, 324).
+  const int kvh = blockIdx.y, split = (blockIdx.x + (blockIdx.z >> 3)) % gridDim.x;
   int seq, tile;
   if (!find_tile(a, blockIdx.z, gridDim.z - 1, lane, &seq, &tile)) return;
   seq = __builtin_amdgcn_readfirstlane(seq);
@@ -1184,7 +1187,8 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   const int keys = range_keys(a, lo, hi);
   const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
   const int end = begin + min(keys, hi - begin);
-  if (begin >= end && a.splits > 1) return;
+  if (begin >= end && split > 0) return;
+  const bool alone = hi - (lo & ~31) <= keys;  // the tile's one range
 
   const int r = min(r0 + 32 * wave + ln, rows - 1);
   int row_lo, row_hi, wave_lo, wave_hi, wave_lo_all, wave_hi_all;
@@ -1468,14 +1472,14 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   const int64_t at = (int64_t)token * a.heads + head;
   float* part = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
   if (h == 0) {
-    if (a.splits > 1) {
+    if (!alone) {
       part[0] = m;
       part[1] = l;
     } else if (a.lse) {
       a.lse[at] = l == 0.0f ? -INFINITY : (m - H::kShift + __builtin_amdgcn_logf(l)) * kLn2;
     }
   }
-  const float inv = a.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = !alone ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int u = 0; u < DT / 2; ++u)
 #pragma unroll
@@ -1484,7 +1488,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = acc[2 * u + (j & 1)][4 * i + (j >> 1)] * inv;
       const int d = dim_of(2 * u, 8 * i + 4 * h);
-      if (a.splits > 1) {
+      if (!alone) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) *reinterpret_cast<float2*>(part + 2 + d + j) = make_float2(o[j], o[j + 1]);
       } else {
@@ -1558,7 +1562,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
     spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
     spk_paged::visible(sq, (min(r0 + 256, rows) - 1) / a.group, a.window, &x, &hi);
     const int span = hi - (lo & ~31), keys = range_keys(a, lo, hi);
-    n = span <= 0 ? 0 : (int)(((int64_t)span + keys - 1) / keys);
+    if (span <= keys) return;
+    n = (int)(((int64_t)span + keys - 1) / keys);
     step = (int64_t)a.c.total_tokens * a.heads * (D + 2);
     part = a.part + at * (D + 2);
   }
