@@ -216,7 +216,7 @@ struct Attn {
   int32_t shares, share_rows;  // few rows: workgroups, and rows of one
   int32_t alone;               // few rows: no ranges
   int32_t splits, chunk;       // many rows: key ranges of a tile and the least keys of one
-  int32_t join_few;            // the join has [num_seqs][kv_heads][64] rows, for sequences of few; else [total_tokens][heads]
+  int32_t few;                 // the join has [num_seqs][kv_heads][few] rows; 0: [total_tokens][heads]
   float scale_log2;  // scale * log2(e)
 };
 
@@ -534,6 +534,11 @@ __device__ __forceinline__ void store_out(const Attn& a, int token, int head, in
 // 16-byte row pieces by pairing halfwords of two keys.  A weight enters as
 // two 16-bit parts (value and remainder): the kernel waits for memory, and the
 // second product keeps a few heavy keys' rounding out of the result.
+//
+// What bounds it: memory.  64 sequences of 300 to 16000 keys, heads of 256: 1.07 GB
+// in 185 us, 5.8 TB/s, where reading alone reaches 7.1; one sequence of 130,001 keys:
+// 98 us, 5.4 TB/s.  Values are loaded past the caches' replacement (they are
+// read once); the keys, whose rows' other halves come later, are not.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
   using H = Half<BF>;
@@ -832,8 +837,8 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
   }
 }
 
-// A middle number of rows per sequence and KV head (17 .. 64: a few drafted
-// tokens): too many for the registers of one wave beside the keys on their
+// A middle number of rows per sequence and KV head (17 .. 128, in pieces of 64: a
+// few drafted tokens): too many for the registers of one wave beside the keys on their
 // way, too few to be bound by anything but memory.  A workgroup takes 64 rows,
 // 16 to each of its 4 waves, and all waves read every step of 32 keys from
 // LDS.  A wave loads its part of a step's keys and values two steps ahead, into
@@ -845,6 +850,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
 // rows 0..7 are read side by side, and by 32 for the values, which are read
 // by the transposing load: 16 lanes take 4 keys' pieces of 16 dimensions and
 // get 4 keys of a dimension each.
+//
+// What bounds it: 16 sequences with 9 tokens of 4 heads (36 rows), heads of 256, take
+// 44 us for 168 MB, 3.8 TB/s: in 64 rows' time on the matrix units and in LDS
+// for 36, and in 32 workgroups' ranges of unequal lengths.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   using H = Half<BF>;
@@ -1146,6 +1155,14 @@ __device__ __forceinline__ void in_turn(Read read, Use use) {
 // thread reads 2 dimensions of 8 keys and writes 8 keys of each, in fragment
 // order; the dimension of row m of output tile 2 u + e is 2 (m + 32 u) + e,
 // which makes these writes (and a lane's output) contiguous.
+//
+// What bounds it: one workgroup of 8 waves to a CU (a wave's outputs and queries
+// fill its registers).  2048 tokens at 16384 keys, heads of 256: 295 us without the
+// join, 870 TFLOP/s; matrix instructions run 38% of the time at the 2.05 GHz the
+// chip keeps, LDS reads 25%, waves wait for one or the other in half of theirs,
+// as no registers are left to read ahead.  Six ragged prompts, heads of 128: 167
+// us, 650 TFLOP/s: a step's exponentials take as long as its matrix
+// instructions, and the longest tile alone is three quarters of the time.
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   using H = Half<BF>;
@@ -1171,7 +1188,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 31, h = lane >> 5;
   // Workgroups go to the 8 XCDs in turn.  Every 8 tiles another range goes to an
-  // XCD, or one has all the short last ranges (2048 tokens after 4096: 335 us ->
+  // XCD, or one has all the short last ranges (2048 tokens at 16384 keys: 335 us ->
   // 316; with another at every tile, which shares fewer keys in an L2, 324).
   const int kvh = blockIdx.y, split = (blockIdx.x + (blockIdx.z >> 3)) % gridDim.x;
   int seq, tile;
@@ -1497,36 +1514,30 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
     }
 }
 
-// Joins the key ranges of a row: 256 / LANES rows to a workgroup, for many rows
-// of few ranges 64 lanes to each, for few rows of many ranges all 256.  The
-// ranges' maxima and sums are read by the lanes side by side; D / 4 lanes add
-// a range's output, the other lanes take other ranges, and LDS joins them.
-template <int D, int LANES, bool BF>
+// Joins the key ranges of a row: a wave to each, as fast as a whole workgroup to
+// each where there are few rows of many ranges (32 rows of 64: 106 us with the
+// attention either way) and faster where there are many (1024 rows: 24 us, 27).
+// The ranges' maxima and sums are read by the lanes side by side; D / 4 lanes
+// add a range's output, the other lanes take other ranges, and LDS joins them.
+template <int D, bool BF>
 __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
-  constexpr int L = D / 4 < LANES ? D / 4 : LANES, W = LANES / L;  // lanes of a range, ranges at a time
-  constexpr int ROWS = 256 / LANES;
-  __shared__ float weights[ROWS][LANES];
-  __shared__ float reds[ROWS][4];
-  __shared__ float4 all[ROWS][W][L];
-  const int lane = threadIdx.x & 63, tid = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+  constexpr int L = D / 4, W = 64 / L;  // lanes of a range, ranges at a time
+  __shared__ float weights[4][64];
+  __shared__ float4 all[4][W][L];
+  const int lane = threadIdx.x & 63, mine = threadIdx.x >> 6;
   float* weight = weights[mine];
-  float* red = reds[mine];
-  auto together = [&]() {  // a row of 64 lanes is one wave
-    if constexpr (LANES == 256) {
-      __syncthreads();
-    } else {
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
+  auto together = [&]() {  // of a wave's lanes
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  int64_t at = (int64_t)blockIdx.x * ROWS + mine;
+  int64_t at = (int64_t)blockIdx.x * 4 + mine;
   int s, token, head, kvh, r;
   Seq sq;
-  if (a.join_few) {
-    r = (int)(at & 63);
-    s = (int)((at >> 6) / a.kv_heads);
-    kvh = (int)(at >> 6) - s * a.kv_heads;
+  if (a.few) {
+    r = (int)(at % a.few);
+    s = (int)(at / a.few / a.kv_heads);
+    kvh = (int)(at / a.few) - s * a.kv_heads;
     if (s >= a.c.num_seqs) return;
     sq = spk_paged::seq_at(a.c, s);
     if (r >= sq.n * a.group || sq.n * a.group >= a.many) return;
@@ -1569,74 +1580,52 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
   }
 
   float top = -INFINITY;
-  for (int j = tid; j < n; j += LANES) top = fmaxf(top, part[j * step]);
+  for (int j = lane; j < n; j += 64) top = fmaxf(top, part[j * step]);
   top = spk::wave_max(top);
-  if constexpr (LANES == 256) {
-    if (lane == 0) red[tid >> 6] = top;
-    together();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  }
-  constexpr int E = D / (4 * L);  // groups of four elements of a lane
   float sum = 0.0f;
-  float4 o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int j0 = 0; j0 < n; j0 += LANES) {
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int j0 = 0; j0 < n; j0 += 64) {
     together();
-    if (j0 + tid < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(part + (j0 + tid) * step);
+    if (j0 + lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(part + (j0 + lane) * step);
       const float f = top == -INFINITY ? 1.0f : exp2_fast(ml.x - top);
-      weight[tid] = f;
+      weight[lane] = f;
       sum += f * ml.y;
     }
     together();
-    const int m = min(LANES, n - j0);
+    const int m = min(64, n - j0);
 #pragma unroll 4
-    for (int j = tid / L; j < m; j += W) {
+    for (int j = lane / L; j < m; j += W) {
       const float f = weight[j];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float* p = part + (j0 + j) * step + 2 + 4 * (tid % L + L * e);
-        const float2 u = *reinterpret_cast<const float2*>(p), v = *reinterpret_cast<const float2*>(p + 2);
-        o[e].x += f * u.x;
-        o[e].y += f * u.y;
-        o[e].z += f * v.x;
-        o[e].w += f * v.y;
-      }
+      const float* p = part + (j0 + j) * step + 2 + 4 * (lane % L);
+      const float2 u = *reinterpret_cast<const float2*>(p), v = *reinterpret_cast<const float2*>(p + 2);
+      o.x += f * u.x;
+      o.y += f * u.y;
+      o.z += f * v.x;
+      o.w += f * v.y;
     }
   }
   sum = wave_sum(sum);
-  if constexpr (LANES == 256) {
-    together();
-    if (lane == 0) red[tid >> 6] = sum;
-  }
   if constexpr (W > 1) {
-    all[mine][tid / L][tid % L] = o[0];
+    all[mine][lane / L][lane % L] = o;
     together();
-    if (tid < L) {
+    if (lane < L) {
 #pragma unroll
       for (int w = 1; w < W; ++w) {
-        const float4 u = all[mine][w][tid];
-        o[0].x += u.x;
-        o[0].y += u.y;
-        o[0].z += u.z;
-        o[0].w += u.w;
+        const float4 u = all[mine][w][lane];
+        o.x += u.x;
+        o.y += u.y;
+        o.z += u.z;
+        o.w += u.w;
       }
     }
   }
-  if constexpr (LANES == 256) {
-    if constexpr (W == 1) together();
-    sum = (red[0] + red[1]) + (red[2] + red[3]);
-  }
-  if (tid < L) {
+  if (lane < L) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float y[4] = {o[e].x * inv, o[e].y * inv, o[e].z * inv, o[e].w * inv};
-      store_out<BF, 4>(a, token, head, 4 * (tid + L * e), y);
-    }
+    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    store_out<BF, 4>(a, token, head, 4 * lane, y);
   }
-  if (tid == 0 && a.lse)
+  if (lane == 0 && a.lse)
     a.lse[at] = sum == 0.0f ? -INFINITY : (top - Half<BF>::kShift + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
@@ -1689,6 +1678,8 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
   return SPK_OK;
 }
 
+constexpr int kFew = 128;  // rows of a sequence that are not many
+
 // How a call's rows and keys are dealt to the kernels.
 struct Plan {
   int many, shares, share_rows, tiles, splits, chunk;
@@ -1704,30 +1695,34 @@ Plan plan_of(const SpkPagedAttnArgs& p) {
   Plan r;
   // a call of one sequence that may have many rows goes to their kernel
   // whatever it has; one that has none to the others
-  const bool any_many = longest > 64;
-  r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : 65;
-  const int64_t few = std::min<int64_t>(longest, 64);
-  r.share_rows = few <= 16 ? 16 : 64;
+  // Many are more than 128, two pieces of 64 (16 sequences at 4000 keys, heads of
+  // 128: 128 rows 68 us, 83 as many; 192 rows 88 as many, 118 in three pieces).
+  const bool any_many = longest > kFew;
+  r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : kFew + 1;
+  // pieces of 16 rows where none has more (16 rows: 35 us, 38 in pieces of 64;
+  // 36 rows: 42 in one of 64, 68 in three of 16)
+  r.share_rows = longest <= 16 ? 16 : 64;
   int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
   if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
   const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
 
   // sequences of few rows: all of them, unless the one there is has many.  As
-  // many workgroups as the chip holds at once (2 to a CU; 4 with heads of 64),
-  // more only where the pieces alone are more, and no more than ranges of 128
-  // keys.
-  // Next to many rows a sequence of few is one piece; else the bound may be low.
-  const int64_t pieces = !any_many ? (all / r.share_rows + c.num_seqs) * c.num_kv_heads
-                         : c.num_seqs > 1 ? std::min<int64_t>(c.num_seqs, all) * c.num_kv_heads : 0;
-  const int64_t slots = c.head_dim == 64 ? 1024 : 512;
+  // many workgroups as the chip holds at once (2 to a CU; with 4, 32 sequences of
+  // one token at 4000 keys take 36 us for 33), more only where the pieces alone
+  // are more, and no more than ranges of 128 keys.
+  // Next to many rows a sequence of few is two pieces; else the bound may be low.
+  const int64_t some = all / r.share_rows + c.num_seqs;
+  const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(2 * (int64_t)c.num_seqs, some) : 0);
+  const int64_t slots = 512;
   r.shares = (int)std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)),
                                     INT32_MAX);
 
   // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
   // the number of ranges that takes the fewest rounds of 256 workgroups times
   // steps in each; a range's share of the join costs as much as some 4 steps
-  // (2048 tokens after 4096 in 64 workgroups: 347 us in 3 ranges, 322 in 4, where 4 fill the chip).
-  const int64_t seqs = std::min<int64_t>(c.num_seqs, all / 65 + 1);
+  // (2048 tokens at 16384 keys, 64 workgroups: 347 us in 3 ranges, 322 in the 4 that
+  // fill the chip; six prompts in 500 workgroups: 184 us, 210 in 2 ranges each).
+  const int64_t seqs = std::min<int64_t>(c.num_seqs, all / (kFew + 1) + 1);
   r.tiles = any_many ? (int)std::min<int64_t>((all + 255 * seqs) / 256, INT32_MAX) : 0;
   const int64_t groups = std::max<int64_t>(1, (int64_t)r.tiles * c.num_kv_heads);
   int64_t per = steps, least = (groups + 255) / 256 * steps;
@@ -1739,7 +1734,7 @@ Plan plan_of(const SpkPagedAttnArgs& p) {
   r.splits = r.tiles ? (int)((steps + per - 1) / per) : 1;
   r.join = r.splits > 1 || (r.shares && steps > 1);
   // rows to join: all tokens', or of each sequence those that few can be
-  const int64_t every = (int64_t)c.total_tokens * p.num_q_heads, of_few = (int64_t)c.num_seqs * c.num_kv_heads * 64;
+  const int64_t every = (int64_t)c.total_tokens * p.num_q_heads, of_few = (int64_t)c.num_seqs * c.num_kv_heads * kFew;
   r.join_few = any_many && r.splits == 1 && of_few < every;
   r.join_rows = r.join_few ? of_few : every;
   return r;
@@ -1782,11 +1777,7 @@ void launch_attn(const Attn& a, const Plan& r, hipStream_t s) {
   if (r.tiles)
     hipLaunchKernelGGL((paged_tiles_kernel<D, BF>), dim3(r.splits, a.kv_heads, r.tiles), dim3(512), 0, s, a);
   if (!r.join) return;
-  const int64_t rows = r.join_rows;
-  if (rows >= 1024)
-    hipLaunchKernelGGL((paged_join_kernel<D, 64, BF>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((paged_join_kernel<D, 256, BF>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((paged_join_kernel<D, BF>), dim3((unsigned)((r.join_rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 template <int D, bool BF>
@@ -1915,7 +1906,7 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
   a.alone = !r.join;
   a.splits = r.splits;
   a.chunk = r.chunk;
-  a.join_few = r.join_few;
+  a.few = r.join_few ? kFew : 0;
   const float scale = p->scale != 0.0f ? p->scale : 1.0f / std::sqrt((float)c.head_dim);
   a.scale_log2 = scale * 1.44269504088896341f;
   hipStream_t s = spk::to_hip(stream);
