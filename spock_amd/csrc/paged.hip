@@ -105,6 +105,11 @@ struct Mrope {
 // that rotate together (HALVES: chunk j and j + rot/16; ADJACENT: the pairs
 // lie inside a chunk), so the angles of a lane are the same for every head of
 // the token and are read once.
+//
+// What bounds it: memory.  32,768 tokens of 16 + 4 + 4 heads of 128 take 107 us for
+// 405 MB read and written, 3.8 TB/s (a plain copy reaches 5.1); a lane's next row
+// loaded while it turns one costs registers that other waves' loads need (115
+// us).  A decode step's is the launch.
 template <int D, bool BF, bool ADJ>
 __global__ __launch_bounds__(256) void mrope_append_kernel(Mrope a) {
   constexpr int L = D / 16, RG = 64 / L;  // lanes of a head, heads at a time
