@@ -557,9 +557,14 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * workspace: 256-byte aligned, spk_paged_attention_workspace_size() bytes,
  * contents ignored (may be 0 bytes: then NULL is fine).  Calls that overlap on
  * one workspace race.
+ * Limits: page_stride and token_stride below 2^32 elements, max_pages *
+ * page_size at most 2^31 - 4096 positions, 65535 KV heads, and as many row
+ * tiles (of 256) in a call.
  * Numerics: products of 16-bit values accumulate in fp32, softmax statistics
- * in fp32; the weights are rounded to the 16-bit type before the product with
- * V (they enter the sum of weights unrounded), out is rounded once. */
+ * in fp32, out is rounded once.  Weights enter the sum of weights unrounded;
+ * before the product with V they are two 16-bit parts (value and remainder) in
+ * sequences of up to 128 rows (new tokens times heads of a KV head), and rounded
+ * to one in longer ones and in a call of one sequence whose bound is longer. */
 typedef struct SpkPagedAttnArgs {
   SpkPagedCache cache;
   int32_t num_q_heads;
