@@ -558,8 +558,8 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * contents ignored (may be 0 bytes: then NULL is fine).  Calls that overlap on
  * one workspace race.
  * Limits: page_stride and token_stride below 2^32 elements, max_pages *
- * page_size at most 2^31 - 4096 positions, 65535 KV heads, and as many row
- * tiles (of 256) in a call.
+ * page_size at most 2^31 - 4096 positions, 65535 KV heads and row tiles (of
+ * 256) in a call, and 2^24 workgroups of a launch (some 67 million rows).
  * Numerics: products of 16-bit values accumulate in fp32, softmax statistics
  * in fp32, out is rounded once.  Weights enter the sum of weights unrounded;
  * before the product with V they are two 16-bit parts (value and remainder) in

@@ -1684,6 +1684,7 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
 }
 
 constexpr int kFew = 128;  // rows of a sequence that are not many
+constexpr int64_t kMostGroups = 16777215;  // workgroups of 256 in a launch: below 2^32 threads
 
 // How a call's rows and keys are dealt to the kernels.
 struct Plan {
@@ -1802,7 +1803,9 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
   Mrope a{};
   if (const int rc = check_cache(p->cache, who, &a.c)) return rc;
   const SpkPagedCache& c = p->cache;
-  if (p->num_q_heads <= 0) return spk::fail(SPK_ERR_SHAPE, "%s: %d query heads", who, p->num_q_heads);
+  if (p->num_q_heads <= 0 || c.total_tokens > 4 * kMostGroups)
+    return spk::fail(SPK_ERR_SHAPE, "%s: %d query heads, %d tokens (%lld at most)", who, p->num_q_heads, c.total_tokens,
+                     (long long)(4 * kMostGroups));
   if (p->rot_dim <= 0 || p->rot_dim % 16 || p->rot_dim > c.head_dim)
     return spk::fail(SPK_ERR_SHAPE, "%s: rot_dim %d (a multiple of 16 up to head_dim %d)", who, p->rot_dim, c.head_dim);
   if (p->pairing != SPK_ROPE_HALVES && p->pairing != SPK_ROPE_ADJACENT)
@@ -1881,6 +1884,9 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
       (p->gate && !strides_ok(p->gate_token_stride, p->gate_head_stride)))
     return spk::fail(SPK_ERR_ALIGN, "%s: q, gate and out and their strides must be 16-byte aligned", who);
   const Plan r = plan_of(*p);
+  if (r.shares > kMostGroups || (r.join && (r.join_rows + 3) / 4 > kMostGroups))
+    return spk::fail(SPK_ERR_SHAPE, "%s: %d tokens of %d heads, %d sequences are more than one launch holds", who,
+                     c.total_tokens, p->num_q_heads, c.num_seqs);
   const size_t need = workspace_of(*p, r);
   if (need && (!p->workspace || p->workspace_bytes < need || !spk::aligned(p->workspace, 256)))
     return spk::fail(p->workspace ? SPK_ERR_ARG : SPK_ERR_NULL, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)",

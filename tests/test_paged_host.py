@@ -164,6 +164,19 @@ def test_mrope_refusals(over, code):
     assert lib.spk_mrope_append(C.byref(a), None) == code, lib.spk_last_error()
 
 
+def test_more_rows_than_a_launch_holds():
+    from spock_amd import _lib
+    lib = _lib.lib()
+    for tokens, seqs, bound, context in ((120_000_000, 120_000_000, 1, 64), (120_000_000, 1, 1, 60000)):
+        a = _lib.SpkPagedAttnArgs(_cache(_lib, num_kv_heads=16, head_stride=64, token_stride=1024, total_tokens=tokens, num_seqs=seqs,
+                                         max_pages=4000, table_stride=4000), 16, bound, context, 0, 0.0, 256, 256, 64, None, 0, 0,
+                                  256, 256, 64, None, 256, 1 << 62)
+        assert lib.spk_paged_attention(C.byref(a), None) == -2 and b"launch" in lib.spk_last_error(), lib.spk_last_error()
+    m = _lib.SpkMropeArgs(_cache(_lib, total_tokens=70_000_000), 4, 32, 0, 1, bytes(16), 256, 70_000_000, 256, 10, 0.0, 256, 256, 64,
+                          256, 128, 64, 256, 128, 64, None, None, 256, 256, 64)
+    assert lib.spk_mrope_append(C.byref(m), None) == -2
+
+
 def test_nothing_to_do():
     from spock_amd import _lib
     lib = _lib.lib()
