@@ -214,6 +214,7 @@ struct Attn {
   uint16_t* out;
   float* lse;
   float* shared;  // few rows: [shares][share_rows][D + 2], of the shares that are not alone
+  int2* ranges;   // [total_tokens * heads]: where the row's first part lies in `shared` (-1: in `part`) and how many; NULL: no join
   float* part;    // many rows: [splits][total_tokens * heads][D + 2] where splits > 1
   int64_t qt, qh, gt, gh, ot, oh;
   int32_t heads, kv_heads, group, window;
@@ -307,8 +308,8 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The share numbered `at`, or (seq >= 0) the first of the piece (seq, tile, kvh).  false: there is none.
-__device__ __forceinline__ bool find_share(const Attn& a, int at, int seq, int tile, int kvh, int lane, Share* out) {
+// The share numbered `at`.  false: there is none.
+__device__ __forceinline__ bool find_share(const Attn& a, int at, int lane, Share* out) {
   constexpr int N = 4;  // sequences of a lane at a time
   Load mine[N];
   long long keys = 0;
@@ -350,16 +351,16 @@ __device__ __forceinline__ bool find_share(const Attn& a, int at, int seq, int t
       n += mine[j].tiles * a.kv_heads * ranges_of(mine[j], c);
     }
     const int sum = wave_scan(n), total = __builtin_amdgcn_readlane(sum, 63);
-    if (seq >= 0 ? seq < s0 + 64 * N : at < before + total) {
+    if (at < before + total) {
       // the lane that holds it, then the one of its sequences
-      const int l = __builtin_amdgcn_readfirstlane(seq >= 0 ? (seq - s0) / N : __popcll(__ballot(before + sum <= at)));
+      const int l = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + sum <= at)));
       int first = before + sum - n;
       Load found{0, 0};
       int s = -1;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int count = mine[j].tiles * a.kv_heads * ranges_of(mine[j], c);
-        const bool here = seq >= 0 ? s0 + N * lane + j == seq : at >= first && at < first + count;
+        const bool here = at >= first && at < first + count;
         if (s < 0) {
           if (here) {
             s = s0 + N * lane + j;
@@ -377,16 +378,10 @@ __device__ __forceinline__ bool find_share(const Attn& a, int at, int seq, int t
       out->seq = s;
       out->ranges = ranges_of(found, c);
       out->keys = (((found.span + out->ranges - 1) / out->ranges) + 127) & ~127;
-      if (seq >= 0) {
-        out->tile = tile;
-        out->kvh = kvh;
-        out->range = 0;
-      } else {
-        const int rest = at - first, piece = rest / out->ranges;
-        out->range = rest - piece * out->ranges;
-        out->tile = piece / a.kv_heads;
-        out->kvh = piece - out->tile * a.kv_heads;
-      }
+      const int rest = at - first, piece = rest / out->ranges;
+      out->range = rest - piece * out->ranges;
+      out->tile = piece / a.kv_heads;
+      out->kvh = piece - out->tile * a.kv_heads;
       out->first = first + (out->tile * a.kv_heads + out->kvh) * out->ranges;
       int x;
       spk_paged::visible(spk_paged::seq_at(a.c, out->seq), 0, a.window, &out->lo, &x);
@@ -396,6 +391,12 @@ __device__ __forceinline__ bool find_share(const Attn& a, int at, int seq, int t
     before += total;
   }
   return false;
+}
+
+// Tells the join where the parts of row r of a piece or tile lie.
+__device__ __forceinline__ void tell(const Attn& a, const Seq& sq, int kvh, int r, int first, int ranges) {
+  const int i = r / a.group;
+  a.ranges[(int64_t)(sq.first + i) * a.heads + kvh * a.group + r - i * a.group] = make_int2(first, ranges);
 }
 
 // Keys in one range of a tile of many rows that sees [lo, hi): the plan's, or
@@ -541,8 +542,8 @@ __device__ __forceinline__ void store_out(const Attn& a, int token, int head, in
 // second product keeps a few heavy keys' rounding out of the result.
 //
 // What bounds it: memory.  64 sequences of 300 to 16000 keys, heads of 256: 1.07 GB
-// in 185 us, 5.8 TB/s, where reading alone reaches 7.1; one sequence of 130,001 keys:
-// 98 us, 5.4 TB/s.  Values are loaded past the caches' replacement (they are
+// in 182 us, 5.9 TB/s, where reading alone reaches 7.1; one sequence of 130,001 keys:
+// 96 us, 5.5 TB/s.  Values are loaded past the caches' replacement (they are
 // read once); the keys, whose rows' other halves come later, are not.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
@@ -558,11 +559,13 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int ln = lane & 15, g = lane >> 4;
   Share sh;
-  if (!find_share(a, blockIdx.x, -1, 0, 0, lane, &sh)) return;
+  if (!find_share(a, blockIdx.x, lane, &sh)) return;
   const int seq = sh.seq, kvh = sh.kvh;
   const Seq sq = spk_paged::seq_at(a.c, seq);
   const int rows = sq.n * a.group;
   const int r0 = sh.tile * 16;
+  if (a.ranges && sh.range == 0 && threadIdx.x < 16 && r0 + (int)threadIdx.x < rows)
+    tell(a, sq, kvh, r0 + threadIdx.x, sh.first * 16 + threadIdx.x, sh.ranges);
   // keys of the range that any row of the tile sees, and those that all see
   int lo, hi, lo_all, hi_all;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
@@ -857,8 +860,9 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
 // get 4 keys of a dimension each.
 //
 // What bounds it: 16 sequences with 9 tokens of 4 heads (36 rows), heads of 256, take
-// 44 us for 168 MB, 3.8 TB/s: in 64 rows' time on the matrix units and in LDS
-// for 36, and in 32 workgroups' ranges of unequal lengths.
+// 44 us for 168 MB, 3.8 TB/s.  Matrix instructions run 10% of the time and LDS
+// reads 14%; some 10 us are the way to the first keys (lengths, shares, page ids),
+// the rest is memory.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   using H = Half<BF>;
@@ -873,11 +877,12 @@ __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 15, g = lane >> 4;
   Share sh;
-  if (!find_share(a, blockIdx.x, -1, 0, 0, lane, &sh)) return;
+  if (!find_share(a, blockIdx.x, lane, &sh)) return;
   const int seq = sh.seq, kvh = sh.kvh;
   const Seq sq = spk_paged::seq_at(a.c, seq);
   const int rows = sq.n * a.group;
   const int r0 = sh.tile * 64;
+  if (a.ranges && sh.range == 0 && tid < 64 && r0 + tid < rows) tell(a, sq, kvh, r0 + tid, sh.first * 64 + tid, sh.ranges);
   int lo, hi, lo_all, hi_all, x;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
   spk_paged::visible(sq, (min(r0 + 64, rows) - 1) / a.group, a.window, &x, &hi);
@@ -1211,6 +1216,8 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   const int end = begin + min(keys, hi - begin);
   if (begin >= end && split > 0) return;
   const bool alone = hi - (lo & ~31) <= keys;  // the tile's one range
+  if (a.ranges && split == 0 && tid < r1 - r0)
+    tell(a, sq, kvh, r0 + tid, -1, alone ? 1 : (hi - (lo & ~31) + keys - 1) / keys);
 
   const int r = min(r0 + 32 * wave + ln, rows - 1);
   int row_lo, row_hi, wave_lo, wave_hi, wave_lo_all, wave_hi_all;
@@ -1524,6 +1531,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
 // attention either way) and faster where there are many (1024 rows: 24 us, 27).
 // The ranges' maxima and sums are read by the lanes side by side; D / 4 lanes
 // add a range's output, the other lanes take other ranges, and LDS joins them.
+// Where the parts lie the kernels that made them say (`tell`).
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
   constexpr int L = D / 4, W = 64 / L;  // lanes of a range, ranges at a time
@@ -1537,78 +1545,74 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Attn a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
   int64_t at = (int64_t)blockIdx.x * 4 + mine;
-  int s, token, head, kvh, r;
-  Seq sq;
+  int token, head;
+  int2 ranges;
   if (a.few) {
-    r = (int)(at % a.few);
-    s = (int)(at / a.few / a.kv_heads);
-    kvh = (int)(at / a.few) - s * a.kv_heads;
+    const int r = (int)(at % a.few), s = (int)(at / a.few / a.kv_heads), kvh = (int)(at / a.few) - s * a.kv_heads;
     if (s >= a.c.num_seqs) return;
-    sq = spk_paged::seq_at(a.c, s);
+    const Seq sq = spk_paged::seq_at(a.c, s);
     if (r >= sq.n * a.group || sq.n * a.group >= a.many) return;
     token = sq.first + r / a.group;
     head = kvh * a.group + r % a.group;
     at = (int64_t)token * a.heads + head;
+    ranges = a.ranges[at];
   } else {
     token = (int)(at / a.heads);
     head = (int)(at - (int64_t)token * a.heads);
     if (token >= a.c.total_tokens) return;
-    s = spk_paged::seq_of_token(a.c.cu, a.c.num_seqs, token, lane);
-    if (s >= a.c.num_seqs) return;
-    sq = spk_paged::seq_at(a.c, s);
-    if (token < sq.first || token >= sq.first + sq.n) return;
-    kvh = head / a.group;
-    r = (token - sq.first) * a.group + head - kvh * a.group;
+    ranges = a.ranges[at];  // asked for before the lengths: of a row of no sequence it is anything
+    bool there = false;
+    for (int s0 = 0; s0 < a.c.num_seqs && !there; s0 += 64) {
+      const int s = min(s0 + lane, a.c.num_seqs - 1);
+      there = __any(a.c.cu[s] <= token && token < a.c.cu[s + 1]);
+    }
+    if (!there) return;
   }
-  // the ranges that the row's tile had
-  const int rows = sq.n * a.group;
-  int n;
-  int64_t step;
-  const float* part;
-  if (rows < a.many) {
-    Share sh;
-    if (!find_share(a, 0, s, r / a.share_rows, kvh, lane, &sh) || sh.ranges == 1) return;
-    n = sh.ranges;
-    step = (int64_t)a.share_rows * (D + 2);
-    part = a.shared + sh.first * step + r % a.share_rows * (D + 2);
-  } else {
-    if (a.splits == 1) return;
-    const int r0 = r & ~255;
-    int lo, hi, x;
-    spk_paged::visible(sq, r0 / a.group, a.window, &lo, &x);
-    spk_paged::visible(sq, (min(r0 + 256, rows) - 1) / a.group, a.window, &x, &hi);
-    const int span = hi - (lo & ~31), keys = range_keys(a, lo, hi);
-    if (span <= keys) return;
-    n = (int)(((int64_t)span + keys - 1) / keys);
-    step = (int64_t)a.c.total_tokens * a.heads * (D + 2);
-    part = a.part + at * (D + 2);
-  }
+  const bool many = ranges.x < 0;
+  // what a row of sequences that overlap left unwritten stays inside the workspace
+  const int most = many ? a.splits : (int)(((int64_t)a.shares * a.share_rows - 1 - ranges.x) / a.share_rows) + 1;
+  const int n = min(ranges.y, most);
+  if (n <= 1) return;
+  const int64_t step = many ? (int64_t)a.c.total_tokens * a.heads * (D + 2) : (int64_t)a.share_rows * (D + 2);
+  const float* part = many ? a.part + at * (D + 2) : a.shared + (int64_t)ranges.x * (D + 2);
 
-  float top = -INFINITY;
-  for (int j = lane; j < n; j += 64) top = fmaxf(top, part[j * step]);
+  float2 ml = lane < n ? *reinterpret_cast<const float2*>(part + lane * step) : make_float2(-INFINITY, 0.0f);
+  float top = ml.x;
+  for (int j = lane + 64; j < n; j += 64) top = fmaxf(top, part[j * step]);
   top = spk::wave_max(top);
   float sum = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int j0 = 0; j0 < n; j0 += 64) {
+  for (int j0 = 0;;) {
     together();
     if (j0 + lane < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(part + (j0 + lane) * step);
       const float f = top == -INFINITY ? 1.0f : exp2_fast(ml.x - top);
       weight[lane] = f;
       sum += f * ml.y;
     }
     together();
     const int m = min(64, n - j0);
-#pragma unroll 4
-    for (int j = lane / L; j < m; j += W) {
-      const float f = weight[j];
-      const float* p = part + (j0 + j) * step + 2 + 4 * (lane % L);
-      const float2 u = *reinterpret_cast<const float2*>(p), v = *reinterpret_cast<const float2*>(p + 2);
-      o.x += f * u.x;
-      o.y += f * u.y;
-      o.z += f * v.x;
-      o.w += f * v.y;
+    constexpr int B = 8;  // loads under way, without a branch between them
+    for (int j = lane / L; j < m; j += B * W) {
+      float2 u[B], v[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const float* p = part + (j0 + min(j + i * W, m - 1)) * step + 2 + 4 * (lane % L);
+        u[i] = *reinterpret_cast<const float2*>(p);
+        v[i] = *reinterpret_cast<const float2*>(p + 2);
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const bool there = j + i * W < m;
+        const float f = weight[min(j + i * W, m - 1)];
+        o.x += there ? f * u[i].x : 0.0f;
+        o.y += there ? f * u[i].y : 0.0f;
+        o.z += there ? f * v[i].x : 0.0f;
+        o.w += there ? f * v[i].y : 0.0f;
+      }
     }
+    j0 += 64;
+    if (j0 >= n) break;
+    ml = *reinterpret_cast<const float2*>(part + min(j0 + lane, n - 1) * step);
   }
   sum = wave_sum(sum);
   if constexpr (W > 1) {
@@ -1767,11 +1771,16 @@ size_t shared_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
   return r.join ? (n + 255) & ~(size_t)255 : 0;
 }
 
+size_t ranges_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
+  const size_t n = (size_t)p.cache.total_tokens * p.num_q_heads * sizeof(int2);
+  return r.join ? (n + 255) & ~(size_t)255 : 0;
+}
+
 size_t workspace_of(const SpkPagedAttnArgs& p, const Plan& r) {
   const size_t part = r.splits <= 1 ? 0
                                     : (size_t)r.splits * p.cache.total_tokens * p.num_q_heads *
                                           (p.cache.head_dim + 2) * sizeof(float);
-  return shared_bytes(p, r) + part;
+  return shared_bytes(p, r) + ranges_bytes(p, r) + part;
 }
 
 template <int D, bool BF>
@@ -1900,7 +1909,8 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
   a.out = static_cast<uint16_t*>(p->out);
   a.lse = p->lse;
   a.shared = static_cast<float*>(p->workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + shared_bytes(*p, r));
+  if (r.join) a.ranges = reinterpret_cast<int2*>(static_cast<char*>(p->workspace) + shared_bytes(*p, r));
+  a.part = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + shared_bytes(*p, r) + ranges_bytes(*p, r));
   a.qt = p->q_token_stride;
   a.qh = p->q_head_stride;
   a.gt = p->gate_token_stride;
