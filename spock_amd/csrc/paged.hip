@@ -101,6 +101,12 @@ struct Mrope {
   uint8_t axis[128];
 };
 
+// A load of what is read once.
+__device__ __forceinline__ uint4 load_once(const uint16_t* p) {
+  typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)));
+}
+
 // One wave per token.  D / 16 lanes hold a head, 16 elements each: chunks of 8
 // that rotate together (HALVES: chunk j and j + rot/16; ADJACENT: the pairs
 // lie inside a chunk), so the angles of a lane are the same for every head of
@@ -109,7 +115,8 @@ struct Mrope {
 // What bounds it: memory.  32,768 tokens of 16 + 4 + 4 heads of 128 take 107 us for
 // 405 MB read and written, 3.8 TB/s (a plain copy reaches 5.1); a lane's next row
 // loaded while it turns one costs registers that other waves' loads need (115
-// us).  A decode step's is the launch.
+// us).  Rows are read past the caches' replacement: 120 us from call to result for
+// 129.  A decode step's is the launch.
 template <int D, bool BF, bool ADJ>
 __global__ __launch_bounds__(256) void mrope_append_kernel(Mrope a) {
   constexpr int L = D / 16, RG = 64 / L;  // lanes of a head, heads at a time
@@ -151,8 +158,8 @@ __global__ __launch_bounds__(256) void mrope_append_kernel(Mrope a) {
     const uint16_t* src = isq ? a.q + t * a.qt + h * a.qh : isv ? a.v + t * a.vt + h * a.vh : a.k + t * a.kt + h * a.kh;
     uint16_t* dst = isq ? a.qo + t * a.ot + h * a.oh : (isv ? a.vc : a.kc) + slot + h * a.c.head_stride;
     const uint16_t* w = isq ? a.qw : isv ? nullptr : a.kw;
-    uint4 u0 = *reinterpret_cast<const uint4*>(src + 8 * c0);
-    uint4 u1 = *reinterpret_cast<const uint4*>(src + 8 * c1);
+    uint4 u0 = load_once(src + 8 * c0);
+    uint4 u1 = load_once(src + 8 * c1);
     if (!isv) {
       float x[16];
 #pragma unroll
@@ -231,11 +238,6 @@ constexpr float kBehind = 8.0f;  // binades that the running maximum may lag
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A load of what is read once.
-__device__ __forceinline__ uint4 load_once(const uint16_t* p) {
-  typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(p)));
-}
 
 // The work of the sequences of few rows, dealt to the workgroups of a launch:
 // each takes the rows of one sequence, tile of rows and KV head over one range
