@@ -551,6 +551,9 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * sees nothing that weighs (a position before the first, bad pages, every
  * score -inf) is zero with lse -inf; keys and values that a row does not see
  * cannot reach it, whatever they hold.
+ * Values that it sees count as they are: an infinity stays one under any weight
+ * that 16 bits hold (from 2^-30 of the row's largest on in fp16, 2^-126 in bf16),
+ * and becomes NaN under a smaller one, as 0 times it does.
  * max_query_len and max_context_len: host bounds of the sequences' lengths;
  * they choose the kernels and the split of the keys, not the result, which
  * follows the device's lengths.

@@ -22,6 +22,12 @@ typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
+// Both halfwords less one, no lower than zero.
+__device__ __forceinline__ uint32_t step_down(uint32_t u) {
+  typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2_t, u), ushort2_t{1, 1}));
+}
+
 // The two 16-bit types: conversions (round to nearest even) and products.
 template <bool BF>
 struct Half;
@@ -37,6 +43,13 @@ struct Half<false> {
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, half2_t{(_Float16)a, (_Float16)b});
+  }
+  // Two numbers >= 0, each rounded toward zero and one step further: what is left
+  // of a number is then larger than zero wherever the rounded one is, so that
+  // both parts of a weight give an infinity its sign.  Rounded to nearest, what is
+  // left may be zero or less, and a row that sees an infinity got NaN.
+  static __device__ __forceinline__ uint32_t below(float a, float b) {
+    return step_down(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)));
   }
   static __device__ __forceinline__ uint16_t one(float a) { return __builtin_bit_cast(uint16_t, (_Float16)a); }
   static __device__ __forceinline__ float widen(uint16_t u) { return (float)__builtin_bit_cast(_Float16, u); }
@@ -65,6 +78,9 @@ struct Half<true> {
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, bf2_t{(__bf16)a, (__bf16)b});
+  }
+  static __device__ __forceinline__ uint32_t below(float a, float b) {
+    return step_down(__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u));
   }
   static __device__ __forceinline__ uint16_t one(float a) { return __builtin_bit_cast(uint16_t, (__bf16)a); }
   static __device__ __forceinline__ float widen(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
@@ -540,8 +556,9 @@ __device__ __forceinline__ void store_out(const Attn& a, int token, int head, in
 // product is free: lane group g supplies keys 4g..4g+3 and 16+4g..+3, which are the
 // ones its scores are.  V's A operand (8 keys of one dimension) is made from
 // 16-byte row pieces by pairing halfwords of two keys.  A weight enters as
-// two 16-bit parts (value and remainder): the kernel waits for memory, and the
-// second product keeps a few heavy keys' rounding out of the result.
+// two 16-bit parts (value and remainder, `below`: some 20 bits together in fp16,
+// 14 in bf16): the kernel waits for memory, and the second product keeps a few
+// heavy keys' rounding out of the result.
 //
 // What bounds it: memory.  64 sequences of 300 to 16000 keys, heads of 256: 1.07 GB
 // in 182 us, 5.9 TB/s, where reading alone reaches 7.1; one sequence of 130,001 keys:
@@ -712,7 +729,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
     uint4 p0, p1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = H::pack(w[2 * i], w[2 * i + 1]);
+      const uint32_t u = H::below(w[2 * i], w[2 * i + 1]);
       const float2_t x = H::unpack(u);
       (&p0.x)[i] = u;
       (&p1.x)[i] = H::pack(w[2 * i] - x.x, w[2 * i + 1] - x.y);
@@ -1024,7 +1041,7 @@ __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
     uint4 p0, p1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = H::pack(w[2 * i], w[2 * i + 1]);
+      const uint32_t u = H::below(w[2 * i], w[2 * i + 1]);
       const float2_t v = H::unpack(u);
       (&p0.x)[i] = u;
       (&p1.x)[i] = H::pack(w[2 * i] - v.x, w[2 * i + 1] - v.y);
