@@ -599,8 +599,9 @@ int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
  * SPK_VERIFY_LOGITS: rows are logits, distributions softmax(row /
  * temperature[s]) (NULL: 1); temperature <= 0 (or NaN) is greedy: a draft is
  * accepted when it is the row's largest logit, lowest index first (NaN never
- * is), and that token is the one drawn.  SPK_VERIFY_PROBS: rows are
- * probabilities (temperature must be NULL).
+ * is), and that token is the one drawn.  A temperature between 0 and 1e-30 counts
+ * as 1e-30, one of +inf as the largest finite float.  SPK_VERIFY_PROBS: rows
+ * are probabilities (temperature must be NULL).
  * out_tokens[t] = the token emitted after row t: the accepted drafts, then the
  * drawn token, then -1.  accepted[s] = accepted drafts.  logprobs (nullable):
  * log target(out_tokens[t]) (greedy: at temperature 1), 0 where -1.

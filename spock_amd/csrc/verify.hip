@@ -67,8 +67,10 @@ __device__ __forceinline__ bool better(float m, int a, float om, int oa) {
   return om > m || (om == m && (uint32_t)oa < (uint32_t)a);  // -1 is the largest index
 }
 
-// log2(e) / T, also as two floats; greedy rows count at T = 1.  The second is
-// larger than 0, so that a logit of -inf stays one.
+// log2(e) / T, also as two floats; greedy rows count at T = 1.  Both are larger
+// than 0, so that a logit of -inf stays one: T is at most the largest finite
+// float, and the second, a denormal from some 7e30 on, at least the smallest of
+// them (off by half a step of theirs, 1.7e-7 of log2(e) / T where T is largest).
 struct Heat {
   float c, lo;
   double scale;
@@ -79,9 +81,9 @@ __device__ __forceinline__ Heat heat_of(const Verify& a, int s) {
   Heat h;
   h.greedy = !(t > 0.0f);
   if (h.greedy) t = 1.0f;
-  h.scale = 1.4426950408889634 / fmax((double)t, 1e-30);
+  h.scale = 1.4426950408889634 / fmin(fmax((double)t, 1e-30), 3.4028234663852886e38);
   h.c = __uint_as_float(__float_as_uint((float)h.scale) - 1);
-  h.lo = (float)(h.scale - (double)h.c);
+  h.lo = fmaxf((float)(h.scale - (double)h.c), __uint_as_float(1));
   return h;
 }
 
