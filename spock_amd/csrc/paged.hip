@@ -8,11 +8,14 @@
 #include "capi_common.hpp"
 #include "numerics.hpp"
 #include "paged.hpp"
+#include "paged_deal.hpp"
 
 namespace {
 
 using spk_paged::Cache;
+using spk_paged::Plan;
 using spk_paged::Seq;
+using spk_paged::Share;
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
@@ -231,8 +234,7 @@ __global__ __launch_bounds__(256) void mrope_append_kernel(Mrope a) {
 // Attention over the pages.
 // ---------------------------------------------------------------------------
 
-struct Attn {
-  Cache c;
+struct Attn : spk_paged::Deal {
   const uint16_t *q, *k, *v, *gate;
   uint16_t* out;
   float* lse;
@@ -240,12 +242,8 @@ struct Attn {
   int2* ranges;   // [total_tokens * heads]: where the row's first part lies in `shared` (-1: in `part`) and how many; NULL: no join
   float* part;    // many rows: [splits][total_tokens * heads][D + 2] where splits > 1
   int64_t qt, qh, gt, gh, ot, oh;
-  int32_t heads, kv_heads, group, window;
-  int32_t many;                // a sequence has many rows from this on
-  int32_t shares, share_rows;  // few rows: workgroups, and rows of one
-  int32_t alone;               // few rows: no ranges
-  int32_t splits, chunk;       // many rows: key ranges of a tile and the least keys of one
-  int32_t few;                 // the join has [num_seqs][kv_heads][few] rows; 0: [total_tokens][heads]
+  int32_t heads;
+  int32_t few;       // the join has [num_seqs][kv_heads][few] rows; 0: [total_tokens][heads]
   float scale_log2;  // scale * log2(e)
 };
 
@@ -254,38 +252,6 @@ constexpr float kBehind = 8.0f;  // binades that the running maximum may lag
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-
-// The work of the sequences of few rows, dealt to the workgroups of a launch:
-// each takes the rows of one sequence, tile of rows and KV head over one range
-// of its keys.  The ranges' length follows from the lengths on the device, so
-// that they fill the launch once and are nearly equal: with pieces = (sequence,
-// tile, head) the number of shares for ranges of c keys is the sum of
-// ceil(keys / c) over the pieces, and c the smallest tried with no more shares
-// than workgroups.  Every workgroup finds c and its share by itself.
-struct Share {
-  int seq, tile, kvh;
-  int range, ranges, keys;  // this one of the piece's, and the keys of each
-  int lo;                   // where the first range begins
-  int first;                // the piece's first share
-};
-
-struct Load {
-  int tiles, span;  // tiles of rows, keys that they see
-};
-
-// Of sequence s; nothing past the last.  No branch before the loads: those of
-// several sequences are under way together.
-__device__ __forceinline__ Load load_of(const Attn& a, int s) {
-  const Seq sq = spk_paged::seq_at(a.c, min(s, a.c.num_seqs - 1));
-  const int rows = s < a.c.num_seqs ? sq.n * a.group : 0;
-  int lo, hi, x;
-  spk_paged::visible(sq, 0, a.window, &lo, &x);
-  spk_paged::visible(sq, sq.n - 1, a.window, &x, &hi);
-  const bool few = rows > 0 && rows < a.many;
-  return {few ? (rows + a.share_rows - 1) / a.share_rows : 0, few ? max(hi - (lo & ~31), 1) : 0};
-}
-
-__device__ __forceinline__ int ranges_of(const Load& l, int c) { return (l.span - 1) / c + (l.span > 0); }
 
 // Sum over the wave, in every lane; and the inclusive running sum.  Lane swaps
 // and DPP moves: an LDS permute is ten times as long, and every workgroup
@@ -326,102 +292,21 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The share numbered `at`.  false: there is none.
-__device__ __forceinline__ bool find_share(const Attn& a, int at, int lane, Share* out) {
-  constexpr int N = 4;  // sequences of a lane at a time
-  Load mine[N];
-  long long keys = 0;
-  int pieces = 0, low = 0, high = 0;  // keys = high * 2^16 + low
-  for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64 * N)
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      mine[j] = load_of(a, s0 + N * lane + j);
-      keys += (long long)mine[j].tiles * mine[j].span;
-      pieces += mine[j].tiles;
-    }
-  low = (int)(keys & 0xffff);
-  high = (int)(keys >> 16);
-  keys = (((long long)__builtin_amdgcn_readfirstlane(wave_sum(high)) << 16) + __builtin_amdgcn_readfirstlane(wave_sum(low))) *
-         a.kv_heads;
-  pieces = __builtin_amdgcn_readfirstlane(wave_sum(pieces)) * a.kv_heads;
-  if (pieces == 0) return false;
-  // enough for any lengths: each piece's last range may be short
-  auto whole = [](long long k) { return (int)((min(k, (long long)INT32_MAX - 128) + 127) & ~127ll); };
-  int c = INT32_MAX;
-  if (!a.alone) {
-    const int room = max(a.shares - pieces, 1);
-    c = __builtin_amdgcn_readfirstlane(whole((keys + room - 1) / room));
-  }
-  if (!a.alone && a.c.num_seqs <= 64 * N) {
-    for (int t = __builtin_amdgcn_readfirstlane(whole((keys + a.shares - 1) / a.shares)); t < c; t += max(128, (t >> 4) & ~127)) {
-      int n = 0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) n += mine[j].tiles * ranges_of(mine[j], t);
-      if (__builtin_amdgcn_readfirstlane(wave_sum(n)) * a.kv_heads <= a.shares) c = t;
-    }
-  }
-  int before = 0;
-  for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64 * N) {
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (a.c.num_seqs > 64 * N) mine[j] = load_of(a, s0 + N * lane + j);
-      n += mine[j].tiles * a.kv_heads * ranges_of(mine[j], c);
-    }
-    const int sum = wave_scan(n), total = __builtin_amdgcn_readlane(sum, 63);
-    if (at < before + total) {
-      // the lane that holds it, then the one of its sequences
-      const int l = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + sum <= at)));
-      int first = before + sum - n;
-      Load found{0, 0};
-      int s = -1;
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int count = mine[j].tiles * a.kv_heads * ranges_of(mine[j], c);
-        const bool here = at >= first && at < first + count;
-        if (s < 0) {
-          if (here) {
-            s = s0 + N * lane + j;
-            found = mine[j];
-          } else {
-            first += count;
-          }
-        }
-      }
-      s = __builtin_amdgcn_readlane(s, l);
-      first = __builtin_amdgcn_readlane(first, l);
-      found.tiles = __builtin_amdgcn_readlane(found.tiles, l);
-      found.span = __builtin_amdgcn_readlane(found.span, l);
-      if (s < 0 || found.tiles == 0) return false;
-      out->seq = s;
-      out->ranges = ranges_of(found, c);
-      out->keys = (((found.span + out->ranges - 1) / out->ranges) + 127) & ~127;
-      const int rest = at - first, piece = rest / out->ranges;
-      out->range = rest - piece * out->ranges;
-      out->tile = piece / a.kv_heads;
-      out->kvh = piece - out->tile * a.kv_heads;
-      out->first = first + (out->tile * a.kv_heads + out->kvh) * out->ranges;
-      int x;
-      spk_paged::visible(spk_paged::seq_at(a.c, out->seq), 0, a.window, &out->lo, &x);
-      out->lo &= ~31;
-      return true;
-    }
-    before += total;
-  }
-  return false;
-}
+// What the dealing of work does with a wave together (the lengths that it finds
+// are the same in all lanes: in scalar registers from there on).
+struct Wave {
+  static __device__ __forceinline__ int first(int v) { return __builtin_amdgcn_readfirstlane(v); }
+  static __device__ __forceinline__ int at(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+  static __device__ __forceinline__ int count(bool b) { return __popcll(__ballot(b)); }
+  static __device__ __forceinline__ int sum(int v) { return wave_sum(v); }
+  static __device__ __forceinline__ int max(int v) { return wave_max(v); }
+  static __device__ __forceinline__ int scan(int v) { return wave_scan(v); }
+};
 
 // Tells the join where the parts of row r of a piece or tile lie.
 __device__ __forceinline__ void tell(const Attn& a, const Seq& sq, int kvh, int r, int first, int ranges) {
   const int i = r / a.group;
   a.ranges[(int64_t)(sq.first + i) * a.heads + kvh * a.group + r - i * a.group] = make_int2(first, ranges);
-}
-
-// Keys in one range of a tile of many rows that sees [lo, hi): the plan's, or
-// more where the lengths pass the host's bound.
-__device__ __forceinline__ int range_keys(const Attn& a, int lo, int hi) {
-  const int span = max(hi - (lo & ~31), 0);
-  return max(a.chunk, (int)((((int64_t)span + a.splits - 1) / a.splits + 127) & ~127));
 }
 
 // Bit n: a row that sees keys [lo, hi) sees key k0 + n, where `has` says that
@@ -430,85 +315,6 @@ __device__ __forceinline__ uint32_t seen(uint32_t has, int k0, int lo, int hi) {
   const int first = lo - k0, last = hi - k0;
   if (first > 31 || last <= 0) return 0;
   return has & (0xffffffffu << max(first, 0)) & (0xffffffffu >> (32 - min(last, 32)));
-}
-
-// Tile `at` of the tiles of 256 of the n * group rows of the sequences of many:
-// its sequence and its index there.  false past the last of them.  Those that
-// see the most keys come first, to within 128 keys, so that the last that
-// workgroups take are short (six prompts of 16 heads over 4: 180 us, 185 with
-// the last sequence's last tile first).
-__device__ __forceinline__ bool find_tile(const Attn& a, int at, int last, int lane, int* seq, int* tile) {
-  constexpr int N = 4;  // sequences of a lane
-  if (a.c.num_seqs > 64 * N) {  // more than are looked at together: by sequence, the last tiles first
-    at = last - at;
-    for (int s0 = 0; s0 < a.c.num_seqs; s0 += 64) {
-      int mine = 0;
-      if (s0 + lane < a.c.num_seqs) {
-        const int n = spk_paged::make_seq(a.c, a.c.cu[s0 + lane], a.c.cu[s0 + lane + 1], 0).n * a.group;
-        if (n >= a.many) mine = (n + 255) / 256;
-      }
-      const int sum = wave_scan(mine), total = __builtin_amdgcn_readlane(sum, 63);
-      if (at < total) {
-        const int l = __popcll(__ballot(sum <= at));
-        *seq = s0 + l;
-        *tile = at - __builtin_amdgcn_readlane(sum - mine, l);
-        return true;
-      }
-      at -= total;
-    }
-    return false;
-  }
-  Seq sq[N];
-  int tiles[N], total = 0, top = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) sq[j] = spk_paged::seq_at(a.c, min(N * lane + j, a.c.num_seqs - 1));
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int rows = N * lane + j < a.c.num_seqs ? sq[j].n * a.group : 0;
-    tiles[j] = rows >= a.many ? (rows + 255) / 256 : 0;
-    if (tiles[j] == 0) sq[j] = {0, 0, 0};  // no tokens: past() is 0
-    total += tiles[j];
-    top = max(top, sq[j].ctx);
-  }
-  if (at >= __builtin_amdgcn_readfirstlane(wave_sum(total))) return false;
-  // tiles of the lane's sequence j that see past key 128 * level; all for -1
-  auto past = [&](int j, int level) {
-    const int64_t d = 128ll * level - sq[j].ctx + sq[j].n;  // its tokens that do not
-    return level < 0 || d <= 0 ? tiles[j] : d >= sq[j].n ? 0 : tiles[j] - ((int)d * a.group >> 8);
-  };
-  int low = -1, high = __builtin_amdgcn_readfirstlane(wave_max(top)) / 128 + 1;
-  int before = 0;  // tiles past high
-  while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j) n += past(j, mid);
-    n = __builtin_amdgcn_readfirstlane(wave_sum(n));
-    if (n > at) {
-      low = mid;
-    } else {
-      high = mid;
-      before = n;
-    }
-  }
-  at -= before;
-  int n = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) n += past(j, low) - past(j, high);
-  const int sum = wave_scan(n), l = __popcll(__ballot(sum <= at));
-  int first = sum - n, found = -1, its = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int m = past(j, low) - past(j, high);
-    if (found < 0 && at < first + m) {
-      found = N * lane + j;
-      its = tiles[j] - 1 - past(j, high) - (at - first);
-    }
-    first += m;
-  }
-  *seq = __builtin_amdgcn_readlane(found, l);
-  *tile = __builtin_amdgcn_readlane(its, l);
-  return true;
 }
 
 // 16 lanes' 8-byte pieces of 4 rows (4 lanes a row) turned: lane l of the 16
@@ -578,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int ln = lane & 15, g = lane >> 4;
   Share sh;
-  if (!find_share(a, blockIdx.x, lane, &sh)) return;
+  if (!spk_paged::find_share<Wave>(a, blockIdx.x, lane, &sh)) return;
   const int seq = sh.seq, kvh = sh.kvh;
   const Seq sq = spk_paged::seq_at(a.c, seq);
   const int rows = sq.n * a.group;
@@ -896,7 +702,7 @@ __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ln = lane & 15, g = lane >> 4;
   Share sh;
-  if (!find_share(a, blockIdx.x, lane, &sh)) return;
+  if (!spk_paged::find_share<Wave>(a, blockIdx.x, lane, &sh)) return;
   const int seq = sh.seq, kvh = sh.kvh;
   const Seq sq = spk_paged::seq_at(a.c, seq);
   const int rows = sq.n * a.group;
@@ -1221,7 +1027,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   // 316; with another at every tile, which shares fewer keys in an L2, 324).
   const int kvh = blockIdx.y, split = (blockIdx.x + (blockIdx.z >> 3)) % gridDim.x;
   int seq, tile;
-  if (!find_tile(a, blockIdx.z, gridDim.z - 1, lane, &seq, &tile)) return;
+  if (!spk_paged::find_tile<Wave>(a, blockIdx.z, gridDim.z - 1, lane, &seq, &tile)) return;
   seq = __builtin_amdgcn_readfirstlane(seq);
   tile = __builtin_amdgcn_readfirstlane(tile);
   const Seq sq = spk_paged::seq_at(a.c, seq);
@@ -1230,7 +1036,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   int lo, hi, lo_all, hi_all;
   spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
   spk_paged::visible(sq, (r1 - 1) / a.group, a.window, &lo_all, &hi);
-  const int keys = range_keys(a, lo, hi);
+  const int keys = spk_paged::range_keys(a, lo, hi);
   const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
   const int end = begin + min(keys, hi - begin);
   if (begin >= end && split > 0) return;
@@ -1706,69 +1512,6 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
   return SPK_OK;
 }
 
-constexpr int kFew = 128;  // rows of a sequence that are not many
-constexpr int64_t kMostGroups = 16777215;  // workgroups of 256 in a launch: below 2^32 threads
-
-// How a call's rows and keys are dealt to the kernels.
-struct Plan {
-  int many, shares, share_rows, tiles, splits, chunk;
-  bool join, join_few;
-  int64_t join_rows;
-};
-
-Plan plan_of(const SpkPagedAttnArgs& p) {
-  const SpkPagedCache& c = p.cache;
-  const int group = p.num_q_heads / c.num_kv_heads;
-  const int64_t tokens = std::min(p.max_query_len, c.total_tokens);
-  const int64_t longest = tokens * group, all = (int64_t)c.total_tokens * group;
-  Plan r;
-  // a call of one sequence that may have many rows goes to their kernel
-  // whatever it has; one that has none to the others
-  // Many are more than 128, two pieces of 64 (16 sequences at 4000 keys, heads of
-  // 128: 128 rows 68 us, 83 as many; 192 rows 88 as many, 118 in three pieces).
-  const bool any_many = longest > kFew;
-  r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : kFew + 1;
-  // pieces of 16 rows where none has more (16 rows: 35 us, 38 in pieces of 64;
-  // 36 rows: 42 in one of 64, 68 in three of 16)
-  r.share_rows = longest <= 16 ? 16 : 64;
-  int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
-  if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
-  const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
-
-  // sequences of few rows: all of them, unless the one there is has many.  As
-  // many workgroups as the chip holds at once (2 to a CU; with 4, 32 sequences of
-  // one token at 4000 keys take 36 us for 33), more only where the pieces alone
-  // are more, and no more than ranges of 128 keys.
-  // Next to many rows a sequence of few is two pieces; else the bound may be low.
-  const int64_t some = all / r.share_rows + c.num_seqs;
-  const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(2 * (int64_t)c.num_seqs, some) : 0);
-  const int64_t slots = 512;
-  r.shares = (int)std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)),
-                                    INT32_MAX);
-
-  // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
-  // the number of ranges that takes the fewest rounds of 256 workgroups times
-  // steps in each; a range's share of the join costs as much as some 4 steps
-  // (2048 tokens at 16384 keys, 64 workgroups: 347 us in 3 ranges, 322 in the 4 that
-  // fill the chip; six prompts in 500 workgroups: 184 us, 210 in 2 ranges each).
-  const int64_t seqs = std::min<int64_t>(c.num_seqs, all / (kFew + 1) + 1);
-  r.tiles = any_many ? (int)std::min<int64_t>((all + 255 * seqs) / 256, INT32_MAX) : 0;
-  const int64_t groups = std::max<int64_t>(1, (int64_t)r.tiles * c.num_kv_heads);
-  int64_t per = steps, least = (groups + 255) / 256 * steps;
-  for (int64_t n = 2; n <= std::min<int64_t>(512 / groups + 1, steps / 4); ++n) {
-    const int64_t in = (steps + n - 1) / n, cost = (groups * n + 255) / 256 * (in + 4);
-    if (cost < least) per = in, least = cost;
-  }
-  r.chunk = (int)(128 * per);
-  r.splits = r.tiles ? (int)((steps + per - 1) / per) : 1;
-  r.join = r.splits > 1 || (r.shares && steps > 1);
-  // rows to join: all tokens', or of each sequence those that few can be
-  const int64_t every = (int64_t)c.total_tokens * p.num_q_heads, of_few = (int64_t)c.num_seqs * c.num_kv_heads * kFew;
-  r.join_few = any_many && r.splits == 1 && of_few < every;
-  r.join_rows = r.join_few ? of_few : every;
-  return r;
-}
-
 int check_attn(const SpkPagedAttnArgs* p, Cache* c) {
   if (!p) return spk::fail(SPK_ERR_NULL, "spk_paged_attention: NULL args");
   if (const int rc = check_cache(p->cache, "spk_paged_attention", c)) return rc;
@@ -1783,23 +1526,6 @@ int check_attn(const SpkPagedAttnArgs* p, Cache* c) {
   if ((int64_t)p->cache.total_tokens * p->num_q_heads > INT32_MAX - 65536)
     return spk::fail(SPK_ERR_SHAPE, "spk_paged_attention: %d tokens of %d heads", p->cache.total_tokens, p->num_q_heads);
   return SPK_OK;
-}
-
-size_t shared_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
-  const size_t n = (size_t)r.shares * r.share_rows * (p.cache.head_dim + 2) * sizeof(float);
-  return r.join ? (n + 255) & ~(size_t)255 : 0;
-}
-
-size_t ranges_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
-  const size_t n = (size_t)p.cache.total_tokens * p.num_q_heads * sizeof(int2);
-  return r.join ? (n + 255) & ~(size_t)255 : 0;
-}
-
-size_t workspace_of(const SpkPagedAttnArgs& p, const Plan& r) {
-  const size_t part = r.splits <= 1 ? 0
-                                    : (size_t)r.splits * p.cache.total_tokens * p.num_q_heads *
-                                          (p.cache.head_dim + 2) * sizeof(float);
-  return shared_bytes(p, r) + ranges_bytes(p, r) + part;
 }
 
 template <int D, bool BF>
@@ -1831,9 +1557,9 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
   Mrope a{};
   if (const int rc = check_cache(p->cache, who, &a.c)) return rc;
   const SpkPagedCache& c = p->cache;
-  if (p->num_q_heads <= 0 || c.total_tokens > 4 * kMostGroups)
+  if (p->num_q_heads <= 0 || c.total_tokens > 4 * spk_paged::kMostGroups)
     return spk::fail(SPK_ERR_SHAPE, "%s: %d query heads, %d tokens (%lld at most)", who, p->num_q_heads, c.total_tokens,
-                     (long long)(4 * kMostGroups));
+                     (long long)(4 * spk_paged::kMostGroups));
   if (p->rot_dim <= 0 || p->rot_dim % 16 || p->rot_dim > c.head_dim)
     return spk::fail(SPK_ERR_SHAPE, "%s: rot_dim %d (a multiple of 16 up to head_dim %d)", who, p->rot_dim, c.head_dim);
   if (p->pairing != SPK_ROPE_HALVES && p->pairing != SPK_ROPE_ADJACENT)
@@ -1897,7 +1623,7 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
 extern "C" size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* p) {
   Cache c;
   if (check_attn(p, &c) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
-  return workspace_of(*p, plan_of(*p));
+  return spk_paged::workspace_of(*p, spk_paged::plan_of(*p));
 }
 
 extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t stream) {
@@ -1911,11 +1637,11 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
       !strides_ok(p->q_token_stride, p->q_head_stride) || !strides_ok(p->out_token_stride, p->out_head_stride) ||
       (p->gate && !strides_ok(p->gate_token_stride, p->gate_head_stride)))
     return spk::fail(SPK_ERR_ALIGN, "%s: q, gate and out and their strides must be 16-byte aligned", who);
-  const Plan r = plan_of(*p);
-  if (r.shares > kMostGroups || (r.join && (r.join_rows + 3) / 4 > kMostGroups))
+  const Plan r = spk_paged::plan_of(*p);
+  if (r.shares > spk_paged::kMostGroups || (r.join && (r.join_rows + 3) / 4 > spk_paged::kMostGroups))
     return spk::fail(SPK_ERR_SHAPE, "%s: %d tokens of %d heads, %d sequences are more than one launch holds", who,
                      c.total_tokens, p->num_q_heads, c.num_seqs);
-  const size_t need = workspace_of(*p, r);
+  const size_t need = spk_paged::workspace_of(*p, r);
   if (need && (!p->workspace || p->workspace_bytes < need || !spk::aligned(p->workspace, 256)))
     return spk::fail(p->workspace ? SPK_ERR_ARG : SPK_ERR_NULL, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)",
                      who, p->workspace ? p->workspace_bytes : (size_t)0, need);
@@ -1936,17 +1662,9 @@ extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t strea
   a.gh = p->gate_head_stride;
   a.ot = p->out_token_stride;
   a.oh = p->out_head_stride;
+  static_cast<spk_paged::Deal&>(a) = spk_paged::deal_of(*p, r, a.c);
   a.heads = p->num_q_heads;
-  a.kv_heads = c.num_kv_heads;
-  a.group = p->num_q_heads / c.num_kv_heads;
-  a.window = p->window;
-  a.many = r.many;
-  a.shares = r.shares;
-  a.share_rows = r.share_rows;
-  a.alone = !r.join;
-  a.splits = r.splits;
-  a.chunk = r.chunk;
-  a.few = r.join_few ? kFew : 0;
+  a.few = r.join_few ? spk_paged::kFew : 0;
   const float scale = p->scale != 0.0f ? p->scale : 1.0f / std::sqrt((float)c.head_dim);
   a.scale_log2 = scale * 1.44269504088896341f;
   hipStream_t s = spk::to_hip(stream);
