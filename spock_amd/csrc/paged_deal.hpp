@@ -86,11 +86,12 @@ SPK_HD bool find_share(const Deal& a, int at, int lane, Share* out) {
     c = W::first(whole((keys + room - 1) / room));
   }
   if (!a.alone && a.c.num_seqs <= 64 * N) {
-    for (int t = W::first(whole((keys + a.shares - 1) / a.shares)); t < c; t += larger(128, (t >> 4) & ~127)) {
+    // unsigned: the next t may pass 2^31
+    for (uint32_t t = W::first(whole((keys + a.shares - 1) / a.shares)); t < (uint32_t)c; t += larger(128, (int)(t >> 4) & ~127)) {
       int n = 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) n += mine[j].tiles * ranges_of(mine[j], t);
-      if (W::first(W::sum(n)) * a.kv_heads <= a.shares) c = t;
+      for (int j = 0; j < N; ++j) n += mine[j].tiles * ranges_of(mine[j], (int)t);
+      if (W::first(W::sum(n)) * a.kv_heads <= a.shares) c = (int)t;
     }
   }
   int before = 0;
@@ -128,7 +129,7 @@ SPK_HD bool find_share(const Deal& a, int at, int lane, Share* out) {
       if (s < 0 || found.tiles == 0) return false;
       out->seq = s;
       out->ranges = ranges_of(found, c);
-      out->keys = (((found.span + out->ranges - 1) / out->ranges) + 127) & ~127;
+      out->keys = ((int)(((uint32_t)found.span + out->ranges - 1) / out->ranges) + 127) & ~127;
       const int rest = at - first, piece = rest / out->ranges;
       out->range = rest - piece * out->ranges;
       out->tile = piece / a.kv_heads;

@@ -268,3 +268,18 @@ def test_lengths_and_offsets_from_outside(shim, seed):
     call = Call(shim, cu, ctx, total=500, max_pages=100, max_q=int(rng.choice([1, 40, 500])), max_c=1000)
     call.check_shares(exact=False)
     call.check_tiles(exact=False)
+
+
+def test_lengths_next_to_the_largest(shim):
+    """Contexts of nearly 2^31 positions: the tried length of a range stays below it."""
+    call = Call(shim, *_cu([(1, 2 ** 31 - 2 ** 21)] * 256), heads=8, kv=8, page=2 ** 20, max_pages=2047)
+    assert call.join
+    call.check_shares()
+
+
+def test_more_ranges_of_the_largest_length_than_it_lacks_to_two_to_the_31(shim):
+    call = Call(shim, *_cu([(0, 0)] * 70000 + [(1, 2 ** 31 - 2 ** 13)]), heads=1, kv=1, page=2 ** 12, max_pages=2 ** 19 - 2)
+    for at in (0, 1, 5000):
+        x = call.share_of(at)
+        assert x["seq"] == 70000 and x["range"] == at and x["ranges"] > 2 ** 13 and x["keys"] % 128 == 0
+        assert x["keys"] > 0 and 0 <= x["keys"] * x["ranges"] - (2 ** 31 - 2 ** 13) < 129 * x["ranges"]
