@@ -557,9 +557,12 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * max_query_len and max_context_len: host bounds of the sequences' lengths;
  * they choose the kernels and the split of the keys, not the result, which
  * follows the device's lengths.
- * workspace: 256-byte aligned, spk_paged_attention_workspace_size() bytes,
- * contents ignored (may be 0 bytes: then NULL is fine).  Calls that overlap on
- * one workspace race.
+ * workspace: 256-byte aligned, contents ignored, NULL where 0 bytes suffice.
+ * spk_paged_attention_workspace_size() bytes are enough for the call and for
+ * every one of the same heads and head_dim whose tokens, sequences, bounds,
+ * table and window (0 is the widest) are no larger, so that a caller asks once,
+ * with its largest sizes; a call may need less and takes what it needs.  Calls
+ * that overlap on one workspace race.
  * Limits: page_stride and token_stride below 2^32 elements, max_pages *
  * page_size at most 2^31 - 4096 positions, 65535 KV heads and row tiles (of
  * 256) in a call, and 2^24 workgroups of a launch (some 67 million rows).

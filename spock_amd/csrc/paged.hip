@@ -1623,7 +1623,7 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
 extern "C" size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* p) {
   Cache c;
   if (check_attn(p, &c) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
-  return spk_paged::workspace_of(*p, spk_paged::plan_of(*p));
+  return spk_paged::workspace_bound(*p);
 }
 
 extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t stream) {

@@ -244,7 +244,16 @@ struct Plan {
   int many, shares, share_rows, tiles, splits, chunk;
   bool join, join_few;
   int64_t join_rows;
+  int64_t longest, steps;  // rows of a sequence, and steps of 128 keys, by the bounds
 };
+
+// Workgroups of the sequences of few rows.  As many as the chip holds at once (2 to
+// a CU; with 4, 32 sequences of one token at 4000 keys take 36 us for 33), more
+// only where the pieces alone are more, and no more than ranges of 128 keys.
+inline int64_t shares_of(int64_t pieces, int64_t steps) {
+  const int64_t slots = 512;
+  return std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)), INT32_MAX);
+}
 
 inline Plan plan_of(const SpkPagedAttnArgs& p) {
   const SpkPagedCache& c = p.cache;
@@ -252,6 +261,7 @@ inline Plan plan_of(const SpkPagedAttnArgs& p) {
   const int64_t tokens = std::min(p.max_query_len, c.total_tokens);
   const int64_t longest = tokens * group, all = (int64_t)c.total_tokens * group;
   Plan r;
+  r.longest = longest;
   // a call of one sequence that may have many rows goes to their kernel
   // whatever it has; one that has none to the others
   // Many are more than 128, two pieces of 64 (16 sequences at 4000 keys, heads of
@@ -264,17 +274,13 @@ inline Plan plan_of(const SpkPagedAttnArgs& p) {
   int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
   if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
   const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
+  r.steps = steps;
 
-  // sequences of few rows: all of them, unless the one there is has many.  As
-  // many workgroups as the chip holds at once (2 to a CU; with 4, 32 sequences of
-  // one token at 4000 keys take 36 us for 33), more only where the pieces alone
-  // are more, and no more than ranges of 128 keys.
+  // sequences of few rows: all of them, unless the one there is has many.
   // Next to many rows a sequence of few is two pieces; else the bound may be low.
   const int64_t some = all / r.share_rows + c.num_seqs;
   const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(2 * (int64_t)c.num_seqs, some) : 0);
-  const int64_t slots = 512;
-  r.shares = (int)std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)),
-                                    INT32_MAX);
+  r.shares = (int)shares_of(pieces, steps);
 
   // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
   // the number of ranges that takes the fewest rounds of 256 workgroups times
@@ -299,21 +305,43 @@ inline Plan plan_of(const SpkPagedAttnArgs& p) {
   return r;
 }
 
+inline size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Of one row's part: its maximum, its sum and its output.
+inline size_t part_bytes(const SpkPagedAttnArgs& p) { return (p.cache.head_dim + 2) * sizeof(float); }
+
 inline size_t shared_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
-  const size_t n = (size_t)r.shares * r.share_rows * (p.cache.head_dim + 2) * sizeof(float);
-  return r.join ? (n + 255) & ~(size_t)255 : 0;
+  return r.join ? up((size_t)r.shares * r.share_rows * part_bytes(p)) : 0;
 }
 
 inline size_t ranges_bytes(const SpkPagedAttnArgs& p, const Plan& r) {
-  const size_t n = (size_t)p.cache.total_tokens * p.num_q_heads * 2 * sizeof(int32_t);
-  return r.join ? (n + 255) & ~(size_t)255 : 0;
+  return r.join ? up((size_t)p.cache.total_tokens * p.num_q_heads * 2 * sizeof(int32_t)) : 0;
 }
 
 inline size_t workspace_of(const SpkPagedAttnArgs& p, const Plan& r) {
-  const size_t part = r.splits <= 1 ? 0
-                                    : (size_t)r.splits * p.cache.total_tokens * p.num_q_heads *
-                                          (p.cache.head_dim + 2) * sizeof(float);
+  const size_t part = r.splits <= 1 ? 0 : (size_t)r.splits * p.cache.total_tokens * p.num_q_heads * part_bytes(p);
   return shared_bytes(p, r) + ranges_bytes(p, r) + part;
+}
+
+// Bytes that no call exceeds whose tokens, sequences, bounds, window and table are
+// at most these.  What a plan needs is not monotone in them: more rows leave fewer
+// ranges and pieces of other sizes (one sequence of up to 32,768 keys, 8 heads of 256
+// over 2: 8 MB for one token, 34 for 9, none for 8,192).  So the largest of each
+// part: shares of either size; and with groups = tiles * KV heads, of at most 256
+// rows each, up to 512 / groups + 1 ranges of at least 4 steps while that is more
+// than one.
+inline size_t workspace_bound(const SpkPagedAttnArgs& p) {
+  const SpkPagedCache& c = p.cache;
+  const Plan r = plan_of(p);
+  const int64_t all = (int64_t)c.total_tokens * (p.num_q_heads / c.num_kv_heads), rows = (int64_t)c.total_tokens * p.num_q_heads;
+  if (r.steps <= 1) return 0;
+  auto shared = [&](int64_t share_rows) { return share_rows * shares_of(c.num_kv_heads * (all / share_rows + c.num_seqs), r.steps); };
+  int64_t parts = shared(16);
+  if (r.longest > 16) parts = std::max(parts, shared(64));
+  int64_t split = 0;
+  if (r.longest > kFew && r.steps >= 8)
+    split = std::min(131072 + 256 * std::min<int64_t>(512, (all + 255) / 256 * c.num_kv_heads), rows * (r.steps / 4));
+  return up(parts * part_bytes(p)) + up(rows * 2 * sizeof(int32_t)) + split * part_bytes(p);
 }
 
 // What the kernels know of it.

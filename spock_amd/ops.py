@@ -420,6 +420,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sequences' lengths; scale 0 = 1/sqrt(D); window > 0: only the last `window` positions are seen; gate [T][Hq][D]:
     the output is multiplied by sigmoid(gate).  Returns out [T][Hq][D], or (out, lse [T][Hq] float32) with return_lse
     or an lse buffer.  Rows past cu_seqlens[S] are not written.
+    workspace: paged_attention_workspace_bytes() of the largest sizes in use; one that is too small is left alone and a
+    fresh one taken.
     """
     what = "paged_attention"
     cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
@@ -449,7 +451,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def paged_attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
                                     max_pages: int, num_seqs: int, max_query_len: int, max_context_len: int,
                                     window: int = 0) -> int:
-    """Bytes of paged_attention's workspace for these sizes, for callers that keep one."""
+    """Bytes of a workspace for paged_attention at these sizes and any smaller ones, for callers that keep one."""
     cache = SpkPagedCache(_lib.SPK_F16, kv_heads, head_dim, page_size, 1, max_pages, num_seqs, tokens, 16, 16, 0, 0, 0,
                           16, max_pages, 16, 16)
     a = SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window)

@@ -1,0 +1,39 @@
+"""GPU runs of the paged operators on one workspace that was sized for the
+largest call and holds anything: every smaller call is as with one of its own,
+and nothing behind the size is written."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_paged import DT, _i32, _normal, _tables
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 4096
+
+
+def _kept(need, dev):
+    """A workspace of NaN with a guard behind it."""
+    return torch.full((need + GUARD,), 0xFF, dtype=torch.uint8, device=dev)
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim", [("f16", 8, 2, 256), ("bf16", 12, 3, 64)])
+def test_attention_on_the_largest_calls_workspace(dev, dtype, heads, kv, dim):
+    from spock_amd import ops
+    gen = torch.Generator().manual_seed(dim)
+    page, cols, most_c = 16, 320, 5000
+    need = ops.paged_attention_workspace_bytes(600, heads, kv, dim, page, cols, 8, 500, most_c)
+    ws = _kept(need, dev)
+    for lens in ([(1, 5000)], [(9, 4900)], [(33, 2000)], [(500, 5000)], [(17, 300), (1, 4000)], [(1, 700 + 500 * i) for i in range(8)],
+                 [(100, 900), (200, 5000), (3, 4000), (1, 1)]):
+        print(f"[kept workspace {dtype} {heads}/{kv}x{dim} {lens}]", flush=True)
+        cu, ctx, table, pages = _tables(lens, page, dim)
+        kc, vc = (_normal(gen, pages, page, kv, dim, dtype=DT[dtype]).to(dev) for _ in range(2))
+        q = _normal(gen, cu[-1], heads, dim, dtype=DT[dtype]).to(dev)
+        args = (q, kc, vc, table.to(dev), _i32(cu, dev), _i32(ctx, dev), max(n for n, _ in lens), max(ctx))
+        want = ops.paged_attention(*args, return_lse=True)
+        have = ops.paged_attention(*args, return_lse=True, workspace=ws[:need])
+        torch.cuda.synchronize()
+        assert torch.equal(want[0], have[0]) and torch.equal(want[1], have[1])
+        assert bool((ws[need:] == 0xFF).all())
+    assert bool((ws[:need] != 0xFF).any())

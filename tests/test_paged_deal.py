@@ -122,6 +122,20 @@ int tile_of(int at, int* out) {
   out[2] = tile[0];
   return !torn;
 }
+size_t bound(const int* sizes) {
+  SpkPagedAttnArgs p{};
+  p.num_q_heads = sizes[0];
+  p.cache.num_kv_heads = sizes[1];
+  p.cache.head_dim = sizes[2];
+  p.cache.page_size = sizes[3];
+  p.cache.max_pages = sizes[4];
+  p.cache.num_seqs = sizes[5];
+  p.cache.total_tokens = sizes[6];
+  p.max_query_len = sizes[7];
+  p.max_context_len = sizes[8];
+  p.window = sizes[9];
+  return workspace_bound(p);
+}
 int keys_of(int lo, int hi) { return range_keys(deal, lo, hi); }
 }
 '''
@@ -135,7 +149,7 @@ def shim(tmp_path_factory):
                         str(d / "shim.cpp"), "-o", str(d / "shim.so")], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-2000:]
     lib = C.CDLL(str(d / "shim.so"))
-    lib.plan.restype = C.c_size_t
+    lib.plan.restype = lib.bound.restype = C.c_size_t
     return lib
 
 
@@ -283,3 +297,38 @@ def test_more_ranges_of_the_largest_length_than_it_lacks_to_two_to_the_31(shim):
         x = call.share_of(at)
         assert x["seq"] == 70000 and x["range"] == at and x["ranges"] > 2 ** 13 and x["keys"] % 128 == 0
         assert x["keys"] > 0 and 0 <= x["keys"] * x["ranges"] - (2 ** 31 - 2 ** 13) < 129 * x["ranges"]
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 256), (16, 4, 128), (7, 1, 64), (40, 2, 64), (4, 4, 128)])
+@pytest.mark.parametrize("most", [(8192, 64, 8192, 32768, 0), (300, 300, 9, 5000, 0), (4096, 1, 4096, 131072, 0), (2000, 16, 500, 20000, 1024),
+                                  (64, 64, 1, 200, 0), (700, 3, 600, 1200, 0)], ids=str)
+def test_a_workspace_of_the_largest_sizes_serves_the_smaller(shim, heads, kv, dim, most):
+    out = (C.c_int * 8)()
+
+    def sizes(T, S, q, c, w):
+        return (C.c_int * 10)(heads, kv, dim, 16, 10000, S, T, q, c, w)
+
+    kept, largest = shim.bound(sizes(*most)), 0
+    rng = np.random.default_rng(most[0] + heads)
+    T, S, q, c, w = most
+    log = lambda top: int(round(np.exp(rng.uniform(0, np.log(top)))))
+    tried = [most] + [(log(T), log(S), log(q), log(c), w) for _ in range(6000)]
+    tried += [(t, min(s, S), min(t, q), x, w) for t in list(range(1, min(T, 400))) + list(range(400, T + 1, 97)) for s in (1, 8) for x in (c, c // 3 + 1)]
+    if w == 0:
+        tried += [(log(T), log(S), log(q), c, log(5000)) for _ in range(500)]
+    for x in tried:
+        need = shim.plan(sizes(*x), None, None, out)
+        assert need <= kept and need <= shim.bound(sizes(*x)), (x, need, kept)
+        assert shim.bound(sizes(*x)) <= kept, x
+        largest = max(largest, need)
+    # and not much more than the largest need of them
+    assert kept <= 3.5 * largest + 4096, (kept, largest)
+
+
+def test_the_size_that_the_library_tells(shim):
+    """Through the entry point: one that a smaller call needs more of than a larger one does."""
+    from spock_amd import ops
+    args = dict(heads=8, kv_heads=2, head_dim=256, page_size=16, max_pages=2048, num_seqs=1, max_context_len=32768)
+    kept = ops.paged_attention_workspace_bytes(tokens=8192, max_query_len=8192, **args)
+    for n in (1, 4, 9, 16, 32, 33, 100, 500, 2048, 4000, 8000):
+        assert 0 < ops.paged_attention_workspace_bytes(tokens=n, max_query_len=n, **args) <= kept
