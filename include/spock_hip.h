@@ -613,7 +613,9 @@ int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
  * token is fed.  A drawn row without a distribution (NaN, no mass) emits -1.
  * Tokens outside [0, vocab) are refused; a sequence without rows only gets
  * accepted[s] = 0 and its context.  Comparisons and running sums are fp64.
- * workspace: 256-byte aligned, contents ignored; overlapping calls race on it. */
+ * workspace: 256-byte aligned, contents ignored; overlapping calls race on it.
+ * spk_verify_drafts_workspace_size() bytes serve every call of no larger vocab,
+ * num_seqs and total_tokens.  Limits: 65535 rows and sequences. */
 enum { SPK_VERIFY_LOGITS = 0, SPK_VERIFY_PROBS = 1 };
 typedef struct SpkVerifyArgs {
   int32_t kind;

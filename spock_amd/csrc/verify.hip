@@ -640,12 +640,27 @@ void launch(const Verify& a, hipStream_t s) {
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Bytes of a call, and of the largest with no more entries, sequences and rows: a
+// row has fewer parts the more rows there are, but all of them no more than the
+// 2,048 that fill the chip or one each; and small pieces are chosen up to 512
+// large ones, which are 2,048 small ones.
+size_t workspace_of(int64_t stats, int64_t seqs, int64_t masses) {
+  return up(sizeof(Stat) * 2 * (size_t)stats) + up(sizeof(Left) * (size_t)seqs) + sizeof(double) * 2 * (size_t)masses;
+}
+size_t workspace_of_call(int vocab, int seqs, int rows) {
+  return workspace_of((int64_t)rows * parts_of(vocab, rows), seqs, (int64_t)seqs * pieces_of(vocab, seqs));
+}
+size_t workspace_bound(int vocab, int64_t seqs, int64_t rows) {
+  const int64_t large = seqs * (((int64_t)vocab + 4095) / 4096), small = seqs * (((int64_t)vocab + 1023) / 1024);
+  const int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)vocab + 2047) / 2048);
+  return workspace_of(std::max(rows, std::min<int64_t>(2048, rows * parts)), seqs, std::max(large, std::min<int64_t>(2048, small)));
+}
+
 }  // namespace
 
 extern "C" size_t spk_verify_drafts_workspace_size(int32_t vocab, int32_t num_seqs, int32_t total_tokens) {
   if (vocab <= 0 || num_seqs <= 0 || total_tokens <= 0) return 0;
-  const size_t stats = sizeof(Stat) * 2 * (size_t)total_tokens * parts_of(vocab, total_tokens);
-  return up(stats) + up(sizeof(Left) * (size_t)num_seqs) + sizeof(double) * 2 * (size_t)num_seqs * pieces_of(vocab, num_seqs);
+  return workspace_bound(vocab, num_seqs, total_tokens);
 }
 
 extern "C" int spk_verify_drafts(const SpkVerifyArgs* p, spk_stream_t stream) {
@@ -673,7 +688,7 @@ extern "C" int spk_verify_drafts(const SpkVerifyArgs* p, spk_stream_t stream) {
     const size_t size = p->dtype == SPK_F32 ? 4 : 2;
     if (!spk::aligned(p->target, size) || !spk::aligned(p->draft, size))
       return spk::fail(SPK_ERR_ALIGN, "%s: target and draft must be aligned to their type", who);
-    const size_t need = spk_verify_drafts_workspace_size(p->vocab, p->num_seqs, p->total_tokens);
+    const size_t need = workspace_of_call(p->vocab, p->num_seqs, p->total_tokens);
     if (!p->workspace || p->workspace_bytes < need || !spk::aligned(p->workspace, 256))
       return spk::fail(p->workspace ? SPK_ERR_ARG : SPK_ERR_NULL, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)",
                        who, p->workspace ? p->workspace_bytes : (size_t)0, need);

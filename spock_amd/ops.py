@@ -463,6 +463,7 @@ _KINDS = {"logits": _lib.SPK_VERIFY_LOGITS, "probs": _lib.SPK_VERIFY_PROBS}
 
 
 def verify_workspace_bytes(vocab: int, num_seqs: int, tokens: int) -> int:
+    """Bytes of a workspace for verify_drafts at these sizes and any smaller ones."""
     return int(lib().spk_verify_drafts_workspace_size(vocab, num_seqs, tokens))
 
 
@@ -479,7 +480,8 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     sequence, the last accepted token's first; draft [T][vocab]: the rows that the drafts were drawn from, None for a
     drafter that is certain; temperature [S] float32 (logits; None = 1, 0 = greedy); u_accept [T], u_sample [S] float32
     in [0, 1).  Returns (out_tokens [T] int32, accepted [S] int32, logprobs [T] float32, context_out [S] int32 or None
-    without context_lens).  Rows past cu_seqlens[S] are not written.
+    without context_lens).  Rows past cu_seqlens[S] are not written.  workspace: verify_workspace_bytes() of the largest
+    sizes in use; one that is too small is left alone and a fresh one taken.
     """
     what = "verify_drafts"
     dev = _device(what, target)

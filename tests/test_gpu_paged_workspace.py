@@ -37,3 +37,18 @@ def test_attention_on_the_largest_calls_workspace(dev, dtype, heads, kv, dim):
         assert torch.equal(want[0], have[0]) and torch.equal(want[1], have[1])
         assert bool((ws[need:] == 0xFF).all())
     assert bool((ws[:need] != 0xFF).any())
+
+
+def test_verification_on_the_largest_calls_workspace(dev):
+    from spock_amd import ops
+    from test_gpu_verify import _call, _case, _check, _inputs, _want
+    vocab = 9001
+    need = ops.verify_workspace_bytes(vocab, 40, 200)
+    ws = _kept(need, dev)
+    for v, rows in ((9001, [5] * 40), (9001, [5] * 8), (9001, [1]), (9000, [9, 1, 3]), (70, [2] * 40), (4097, [7] * 20)):
+        print(f"[kept workspace verify {v} x {len(rows)}]", flush=True)
+        c = _case(v + len(rows), v, rows, "f16", temps=(1.0, 0.0, 0.7))
+        got = _call(_inputs(c, dev), workspace=ws[:need])
+        torch.cuda.synchronize()
+        _check(got, _want(c))
+        assert bool((ws[need:] == 0xFF).all())
