@@ -561,8 +561,9 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * spk_paged_attention_workspace_size() bytes are enough for the call and for
  * every one of the same heads and head_dim whose tokens, sequences, bounds,
  * table and window (0 is the widest) are no larger, so that a caller asks once,
- * with its largest sizes; a call may need less and takes what it needs.  Calls
- * that overlap on one workspace race.
+ * with its largest sizes; a call may need less and takes what it needs.  The
+ * query reads the sizes alone: the buffers may be NULL.  Calls that overlap on
+ * one workspace race.
  * Limits: page_stride and token_stride below 2^32 elements, max_pages *
  * page_size at most 2^31 - 4096 positions, 65535 KV heads and row tiles (of
  * 256) in a call, and 2^24 workgroups of a launch (some 67 million rows).

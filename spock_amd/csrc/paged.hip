@@ -1471,8 +1471,9 @@ bool strides_ok(int64_t token, int64_t head) {
   return token >= 0 && head >= 0 && token % 8 == 0 && head % 8 == 0;
 }
 
-// Checks the cache and fills the kernels' view of it.
-int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
+// Checks the cache (its sizes alone where there are no buffers yet) and fills the
+// kernels' view of it.
+int check_cache(const SpkPagedCache& p, const char* who, Cache* c, bool buffers) {
   if (p.dtype != SPK_F16 && p.dtype != SPK_BF16)
     return spk::fail(SPK_ERR_ARG, "%s: dtype %d (SPK_F16 or SPK_BF16)", who, p.dtype);
   if (p.head_dim != 64 && p.head_dim != 128 && p.head_dim != 256)
@@ -1483,7 +1484,7 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
                      who, p.num_kv_heads, p.page_size, p.num_pages, p.max_pages, p.num_seqs, p.total_tokens);
   if ((int64_t)p.max_pages * p.page_size > INT32_MAX - 4096)
     return spk::fail(SPK_ERR_SHAPE, "%s: max_pages %d of %d tokens pass 2^31 positions", who, p.max_pages, p.page_size);
-  if (p.num_seqs && p.total_tokens) {
+  if (buffers && p.num_seqs && p.total_tokens) {
     if (!p.k_cache || !p.v_cache || !p.block_table || !p.cu_seqlens || !p.context_lens)
       return spk::fail(SPK_ERR_NULL, "%s: k_cache, v_cache, block_table, cu_seqlens or context_lens is NULL", who);
     if (!spk::aligned(p.k_cache, 16) || !spk::aligned(p.v_cache, 16) || !strides_ok(p.token_stride, p.head_stride) ||
@@ -1512,9 +1513,9 @@ int check_cache(const SpkPagedCache& p, const char* who, Cache* c) {
   return SPK_OK;
 }
 
-int check_attn(const SpkPagedAttnArgs* p, Cache* c) {
+int check_attn(const SpkPagedAttnArgs* p, Cache* c, bool buffers) {
   if (!p) return spk::fail(SPK_ERR_NULL, "spk_paged_attention: NULL args");
-  if (const int rc = check_cache(p->cache, "spk_paged_attention", c)) return rc;
+  if (const int rc = check_cache(p->cache, "spk_paged_attention", c, buffers)) return rc;
   if (p->num_q_heads <= 0 || p->num_q_heads % p->cache.num_kv_heads)
     return spk::fail(SPK_ERR_SHAPE, "spk_paged_attention: %d query heads over %d KV heads", p->num_q_heads,
                      p->cache.num_kv_heads);
@@ -1555,7 +1556,7 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
   const char* who = "spk_mrope_append";
   if (!p) return spk::fail(SPK_ERR_NULL, "%s: NULL args", who);
   Mrope a{};
-  if (const int rc = check_cache(p->cache, who, &a.c)) return rc;
+  if (const int rc = check_cache(p->cache, who, &a.c, true)) return rc;
   const SpkPagedCache& c = p->cache;
   if (p->num_q_heads <= 0 || c.total_tokens > 4 * spk_paged::kMostGroups)
     return spk::fail(SPK_ERR_SHAPE, "%s: %d query heads, %d tokens (%lld at most)", who, p->num_q_heads, c.total_tokens,
@@ -1622,14 +1623,14 @@ extern "C" int spk_mrope_append(const SpkMropeArgs* p, spk_stream_t stream) {
 
 extern "C" size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* p) {
   Cache c;
-  if (check_attn(p, &c) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
+  if (check_attn(p, &c, false) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
   return spk_paged::workspace_bound(*p);
 }
 
 extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t stream) {
   const char* who = "spk_paged_attention";
   Attn a{};
-  if (const int rc = check_attn(p, &a.c)) return rc;
+  if (const int rc = check_attn(p, &a.c, true)) return rc;
   const SpkPagedCache& c = p->cache;
   if (c.num_seqs == 0 || c.total_tokens == 0) return SPK_OK;
   if (!p->q || !p->out) return spk::fail(SPK_ERR_NULL, "%s: q or out is NULL", who);

@@ -332,3 +332,18 @@ def test_the_size_that_the_library_tells(shim):
     kept = ops.paged_attention_workspace_bytes(tokens=8192, max_query_len=8192, **args)
     for n in (1, 4, 9, 16, 32, 33, 100, 500, 2048, 4000, 8000):
         assert 0 < ops.paged_attention_workspace_bytes(tokens=n, max_query_len=n, **args) <= kept
+
+
+def test_the_size_needs_no_buffers():
+    from spock_amd import _lib, ops
+    lib = _lib.lib()
+    cache = _lib.SpkPagedCache(_lib.SPK_BF16, 2, 256, 16, 100, 2048, 3, 40)
+    a = _lib.SpkPagedAttnArgs(cache, 8, 20, 32768)
+    want = ops.paged_attention_workspace_bytes(40, 8, 2, 256, 16, 2048, 3, 20, 32768)
+    assert lib.spk_paged_attention_workspace_size(C.byref(a)) == want > 0
+    assert lib.spk_paged_attention(C.byref(a), None) == -1      # the call itself does need them
+    for bad in (dict(num_q_heads=7), dict(window=-1), dict(max_context_len=-1)):
+        b = _lib.SpkPagedAttnArgs(cache, 8, 20, 32768)
+        for k, v in bad.items():
+            setattr(b, k, v)
+        assert lib.spk_paged_attention_workspace_size(C.byref(b)) == 0
