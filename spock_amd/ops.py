@@ -311,6 +311,12 @@ def _rows(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape):
     return strides
 
 
+def _workspace(what: str, t: torch.Tensor, dev: int) -> None:
+    """The kernels write all of its bytes in a row: of a view with gaps or repeats those are not its own."""
+    if t.get_device() != dev or not t.is_contiguous():
+        raise _lib.SpockError(f"{what}: workspace must be contiguous and on cuda:{dev}, got strides {t.stride()} on {t.device}")
+
+
 def _device(what: str, t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise _lib.SpockError(f"{what}: expected device tensors")
@@ -441,8 +447,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if need:
         if workspace is None or workspace.numel() * workspace.element_size() < need:
             workspace = q.new_empty(need, dtype=torch.uint8)
-        elif workspace.get_device() != dev:
-            raise _lib.SpockError(f"{what}: workspace must be on cuda:{dev}, got {workspace.device}")
+        else:
+            _workspace(what, workspace, dev)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _call(lib().spk_paged_attention, a, dev, what)
     return out if lse is None else (out, lse)
@@ -524,8 +530,8 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     need = lib().spk_verify_drafts_workspace_size(vocab, S, T)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=target.device)
-    elif workspace.get_device() != dev:
-        raise _lib.SpockError(f"{what}: workspace must be on cuda:{dev}, got {workspace.device}")
+    else:
+        _workspace(what, workspace, dev)
     a = SpkVerifyArgs(_KINDS[kind], _ROWS[target.dtype], vocab, S, T, cu_seqlens.data_ptr(), tokens.data_ptr(),
                       target.data_ptr(), stride, _ptr(draft), draft_stride, _ptr(temperature), u_accept.data_ptr(),
                       u_sample.data_ptr(), out_tokens.data_ptr(), accepted.data_ptr(), logprobs.data_ptr(),

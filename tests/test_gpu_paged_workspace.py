@@ -52,3 +52,23 @@ def test_verification_on_the_largest_calls_workspace(dev):
         torch.cuda.synchronize()
         _check(got, _want(c))
         assert bool((ws[need:] == 0xFF).all())
+
+
+def test_workspaces_that_are_no_buffer_are_refused(dev):
+    """Views with gaps or repeats, whose bytes in a row are not their own, and other devices."""
+    from spock_amd import _lib, ops
+    from test_gpu_verify import _call, _case, _inputs
+    need = ops.paged_attention_workspace_bytes(1, 8, 2, 64, 16, 320, 1, 1, 5000)
+    cu, ctx, table, pages = _tables([(1, 5000)], 16, 0)
+    c = torch.zeros(pages, 16, 2, 64, dtype=torch.float16, device=dev)
+    q = torch.zeros(1, 8, 64, dtype=torch.float16, device=dev)
+    args = (q, c, c, table.to(dev), _i32(cu, dev), _i32(ctx, dev), 1, 5000)
+    v = _inputs(_case(1, 64, [2, 2], "f16"), dev)
+    for size, call in ((need, lambda ws: ops.paged_attention(*args, workspace=ws)),
+                       (ops.verify_workspace_bytes(64, 2, 4), lambda ws: _call(v, workspace=ws))):
+        call(torch.empty(size, dtype=torch.uint8, device=dev))
+        for ws in (torch.empty(2 * size, dtype=torch.uint8, device=dev)[::2], torch.empty(1, dtype=torch.uint8, device=dev).expand(size),
+                   torch.empty(size, dtype=torch.uint8)):
+            with pytest.raises(_lib.SpockError, match="workspace"):
+                call(ws)
+    torch.cuda.synchronize()
