@@ -373,7 +373,8 @@ def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary positions with several axes, and the store into the pages (spk_mrope_append).
 
-    q [T][Hq][D], k, v [T][Hkv][D] (float16 or bfloat16, any token and head strides); positions [axes][T] int32;
+    q [T][Hq][D], k, v [T][Hkv][D] (float16 or bfloat16, any token and head strides); positions [axes][T] int32 (for text
+    also one row expanded to all axes);
     rope [rows][rot_dim] float32, (cos, sin) per pair; pair_axis: the axis of each of the rot_dim / 2 pairs (host);
     caches [pages][page_size][Hkv][D] (any page, token and head strides, the same for both); block_table
     [S][max_pages], cu_seqlens [S+1], context_lens [S] int32 on the device.  q and k are normalised first where a
@@ -399,6 +400,10 @@ def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     _on(what, "positions", positions, dev, torch.int32, (num_axes, T))
     if T > 1 and positions.stride(1) != 1:
         raise _lib.SpockError(f"{what}: positions must have contiguous rows")
+    if 1 < num_axes <= 4 and positions.stride(0) == 0:  # one row broadcast to all axes
+        if max(axes, default=0) >= num_axes:
+            raise _lib.SpockError(f"{what}: pair_axis names axis {max(axes)} of {num_axes}")
+        num_axes, axes = 1, bytes(len(axes))
     if q_norm_weight is not None:
         _flat(what, "q_norm_weight", q_norm_weight, dev, dtype, (D,))
     if k_norm_weight is not None:
