@@ -612,6 +612,7 @@ int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
  * context_out (nullable, with context_lens; may be the same buffer):
  * context_lens[s] less the refused drafts, the cache's length before the drawn
  * token is fed.  A drawn row without a distribution (NaN, no mass) emits -1.
+ * Apart from context_out no output may overlap an input, nor another output.
  * Tokens outside [0, vocab) are refused; a sequence without rows only gets
  * accepted[s] = 0 and its context.  Comparisons and running sums are fp64.
  * workspace: 256-byte aligned, contents ignored; overlapping calls race on it.

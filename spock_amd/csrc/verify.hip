@@ -693,6 +693,15 @@ extern "C" int spk_verify_drafts(const SpkVerifyArgs* p, spk_stream_t stream) {
       return spk::fail(p->workspace ? SPK_ERR_ARG : SPK_ERR_NULL, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)",
                        who, p->workspace ? p->workspace_bytes : (size_t)0, need);
   }
+  // every workgroup of a sequence reads its inputs, and one writes
+  const void* ins[] = {p->cu_seqlens, p->tokens, p->target, p->draft, p->temperature, p->u_accept, p->u_sample, p->context_lens};
+  const void* outs[] = {p->out_tokens, p->accepted, p->logprobs, p->context_out};
+  for (int i = 0; i < 4; ++i) {
+    bool own = true;
+    for (const void* in : ins) own = own && (outs[i] != in || (i == 3 && in == p->context_lens));
+    for (int j = 0; j < i; ++j) own = own && outs[i] != outs[j];
+    if (outs[i] && !own) return spk::fail(SPK_ERR_ARG, "%s: an output is an input or another output", who);
+  }
   Verify a{};
   a.target = p->target;
   a.draft = p->draft;

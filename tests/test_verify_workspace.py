@@ -1,6 +1,6 @@
-"""What spk_verify_drafts needs of its workspace, as its refusal of a misaligned
-one states it, never passes what the size query told for a larger call.  No
-GPU: every call here is refused."""
+"""What spk_verify_drafts refuses of its buffers, without a GPU.  What it needs of
+its workspace, as its refusal of a misaligned one states it, never passes what
+the size query told for a larger call."""
 import ctypes as C
 import re
 
@@ -31,3 +31,23 @@ def test_a_workspace_of_the_largest_sizes_serves_the_smaller(vocab, seqs, rows):
         assert need <= size(v, s, r) <= kept, (v, s, r, need, kept)
         largest = max(largest, need)
     assert kept <= 2 * largest + 4096, (kept, largest)
+
+
+@pytest.mark.parametrize("out", ["out_tokens", "accepted", "logprobs", "context_out"])
+@pytest.mark.parametrize("other", ["cu_seqlens", "tokens", "target", "draft", "temperature", "u_accept", "u_sample", "context_lens", "out_tokens",
+                                   "accepted", "logprobs", "context_out"])
+def test_an_output_is_no_other_buffer(out, other):
+    """A workgroup would read what another one wrote."""
+    from spock_amd import _lib
+    lib = _lib.lib()
+    if out == other or (out, other) in (("context_out", "context_lens"), ("out_tokens", "tokens")):
+        return
+    names = ("cu_seqlens", "tokens", "target", "draft", "temperature", "u_accept", "u_sample", "out_tokens", "accepted", "logprobs",
+             "context_lens", "context_out", "workspace")
+    a = _lib.SpkVerifyArgs(0, _lib.SPK_F16, 100, 2, 6)
+    for i, n in enumerate(names):
+        setattr(a, n, 4096 * (i + 1))
+    a.target_stride = a.draft_stride = 100
+    a.workspace_bytes = 1 << 20
+    setattr(a, out, getattr(a, other))
+    assert lib.spk_verify_drafts(C.byref(a), None) == -5 and b"output" in lib.spk_last_error(), lib.spk_last_error()
