@@ -303,12 +303,12 @@ def _flat(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape) -> None
 
 
 def _rows(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape):
-    """Strides of a [tokens][heads][dim] view: any of the first two dimensions."""
+    """Token and head strides of a [tokens][heads][dim] view: any, and 0 where there is one."""
     _on(what, name, t, dev, dtype, shape)
-    strides = t.stride()
-    if strides[2] != 1:
+    token, head, last = t.stride()
+    if last != 1:
         raise _lib.SpockError(f"{what}: the last dimension of {name} must be contiguous")
-    return strides
+    return (token if shape[0] > 1 else 0), (head if shape[1] > 1 else 0)
 
 
 def _workspace(what: str, t: torch.Tensor, dev: int) -> None:
@@ -338,10 +338,12 @@ def _paged_cache(what: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise _lib.SpockError(f"{what}: q has head_dim {q_dim}, the cache {dim}")
     _on(what, "k_cache", k_cache, dev, dtype)
     _on(what, "v_cache", v_cache, dev, dtype, shape)
-    strides = k_cache.stride()
-    if v_cache.stride() != strides or strides[3] != 1:
+    strides, v_strides = k_cache.stride(), v_cache.stride()
+    if 1 in shape:  # a stride of one element is not read
+        strides, v_strides = ([n if size > 1 else 0 for n, size in zip(t, shape)] for t in (strides, v_strides))
+    if v_strides != strides or strides[3] != 1:
         raise _lib.SpockError(f"{what}: k_cache and v_cache need equal strides and a contiguous last dimension, "
-                              f"got {strides} and {v_cache.stride()}")
+                              f"got {k_cache.stride()} and {v_cache.stride()}")
     seqs = context_lens.numel()
     _on(what, "block_table", block_table, dev, torch.int32)
     _flat(what, "cu_seqlens", cu_seqlens, dev, torch.int32, (seqs + 1,))
