@@ -555,8 +555,8 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * that 16 bits hold (from 2^-30 of the row's largest on in fp16, 2^-126 in bf16),
  * and becomes NaN under a smaller one, as 0 times it does.
  * max_query_len and max_context_len: host bounds of the sequences' lengths;
- * they choose the kernels and the split of the keys, not the result, which
- * follows the device's lengths.
+ * they choose the kernels and the split of the keys, and with them the rounding.
+ * What is computed follows the device's lengths, also where a bound is too low.
  * workspace: 256-byte aligned, contents ignored, NULL where 0 bytes suffice.
  * spk_paged_attention_workspace_size() bytes are enough for the call and for
  * every one of the same heads and head_dim whose tokens, sequences, bounds,
@@ -571,7 +571,8 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * in fp32, out is rounded once.  Weights enter the sum of weights unrounded;
  * before the product with V they are two 16-bit parts (value and remainder) in
  * sequences of up to 128 rows (new tokens times heads of a KV head), and rounded
- * to one in longer ones and in a call of one sequence whose bound is longer. */
+ * to one in longer ones and in a call of one sequence whose bound is longer (an
+ * error of a third more than out's own rounding). */
 typedef struct SpkPagedAttnArgs {
   SpkPagedCache cache;
   int32_t num_q_heads;
@@ -614,7 +615,9 @@ int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
  * token is fed.  A drawn row without a distribution (NaN, no mass) emits -1.
  * Apart from context_out no output may overlap an input, nor another output.
  * Tokens outside [0, vocab) are refused; a sequence without rows only gets
- * accepted[s] = 0 and its context.  Comparisons and running sums are fp64.
+ * accepted[s] = 0 and its context.  Comparisons and running sums are fp64; what
+ * normalises a row of logits is a sum of fp32 exponentials (within 10 x 2^-23), so
+ * that an acceptance may come out otherwise where its two sides are that near.
  * workspace: 256-byte aligned, contents ignored; overlapping calls race on it.
  * spk_verify_drafts_workspace_size() bytes serve every call of no larger vocab,
  * num_seqs and total_tokens.  Limits: 65535 rows and sequences. */

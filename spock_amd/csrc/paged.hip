@@ -685,9 +685,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(Attn a) {
 // get 4 keys of a dimension each.
 //
 // What bounds it: 16 sequences with 9 tokens of 4 heads (36 rows), heads of 256, take
-// 44 us for 168 MB, 3.8 TB/s.  Matrix instructions run 10% of the time and LDS
+// 44 us for 168 MB, 3.8 TB/s.  Matrix instructions run 9% of the time and LDS
 // reads 14%; some 10 us are the way to the first keys (lengths, shares, page ids),
-// the rest is memory.
+// the rest is memory.  Heads of 256 fill the registers: 20 bytes of a lane's
+// addresses lie in memory, outside the products.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   using H = Half<BF>;
@@ -991,13 +992,21 @@ __device__ __forceinline__ void in_turn(Read read, Use use) {
 // order; the dimension of row m of output tile 2 u + e is 2 (m + 32 u) + e,
 // which makes these writes (and a lane's output) contiguous.
 //
+// A weight enters the product with V as one 16-bit value, half a step off at
+// most; the sum of weights has it unrounded.  In two parts, as the other kernels
+// have them, the product is twice as many matrix instructions: 453 us for 337 with
+// the first shape below, 249 for 191 with the second, for an error of 2.1e-4 instead
+// of 2.8e-4 (fp16, 2-norm against 64 bits) and 1.65e-3 instead of 2.2e-3 (bf16),
+// most of which is the result's own rounding.
+//
 // What bounds it: one workgroup of 8 waves to a CU (a wave's outputs and queries
-// fill its registers).  2048 tokens at 16384 keys, heads of 256: 295 us without the
-// join, 870 TFLOP/s; matrix instructions run 38% of the time at the 2.05 GHz the
-// chip keeps, LDS reads 25%, waves wait for one or the other in half of theirs,
-// as no registers are left to read ahead.  Six ragged prompts, heads of 128: 167
-// us, 650 TFLOP/s: a step's exponentials take as long as its matrix
-// instructions, and the longest tile alone is three quarters of the time.
+// fill its registers).  2048 tokens at 16384 keys, heads of 256: 295 to 325 us
+// without the join (one chip's clock under load and another's), 790 to 870
+// TFLOP/s; matrix instructions run 37% of the time at some 2 GHz, LDS reads 25%,
+// waves wait for one or the other in half of theirs, as no registers are left to
+// read ahead.  Six ragged prompts, heads of 128: 167 to 180 us, 600 to 650
+// TFLOP/s: a step's exponentials take as long as its matrix instructions, and the
+// longest tile alone is three quarters of the time.
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   using H = Half<BF>;
@@ -1012,8 +1021,9 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(Attn a) {
   constexpr int U = KT > 64 ? 2 : 1;       // lookups of a lane per tile
   constexpr int NB = D == 256 ? 1 : 2;     // blocks of 32 keys at a time
   // LDS reads ahead of the matrix instruction that uses them.  Heads of 256 have
-  // no registers left for it: 2 ahead spills and takes 356 us for 347, while with
-  // heads of 128, 4 ahead take 207 us for 217.
+  // no registers left for it: the kernel keeps 28 bytes of a lane's address
+  // arithmetic in memory as it is, outside the products, and 44 with reads 2 ahead,
+  // which take 321 us for 317.  With heads of 128, 4 ahead take 181 us for 189.
   constexpr int AHEAD = D == 256 ? 0 : 4;
   // keys, values as they come: three tiles, as separate arrays: a load into one is then known not to touch the others
   __shared__ __align__(16) uint4 ka[16 * 65], kb[16 * 65], kc[16 * 65], ra[1024], rb[1024], rc[1024];
