@@ -517,7 +517,8 @@ typedef struct SpkPagedCache {
  * [rope_rows][rot_dim], (cos, sin) per pair (rope_apply.comp's table;
  * positions outside it take its first or last row).  Text has one axis, or
  * equal positions on all; images and videos have time, height and width.
- * q_out receives the queries (it may be q), the pages the keys and values.
+ * q_out receives the queries (it may be q), the pages the keys and values; two
+ * tokens of a step that the tables give one slot race for it.
  * fp32 throughout, one rounding at the end (rope_apply.comp's separate
  * dispatches round after the norm as well). */
 enum { SPK_ROPE_HALVES = 0 /* pairs (i, i + rot_dim/2) */, SPK_ROPE_ADJACENT = 1 /* pairs (2i, 2i + 1) */ };
@@ -552,7 +553,7 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * score -inf) is zero with lse -inf; keys and values that a row does not see
  * cannot reach it, whatever they hold.
  * Values that it sees count as they are: an infinity stays one under any weight
- * that 16 bits hold (from 2^-30 of the row's largest on in fp16, 2^-126 in bf16),
+ * that 16 bits hold (from 2^-30 of the row's largest on in fp16, 2^-125 in bf16),
  * and becomes NaN under a smaller one, as 0 times it does.
  * max_query_len and max_context_len: host bounds of the sequences' lengths;
  * they choose the kernels and the split of the keys, and with them the rounding.

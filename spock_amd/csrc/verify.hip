@@ -14,8 +14,8 @@
 // two values, the exponentials of the drawn row, the running sums) but for what
 // normalises a row of logits: that sum is of fp32 exponentials, each off by a few
 // units in the last place but none in common (log2(e) / T enters as two floats),
-// eight at a time in fp32 and those in fp64.  fp64 exponentials there would be as
-// many again as step 2's, of every row instead of two.
+// eight at a time in fp32 and those in fp64 (fp64 exponentials of every row would
+// take several times as long as step 2, which has them for two a sequence).
 //
 // What bounds it (64 sequences, 222 rows and 158 drafts' rows of 248,320 fp16
 // logits): step 1 reads 190 MB in 39 us, 4.8 TB/s, with as much time in its

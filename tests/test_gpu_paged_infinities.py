@@ -2,7 +2,7 @@
 row sees: softmax . V says what they give, wherever in the context they lie.
 
 An infinity times a weight that rounds to zero (below 2^-30 of the row's largest
-in fp16, 2^-126 in bf16) is NaN; scores of these inputs are normal with deviation
+in fp16, 2^-125 in bf16) is NaN; scores of these inputs are normal with deviation
 1, so no weight comes near that."""
 import math
 
