@@ -562,9 +562,11 @@ int spk_mrope_append(const SpkMropeArgs* args, spk_stream_t stream);
  * spk_paged_attention_workspace_size() bytes are enough for the call and for
  * every one of the same heads and head_dim whose tokens, sequences, bounds,
  * table and window (0 is the widest) are no larger, so that a caller asks once,
- * with its largest sizes; a call may need less and takes what it needs.  The
- * query reads the sizes alone: the buffers may be NULL.  Calls that overlap on
- * one workspace race.
+ * with its largest sizes; a call may need less and takes what it needs, which
+ * spk_paged_attention_workspace_need() tells a caller that allocates for each
+ * call (a prompt of 16,384 tokens may need nothing, smaller calls of as many rows
+ * hundreds of megabytes).  Both read the sizes alone: the buffers may be NULL.
+ * Calls that overlap on one workspace race.
  * Limits: page_stride and token_stride below 2^32 elements, max_pages *
  * page_size at most 2^31 - 4096 positions, 65535 KV heads and row tiles (of
  * 256) in a call, and 2^24 workgroups of a launch (some 67 million rows).
@@ -589,6 +591,7 @@ typedef struct SpkPagedAttnArgs {
   size_t workspace_bytes;
 } SpkPagedAttnArgs;
 size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* args);
+size_t spk_paged_attention_workspace_need(const SpkPagedAttnArgs* args);
 int spk_paged_attention(const SpkPagedAttnArgs* args, spk_stream_t stream);
 
 /* Verification of drafted tokens.  The rows of a step are packed as above:

@@ -68,6 +68,7 @@ SIGNATURES = {
     # a serving step over a paged cache
     "spk_mrope_append": (C.c_int, [_p, _p]),
     "spk_paged_attention_workspace_size": (_sz, [_p]),
+    "spk_paged_attention_workspace_need": (_sz, [_p]),
     "spk_paged_attention": (C.c_int, [_p, _p]),
     "spk_verify_drafts_workspace_size": (_sz, [_i32, _i32, _i32]),
     "spk_verify_drafts": (C.c_int, [_p, _p]),

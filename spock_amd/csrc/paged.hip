@@ -1637,6 +1637,12 @@ extern "C" size_t spk_paged_attention_workspace_size(const SpkPagedAttnArgs* p) 
   return spk_paged::workspace_bound(*p);
 }
 
+extern "C" size_t spk_paged_attention_workspace_need(const SpkPagedAttnArgs* p) {
+  Cache c;
+  if (check_attn(p, &c, false) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
+  return spk_paged::workspace_of(*p, spk_paged::plan_of(*p));
+}
+
 extern "C" int spk_paged_attention(const SpkPagedAttnArgs* p, spk_stream_t stream) {
   const char* who = "spk_paged_attention";
   Attn a{};

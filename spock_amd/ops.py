@@ -450,7 +450,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         lse = q.new_empty(shape[:2], dtype=torch.float32)
     a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale, q.data_ptr(), qs[0], qs[1],
                          _ptr(gate), gs[0], gs[1], out.data_ptr(), outs[0], outs[1], _ptr(lse), None, 0)
-    need = lib().spk_paged_attention_workspace_size(C.byref(a))
+    need = lib().spk_paged_attention_workspace_need(C.byref(a))
     if need:
         if workspace is None or workspace.numel() * workspace.element_size() < need:
             workspace = q.new_empty(need, dtype=torch.uint8)

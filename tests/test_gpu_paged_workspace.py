@@ -39,6 +39,24 @@ def test_attention_on_the_largest_calls_workspace(dev, dtype, heads, kv, dim):
     assert bool((ws[:need] != 0xFF).any())
 
 
+def test_a_call_takes_no_more_than_it_needs(dev):
+    """Without a workspace of the caller's: a prompt whose tiles fill the chip takes none, not what smaller calls would."""
+    from spock_amd import ops
+    gen = torch.Generator().manual_seed(2)
+    cu, ctx, table, pages = _tables([(4096, 4096)], 64, 2)
+    kc, vc = (_normal(gen, pages, 64, 4, 64, dtype=torch.float16).to(dev) for _ in range(2))
+    q = _normal(gen, 4096, 64, 64, dtype=torch.float16).to(dev)
+    out = torch.empty_like(q)
+    args = (q, kc, vc, table.to(dev), _i32(cu, dev), _i32(ctx, dev), 4096, 4096)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.paged_attention(*args, out=out)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() == before
+    assert ops.paged_attention_workspace_bytes(4096, 64, 4, 64, 64, table.shape[1], 1, 4096, 4096) > 2 ** 26
+
+
 def test_verification_on_the_largest_calls_workspace(dev):
     from spock_amd import ops
     from test_gpu_verify import _call, _case, _check, _inputs, _want

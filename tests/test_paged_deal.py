@@ -347,3 +347,22 @@ def test_the_size_needs_no_buffers():
         for k, v in bad.items():
             setattr(b, k, v)
         assert lib.spk_paged_attention_workspace_size(C.byref(b)) == 0
+
+
+def test_what_one_call_needs(shim):
+    """The need of the call alone, as the plan and the refusal of a misaligned workspace have it."""
+    import re
+    from spock_amd import _lib
+    lib = _lib.lib()
+    assert lib.spk_paged_attention_workspace_need(None) == 0
+    out = (C.c_int * 8)()
+    for tokens, seqs, q, c in ((1, 1, 1, 32768), (9, 1, 9, 32768), (8192, 1, 8192, 32768), (16384, 1, 16384, 131072), (64, 64, 1, 16000), (700, 6, 500, 3000)):
+        cache = _lib.SpkPagedCache(_lib.SPK_F16, 2, 256, 16, 100, 8192, seqs, tokens, 256, 256, 16384, 1024, 256, 256, 8192, 256, 256)
+        a = _lib.SpkPagedAttnArgs(cache, 8, q, c, 0, 0.0, 256, 256, 256, None, 0, 0, 256, 256, 256, None, 264, 1 << 60)
+        need = lib.spk_paged_attention_workspace_need(C.byref(a))
+        assert need == shim.plan((C.c_int * 10)(8, 2, 256, 16, 8192, seqs, tokens, q, c, 0), None, None, out)
+        assert need <= lib.spk_paged_attention_workspace_size(C.byref(a))
+        if need:    # else it would be launched
+            assert lib.spk_paged_attention(C.byref(a), None) == -5
+            assert int(re.search(rb"(\d+) needed", lib.spk_last_error()).group(1)) == need
+    assert lib.spk_paged_attention_workspace_need(C.byref(a)) > 0
