@@ -651,6 +651,80 @@ size_t spk_verify_drafts_workspace_size(int32_t vocab, int32_t num_seqs, int32_t
 int spk_verify_drafts(const SpkVerifyArgs* args, spk_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Serving in 4 bits (no reference counterpart): microscaled 4-bit floating point
+ * (OCP MX: E2M1 elements, E8M0 scales).  32 consecutive values of a row share a
+ * scale 2^e, one byte e + 127; a value is a code of 4 bits, sign and one of 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6, times the scale.  Two codes a byte, the first in the low
+ * half: a row of n values is n / 2 bytes of codes and n / 32 bytes of scales.
+ * Byte 255: the block's values are NaN.
+ * ---------------------------------------------------------------------- */
+
+/* Rows of such values: codes 16-byte aligned with code_stride a multiple of 16,
+ * scales anywhere; strides in bytes between rows. */
+typedef struct SpkMx4 {
+  uint8_t* codes;   int64_t code_stride;
+  uint8_t* scales;  int64_t scale_stride;
+} SpkMx4;
+
+/* Quantises rows of x (dtype SPK_F32, SPK_F16 or SPK_BF16; cols a multiple of
+ * 32; 16-byte aligned, x_stride elements between rows, a multiple of 16 bytes):
+ * e = floor(log2 of the block's largest magnitude) - 2, at least -127; a code is
+ * the nearest of x / 2^e, ties to even, magnitudes above 6 (the last quarter
+ * of a binade) 6.  A block that holds an infinity or NaN gets byte 255 and codes
+ * 0.  Exact but for that one rounding.  Limit: 2^31 groups of 8 values. */
+int spk_mx4_quantize(const void* x, int32_t dtype, int64_t x_stride, int64_t rows, int32_t cols,
+                     const SpkMx4* out, spk_stream_t stream);
+/* The values, rounded to dtype (bf16 and fp32 hold them all but for the largest
+ * scales; fp16 those of scales 2^-23 to 2^13; what passes it is infinite). */
+int spk_mx4_dequantize(const SpkMx4* m, int64_t rows, int32_t cols, int32_t dtype, void* y,
+                       int64_t y_stride, spk_stream_t stream);
+
+/* out[m][n] = x[m] . w[n] (+ residual[m][n]), rounded once; fp32 accumulation.
+ * The products of spk_matvec_f16 and spk_gemm_f16 with weights in 4 bits.
+ * x: rows of 16 bits (dtype; 16-byte aligned, x_stride a multiple of 8
+ * elements), or, with x == NULL, rows in 4 bits too (x4).  w: out_dim rows of
+ * in_dim values.  With 16-bit rows a weight enters rounded to their type (as
+ * spk_mx4_dequantize; bf16 holds every one), with x4 exactly.  residual
+ * (nullable) may be out; out overlaps no other input.  in_dim % 32 == 0; rows
+ * and out_dim any. */
+typedef struct SpkMx4MatmulArgs {
+  int32_t dtype;               /* SPK_F16 or SPK_BF16: x, residual and out */
+  int32_t rows, out_dim, in_dim;
+  const void* x;               int64_t x_stride;
+  SpkMx4 x4;
+  SpkMx4 w;
+  const void* residual;        int64_t residual_stride;
+  void* out;                   int64_t out_stride;
+} SpkMx4MatmulArgs;
+int spk_mx4_matmul(const SpkMx4MatmulArgs* args, spk_stream_t stream);
+
+/* The paged cache in 4 bits.  SpkPagedCache then holds the codes (k_cache,
+ * v_cache; strides in BYTES, multiples of 16) and dtype is that of q, k, v, gate,
+ * out and weights; the scales of a position's row, head_dim / 32 bytes, lie in
+ * pools of their own, strides in bytes. */
+typedef struct SpkPagedScales {
+  uint8_t* k_scales;
+  uint8_t* v_scales;
+  int64_t page_stride, token_stride, head_stride;
+} SpkPagedScales;
+
+/* spk_mrope_append with the pages in 4 bits.  The queries are its, bit for bit.  Keys
+ * are normalised, rotated and quantised in one rounding (in 64 bits before
+ * it), values as they come; with fp16 a scale is at most 2^13, with bf16 2^125,
+ * and what passes 6 times it is cut there. */
+int spk_mrope_append_mx4(const SpkMropeArgs* args, const SpkPagedScales* scales, spk_stream_t stream);
+
+/* spk_paged_attention over pages in 4 bits: its arguments, bounds and results,
+ * with a workspace of its own sizes.  Keys and values enter as spk_mx4_dequantize
+ * gives them in dtype; a block whose scale passes 2^13 (fp16) or 2^125 (bf16)
+ * counts as NaN, as one of byte 255 does: a row that sees such a value has NaN in
+ * that block's dimensions, one that sees such a key is NaN, and no other row is
+ * touched.  Weights are rounded to dtype before the product with V. */
+size_t spk_paged_attention_mx4_workspace_size(const SpkPagedAttnArgs* args);
+size_t spk_paged_attention_mx4_workspace_need(const SpkPagedAttnArgs* args);
+int spk_paged_attention_mx4(const SpkPagedAttnArgs* args, const SpkPagedScales* scales, spk_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Diagnostics (no reference counterpart).
  * ---------------------------------------------------------------------- */
 

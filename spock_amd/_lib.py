@@ -72,6 +72,14 @@ SIGNATURES = {
     "spk_paged_attention": (C.c_int, [_p, _p]),
     "spk_verify_drafts_workspace_size": (_sz, [_i32, _i32, _i32]),
     "spk_verify_drafts": (C.c_int, [_p, _p]),
+    # serving in 4 bits
+    "spk_mx4_quantize": (C.c_int, [_p, _i32, _i64, _i64, _i32, _p, _p]),
+    "spk_mx4_dequantize": (C.c_int, [_p, _i64, _i32, _i32, _p, _i64, _p]),
+    "spk_mx4_matmul": (C.c_int, [_p, _p]),
+    "spk_mrope_append_mx4": (C.c_int, [_p, _p, _p]),
+    "spk_paged_attention_mx4_workspace_size": (_sz, [_p]),
+    "spk_paged_attention_mx4_workspace_need": (_sz, [_p]),
+    "spk_paged_attention_mx4": (C.c_int, [_p, _p, _p]),
 }
 
 
@@ -153,6 +161,21 @@ class SpkVerifyArgs(C.Structure):
                 ("draft_stride", _i64), ("temperature", _p), ("u_accept", _p), ("u_sample", _p), ("out_tokens", _p),
                 ("accepted", _p), ("logprobs", _p), ("context_lens", _p), ("context_out", _p),
                 ("workspace", _p), ("workspace_bytes", _sz)]
+
+
+class SpkMx4(C.Structure):
+    _fields_ = [("codes", _p), ("code_stride", _i64), ("scales", _p), ("scale_stride", _i64)]
+
+
+class SpkMx4MatmulArgs(C.Structure):
+    _fields_ = [("dtype", _i32), ("rows", _i32), ("out_dim", _i32), ("in_dim", _i32),
+                ("x", _p), ("x_stride", _i64), ("x4", SpkMx4), ("w", SpkMx4),
+                ("residual", _p), ("residual_stride", _i64), ("out", _p), ("out_stride", _i64)]
+
+
+class SpkPagedScales(C.Structure):
+    _fields_ = [("k_scales", _p), ("v_scales", _p),
+                ("page_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
 
 
 class SpkMatvecDesc(C.Structure):

@@ -1,0 +1,355 @@
+// mx4.hip -- microscaled 4-bit floating point: quantisation and back
+// (spk_mx4_quantize, spk_mx4_dequantize) and the products with such weights
+// (spk_mx4_matmul).
+#include "mx4.hpp"
+
+#include "capi_common.hpp"
+#include "numerics.hpp"
+#include "paged.hpp"
+
+namespace {
+
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
+
+// ---------------------------------------------------------------------------
+// Quantisation.
+// ---------------------------------------------------------------------------
+
+// Rows cut into groups of 8 values, a group to a thread: four groups are a block,
+// and its four lanes find the largest magnitude together.
+struct Rows {
+  const void* x;
+  void* y;
+  uint8_t *codes, *scales;
+  int64_t stride, code_stride, scale_stride;  // of x or y in elements
+  uint32_t groups, per_row;
+  spk_paged::PageDiv div;  // by per_row
+};
+
+struct Group {
+  int64_t row;
+  uint32_t at;  // in the row
+};
+
+__device__ __forceinline__ Group group_of(const Rows& a, uint32_t i) {
+  const uint32_t row = spk_paged::divide(a.div, i);
+  return {(int64_t)row, i - row * a.per_row};
+}
+
+template <typename T>
+__device__ __forceinline__ T xor_max4(T v) {  // over the four lanes of a block
+  v = max(v, (T)spk::lane_xor1_u((uint32_t)v));
+  return max(v, (T)spk::lane_xor2_u((uint32_t)v));
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(Rows a) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.groups) return;  // whole blocks: groups is a multiple of 4
+  const Group g = group_of(a, i);
+  uint32_t byte, codes;
+  if constexpr (DT == SPK_F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + g.row * a.stride + 8 * (int64_t)g.at);
+    const float4 u = p[0], v = p[1];
+    const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(x[k]) & 0x7fffffffu);
+    byte = spk_mx4::scale_byte(xor_max4(most));
+    codes = spk_mx4::codes_of(x, spk_mx4::scale_of(byte));
+  } else {
+    constexpr bool BF = DT == SPK_BF16;
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + g.row * a.stride + 8 * (int64_t)g.at);
+    byte = spk_mx4::scale_byte16<BF>(xor_max4(spk_mx4::most_of(u)));
+    codes = spk_mx4::codes_of<BF>(u, spk_mx4::scale_of(byte));
+  }
+  if (byte == spk_mx4::kNone) codes = 0;
+  *reinterpret_cast<uint32_t*>(a.codes + g.row * a.code_stride + 4 * (int64_t)g.at) = codes;
+  if ((g.at & 3) == 0) a.scales[g.row * a.scale_stride + g.at / 4] = (uint8_t)byte;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(Rows a) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.groups) return;
+  const Group g = group_of(a, i);
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(a.codes + g.row * a.code_stride + 4 * (int64_t)g.at);
+  const float scale = spk_mx4::scale_of(a.scales[g.row * a.scale_stride + g.at / 4]);
+  const int64_t to = g.row * a.stride + 8 * (int64_t)g.at;
+  if constexpr (DT == SPK_F32) {
+    const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, scale, 0), q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, scale, 1);
+    const auto r = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, scale, 2), s = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, scale, 3);
+    float4* y = reinterpret_cast<float4*>(static_cast<float*>(a.y) + to);
+    y[0] = make_float4(p[0], p[1], q[0], q[1]);
+    y[1] = make_float4(r[0], r[1], s[0], s[1]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + to) = spk_mx4::expand<DT == SPK_BF16>(u, scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products.
+// ---------------------------------------------------------------------------
+
+struct Mm {
+  const uint16_t* x;
+  const uint8_t *xc, *xs, *wc, *ws;
+  const uint16_t* res;
+  uint16_t* out;
+  int64_t xt, xct, xst, wct, wst, rt, ot;
+  int32_t rows, cols, depth;  // of the product: m, n, k
+};
+
+__device__ const uint4 kZero[4] = {};  // what lanes past the last value of a row read
+
+template <bool BF>
+__device__ __forceinline__ floatx4 mfma16(uint4 a, uint4 b, floatx4 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// Four codes' dwords as an operand of the scaled products (of 8, the upper are not read).
+__device__ __forceinline__ intx8 four_bits(uint4 u) {
+  return intx8{(int)u.x, (int)u.y, (int)u.z, (int)u.w, 0, 0, 0, 0};
+}
+
+template <bool BF>
+__device__ __forceinline__ float widen(uint16_t u) {
+  if constexpr (BF) return __uint_as_float((uint32_t)u << 16);
+  return (float)__builtin_bit_cast(_Float16, u);
+}
+template <bool BF>
+__device__ __forceinline__ uint16_t narrow(float f) {
+  if constexpr (BF) return __builtin_bit_cast(uint16_t, (__bf16)f);
+  return __builtin_bit_cast(uint16_t, (_Float16)f);
+}
+
+// Up to 16 MT rows of x: a workgroup takes 16 NT rows of w and all of their depth, 128
+// at a time, every NW-th step to a wave; the waves' sums meet in LDS, in their order.
+// A lane of the 16x16 products' A operand holds one block of a row of w, 32 codes
+// under one scale, as four contraction steps of 8 (rows in 16 bits) or as they
+// are (rows in 4 bits, whose scales the instruction applies).
+template <bool X4, bool BF, int MT, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void mx4_few_rows_kernel(Mm a) {
+  __shared__ float sums[NW][NT * 16][MT * 16 + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ln = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+  const uint8_t *wc[NT], *ws[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = min(n0 + 16 * t + ln, a.cols - 1);
+    wc[t] = a.wc + n * a.wct;
+    ws[t] = a.ws + n * a.wst;
+  }
+  const uint16_t* x[MT];
+  const uint8_t *xc[MT], *xs[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int64_t m = min(m0 + 16 * t + ln, a.rows - 1);
+    if constexpr (X4) {
+      xc[t] = a.xc + m * a.xct;
+      xs[t] = a.xs + m * a.xst;
+    } else {
+      x[t] = a.x + m * a.xt;
+    }
+  }
+  floatx4 acc[NT][MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u) acc[t][u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k = 128 * wave; k < a.depth; k += 128 * NW) {
+    const int b = k / 32 + g;  // this lane's block
+    const bool there = 32 * b < a.depth;
+    uint4 w[NT];
+    uint32_t s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      w[t] = *(there ? reinterpret_cast<const uint4*>(wc[t] + 16 * b) : kZero);
+      s[t] = *(there ? ws[t] + b : reinterpret_cast<const uint8_t*>(kZero));
+    }
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      if constexpr (X4) {
+        const uint4 v = *(there ? reinterpret_cast<const uint4*>(xc[u] + 16 * b) : kZero);
+        const uint32_t vs = *(there ? xs[u] + b : reinterpret_cast<const uint8_t*>(kZero));
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(four_bits(w[t]), four_bits(v), acc[t][u], 4, 4, 0,
+                                                                       (int)s[t], 0, (int)vs);
+      } else {
+        const uint4* p = there ? reinterpret_cast<const uint4*>(x[u] + 32 * b) : kZero;
+        uint4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = p[c];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            acc[t][u] = mfma16<BF>(spk_mx4::expand<BF>((&w[t].x)[c], spk_mx4::scale_of(s[t])), v[c], acc[t][u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[wave][16 * t + 4 * g + i][16 * u + ln] = acc[t][u][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 256 * NT * MT; i += 64 * NW) {
+    const int n = i % (16 * NT), m = i / (16 * NT);
+    if (m0 + m >= a.rows || n0 + n >= a.cols) continue;
+    float sum = sums[0][n][m];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum += sums[w][n][m];
+    if (a.res) sum += widen<BF>(a.res[(m0 + m) * a.rt + n0 + n]);
+    a.out[(m0 + m) * a.ot + n0 + n] = narrow<BF>(sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+
+size_t size_of(int dtype) { return dtype == SPK_F32 ? 4 : 2; }
+
+int check_mx4(const SpkMx4& m, int64_t rows, int32_t cols, const char* who, const char* name) {
+  if (!m.codes || !m.scales) return spk::fail(SPK_ERR_NULL, "%s: codes or scales of %s is NULL", who, name);
+  if (!spk::aligned(m.codes, 16) || m.code_stride % 16)
+    return spk::fail(SPK_ERR_ALIGN, "%s: codes of %s and their stride (%lld bytes) must be 16-byte aligned", who, name,
+                     (long long)m.code_stride);
+  if (rows > 1 && (m.code_stride < cols / 2 || m.scale_stride < cols / 32))
+    return spk::fail(SPK_ERR_SHAPE, "%s: strides of %s (codes %lld, scales %lld) are less than a row of %d values", who,
+                     name, (long long)m.code_stride, (long long)m.scale_stride, cols);
+  return SPK_OK;
+}
+
+// The arguments that quantisation and its inverse share.  1: there is nothing to do.
+int fill_rows(const SpkMx4* m, const void* x, int32_t dtype, int64_t stride, int64_t rows, int32_t cols, const char* who,
+              Rows* a) {
+  if (!m) return spk::fail(SPK_ERR_NULL, "%s: NULL args", who);
+  if (dtype != SPK_F32 && dtype != SPK_F16 && dtype != SPK_BF16)
+    return spk::fail(SPK_ERR_ARG, "%s: dtype %d (SPK_F32, SPK_F16 or SPK_BF16)", who, dtype);
+  if (rows < 0 || cols < 0 || cols % 32)
+    return spk::fail(SPK_ERR_SHAPE, "%s: %lld rows of %d values (a multiple of 32)", who, (long long)rows, cols);
+  if (rows == 0 || cols == 0) return 1;
+  if (rows > INT32_MAX || rows * (cols / 8) > INT32_MAX)
+    return spk::fail(SPK_ERR_SHAPE, "%s: %lld rows of %d values (below 2^34 in all)", who, (long long)rows, cols);
+  if (!x) return spk::fail(SPK_ERR_NULL, "%s: the rows are NULL", who);
+  if (!spk::aligned(x, 16) || stride * (int64_t)size_of(dtype) % 16)
+    return spk::fail(SPK_ERR_ALIGN, "%s: the rows and their stride (%lld elements) must be 16-byte aligned", who,
+                     (long long)stride);
+  if (rows > 1 && stride < cols)
+    return spk::fail(SPK_ERR_SHAPE, "%s: stride %lld of rows of %d values", who, (long long)stride, cols);
+  if (const int rc = check_mx4(*m, rows, cols, who, "the 4-bit rows")) return rc;
+  a->codes = m->codes;
+  a->scales = m->scales;
+  a->stride = stride;
+  a->code_stride = m->code_stride;
+  a->scale_stride = m->scale_stride;
+  a->groups = (uint32_t)(rows * (cols / 8));
+  a->per_row = (uint32_t)cols / 8;
+  a->div = spk_paged::page_div(a->per_row);
+  return SPK_OK;
+}
+
+template <bool X4, bool BF>
+void launch_matmul(const Mm& a, hipStream_t s) {
+  const dim3 grid((a.cols + 31) / 32, (a.rows + 63) / 64);
+  hipLaunchKernelGGL((mx4_few_rows_kernel<X4, BF, 4, 2, 4>), grid, dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" int spk_mx4_quantize(const void* x, int32_t dtype, int64_t x_stride, int64_t rows, int32_t cols,
+                                const SpkMx4* out, spk_stream_t stream) {
+  const char* who = "spk_mx4_quantize";
+  Rows a{};
+  if (const int rc = fill_rows(out, x, dtype, x_stride, rows, cols, who, &a)) return rc < 0 ? rc : SPK_OK;
+  a.x = x;
+  hipStream_t s = spk::to_hip(stream);
+  const dim3 grid((a.groups + 255) / 256);
+  if (dtype == SPK_F32)
+    hipLaunchKernelGGL(mx4_quantize_kernel<SPK_F32>, grid, dim3(256), 0, s, a);
+  else if (dtype == SPK_F16)
+    hipLaunchKernelGGL(mx4_quantize_kernel<SPK_F16>, grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(mx4_quantize_kernel<SPK_BF16>, grid, dim3(256), 0, s, a);
+  return spk::check_launch(who);
+}
+
+extern "C" int spk_mx4_dequantize(const SpkMx4* m, int64_t rows, int32_t cols, int32_t dtype, void* y, int64_t y_stride,
+                                  spk_stream_t stream) {
+  const char* who = "spk_mx4_dequantize";
+  Rows a{};
+  if (const int rc = fill_rows(m, y, dtype, y_stride, rows, cols, who, &a)) return rc < 0 ? rc : SPK_OK;
+  a.y = y;
+  hipStream_t s = spk::to_hip(stream);
+  const dim3 grid((a.groups + 255) / 256);
+  if (dtype == SPK_F32)
+    hipLaunchKernelGGL(mx4_dequantize_kernel<SPK_F32>, grid, dim3(256), 0, s, a);
+  else if (dtype == SPK_F16)
+    hipLaunchKernelGGL(mx4_dequantize_kernel<SPK_F16>, grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(mx4_dequantize_kernel<SPK_BF16>, grid, dim3(256), 0, s, a);
+  return spk::check_launch(who);
+}
+
+extern "C" int spk_mx4_matmul(const SpkMx4MatmulArgs* p, spk_stream_t stream) {
+  const char* who = "spk_mx4_matmul";
+  if (!p) return spk::fail(SPK_ERR_NULL, "%s: NULL args", who);
+  if (p->dtype != SPK_F16 && p->dtype != SPK_BF16)
+    return spk::fail(SPK_ERR_ARG, "%s: dtype %d (SPK_F16 or SPK_BF16)", who, p->dtype);
+  if (p->rows < 0 || p->out_dim < 0 || p->in_dim <= 0 || p->in_dim % 32)
+    return spk::fail(SPK_ERR_SHAPE, "%s: rows %d out_dim %d in_dim %d (a positive multiple of 32)", who, p->rows, p->out_dim,
+                     p->in_dim);
+  if (p->rows == 0 || p->out_dim == 0) return SPK_OK;
+  if (const int rc = check_mx4(p->w, p->out_dim, p->in_dim, who, "w")) return rc;
+  if (p->x) {
+    if (!spk::aligned(p->x, 16) || p->x_stride % 8)
+      return spk::fail(SPK_ERR_ALIGN, "%s: x and its stride (%lld elements) must be 16-byte aligned", who, (long long)p->x_stride);
+    if (p->rows > 1 && p->x_stride < p->in_dim)
+      return spk::fail(SPK_ERR_SHAPE, "%s: x_stride %lld < in_dim %d", who, (long long)p->x_stride, p->in_dim);
+  } else if (const int rc = check_mx4(p->x4, p->rows, p->in_dim, who, "x4")) {
+    return rc;
+  }
+  if (!p->out) return spk::fail(SPK_ERR_NULL, "%s: out is NULL", who);
+  if (!spk::aligned(p->out, 2) || !spk::aligned(p->residual, 2))
+    return spk::fail(SPK_ERR_ALIGN, "%s: out and residual must be 2-byte aligned", who);
+  if (p->rows > 1 && (p->out_stride < p->out_dim || (p->residual && p->residual_stride < p->out_dim)))
+    return spk::fail(SPK_ERR_SHAPE, "%s: out_stride %lld, residual_stride %lld < out_dim %d", who, (long long)p->out_stride,
+                     (long long)p->residual_stride, p->out_dim);
+  if (p->out == p->residual && p->rows > 1 && p->out_stride != p->residual_stride)
+    return spk::fail(SPK_ERR_ARG, "%s: out is residual with another stride", who);
+  Mm a{};
+  a.x = static_cast<const uint16_t*>(p->x);
+  a.xc = p->x4.codes;
+  a.xs = p->x4.scales;
+  a.wc = p->w.codes;
+  a.ws = p->w.scales;
+  a.res = static_cast<const uint16_t*>(p->residual);
+  a.out = static_cast<uint16_t*>(p->out);
+  a.xt = p->x_stride;
+  a.xct = p->x4.code_stride;
+  a.xst = p->x4.scale_stride;
+  a.wct = p->w.code_stride;
+  a.wst = p->w.scale_stride;
+  a.rt = p->residual_stride;
+  a.ot = p->out_stride;
+  a.rows = p->rows;
+  a.cols = p->out_dim;
+  a.depth = p->in_dim;
+  hipStream_t s = spk::to_hip(stream);
+  if (p->dtype == SPK_BF16)
+    p->x ? launch_matmul<false, true>(a, s) : launch_matmul<true, true>(a, s);
+  else
+    p->x ? launch_matmul<false, false>(a, s) : launch_matmul<true, false>(a, s);
+  return spk::check_launch(who);
+}

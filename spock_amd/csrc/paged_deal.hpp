@@ -305,6 +305,26 @@ inline Plan plan_of(const SpkPagedAttnArgs& p) {
   return r;
 }
 
+// The plan over a cache in 4 bits: pieces of 16 rows.
+inline Plan plan_mx4(const SpkPagedAttnArgs& p) {
+  const SpkPagedCache& c = p.cache;
+  const int group = p.num_q_heads / c.num_kv_heads;
+  const int64_t tokens = std::min(p.max_query_len, c.total_tokens), all = (int64_t)c.total_tokens * group;
+  int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
+  if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
+  Plan r{};
+  r.longest = tokens * group;
+  r.steps = std::max<int64_t>(1, (span + 127) / 128);
+  r.many = INT32_MAX;
+  r.share_rows = 16;
+  r.shares = (int)shares_of(c.num_kv_heads * (all / 16 + c.num_seqs), r.steps);
+  r.splits = 1;
+  r.chunk = (int)(128 * r.steps);
+  r.join = r.steps > 1;
+  r.join_rows = (int64_t)c.total_tokens * p.num_q_heads;
+  return r;
+}
+
 inline size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Of one row's part: its maximum, its sum and its output.

@@ -7,14 +7,14 @@ hand-written gfx950 kernel behind include/spock_hip.h.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (SpkChunkArgs, SpkDecodeArgs, SpkMatvecDesc, SpkMropeArgs, SpkPagedAttnArgs, SpkPagedCache,
-                   SpkVerifyArgs, check, lib)
+from ._lib import (SpkChunkArgs, SpkDecodeArgs, SpkMatvecDesc, SpkMropeArgs, SpkMx4, SpkMx4MatmulArgs, SpkPagedAttnArgs,
+                   SpkPagedCache, SpkPagedScales, SpkVerifyArgs, check, lib)
 
 KEY_DIM = 128
 VALUE_DIM = 128
@@ -368,23 +368,9 @@ def _call(fn, a, dev: int, what: str) -> None:
         check(rc, what)
 
 
-def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor,
-                 pair_axis: Sequence[int], k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
-                 cu_seqlens: torch.Tensor, context_lens: torch.Tensor, q_norm_weight: Optional[torch.Tensor] = None,
-                 k_norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, pairing: str = "halves",
-                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Rotary positions with several axes, and the store into the pages (spk_mrope_append).
-
-    q [T][Hq][D], k, v [T][Hkv][D] (float16 or bfloat16, any token and head strides); positions [axes][T] int32 (for text
-    also one row expanded to all axes);
-    rope [rows][rot_dim] float32, (cos, sin) per pair; pair_axis: the axis of each of the rot_dim / 2 pairs (host);
-    caches [pages][page_size][Hkv][D] (any page, token and head strides, the same for both); block_table
-    [S][max_pages], cu_seqlens [S+1], context_lens [S] int32 on the device.  q and k are normalised first where a
-    norm weight [D] is given (RMSNorm, 1 + w).  Writes the new tokens' keys and values into the caches and returns
-    the queries (in `out`, which may be q; rows past cu_seqlens[S] are not written).
-    """
-    what = "mrope_append"
-    cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
+def _mrope_args(what: str, cache: SpkPagedCache, q, k, v, positions, rope, pair_axis, q_norm_weight, k_norm_weight, eps, pairing,
+                out):
+    """(SpkMropeArgs, out) of a rotation and store into `cache`, checked."""
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
     T, heads, D = shape
     kv_shape = (T, cache.num_kv_heads, D)
@@ -418,8 +404,54 @@ def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: t
     a = SpkMropeArgs(cache, heads, rot, _PAIRINGS[pairing], num_axes, axes, positions.data_ptr(), positions.stride(0),
                      rope.data_ptr(), rows, eps, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
                      v.data_ptr(), vs[0], vs[1], _ptr(q_norm_weight), _ptr(k_norm_weight), out.data_ptr(), outs[0], outs[1])
-    _call(lib().spk_mrope_append, a, dev, what)
+    return a, out
+
+
+def mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor,
+                 pair_axis: Sequence[int], k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                 cu_seqlens: torch.Tensor, context_lens: torch.Tensor, q_norm_weight: Optional[torch.Tensor] = None,
+                 k_norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, pairing: str = "halves",
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions with several axes, and the store into the pages (spk_mrope_append).
+
+    q [T][Hq][D], k, v [T][Hkv][D] (float16 or bfloat16, any token and head strides); positions [axes][T] int32 (for text
+    also one row expanded to all axes);
+    rope [rows][rot_dim] float32, (cos, sin) per pair; pair_axis: the axis of each of the rot_dim / 2 pairs (host);
+    caches [pages][page_size][Hkv][D] (any page, token and head strides, the same for both); block_table
+    [S][max_pages], cu_seqlens [S+1], context_lens [S] int32 on the device.  q and k are normalised first where a
+    norm weight [D] is given (RMSNorm, 1 + w).  Writes the new tokens' keys and values into the caches and returns
+    the queries (in `out`, which may be q; rows past cu_seqlens[S] are not written).
+    """
+    what = "mrope_append"
+    cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
+    a, out = _mrope_args(what, cache, q, k, v, positions, rope, pair_axis, q_norm_weight, k_norm_weight, eps, pairing, out)
+    _call(lib().spk_mrope_append, a, q.get_device(), what)
     return out
+
+
+def _attention_args(what: str, cache: SpkPagedCache, q, max_query_len, max_context_len, scale, window, gate, out, return_lse, lse,
+                    workspace, need_of):
+    """(SpkPagedAttnArgs, out, lse, workspace) of an attention over `cache`, checked."""
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    qs = _rows(what, "q", q, dev, dtype, shape)
+    gs = (0, 0) if gate is None else _rows(what, "gate", gate, dev, dtype, shape)
+    if out is None:
+        out = q.new_empty(shape)
+    outs = _rows(what, "out", out, dev, dtype, shape)
+    if lse is not None:
+        _flat(what, "lse", lse, dev, torch.float32, shape[:2])
+    elif return_lse:
+        lse = q.new_empty(shape[:2], dtype=torch.float32)
+    a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale, q.data_ptr(), qs[0], qs[1],
+                         _ptr(gate), gs[0], gs[1], out.data_ptr(), outs[0], outs[1], _ptr(lse), None, 0)
+    need = need_of(C.byref(a))
+    if need:
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = q.new_empty(need, dtype=torch.uint8)
+        else:
+            _workspace(what, workspace, dev)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return a, out, lse, workspace
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -438,36 +470,24 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """
     what = "paged_attention"
     cache = _paged_cache(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
-    shape, dtype, dev = q.shape, q.dtype, q.get_device()
-    qs = _rows(what, "q", q, dev, dtype, shape)
-    gs = (0, 0) if gate is None else _rows(what, "gate", gate, dev, dtype, shape)
-    if out is None:
-        out = q.new_empty(shape)
-    outs = _rows(what, "out", out, dev, dtype, shape)
-    if lse is not None:
-        _flat(what, "lse", lse, dev, torch.float32, shape[:2])
-    elif return_lse:
-        lse = q.new_empty(shape[:2], dtype=torch.float32)
-    a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale, q.data_ptr(), qs[0], qs[1],
-                         _ptr(gate), gs[0], gs[1], out.data_ptr(), outs[0], outs[1], _ptr(lse), None, 0)
-    need = lib().spk_paged_attention_workspace_need(C.byref(a))
-    if need:
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = q.new_empty(need, dtype=torch.uint8)
-        else:
-            _workspace(what, workspace, dev)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(lib().spk_paged_attention, a, dev, what)
+    a, out, lse, _held = _attention_args(what, cache, q, max_query_len, max_context_len, scale, window, gate, out, return_lse, lse,
+                                         workspace, lib().spk_paged_attention_workspace_need)
+    _call(lib().spk_paged_attention, a, q.get_device(), what)
     return out if lse is None else (out, lse)
+
+
+def _attention_sizes(tokens, heads, kv_heads, head_dim, page_size, max_pages, num_seqs, max_query_len, max_context_len, window):
+    """SpkPagedAttnArgs of these sizes, without buffers."""
+    cache = SpkPagedCache(_lib.SPK_F16, kv_heads, head_dim, page_size, 1, max_pages, num_seqs, tokens, 16, 16, 0, 0, 0,
+                          16, max_pages, 16, 16)
+    return SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window)
 
 
 def paged_attention_workspace_bytes(tokens: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
                                     max_pages: int, num_seqs: int, max_query_len: int, max_context_len: int,
                                     window: int = 0) -> int:
     """Bytes of a workspace for paged_attention at these sizes and any smaller ones, for callers that keep one."""
-    cache = SpkPagedCache(_lib.SPK_F16, kv_heads, head_dim, page_size, 1, max_pages, num_seqs, tokens, 16, 16, 0, 0, 0,
-                          16, max_pages, 16, 16)
-    a = SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window)
+    a = _attention_sizes(tokens, heads, kv_heads, head_dim, page_size, max_pages, num_seqs, max_query_len, max_context_len, window)
     return int(lib().spk_paged_attention_workspace_size(C.byref(a)))
 
 
@@ -545,3 +565,217 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
                       _ptr(context_lens), _ptr(context_out), workspace.data_ptr(), workspace.numel() * workspace.element_size())
     _call(lib().spk_verify_drafts, a, dev, what)
     return out_tokens, accepted, logprobs, context_out
+
+
+# ----------------------------------------------------------------------------
+# serving in 4 bits
+# ----------------------------------------------------------------------------
+class Mx4(NamedTuple):
+    """Microscaled 4-bit rows: codes [..., n / 2] and scales [..., n / 32], both uint8 (include/spock_hip.h)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _mx4_rows(what: str, name: str, m: Mx4, dev: int):
+    """(SpkMx4, rows, values of a row) of 4-bit rows: two dimensions with any stride between rows, others contiguous."""
+    if not isinstance(m, Mx4):
+        raise _lib.SpockError(f"{what}: {name} must be an Mx4, got {type(m).__name__}")
+    codes, scales = m
+    if codes.dim() < 1 or codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1] or \
+            codes.shape[-1] != 16 * scales.shape[-1]:
+        raise _lib.SpockError(f"{what}: {name} must have codes [..., n / 2] and scales [..., n / 32], "
+                              f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    for t in m:
+        _on(what, name, t, dev, torch.uint8)
+    rows, cols = codes.shape[:-1].numel(), 2 * codes.shape[-1]
+    return SpkMx4(codes.data_ptr(), _row_stride(what, name, codes), scales.data_ptr(),
+                  _row_stride(what, name, scales)), rows, cols
+
+
+def _row_stride(what: str, name: str, t: torch.Tensor) -> int:
+    """Elements between the rows of [..., n]: any in two dimensions, else those of a contiguous tensor."""
+    if t.dim() == 2:
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise _lib.SpockError(f"{what}: {name} must have contiguous rows, got strides {t.stride()}")
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if not t.is_contiguous():
+        raise _lib.SpockError(f"{what}: {name} must be two-dimensional or contiguous, got strides {t.stride()}")
+    return t.shape[-1]
+
+
+def mx4_quantize(x: torch.Tensor, out: Optional[Mx4] = None) -> Mx4:
+    """Rows of x [..., n] (float32, float16 or bfloat16, n a multiple of 32) in 4 bits (spk_mx4_quantize)."""
+    what = "mx4_quantize"
+    dev = _device(what, x)
+    if x.dim() < 1 or x.shape[-1] % 32 or x.dtype not in _ROWS:
+        raise _lib.SpockError(f"{what}: x must be [..., a multiple of 32] float16, bfloat16 or float32, "
+                              f"got {tuple(x.shape)} {x.dtype}")
+    n = x.shape[-1]
+    stride = _row_stride(what, "x", x)
+    if out is None:
+        out = Mx4(x.new_empty((*x.shape[:-1], n // 2), dtype=torch.uint8),
+                  x.new_empty((*x.shape[:-1], n // 32), dtype=torch.uint8))
+    m, rows, cols = _mx4_rows(what, "out", out, dev)
+    if out.codes.shape[:-1] != x.shape[:-1] or cols != n:
+        raise _lib.SpockError(f"{what}: out holds {tuple(out.codes.shape[:-1])} rows of {cols} values, x is {tuple(x.shape)}")
+    _launch(dev, what, lib().spk_mx4_quantize, x.data_ptr(), _ROWS[x.dtype], stride, rows, cols, C.byref(m))
+    return out
+
+
+def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values of 4-bit rows, [..., n] in dtype (of `out` where it is given; spk_mx4_dequantize)."""
+    what = "mx4_dequantize"
+    if not isinstance(m, Mx4):
+        raise _lib.SpockError(f"{what}: expected an Mx4, got {type(m).__name__}")
+    dev = _device(what, m.codes)
+    a, rows, cols = _mx4_rows(what, "m", m, dev)
+    shape = (*m.codes.shape[:-1], cols)
+    if out is None:
+        if dtype not in _ROWS:
+            raise _lib.SpockError(f"{what}: dtype must be float16, bfloat16 or float32, got {dtype}")
+        out = m.codes.new_empty(shape, dtype=dtype)
+    elif out.dtype not in _ROWS:
+        raise _lib.SpockError(f"{what}: out must be float16, bfloat16 or float32, got {out.dtype}")
+    _on(what, "out", out, dev, out.dtype, shape)
+    _launch(dev, what, lib().spk_mx4_dequantize, C.byref(a), rows, cols, _ROWS[out.dtype], out.data_ptr(),
+            _row_stride(what, "out", out))
+    return out
+
+
+def _launch(dev: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of the tensors' device, which is made current for the launch."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
+
+
+def mx4_matmul(x, w: Mx4, residual: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x . w^T (+ residual) with weights in 4 bits (spk_mx4_matmul).
+
+    x [..., in] (float16 or bfloat16) or an Mx4 of such rows; w [out, in]; residual [..., out] (may be `out`).  Returns
+    [..., out] in dtype: x's, or for an Mx4 that of residual, out or `dtype` (bfloat16 without any).
+    """
+    what = "mx4_matmul"
+    four = isinstance(x, Mx4)
+    dev = _device(what, x.codes if four else x)
+    a = SpkMx4MatmulArgs()
+    a.w, n, k = _mx4_rows(what, "w", w, dev)
+    if w.codes.dim() != 2:
+        raise _lib.SpockError(f"{what}: w must be [out][in], got codes {tuple(w.codes.shape)}")
+    if four:
+        a.x4, rows, depth = _mx4_rows(what, "x", x, dev)
+        lead = x.codes.shape[:-1]
+        if dtype is None:
+            dtype = residual.dtype if residual is not None else out.dtype if out is not None else torch.bfloat16
+    else:
+        if x.dim() < 1 or dtype not in (None, x.dtype):
+            raise _lib.SpockError(f"{what}: x is {tuple(x.shape)} {x.dtype}, the result {dtype}")
+        lead, depth, dtype = x.shape[:-1], x.shape[-1], x.dtype
+        rows = lead.numel()
+        a.x, a.x_stride = x.data_ptr(), _row_stride(what, "x", x)
+    if dtype not in _HALF:
+        raise _lib.SpockError(f"{what}: rows and result must be float16 or bfloat16, got {dtype}")
+    if depth != k:
+        raise _lib.SpockError(f"{what}: x has rows of {depth} values, w of {k}")
+    shape = (*lead, n)
+    if residual is not None:
+        _on(what, "residual", residual, dev, dtype, shape)
+        a.residual, a.residual_stride = residual.data_ptr(), _row_stride(what, "residual", residual)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=w.codes.device)
+    else:
+        _on(what, "out", out, dev, dtype, shape)
+    a.out, a.out_stride = out.data_ptr(), _row_stride(what, "out", out)
+    a.dtype, a.rows, a.out_dim, a.in_dim = _HALF[dtype], rows, n, k
+    if rows and n:  # of no rows there is no address
+        _call(lib().spk_mx4_matmul, a, dev, what)
+    return out
+
+
+def mx4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda"):
+    """Pools (k_cache, v_cache) of a paged cache in 4 bits, each an Mx4 of [pages][page_size][kv_heads][head_dim] values whose
+    pages hold one head's tokens side by side: a workgroup reads one head, and shares no line of memory with others."""
+    def pool():
+        return Mx4(*(torch.zeros(pages, kv_heads, page_size, n, dtype=torch.uint8, device=device).transpose(1, 2)
+                     for n in (head_dim // 2, head_dim // 32)))
+    return pool(), pool()
+
+
+def _paged_cache_mx4(what: str, q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, block_table, cu_seqlens, context_lens):
+    dev, dtype = _device(what, q), q.dtype
+    if not isinstance(k_cache, Mx4) or not isinstance(v_cache, Mx4):
+        raise _lib.SpockError(f"{what}: the caches must be Mx4, got {type(k_cache).__name__} and {type(v_cache).__name__}")
+    if q.dim() != 3 or k_cache.codes.dim() != 4:
+        raise _lib.SpockError(f"{what}: q must be [tokens][heads][dim] and the caches' codes [pages][page_size][kv_heads][dim / 2], "
+                              f"got {tuple(q.shape)} and {tuple(k_cache.codes.shape)}")
+    if dtype not in _HALF:
+        raise _lib.SpockError(f"{what}: q must be float16 or bfloat16, got {dtype}")
+    pages, page_size, kv_heads, half = k_cache.codes.shape
+    tokens, _, dim = q.shape
+    if dim != 2 * half or dim % 32:
+        raise _lib.SpockError(f"{what}: q has head_dim {dim}, the cache {2 * half}")
+    strides = []
+    for name, n, pair in (("codes", half, (k_cache.codes, v_cache.codes)), ("scales", dim // 32, (k_cache.scales, v_cache.scales))):
+        shape = (pages, page_size, kv_heads, n)
+        for t in pair:
+            _on(what, name, t, dev, torch.uint8, shape)
+        # a stride of one element is not read
+        k, v = ([s if size > 1 else 0 for s, size in zip(t.stride(), shape)] for t in pair)
+        if k != v or (n > 1 and k[3] != 1):
+            raise _lib.SpockError(f"{what}: the {name} of k_cache and v_cache need equal strides and a contiguous last dimension, "
+                                  f"got {pair[0].stride()} and {pair[1].stride()}")
+        strides.append(k)
+    seqs = context_lens.numel()
+    _on(what, "block_table", block_table, dev, torch.int32)
+    _flat(what, "cu_seqlens", cu_seqlens, dev, torch.int32, (seqs + 1,))
+    _flat(what, "context_lens", context_lens, dev, torch.int32, (seqs,))
+    if block_table.dim() != 2 or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise _lib.SpockError(f"{what}: block_table must be [{seqs}][max_pages] with contiguous rows, "
+                              f"got {tuple(block_table.shape)}")
+    c, s = strides
+    cache = SpkPagedCache(_HALF[dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, tokens,
+                          k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), c[0], c[1], c[2],
+                          block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), context_lens.data_ptr())
+    return cache, SpkPagedScales(k_cache.scales.data_ptr(), v_cache.scales.data_ptr(), s[0], s[1], s[2])
+
+
+def mrope_append_mx4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor,
+                     pair_axis: Sequence[int], k_cache: Mx4, v_cache: Mx4, block_table: torch.Tensor,
+                     cu_seqlens: torch.Tensor, context_lens: torch.Tensor, q_norm_weight: Optional[torch.Tensor] = None,
+                     k_norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, pairing: str = "halves",
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mrope_append into pages in 4 bits (spk_mrope_append_mx4): its arguments and result, the caches Mx4 of
+    [pages][page_size][Hkv][D] values (mx4_cache; any page, token and head strides, the same for both)."""
+    what = "mrope_append_mx4"
+    cache, scales = _paged_cache_mx4(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
+    a, out = _mrope_args(what, cache, q, k, v, positions, rope, pair_axis, q_norm_weight, k_norm_weight, eps, pairing, out)
+    _launch(q.get_device(), what, lib().spk_mrope_append_mx4, C.byref(a), C.byref(scales))
+    return out
+
+
+def paged_attention_mx4(q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                        context_lens: torch.Tensor, max_query_len: int, max_context_len: int, scale: float = 0.0,
+                        window: int = 0, gate: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                        return_lse: bool = False, lse: Optional[torch.Tensor] = None,
+                        workspace: Optional[torch.Tensor] = None):
+    """paged_attention over pages in 4 bits (spk_paged_attention_mx4): its arguments and results, the caches as in
+    mrope_append_mx4, the workspace paged_attention_mx4_workspace_bytes()."""
+    what = "paged_attention_mx4"
+    cache, scales = _paged_cache_mx4(what, q, k_cache, v_cache, block_table, cu_seqlens, context_lens)
+    a, out, lse, _held = _attention_args(what, cache, q, max_query_len, max_context_len, scale, window, gate, out, return_lse, lse,
+                                         workspace, lib().spk_paged_attention_mx4_workspace_need)
+    _launch(q.get_device(), what, lib().spk_paged_attention_mx4, C.byref(a), C.byref(scales))
+    return out if lse is None else (out, lse)
+
+
+def paged_attention_mx4_workspace_bytes(tokens: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
+                                        max_pages: int, num_seqs: int, max_query_len: int, max_context_len: int,
+                                        window: int = 0) -> int:
+    """Bytes of a workspace for paged_attention_mx4 at these sizes and any smaller ones, for callers that keep one."""
+    a = _attention_sizes(tokens, heads, kv_heads, head_dim, page_size, max_pages, num_seqs, max_query_len, max_context_len, window)
+    return int(lib().spk_paged_attention_mx4_workspace_size(C.byref(a)))
