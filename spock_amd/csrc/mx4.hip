@@ -12,6 +12,7 @@ namespace {
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef int intx8 __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------------------
@@ -111,6 +112,14 @@ __device__ __forceinline__ floatx4 mfma16(uint4 a, uint4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+template <bool BF>
+__device__ __forceinline__ floatx16 mfma32(uint4 a, uint4 b, floatx16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8_t, a), __builtin_bit_cast(bf8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
 
 // Four codes' dwords as an operand of the scaled products (of 8, the upper are not read).
@@ -214,6 +223,307 @@ __global__ __launch_bounds__(64 * NW) void mx4_few_rows_kernel(Mm a) {
   }
 }
 
+// A wave's tiles into out: row m and column n are this lane's first.  vec: out's and
+// residual's groups of four values are aligned.
+template <bool BF, int TM, int TN>
+__device__ __forceinline__ void store_tile(const Mm& a, int vec, int m, int n, const floatx16 (&acc)[TN][TM]) {
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int64_t row = m + 32 * i;
+    if (row >= a.rows) continue;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int col = n + 32 * j + 2 * e;
+        float y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = acc[j][i][e + k];
+        uint16_t* to = a.out + row * a.ot + col;
+        const uint16_t* r = a.res + row * a.rt + col;
+        if (vec && col + 4 <= a.cols) {
+          if (a.res) {
+            const ushort4 u = *reinterpret_cast<const ushort4*>(r);
+            y[0] += widen<BF>(u.x);
+            y[1] += widen<BF>(u.y);
+            y[2] += widen<BF>(u.z);
+            y[3] += widen<BF>(u.w);
+          }
+          *reinterpret_cast<ushort4*>(to) = make_ushort4(narrow<BF>(y[0]), narrow<BF>(y[1]), narrow<BF>(y[2]), narrow<BF>(y[3]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (col + k >= a.cols) continue;
+            if (a.res) y[k] += widen<BF>(r[k]);
+            to[k] = narrow<BF>(y[k]);
+          }
+        }
+      }
+  }
+}
+
+// A wave's load straight into LDS, side by side at `to`: B bytes of a lane (of one byte
+// a dword is written).
+template <int B, typename T>
+__device__ __forceinline__ void load_lds(const uint8_t* from, T* to) {
+  const auto g = (const __attribute__((address_space(1))) void*)from;
+  const auto l = (__attribute__((address_space(3))) void*)to;
+  if constexpr (B == 16)
+    __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else if constexpr (B == 4)
+    __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
+  else
+    __builtin_amdgcn_global_load_lds(g, l, 1, 0, 0);
+}
+
+// All loads but the newest N of this wave have arrived, its LDS reads are done, and so are
+// those of the workgroup's other waves.
+template <int N>
+__device__ __forceinline__ void meet_after() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The tile of a workgroup: those of an XCD (its ids are 8 apart) side by side, 8 tiles
+// of rows to each tile of columns, so that what they share is in its L2.
+__device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int* tm, int* tn) {
+  const int total = tiles_m * tiles_n, q = total / 8, r = total % 8, xcd = id % 8;
+  int t = xcd * q + min(xcd, r) + id / 8;
+  const int panel = t / (8 * tiles_n), high = min(8, tiles_m - 8 * panel);
+  t -= panel * 8 * tiles_n;
+  *tn = t / high;
+  *tm = 8 * panel + t - *tn * high;
+}
+
+// Many rows: a workgroup of WM x WN waves takes a tile of rows of x and rows of w, a wave TM x TN
+// tiles of 32 x 32 of it, the depth in stages that go straight into LDS, ahead of
+// their use.  The tile is formed transposed (w is the A operand), so that a lane's
+// outputs lie side by side in a row of out.  All that is loaded goes to LDS, also
+// the scales: a load to registers among the others would make the compiler wait for all.
+// TAIL: the depth ends inside a stage; what lies past it is zero in x and w.
+
+// Rows in 16 bits: a stage is 64 values, 128 bytes of a row of x and 32 of w.  Pieces of 16
+// bytes are exchanged within a row so that 8 rows read side by side are in different
+// banks: of x by the row's number (p ^ row % 8), of w in every other four rows.  Of w a lane
+// needs one block, whose 4 dwords of codes are 4 products' operands.
+template <bool BF, int WM, int WN, int TM, int TN, bool TAIL>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles16_kernel(Mm a, int vec) {
+  constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN;
+  constexpr int PX = BM / (8 * NW), PW = BN / (32 * NW), PS = BN / (32 * NW);  // loads of a wave and stage
+  constexpr int P = PX + PW + PS;
+  static_assert(BM % (8 * NW) == 0 && BN % (32 * NW) == 0, "whole loads");
+  // x, w and the scales of three stages, an array to each: a load into one is then known
+  // not to touch the others (the compiler tells eight apart)
+  __shared__ __align__(16) uint4 sa[BM * 8 + BN * 2 + BN / 2], sb[BM * 8 + BN * 2 + BN / 2], sc[BM * 8 + BN * 2 + BN / 2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, h = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  tile_at(blockIdx.x, (a.rows + BM - 1) / BM, (a.cols + BN - 1) / BN, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int blocks = a.depth / 32, stages = (blocks + 1) / 2;
+
+  const int px = lane % 8 ^ lane / 8, pw = lane % 2 ^ (lane >> 3 & 1);
+  const uint8_t *xp[PX], *wp[PW], *sp[PS];
+#pragma unroll
+  for (int i = 0; i < PX; ++i)
+    xp[i] = reinterpret_cast<const uint8_t*>(a.x + min(m0 + 8 * (i * NW + wave) + lane / 8, a.rows - 1) * a.xt) + 16 * px;
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    const int n = min(n0 + 32 * (i * NW + wave) + lane / 2, a.cols - 1);
+    wp[i] = a.wc + n * a.wct + 16 * pw;
+    sp[i] = a.ws + n * a.wst + lane % 2;
+  }
+  auto load = [&](int st, uint4* x) __attribute__((always_inline)) {
+    uint4* w = x + BM * 8;
+    uint32_t* s = reinterpret_cast<uint32_t*>(w + BN * 2);
+    st = min(st, stages - 1);  // past the end the last one again, which nobody reads
+    const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
+#pragma unroll
+    for (int i = 0; i < PX; ++i)
+      load_lds<16>(!TAIL || 2 * st + px / 4 < blocks ? xp[i] + 128 * (int64_t)st : zero, x + 64 * (i * NW + wave));
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      load_lds<16>(!TAIL || 2 * st + pw < blocks ? wp[i] + 32 * (int64_t)st : zero, w + 64 * (i * NW + wave));
+      load_lds<1>(!TAIL || 2 * st + lane % 2 < blocks ? sp[i] + 2 * (int64_t)st : zero, s + 64 * (i * NW + wave));
+    }
+  };
+  floatx16 acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
+  const int xbase = (32 * wm * TM + ln) * 8, nbase = 32 * wn * TN + ln;
+  const int flip = ln & 7, wat = 2 * nbase + (h ^ (ln >> 2 & 1)), sat = 2 * nbase + h;
+  auto step = [&](int st, const uint4* x, uint4* to) __attribute__((always_inline)) {
+    const uint4* w = x + BM * 8;
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(w + BN * 2);
+    load(st + 2, to);
+    __builtin_amdgcn_sched_barrier(0);
+    uint4 codes[TN], v[2][TM];
+    float scale[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      codes[j] = w[wat + 64 * j];
+      scale[j] = spk_mx4::scale_of(s[sat + 64 * j]);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) v[0][i] = x[xbase + 256 * i + (4 * h ^ flip)];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (c < 3) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) v[(c + 1) & 1][i] = x[xbase + 256 * i + ((4 * h + c + 1) ^ flip)];
+      }
+      uint4 f[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) f[j] = spk_mx4::expand<BF>((&codes[j].x)[c], scale[j]);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[j][i] = mfma32<BF>(f[j], v[c & 1][i], acc[j][i]);
+    }
+    meet_after<P>();  // all but what this step asked for
+  };
+  load(0, sa);
+  load(1, sb);
+  meet_after<P>();
+  int st = 0;
+  for (; st + 3 <= stages; st += 3) {
+    step(st, sa, sc);
+    step(st + 1, sb, sa);
+    step(st + 2, sc, sb);
+  }
+  if (st < stages) step(st, sa, sc);
+  if (st + 1 < stages) step(st + 1, sb, sa);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
+  store_tile<BF, TM, TN>(a, vec, m0 + 32 * wm * TM + ln, n0 + 32 * wn * TN + 4 * h, acc);
+}
+
+// Rows in 4 bits: a stage is 128 values, 64 bytes of a row of x and of w (pieces exchanged by
+// half of the row's number) and their four scales, which the products apply.  Without
+// TAIL a row's four scales are an aligned dword, with it they are bytes apart.
+template <bool BF, int WM, int WN, int TM, int TN, bool TAIL>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles4_kernel(Mm a, int vec) {
+  constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, B = TAIL ? 4 : 1;
+  constexpr int PX = BM / (16 * NW), PW = BN / (16 * NW), PS = (BM + BN) / (64 * NW);  // loads of a wave and stage
+  constexpr int P = PX + PW + PS * B;
+  static_assert(BM % (16 * NW) == 0 && BN % (16 * NW) == 0 && (BM + BN) % (64 * NW) == 0, "whole loads");
+  constexpr int N = (BM + BN) * 4 + (BM + BN) * B / 4;
+  __shared__ __align__(16) uint4 sa[N], sb[N], sc[N], sd[N];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, h = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  tile_at(blockIdx.x, (a.rows + BM - 1) / BM, (a.cols + BN - 1) / BN, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int blocks = a.depth / 32, stages = (blocks + 3) / 4;
+
+  const int piece = lane % 4 ^ (lane / 8 & 3);
+  const uint8_t *xp[PX], *wp[PW], *sp[PS];
+#pragma unroll
+  for (int i = 0; i < PX; ++i) xp[i] = a.xc + min(m0 + 16 * (i * NW + wave) + lane / 4, a.rows - 1) * a.xct + 16 * piece;
+#pragma unroll
+  for (int i = 0; i < PW; ++i) wp[i] = a.wc + min(n0 + 16 * (i * NW + wave) + lane / 4, a.cols - 1) * a.wct + 16 * piece;
+#pragma unroll
+  for (int i = 0; i < PS; ++i) {  // rows of x, then of w
+    const int row = 64 * (i * NW + wave) + lane;
+    sp[i] = row < BM ? a.xs + min(m0 + row, a.rows - 1) * a.xst : a.ws + min(n0 + row - BM, a.cols - 1) * a.wst;
+  }
+  auto load = [&](int st, uint4* x) __attribute__((always_inline)) {
+    uint4* w = x + BM * 4;
+    uint32_t* s = reinterpret_cast<uint32_t*>(w + BN * 4);
+    st = min(st, stages - 1);
+    const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
+#pragma unroll
+    for (int i = 0; i < PX; ++i)
+      load_lds<16>(!TAIL || 4 * st + piece < blocks ? xp[i] + 64 * (int64_t)st : zero, x + 64 * (i * NW + wave));
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      load_lds<16>(!TAIL || 4 * st + piece < blocks ? wp[i] + 64 * (int64_t)st : zero, w + 64 * (i * NW + wave));
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      if constexpr (TAIL) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          load_lds<1>(4 * st + b < blocks ? sp[i] + 4 * (int64_t)st + b : zero, s + b * (BM + BN) + 64 * (i * NW + wave));
+      } else {
+        load_lds<4>(sp[i] + 4 * (int64_t)st, s + 64 * (i * NW + wave));
+      }
+    }
+  };
+  floatx16 acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
+  const int mbase = 32 * wm * TM + ln, nbase = 32 * wn * TN + ln, flip = ln >> 1 & 3;
+  auto step = [&](int st, const uint4* x, uint4* to) __attribute__((always_inline)) {
+    const uint4* w = x + BM * 4;
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(w + BN * 4);
+    load(st + 3, to);
+    __builtin_amdgcn_sched_barrier(0);
+    // the scales of this half's blocks: bytes 0 and 2, or two dwords
+    uint32_t xsc[TM][2], wsc[TN][2];
+    auto scales = [&](uint32_t (&to)[2], int row) __attribute__((always_inline)) {
+      if constexpr (TAIL) {
+        to[0] = s[row + h * (BM + BN)];
+        to[1] = s[row + (2 + h) * (BM + BN)];
+      } else {
+        to[0] = to[1] = s[row] >> (8 * h);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < TM; ++i) scales(xsc[i], mbase + 32 * i);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) scales(wsc[j], BM + nbase + 32 * j);
+    uint4 f[2][TN], v[2][TM];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) f[b][j] = w[4 * nbase + 128 * j + ((2 * b + h) ^ flip)];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) v[b][i] = x[4 * mbase + 128 * i + ((2 * b + h) ^ flip)];
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(four_bits(f[0][j]), four_bits(v[0][i]), acc[j][i], 4, 4, 0,
+                                                                    (int)wsc[j][0], 0, (int)xsc[i][0]);
+    constexpr int second = TAIL ? 0 : 2;  // byte of the second scale
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(four_bits(f[1][j]), four_bits(v[1][i]), acc[j][i], 4, 4, second,
+                                                                    (int)wsc[j][1], second, (int)xsc[i][1]);
+    meet_after<2 * P>();
+  };
+  load(0, sa);
+  load(1, sb);
+  load(2, sc);
+  meet_after<2 * P>();
+  int st = 0;
+  for (; st + 4 <= stages; st += 4) {
+    step(st, sa, sd);
+    step(st + 1, sb, sa);
+    step(st + 2, sc, sb);
+    step(st + 3, sd, sc);
+  }
+  if (st < stages) step(st, sa, sd);
+  if (st + 1 < stages) step(st + 1, sb, sa);
+  if (st + 2 < stages) step(st + 2, sc, sb);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
+  store_tile<BF, TM, TN>(a, vec, m0 + 32 * wm * TM + ln, n0 + 32 * wn * TN + 4 * h, acc);
+}
+
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
@@ -260,10 +570,35 @@ int fill_rows(const SpkMx4* m, const void* x, int32_t dtype, int64_t stride, int
   return SPK_OK;
 }
 
+template <bool X4, bool BF, int WM, int WN, int TM, int TN>
+void launch_tiles(const Mm& a, int vec, hipStream_t s) {
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
+  const dim3 grid(((a.rows + BM - 1) / BM) * ((a.cols + BN - 1) / BN)), block(64 * WM * WN);
+  if constexpr (X4) {
+    const bool dwords = a.depth % 128 == 0 && a.xst % 4 == 0 && a.wst % 4 == 0 && spk::aligned(a.xs, 4) && spk::aligned(a.ws, 4);
+    if (dwords)
+      hipLaunchKernelGGL((mx4_tiles4_kernel<BF, WM, WN, TM, TN, false>), grid, block, 0, s, a, vec);
+    else
+      hipLaunchKernelGGL((mx4_tiles4_kernel<BF, WM, WN, TM, TN, true>), grid, block, 0, s, a, vec);
+  } else if (a.depth % 64 == 0) {
+    hipLaunchKernelGGL((mx4_tiles16_kernel<BF, WM, WN, TM, TN, false>), grid, block, 0, s, a, vec);
+  } else {
+    hipLaunchKernelGGL((mx4_tiles16_kernel<BF, WM, WN, TM, TN, true>), grid, block, 0, s, a, vec);
+  }
+}
+
 template <bool X4, bool BF>
 void launch_matmul(const Mm& a, hipStream_t s) {
-  const dim3 grid((a.cols + 31) / 32, (a.rows + 63) / 64);
-  hipLaunchKernelGGL((mx4_few_rows_kernel<X4, BF, 4, 2, 4>), grid, dim3(256), 0, s, a);
+  const int vec = spk::aligned(a.out, 8) && a.ot % 4 == 0 && (!a.res || (spk::aligned(a.res, 8) && a.rt % 4 == 0));
+  const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.cols + 255) / 256);
+  if (a.rows <= 64) {
+    const dim3 grid((a.cols + 31) / 32, (a.rows + 63) / 64);
+    hipLaunchKernelGGL((mx4_few_rows_kernel<X4, BF, 4, 2, 4>), grid, dim3(256), 0, s, a);
+  } else if (big >= 128) {
+    launch_tiles<X4, BF, 2, 4, 4, 2>(a, vec, s);
+  } else {
+    launch_tiles<X4, BF, 2, 2, 2, 2>(a, vec, s);
+  }
 }
 
 }  // namespace
