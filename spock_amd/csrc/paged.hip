@@ -674,27 +674,6 @@ __global__ __launch_bounds__(256, 2) void paged_mid_kernel(Attn a) {
   }
 }
 
-// use(c, read(c)) for c below N, with the reads AHEAD of their use, or as the
-// compiler has them.
-template <int N, int AHEAD, typename Read, typename Use>
-__device__ __forceinline__ void in_turn(Read read, Use use) {
-  if constexpr (AHEAD == 0) {
-#pragma unroll
-    for (int c = 0; c < N; ++c) use(c, read(c));
-  } else {
-    uint4 f[N];
-#pragma unroll
-    for (int c = 0; c < (AHEAD < N ? AHEAD : N); ++c) f[c] = read(c);
-    __builtin_amdgcn_sched_barrier(6);  // only scalar and vector arithmetic may move past it
-#pragma unroll
-    for (int c = 0; c < N; ++c) {
-      if (c + AHEAD < N) f[c + AHEAD] = read(c + AHEAD);
-      use(c, f[c]);
-      __builtin_amdgcn_sched_barrier(6);
-    }
-  }
-}
-
 // Many rows per sequence and KV head: a workgroup of 8 waves takes 256 of the
 // n * group rows, 32 to a wave, and walks the keys in tiles of KT (16 KiB of
 // keys) that all waves share in LDS.  Loads go straight into LDS, the keys' two

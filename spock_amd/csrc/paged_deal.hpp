@@ -255,7 +255,8 @@ inline int64_t shares_of(int64_t pieces, int64_t steps) {
   return std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)), INT32_MAX);
 }
 
-inline Plan plan_of(const SpkPagedAttnArgs& p) {
+// most: rows of the larger of the two sizes of pieces of few rows.
+inline Plan plan_with(const SpkPagedAttnArgs& p, int most) {
   const SpkPagedCache& c = p.cache;
   const int group = p.num_q_heads / c.num_kv_heads;
   const int64_t tokens = std::min(p.max_query_len, c.total_tokens);
@@ -270,16 +271,16 @@ inline Plan plan_of(const SpkPagedAttnArgs& p) {
   r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : kFew + 1;
   // pieces of 16 rows where none has more (16 rows: 35 us, 38 in pieces of 64;
   // 36 rows: 42 in one of 64, 68 in three of 16)
-  r.share_rows = longest <= 16 ? 16 : 64;
+  r.share_rows = longest <= 16 ? 16 : most;
   int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
   if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
   const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
   r.steps = steps;
 
   // sequences of few rows: all of them, unless the one there is has many.
-  // Next to many rows a sequence of few is two pieces; else the bound may be low.
+  // Next to many rows a sequence of few is 128 rows at most; else the bound may be low.
   const int64_t some = all / r.share_rows + c.num_seqs;
-  const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(2 * (int64_t)c.num_seqs, some) : 0);
+  const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(kFew / r.share_rows * (int64_t)c.num_seqs, some) : 0);
   r.shares = (int)shares_of(pieces, steps);
 
   // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
@@ -305,25 +306,10 @@ inline Plan plan_of(const SpkPagedAttnArgs& p) {
   return r;
 }
 
-// The plan over a cache in 4 bits: pieces of 16 rows.
-inline Plan plan_mx4(const SpkPagedAttnArgs& p) {
-  const SpkPagedCache& c = p.cache;
-  const int group = p.num_q_heads / c.num_kv_heads;
-  const int64_t tokens = std::min(p.max_query_len, c.total_tokens), all = (int64_t)c.total_tokens * group;
-  int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
-  if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
-  Plan r{};
-  r.longest = tokens * group;
-  r.steps = std::max<int64_t>(1, (span + 127) / 128);
-  r.many = INT32_MAX;
-  r.share_rows = 16;
-  r.shares = (int)shares_of(c.num_kv_heads * (all / 16 + c.num_seqs), r.steps);
-  r.splits = 1;
-  r.chunk = (int)(128 * r.steps);
-  r.join = r.steps > 1;
-  r.join_rows = (int64_t)c.total_tokens * p.num_q_heads;
-  return r;
-}
+inline Plan plan_of(const SpkPagedAttnArgs& p) { return plan_with(p, 64); }
+
+// Over a cache in 4 bits: the pieces of sequences of few rows have 16.
+inline Plan plan_mx4(const SpkPagedAttnArgs& p) { return plan_with(p, 16); }
 
 inline size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 

@@ -303,6 +303,27 @@ __device__ __forceinline__ void store_out(const Attn& a, int token, int head, in
         make_uint2(Half<BF>::pack(x[i], x[i + 1]), Half<BF>::pack(x[i + 2], x[i + 3]));
 }
 
+// use(c, read(c)) for c below N, with the reads AHEAD of their use, or as the
+// compiler has them.
+template <int N, int AHEAD, typename T = uint4, typename Read, typename Use>
+__device__ __forceinline__ void in_turn(Read read, Use use) {
+  if constexpr (AHEAD == 0) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) use(c, read(c));
+  } else {
+    T f[N];
+#pragma unroll
+    for (int c = 0; c < (AHEAD < N ? AHEAD : N); ++c) f[c] = read(c);
+    __builtin_amdgcn_sched_barrier(6);  // only scalar and vector arithmetic may move past it
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (c + AHEAD < N) f[c + AHEAD] = read(c + AHEAD);
+      use(c, f[c]);
+      __builtin_amdgcn_sched_barrier(6);
+    }
+  }
+}
+
 // Joins the key ranges of a row: a wave to each, as fast as a whole workgroup to
 // each where there are few rows of many ranges (32 rows of 64: 106 us with the
 // attention either way) and faster where there are many (1024 rows: 24 us, 27).

@@ -479,6 +479,302 @@ __global__ __launch_bounds__(256, 2) void mx4_rows_kernel(AttnMx4 a) {
   }
 }
 
+// LDS reads, DMA-free waits: all LDS work of this wave is done, and the workgroup meets.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0) alone
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Many rows per sequence and KV head: spk_paged_attention's form for them (256 rows to a
+// workgroup of 8 waves, 32 to a wave, the keys in tiles of 8192 / D that all waves
+// share, scores transposed), from 4 bits.
+//
+// A thread holds 16 codes of a key and 16 of a value, a half of a block, loaded into
+// registers three tiles ahead, and turns them into 16-bit values in LDS one tile before they
+// are used: once for 256 rows.  Keys and values lie in LDS alike, rows of pieces of 16
+// bytes exchanged by the row's number, so that neither 8 keys' pieces side by side (the
+// scores' operand) nor 4 values' halves of 32 dimensions (the transposing load's) share
+// banks.  The transposing load makes of 4 keys' values the output's operand.
+template <int D, bool BF>
+__global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
+  using H = Half<BF>;
+  constexpr int KT = 8192 / D;             // keys of a tile
+  constexpr int KS = D / 16;               // contraction steps of the scores
+  constexpr int QR = D == 256 ? 10 : KS;   // of the queries' pieces in registers, the rest in LDS
+  constexpr int DT = D / 32;               // output tiles
+  constexpr int CH = D / 8;                // 16-byte pieces of a row
+  constexpr int TK = D / 16;               // threads of a key
+  constexpr int WK = 64 / TK;              // keys of a wave's threads
+  constexpr int NB = D == 256 ? 1 : 2;     // blocks of 32 keys at a time
+  // LDS reads ahead of the product that uses them, and of the queries' 16 pieces those in
+  // registers, as the registers allow: 2048 tokens at 16384 keys, heads of 256, take 292 us with
+  // (1, 10), 295 with (1, 8), 297 with (2, 6), 325 with (0, 12) and 337 with (0, 10).  Heads of 128: 4
+  // and 6 ahead 173 and 177 us (six prompts).
+  constexpr int AHEAD = D == 256 ? 1 : 4;
+  __shared__ __align__(16) uint4 ks[2][1024], vs[2][1024];
+  __shared__ __align__(16) uint4 qs[KS > QR ? (KS - QR) * 512 : 1];
+  __shared__ __align__(16) uint32_t there[2][8];  // keys of a tile that exist, by wave of the threads that hold them
+  __shared__ uint32_t odd_of[3][KT / 32];  // keys of a tile with blocks that are no numbers (tile number % 3)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.y, split = (blockIdx.x + (blockIdx.z >> 3)) % gridDim.x;  // another range to an XCD every 8 tiles
+  int seq, tile;
+  if (!spk_paged::find_tile<Wave>(a, blockIdx.z, gridDim.z - 1, lane, &seq, &tile)) return;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const Seq sq = spk_paged::seq_at(a.c, seq);
+  const int rows = sq.n * a.group;
+  const int r0 = tile * 256, r1 = min(r0 + 256, rows);
+  int lo, hi, lo_all, hi_all;
+  spk_paged::visible(sq, r0 / a.group, a.window, &lo, &hi_all);
+  spk_paged::visible(sq, (r1 - 1) / a.group, a.window, &lo_all, &hi);
+  const int keys = spk_paged::range_keys(a, lo, hi);
+  const int begin = (int)min((int64_t)(lo & ~31) + (int64_t)split * keys, (int64_t)hi);
+  const int end = begin + min(keys, hi - begin);
+  if (begin >= end && split > 0) return;
+  const bool alone = hi - (lo & ~31) <= keys;  // the tile's one range
+  if (a.ranges && split == 0 && tid < r1 - r0)
+    tell(a, sq, kvh, r0 + tid, -1, alone ? 1 : (hi - (lo & ~31) + keys - 1) / keys);
+
+  // this wave's rows, and the lane's
+  const int w0 = r0 + 32 * wave;
+  int row_lo, row_hi, wave_lo, wave_hi, wave_lo_all, wave_hi_all;
+  spk_paged::visible(sq, min(w0, rows - 1) / a.group, a.window, &wave_lo, &wave_hi_all);
+  spk_paged::visible(sq, min(w0 + 31, rows - 1) / a.group, a.window, &wave_lo_all, &wave_hi);
+  wave_hi = min(wave_hi, end);
+  uint4 q[QR];
+  {
+    const int r = min(w0 + ln, rows - 1), i = r / a.group;
+    spk_paged::visible(sq, i, a.window, &row_lo, &row_hi);
+    const uint16_t* src = a.q + (sq.first + i) * a.qt + (kvh * a.group + r - i * a.group) * a.qh + 8 * h;
+#pragma unroll
+    for (int c = 0; c < QR; ++c) q[c] = *reinterpret_cast<const uint4*>(src + 16 * c);
+#pragma unroll
+    for (int c = QR; c < KS; ++c) qs[(c - QR) * 512 + tid] = *reinterpret_cast<const uint4*>(src + 16 * c);
+  }
+  floatx16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+  float m = -INFINITY, shift = H::kShift, l = 0.0f;  // shift: less the maximum that the weights are relative to
+  const int32_t* table = a.c.table + (int64_t)seq * a.c.table_stride;
+
+  // this thread's key of a tile, and its 16 dimensions
+  const int kt = tid / TK, part = tid % TK;
+  const uint8_t* kcode = a.kcode + kvh * a.c.head_stride;
+  const uint8_t* vcode = a.vcode + kvh * a.c.head_stride;
+  const uint8_t* kscale = a.kscale + kvh * a.sc.head_stride;
+  const uint8_t* vscale = a.vscale + kvh * a.sc.head_stride;
+  struct Part {
+    uint2 k, v;
+    uint32_t kscale, vscale;
+    bool there;
+  };
+  auto ask = [&](int k0) __attribute__((always_inline)) {
+    return table[spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + kt, lo), end - 1))];
+  };
+  auto load = [&](int k0, int page, Part& p) __attribute__((always_inline)) {
+    const int key = k0 + kt;
+    const Place o = place_in(a.c, a.sc, page, min(max(key, lo), end - 1));
+    p.there = key >= lo && key < end && o.codes >= 0;
+    // without a place the pool's first row, masked
+    const int64_t code = (p.there ? o.codes : 0) + 8 * part, scale = (p.there ? o.scales : 0) + part / 2;
+    p.k = *reinterpret_cast<const uint2*>(kcode + code);
+    p.v = *reinterpret_cast<const uint2*>(vcode + code);
+    p.kscale = kscale[scale];
+    p.vscale = vscale[scale];
+  };
+  // Both exchanges are one: rows 0..7 have 0, 2, 4, 6, 1, 3, 5, 7.
+  auto swapped = [](int row) { return (row & 3) << 1 | (row >> 2 & 1); };
+  const int put = kt * CH + (2 * part ^ swapped(kt));  // the first piece's place; the other's is put ^ 1
+  // A block of values that is no number must not meet the zero weight of a row that does
+  // not see it: where some row of the workgroup does not, it counts as zeros, and is added
+  // row by row.
+  auto store = [&](int k0, int buf, int third, const Part& p) __attribute__((always_inline)) {
+    const float s = cached_scale<BF>(p.kscale);
+    const bool none = p.vscale > kMost<BF> && (k0 + kt < lo_all || k0 + kt >= hi_all);
+    if (p.there && none) atomicOr(&odd_of[third][kt >> 5], 1u << (kt & 31));
+    const bool take = p.there && !none;
+    const float t = take ? cached_scale<BF>(p.vscale) : 0.0f;
+    ks[buf][put] = spk_mx4::expand<BF>(p.k.x, s);
+    ks[buf][put ^ 1] = spk_mx4::expand<BF>(p.k.y, s);
+    vs[buf][put] = spk_mx4::expand<BF>(take ? p.v.x : 0, t);
+    vs[buf][put ^ 1] = spk_mx4::expand<BF>(take ? p.v.y : 0, t);
+    const bool mine = __shfl((int)p.there, lane * TK & 63);
+    const uint32_t bits = (uint32_t)__ballot(mine && lane < WK);
+    if (lane == 0) there[buf][wave] = bits;
+  };
+  // piece 2 c + h of a key: 2 c exchanges bits of the place of piece h
+  const int kread = ln * CH + (h ^ swapped(ln));
+  // the transposing load's row, half of 32 dimensions, and 8-byte piece
+  const int vrow = 4 * h + (lane >> 2 & 3), vflip = swapped(vrow), vpiece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+  const int vread = 2 * (vrow * CH + (vpiece ^ (vflip & 3))) + (lane & 1);
+  if (tid < 3 * (KT / 32)) odd_of[tid / (KT / 32)][tid % (KT / 32)] = 0;
+
+  // Tile number n at k0 (n % 3 = third, n % 2 = buf): the values of n + 1 go to LDS, the
+  // codes of n + 3 are loaded, tile n is used.
+  int page = 0;  // of tile n + 3
+  auto step = [&](int k0, int third, int buf, Part& p) __attribute__((always_inline)) {
+    store(k0 + KT, buf ^ 1, third == 2 ? 0 : third + 1, p);
+    const int next = ask(k0 + 4 * KT);
+    load(k0 + 3 * KT, page, p);
+    page = next;
+    if (tid < KT / 32) odd_of[third == 0 ? 2 : third - 1][tid] = 0;  // the tile before this one's
+    uint32_t has[KT / 32];
+#pragma unroll
+    for (int j = 0; j < KT / 32; ++j) {
+      has[j] = 0;
+#pragma unroll
+      for (int w = 0; w < 32 / WK; ++w) has[j] |= there[buf][j * (32 / WK) + w] << (w * WK % 32);
+    }
+    const bool some = k0 < lo_all || k0 + KT > hi_all;  // some row does not see some key
+    const uint4* kk = ks[buf];
+    const uint2* vv = reinterpret_cast<const uint2*>(vs[buf]);
+#pragma unroll
+    for (int j = 0; j < KT / 32; j += NB) {
+      const int kj = k0 + 32 * j;
+      if (kj >= wave_hi || kj + 32 * NB <= wave_lo) continue;  // also past the end
+      floatx16 s[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+      in_turn<NB * KS, AHEAD>(
+          [&](int x) {
+            const int c = x / NB;
+            return kk[32 * (j + x % NB) * CH + (c & ~3) * 2 + (kread ^ 2 * (c & 3))];
+          },
+          [&](int x, uint4 k) {
+            const int c = x / NB;
+            s[x % NB] = H::mfma32(k, c < QR ? q[c] : qs[(c - QR) * 512 + tid], s[x % NB]);
+          });
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int kb = kj + 32 * n;
+        const uint32_t exist = __builtin_amdgcn_readfirstlane(has[j + n]);
+        if (exist == 0xffffffffu && kb >= wave_lo_all && kb + 32 <= wave_hi_all) continue;
+        const uint32_t see = seen(exist, kb, row_lo, row_hi) >> (4 * h);  // a lane's keys at constant places
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[n][i] : -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+      top *= a.scale_log2;
+      if (__any(top > m + kBehind)) {
+        const float next = fmaxf(m, fmaxf(top, spk::lane_xor32(top)));
+        const float f = m == -INFINITY ? 0.0f : exp2_fast(m - next);
+        m = next;
+        shift = H::kShift - (next == -INFINITY ? 0.0f : next);
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[t] *= f;
+      }
+      // the weights of 16 keys while the product of the 16 before them runs
+      uint4 p4[2 * NB];
+      auto weigh = [&](int i, int e0, int e1) __attribute__((always_inline)) {
+        floatx16& x = s[i >> 1];
+#pragma unroll
+        for (int e = 8 * (i & 1) + e0; e < 8 * (i & 1) + e1; ++e) {
+          x[e] = exp2_fast(__builtin_fmaf(x[e], a.scale_log2, shift));
+          l += x[e];
+        }
+        if (e1 == 8) {
+          const int f = 8 * (i & 1);
+          p4[i] = make_uint4(H::pack(x[f], x[f + 1]), H::pack(x[f + 2], x[f + 3]), H::pack(x[f + 4], x[f + 5]),
+                             H::pack(x[f + 6], x[f + 7]));
+        }
+      };
+      weigh(0, 0, 8);
+      in_turn<2 * NB * DT, AHEAD>(
+          [&](int c) {
+            // dimension 32 t + ln of keys 16 i + 4 h .. + 3 and 8 further
+            const int i = c / DT, t = c % DT;
+            const uint2* at = vv + 2 * (32 * j + 16 * i) * CH + 8 * (t & ~1) + (vread + 8 * ((t & 1) ^ (vflip >> 2)));
+            const uint2 u = transposed(at), w = transposed(at + 16 * CH);
+            return make_uint4(u.x, u.y, w.x, w.y);
+          },
+          [&](int c, uint4 v) {
+            const int i = c / DT, t = c % DT;
+            acc[t] = H::mfma32(v, p4[i], acc[t]);
+            if (i + 1 < 2 * NB) weigh(i + 1, 8 * t / DT, 8 * (t + 1) / DT);
+          });
+      if (some) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          uint32_t odd = __builtin_amdgcn_readfirstlane(odd_of[third][j + n]);
+          while (odd) {
+            const int key = kj + 32 * n + __ffs(odd) - 1;
+            odd &= odd - 1;
+            const uint8_t* row = a.vscale + kvh * a.sc.head_stride + max(place_of(a.c, a.sc, seq, key).scales, (int64_t)0);
+            if (key >= row_lo && key < row_hi) {
+#pragma unroll
+              for (int t = 0; t < DT; ++t)
+                if (row[t] > kMost<BF>) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) acc[t][i] = NAN;
+                }
+            }
+          }
+        }
+      }
+    }
+    meet();
+  };
+  if (begin < end) {
+    Part pa, pb;
+    const int first = ask(begin), second = ask(begin + KT), last = ask(begin + 2 * KT);
+    page = ask(begin + 3 * KT);
+    load(begin, first, pa);
+    load(begin + KT, second, pb);
+    __syncthreads();  // odd_of is clear
+    store(begin, 0, 0, pa);
+    load(begin + 2 * KT, last, pa);
+    meet();
+    int third = 0;
+    for (int k0 = begin; k0 < end; k0 += 2 * KT) {
+      step(k0, third, 0, pb);
+      third = third == 2 ? 0 : third + 1;
+      step(k0 + KT, third, 1, pa);
+      third = third == 2 ? 0 : third + 1;
+    }
+  }
+
+  l += spk::lane_xor32(l);
+  const int r = w0 + ln;
+  if (r >= rows) return;
+  const int ri = r / a.group, head = kvh * a.group + r - ri * a.group, token = sq.first + ri;
+  const int64_t at = (int64_t)token * a.heads + head;
+  float* out = a.part + (at + (int64_t)split * a.c.total_tokens * a.heads) * (D + 2);
+  if (h == 0) {
+    if (!alone) {
+      out[0] = m;
+      out[1] = l;
+    } else if (a.lse) {
+      a.lse[at] = l == 0.0f ? -INFINITY : (m - H::kShift + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+  }
+  const float inv = !alone ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float o[4] = {acc[t][4 * i] * inv, acc[t][4 * i + 1] * inv, acc[t][4 * i + 2] * inv, acc[t][4 * i + 3] * inv};
+      const int d = 32 * t + 8 * i + 4 * h;
+      if (!alone) {
+        *reinterpret_cast<float2*>(out + 2 + d) = make_float2(o[0], o[1]);
+        *reinterpret_cast<float2*>(out + 4 + d) = make_float2(o[2], o[3]);
+      } else {
+        store_out<BF, 4>(a, token, head, d, o);
+      }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
@@ -502,7 +798,8 @@ int check_scales(const SpkPagedCache& c, const SpkPagedScales* s, const char* wh
 
 template <int D, bool BF>
 void launch_attn(const AttnMx4& a, const Plan& r, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_rows_kernel<D, BF>), dim3(r.shares), dim3(256), 0, s, a);
+  if (r.shares) hipLaunchKernelGGL((mx4_rows_kernel<D, BF>), dim3(r.shares), dim3(256), 0, s, a);
+  if (r.tiles) hipLaunchKernelGGL((mx4_tiles_kernel<D, BF>), dim3(r.splits, a.kv_heads, r.tiles), dim3(512), 0, s, a);
   if (!r.join) return;
   hipLaunchKernelGGL((paged_join_kernel<D, BF>), dim3((unsigned)((r.join_rows + 3) / 4)), dim3(256), 0, s, a);
 }
