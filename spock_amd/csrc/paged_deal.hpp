@@ -255,8 +255,17 @@ inline int64_t shares_of(int64_t pieces, int64_t steps) {
   return std::min<int64_t>(std::min<int64_t>(2 * pieces <= slots ? slots : pieces + slots, pieces * (steps + 1)), INT32_MAX);
 }
 
-// most: rows of the larger of the two sizes of pieces of few rows.
-inline Plan plan_with(const SpkPagedAttnArgs& p, int most) {
+// Over a cache in 4 bits: whole rounds of the workgroups that the chip holds at once, 2
+// to a piece.
+inline int64_t shares_mx4(const SpkPagedAttnArgs& p, int64_t pieces, int64_t steps) {
+  const int64_t round = p.cache.head_dim == 256 ? 512 : 768;
+  const int64_t n = (2 * pieces + round - 1) / round * round;
+  return std::min<int64_t>(std::min<int64_t>(n, pieces * (steps + 1)), INT32_MAX);
+}
+
+// FOUR: over a cache in 4 bits, where pieces of few rows have 16.
+template <bool FOUR>
+Plan plan_with(const SpkPagedAttnArgs& p) {
   const SpkPagedCache& c = p.cache;
   const int group = p.num_q_heads / c.num_kv_heads;
   const int64_t tokens = std::min(p.max_query_len, c.total_tokens);
@@ -271,7 +280,7 @@ inline Plan plan_with(const SpkPagedAttnArgs& p, int most) {
   r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : kFew + 1;
   // pieces of 16 rows where none has more (16 rows: 35 us, 38 in pieces of 64;
   // 36 rows: 42 in one of 64, 68 in three of 16)
-  r.share_rows = longest <= 16 ? 16 : most;
+  r.share_rows = FOUR || longest <= 16 ? 16 : 64;
   int64_t span = std::min<int64_t>(p.max_context_len, (int64_t)c.max_pages * c.page_size);
   if (p.window > 0) span = std::min<int64_t>(span, (int64_t)p.window + tokens + 31);
   const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);  // of 128 keys
@@ -281,7 +290,7 @@ inline Plan plan_with(const SpkPagedAttnArgs& p, int most) {
   // Next to many rows a sequence of few is 128 rows at most; else the bound may be low.
   const int64_t some = all / r.share_rows + c.num_seqs;
   const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(kFew / r.share_rows * (int64_t)c.num_seqs, some) : 0);
-  r.shares = (int)shares_of(pieces, steps);
+  r.shares = (int)(FOUR ? shares_mx4(p, pieces, steps) : shares_of(pieces, steps));
 
   // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
   // the number of ranges that takes the fewest rounds of 256 workgroups times
@@ -306,10 +315,8 @@ inline Plan plan_with(const SpkPagedAttnArgs& p, int most) {
   return r;
 }
 
-inline Plan plan_of(const SpkPagedAttnArgs& p) { return plan_with(p, 64); }
-
-// Over a cache in 4 bits: the pieces of sequences of few rows have 16.
-inline Plan plan_mx4(const SpkPagedAttnArgs& p) { return plan_with(p, 16); }
+inline Plan plan_of(const SpkPagedAttnArgs& p) { return plan_with<false>(p); }
+inline Plan plan_mx4(const SpkPagedAttnArgs& p) { return plan_with<true>(p); }
 
 inline size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -336,19 +343,26 @@ inline size_t workspace_of(const SpkPagedAttnArgs& p, const Plan& r) {
 // part: shares of either size; and with groups = tiles * KV heads, of at most 256
 // rows each, up to 512 / groups + 1 ranges of at least 4 steps while that is more
 // than one.
-inline size_t workspace_bound(const SpkPagedAttnArgs& p) {
+template <bool FOUR>
+size_t bound_with(const SpkPagedAttnArgs& p) {
   const SpkPagedCache& c = p.cache;
-  const Plan r = plan_of(p);
+  const Plan r = plan_with<FOUR>(p);
   const int64_t all = (int64_t)c.total_tokens * (p.num_q_heads / c.num_kv_heads), rows = (int64_t)c.total_tokens * p.num_q_heads;
   if (r.steps <= 1) return 0;
-  auto shared = [&](int64_t share_rows) { return share_rows * shares_of(c.num_kv_heads * (all / share_rows + c.num_seqs), r.steps); };
+  auto shared = [&](int64_t share_rows) {
+    const int64_t pieces = c.num_kv_heads * (all / share_rows + c.num_seqs);
+    return share_rows * (FOUR ? shares_mx4(p, pieces, r.steps) : shares_of(pieces, r.steps));
+  };
   int64_t parts = shared(16);
-  if (r.longest > 16) parts = std::max(parts, shared(64));
+  if (!FOUR && r.longest > 16) parts = std::max(parts, shared(64));
   int64_t split = 0;
   if (r.longest > kFew && r.steps >= 8)
     split = std::min(131072 + 256 * std::min<int64_t>(512, (all + 255) / 256 * c.num_kv_heads), rows * (r.steps / 4));
   return up(parts * part_bytes(p)) + up(rows * 2 * sizeof(int32_t)) + split * part_bytes(p);
 }
+
+inline size_t workspace_bound(const SpkPagedAttnArgs& p) { return bound_with<false>(p); }
+inline size_t workspace_bound_mx4(const SpkPagedAttnArgs& p) { return bound_with<true>(p); }
 
 // What the kernels know of it.
 inline Deal deal_of(const SpkPagedAttnArgs& p, const Plan& r, const Cache& c) {

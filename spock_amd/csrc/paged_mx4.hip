@@ -190,28 +190,70 @@ struct AttnMx4 : Attn {
   Scales sc;
 };
 
+// A wave's load straight into LDS, side by side at `to`: B bytes of a lane (of one byte
+// a dword is written).
+template <int B, typename T>
+__device__ __forceinline__ void load_lds(const void* from, T* to) {
+  const auto g = (const __attribute__((address_space(1))) void*)from;
+  const auto l = (__attribute__((address_space(3))) void*)to;
+  if constexpr (B == 16)
+    __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else if constexpr (B == 4)
+    __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
+  else
+    __builtin_amdgcn_global_load_lds(g, l, 1, 0, 0);
+}
+
+// All loads of this wave but the newest N have arrived.  (As a builtin, which the compiler
+// takes into account: told in assembly it waits for all of them before it reads what they wrote.)
+template <int N>
+__device__ __forceinline__ void arrived() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
+  asm volatile("" ::: "memory");
+}
+
 // Few rows per sequence and KV head: spk_paged_attention's form for them (16 rows of
 // a sequence and a range of its keys to a workgroup, every fourth step of 32 keys
 // to a wave, scores transposed, the waves' states joined in LDS), from 4 bits.
 //
+// A step's codes, scales and page ids go straight into the wave's own LDS, whole rows to
+// neighbouring lanes: read from memory in the operands' order they took four times
+// the loads (4 bytes a lane of the values, 1 of the scales), and the pipe of addresses was
+// the bound (64 sequences, heads of 128: 174 us, 3.3 TB/s).  At each step a wave asks for
+// the step N - 1 further on, whose page ids it asked for N steps ago, and waits for its
+// own.  Keys lie in LDS as in memory but for pieces exchanged by the row's number, so that
+// 8 rows read side by side are in different banks; key 4 g + j of 16 values lies in row 4 j + g,
+// so that what the four lane groups read lies together.
+//
 // A lane of the scores' A operand holds 32 codes of a key that lie side by side,
 // one block and one scale (heads of 64: half a block), as 4 contraction steps of
-// 8; the queries' dimensions are dealt the same way.  Of the values it holds 8
-// dimensions (heads of 64: 4) of its 8 keys.  Codes become 16-bit values with
-// their scale in the conversion: exact but for what the type cannot hold.  A weight
-// enters the second product rounded to 16 bits: the cache's own rounding is a
-// hundred times as much.
-template <int D, bool BF>
-__global__ __launch_bounds__(256, 2) void mx4_rows_kernel(AttnMx4 a) {
+// 8; the queries' dimensions are dealt the same way.  Of the values it holds D / 16
+// dimensions of its 8 keys.  Codes become 16-bit values with their scale in the conversion:
+// exact but for what the type cannot hold.  A weight enters the second product
+// rounded to 16 bits: the cache's own rounding is a hundred times as much.
+// BYTES: the scales' rows are not aligned to 4 bytes (or have 2), and are loaded by the byte.
+template <int D, bool BF, bool BYTES>
+__global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void mx4_rows_kernel(AttnMx4 a) {
   using H = Half<BF>;
-  constexpr int NB = D >= 128 ? D / 128 : 1;  // blocks of a key in a lane
-  constexpr int NC = D >= 128 ? 4 : 2;        // contraction steps of one
-  constexpr int EV = D >= 128 ? 8 : 4;        // dimensions of a lane's values that lie side by side
-  constexpr int NH = D / (16 * EV);           // such pieces
-  constexpr int LD = D + 4;                   // padded rows of the joint
-  __shared__ __align__(16) float joint[4][16][LD];
-  __shared__ float stat[4][16][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int NB = D >= 128 ? D / 128 : 1;   // blocks of a key in a lane
+  constexpr int NC = D >= 128 ? 4 : 2;         // contraction steps of one
+  constexpr int EV = D / 16;                   // dimensions of a lane's values
+  constexpr int CP = D / 32;                   // 16-byte pieces of a row of codes, and blocks
+  constexpr int RL = 64 / CP;                  // rows of a load
+  constexpr int NL = 32 / RL;                  // loads of a step's keys
+  constexpr int SB = BYTES ? 1 : 4;            // bytes of a lane's load of scales
+  constexpr int NS = CP / SB;                  // such loads, lanes 0..31 of the keys, 32..63 of the values
+  constexpr int N = D == 256 ? 2 : 3;          // steps in LDS
+  constexpr int P = 2 * NL + NS + 1;           // loads of a step
+  constexpr int KW = 32 * CP;                  // 16-byte pieces of a step's keys
+  constexpr int SIZE = 2 * KW + NS * 16;       // of a step
+  constexpr int JW = 68, JOINT = 4 * 16 * JW / 4;  // padded rows of the joint, and its pieces
+  constexpr int FIRST = 4 * SIZE > JOINT ? 4 * SIZE : JOINT;
+  // an array to each step: a load into one is then known not to touch the others
+  __shared__ __align__(16) uint4 sa[FIRST], sb[4 * SIZE], sc[N == 3 ? 4 * SIZE : 1];
+  __shared__ int32_t ia[128], ib[128], ic[N == 3 ? 128 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, g = lane >> 4;
   Share sh;
   if (!spk_paged::find_share<Wave>(a, blockIdx.x, lane, &sh)) return;
@@ -232,108 +274,114 @@ __global__ __launch_bounds__(256, 2) void mx4_rows_kernel(AttnMx4 a) {
   const uint8_t* vcode = a.vcode + kvh * a.c.head_stride;
   const uint8_t* kscale = a.kscale + kvh * a.sc.head_stride;
   const uint8_t* vscale = a.vscale + kvh * a.sc.head_stride;
-  auto load_page = [&](int k0) {
+  const uint8_t* scales = lane < 32 ? kscale : vscale;
+  // the lower lanes ask for the pages of the keys from k0 on
+  auto ask = [&](int k0, int32_t* ids) __attribute__((always_inline)) {
+    if (lane < 32)
+      load_lds<4>(table + spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + lane, lo), end - 1)), ids + 32 * wave);
+  };
+  // what row r of a step's keys and of its values in LDS holds
+  const int kfirst = lane / CP, kpiece = lane % CP ^ (CP == 8 ? kfirst & 7 : CP == 4 ? kfirst >> 1 & 3 : 0);
+  const int idat = 32 * wave + (lane & 31);
+  auto value_key = [](int r) { return (r & ~15) + 4 * (r & 3) + (r >> 2 & 3); };
+  // Asks for the codes and scales of the step at k0; the keys of it that exist.
+  auto load = [&](int k0, const int32_t* ids, uint4* to) __attribute__((always_inline)) {
     const int key = k0 + (lane & 31);
-    return key >= lo && key < end ? table[spk_paged::divide(a.c.div, (uint32_t)key)] : -1;
-  };
-  Place off{0, 0};
-  uint32_t valid = 0;
-  auto look_up = [&](int k0, int page) {
-    off = place_in(a.c, a.sc, page, k0 + (lane & 31));
-    valid = (uint32_t)__ballot(off.codes >= 0);
-    if (off.codes < 0) off = Place{0, 0};
-  };
-  constexpr int kLaneCodes = D >= 128 ? 16 : 8;  // bytes of a lane's part of a key's block
-  uint4 kf[2][NB];
-  uint32_t ks[2][NB];
-  uint32_t v[8][NH], vs[8][NH];
-  auto load_k = [&]() {
+    Place off = place_in(a.c, a.sc, ids[idat], min(max(key, lo), end - 1));
+    const bool there = key >= lo && key < end && off.codes >= 0;
+    if (!there) off = Place{0, 0};  // the pool's first row, masked
+    uint4* x = to + SIZE * wave;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint8_t* p = kcode + __shfl(off.codes, 16 * t + ln) + kLaneCodes * g;
-      const uint8_t* q = kscale + __shfl(off.scales, 16 * t + ln) + (D >= 128 ? g : g / 2);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        if constexpr (D >= 128) {
-          kf[t][b] = *reinterpret_cast<const uint4*>(p + 64 * b);
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(p);
-          kf[t][b] = make_uint4(w.x, w.y, 0, 0);
-        }
-        ks[t][b] = q[4 * b];
-      }
+    for (int i = 0; i < NL; ++i) {
+      const int64_t k = __shfl(off.codes, RL * i + kfirst), v = __shfl(off.codes, value_key(RL * i + kfirst));
+      load_lds<16>(kcode + k + 16 * kpiece, x + 64 * i);
+      load_lds<16>(vcode + v + 16 * (lane % CP), x + KW + 64 * i);
     }
-  };
-  auto load_v = [&]() {
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      const int kl = 16 * (kk >> 2) + 4 * g + (kk & 3);
-      const uint8_t* p = vcode + __shfl(off.codes, kl) + EV / 2 * ln;
-      const uint8_t* q = vscale + __shfl(off.scales, kl) + EV * ln / 32;
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        if constexpr (EV == 8)
-          v[kk][h] = *reinterpret_cast<const uint32_t*>(p + 64 * h);
-        else
-          v[kk][h] = *reinterpret_cast<const uint16_t*>(p);
-        vs[kk][h] = q[4 * h];
-      }
-    }
+    for (int i = 0; i < NS; ++i) load_lds<SB>(scales + off.scales + SB * i, x + 2 * KW + 16 * i);
+    return (uint32_t)__ballot(there);
   };
-
-  int k0 = begin + 32 * wave;
-  int page = -1;  // of the step after the one that is loaded
-  if (k0 < end) {
-    const int first = load_page(k0);
-    page = load_page(k0 + 128);
-    look_up(k0, first);
-    load_k();
-    load_v();
-  }
   const int r = min(r0 + ln, rows - 1);  // this lane's row
   uint4 q[NB][NC];
   int row_lo, row_hi;
   {
     const int i = r / a.group;
     spk_paged::visible(sq, i, a.window, &row_lo, &row_hi);
-    const uint16_t* src = a.q + (sq.first + i) * a.qt + (kvh * a.group + r - i * a.group) * a.qh + 2 * kLaneCodes * g;
+    const uint16_t* src = a.q + (sq.first + i) * a.qt + (kvh * a.group + r - i * a.group) * a.qh + (D >= 128 ? 32 : 16) * g;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int c = 0; c < NC; ++c) q[b][c] = *reinterpret_cast<const uint4*>(src + 128 * b + 8 * c);
   }
   float m = -INFINITY, base = 0.0f, l = 0.0f;
-  floatx4 acc[NH][EV];
+  floatx4 acc[EV];
 #pragma unroll
-  for (int h = 0; h < NH; ++h)
+  for (int e = 0; e < EV; ++e) acc[e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  // Where this lane's parts of a step lie, in bytes.  (As one number each: of an address made
+  // of many parts the compiler no longer knows the array, and waits for all loads before it reads.)
+  const int mine = 16 * SIZE * wave, kflip = CP == 8 ? ln & 7 : ln >> 1 & 3;
+  const int kat0 = D >= 128 ? mine + 16 * (ln * CP + (g ^ kflip)) : mine + 32 * ln + 8 * g;
+  const int kat1 = mine + 16 * (ln * CP + (4 + g ^ kflip));  // heads of 256: the second block's
+  const int vat = mine + 16 * KW + 16 * CP * g + EV / 2 * ln;
+  auto scale_at = [&](int b, int key) { return mine + 32 * KW + 4 * (b / SB * 64 + key) + b % SB; };  // values: key + 32
+  const int ksat0 = scale_at(D >= 128 ? g : g / 2, ln), ksat1 = scale_at(4 + g, ln), vsat = scale_at(ln * EV / 32, 32 + 4 * g);
+  // The step at k0, which lies in `at`; asks for the one N - 1 further, into `to`.
+  auto step = [&](int k0, const uint4* at, uint32_t has, int32_t* ids, uint4* to, uint32_t& next) __attribute__((always_inline)) {
+    next = load(k0 + 128 * (N - 1), ids, to);
+    ask(k0 + 128 * (2 * N - 1), ids);
+    arrived<(N - 1) * P>();
+    if (k0 >= end) return;
+    const auto* x = reinterpret_cast<const uint8_t*>(at);
+    const bool full = has == 0xffffffffu && k0 >= lo_all && k0 + 32 <= hi_all;
+    uint32_t ksc[2][NB], vsc[8], most = 0;
 #pragma unroll
-    for (int e = 0; e < EV; ++e) acc[h][e] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  for (; k0 < end; k0 += 128) {
-    const bool full = valid == 0xffffffffu && k0 >= lo_all && k0 + 32 <= hi_all;
-    const uint32_t has = valid;
-    const bool more = k0 + 128 < end;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) ksc[t][b] = x[(b ? ksat1 : ksat0) + 64 * t];
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) vsc[kk] = x[vsat + 64 * (kk >> 2) + 4 * (kk & 3)];
     floatx4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const float scale = cached_scale<BF>(ks[t][b]);
+        most = max(most, ksc[t][b]);
+        uint4 u;
+        if constexpr (D >= 128) {
+          u = *reinterpret_cast<const uint4*>(x + (b ? kat1 : kat0) + 256 * CP * t);
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(x + kat0 + 512 * t);
+          u = make_uint4(w.x, w.y, 0, 0);
+        }
 #pragma unroll
-        for (int c = 0; c < NC; ++c) s[t] = H::mfma16(spk_mx4::expand<BF>((&kf[t][b].x)[c], scale), q[b][c], s[t]);
+        for (int c = 0; c < NC; ++c)
+          s[t] = H::mfma16(spk_mx4::expand<BF>((&u.x)[c], spk_mx4::scale_of(ksc[t][b])), q[b][c], s[t]);
       }
-    }
-    if (more) {
-      look_up(k0 + 128, page);
-      page = load_page(k0 + 256);
-      load_k();
     }
     float w[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       w[i] = s[0][i];
       w[4 + i] = s[1][i];
+    }
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) most = max(most, vsc[kk]);
+    const bool odd = __any(most > kMost<BF>);  // some block is no number
+    if (odd) {
+      // a key that has one is none: its score is no number, where it is seen
+      uint32_t none = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        bool bad = false;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) bad = bad || ksc[t][b] > kMost<BF>;
+        const unsigned long long v = __ballot(bad);
+        none |= (uint32_t)((v | v >> 16 | v >> 32 | v >> 48) & 0xffff) << (16 * t);
+      }
+      none >>= 4 * g;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = none >> (16 * (i >> 2) + (i & 3)) & 1u ? NAN : w[i];
     }
     if (!full) {
       const uint32_t see = seen(has, k0, row_lo, row_hi) >> (4 * g);  // a lane's keys at constant places
@@ -354,9 +402,7 @@ __global__ __launch_bounds__(256, 2) void mx4_rows_kernel(AttnMx4 a) {
       base = nb;
       l *= f;
 #pragma unroll
-      for (int h = 0; h < NH; ++h)
-#pragma unroll
-        for (int e = 0; e < EV; ++e) acc[h][e] *= f;
+      for (int e = 0; e < EV; ++e) acc[e] *= f;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -364,115 +410,148 @@ __global__ __launch_bounds__(256, 2) void mx4_rows_kernel(AttnMx4 a) {
       l += w[i];
     }
     const uint4 p = make_uint4(H::pack(w[0], w[1]), H::pack(w[2], w[3]), H::pack(w[4], w[5]), H::pack(w[6], w[7]));
-    uint32_t odd_keys = 0;
-    if (!full) {
-      // a block without a number must not meet the zero weight of a row that does
-      // not see it: it counts as zeros here, and is added row by row
+    // a block of values that is no number must not meet the zero weight of a row that
+    // does not see it: it counts as zeros here, and is added row by row below
+    uint32_t odd_keys = 0, zeros = 0;
+    if (odd) {
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        const int kl = 16 * (kk >> 2) + 4 * g + (kk & 3);
-        bool odd = false;
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const bool none = vs[kk][h] > kMost<BF>;
-          odd = odd || (none && (has >> kl & 1u));
-          if (none) {
-            v[kk][h] = 0;
-            vs[kk][h] = 127;
-          }
-        }
-        const unsigned long long b = __ballot(odd);
+        const bool none = vsc[kk] > kMost<BF>;
+        zeros |= (none ? 1u : 0u) << kk;
+        const unsigned long long b = __ballot(none && (has >> (16 * (kk >> 2) + 4 * g + (kk & 3)) & 1u));
 #pragma unroll
         for (int gg = 0; gg < 4; ++gg)
           if ((b >> (16 * gg)) & 0xffffull) odd_keys |= 1u << (16 * (kk >> 2) + 4 * gg + (kk & 3));
       }
     }
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      uint4 x[8];
+    for (int e0 = 0; e0 < EV; e0 += 8) {  // 8 dimensions (heads of 64: 4) at a time
+      uint4 v[8];
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) x[kk] = spk_mx4::expand<BF>(v[kk][h], cached_scale<BF>(vs[kk][h]));
+      for (int kk = 0; kk < 8; ++kk) {
+        const auto* from = x + vat + 16 * CP * (16 * (kk >> 2) + 4 * (kk & 3)) + e0 / 2;
+        uint32_t u;
+        if constexpr (EV == 4)
+          u = *reinterpret_cast<const uint16_t*>(from);
+        else
+          u = *reinterpret_cast<const uint32_t*>(from);
+        v[kk] = spk_mx4::expand<BF>(u, spk_mx4::scale_of(vsc[kk]));
+      }
+      if (odd) {
 #pragma unroll
-      for (int e = 0; e < EV; ++e) {
+        for (int kk = 0; kk < 8; ++kk)
+          if (zeros >> kk & 1u) v[kk] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = e0; e < (EV < e0 + 8 ? EV : e0 + 8); ++e) {
         uint4 f;  // dimension e of the 8 keys
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          (&f.x)[i] = __builtin_amdgcn_perm((&x[2 * i + 1].x)[e >> 1], (&x[2 * i].x)[e >> 1],
+          (&f.x)[i] = __builtin_amdgcn_perm((&v[2 * i + 1].x)[(e & 7) >> 1], (&v[2 * i].x)[(e & 7) >> 1],
                                             e & 1 ? 0x07060302u : 0x05040100u);
-        acc[h][e] = H::mfma16(f, p, acc[h][e]);
+        acc[e] = H::mfma16(f, p, acc[e]);
       }
     }
-    if (more) load_v();
     while (odd_keys) {
       const int kl = __ffs(odd_keys) - 1;
       odd_keys &= odd_keys - 1;
-      const uint8_t* row = vscale + max(place_of(a.c, a.sc, seq, k0 + kl).scales, (int64_t)0);
       if (k0 + kl >= row_lo && k0 + kl < row_hi) {
 #pragma unroll
-        for (int h = 0; h < NH; ++h)
-          if (row[D >= 128 ? 4 * h + g : g / 2] > kMost<BF>) {
+        for (int i = 0; i < 4; ++i)  // this lane's outputs are dimensions EV (4 g + i) + e
+          if (x[scale_at(EV * (4 * g + i) / 32, 32 + kl)] > kMost<BF>) {
 #pragma unroll
-            for (int e = 0; e < EV; ++e) acc[h][e] = floatx4{NAN, NAN, NAN, NAN};
+            for (int e = 0; e < EV; ++e) acc[e][i] = NAN;
           }
       }
     }
+  };
+  int k0 = begin + 32 * wave;
+  if (k0 < end) {
+    uint32_t ha, hb, hc = 0;
+    // the first N steps' page ids, then the first N - 1 steps and N further page ids in the
+    // order in which steps ask for them
+    ask(k0, ia);
+    ask(k0 + 128, ib);
+    if constexpr (N == 3) ask(k0 + 256, ic);
+    arrived<0>();
+    if constexpr (N == 3) {
+      ha = load(k0, ia, sa);
+      ask(k0 + 384, ia);
+      hb = load(k0 + 128, ib, sb);
+      ask(k0 + 512, ib);
+      // step n reads slot n + 2 (mod 3): ids of step 2 are in ic, of 3 in ia, of 4 in ib
+      for (; k0 < end; k0 += 384) {
+        step(k0, sa, ha, ic, sc, hc);
+        step(k0 + 128, sb, hb, ia, sa, ha);
+        step(k0 + 256, sc, hc, ib, sb, hb);
+      }
+    } else {
+      ha = load(k0, ia, sa);
+      ask(k0 + 256, ia);
+      for (; k0 < end; k0 += 256) {
+        step(k0, sa, ha, ib, sb, hb);
+        step(k0 + 128, sb, hb, ia, sa, ha);
+      }
+    }
   }
+  arrived<0>();  // loads past the end still write LDS
 
-  // join the waves
+  // join the waves, 4 dimensions of each 16th of a row at a time
   l += spk::lane_xor16(l);
   l += spk::lane_xor32(l);
-#pragma unroll
-  for (int h = 0; h < NH; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < EV; e += 4)
-        *reinterpret_cast<float4*>(&joint[wave][ln][16 * EV * h + EV * (4 * g + i) + e]) =
-            make_float4(acc[h][e][i], acc[h][e + 1][i], acc[h][e + 2][i], acc[h][e + 3][i]);
+  auto stat = reinterpret_cast<float(*)[16][2]>(sb);
+  __syncthreads();
   if (g == 0) {
     stat[wave][ln][0] = m;
     stat[wave][ln][1] = l;
   }
-  __syncthreads();
-  const int row = threadIdx.x >> 4, rj = r0 + row;
-  if (rj >= rows) return;
-  float top = -INFINITY, sum = 0.0f, f[4];
-#pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][row][0]);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = top == -INFINITY ? 1.0f : exp2_fast(stat[w][row][0] - top);
-    sum += f[w] * stat[w][row][1];
-  }
+  auto joint = reinterpret_cast<float(*)[16][JW]>(sa);
+  const int row = threadIdx.x >> 4, part = threadIdx.x & 15, rj = r0 + row;
   const int i = rj / a.group, token = sq.first + i, head = kvh * a.group + rj - i * a.group;
   const int64_t at = (int64_t)token * a.heads + head;
-  float* part = a.shared + ((int64_t)blockIdx.x * 16 + row) * (D + 2);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float* out = a.shared + ((int64_t)blockIdx.x * 16 + row) * (D + 2);
+  float top = -INFINITY, sum = 0.0f, f[4];
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) {
-    const int d = 64 * c + 4 * (threadIdx.x & 15);
+  for (int c = 0; c < EV; c += 4) {
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      *reinterpret_cast<float4*>(&joint[wave][ln][4 * (4 * g + n)]) = make_float4(acc[c][n], acc[c + 1][n], acc[c + 2][n], acc[c + 3][n]);
+    __syncthreads();
+    if (c == 0) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][row][0]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        f[w] = top == -INFINITY ? 1.0f : exp2_fast(stat[w][row][0] - top);
+        sum += f[w] * stat[w][row][1];
+      }
+    }
+    if (rj >= rows) continue;
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float4 x = *reinterpret_cast<const float4*>(&joint[w][row][d]);
+      const float4 x = *reinterpret_cast<const float4*>(&joint[w][row][4 * part]);
       o[0] += f[w] * x.x;
       o[1] += f[w] * x.y;
       o[2] += f[w] * x.z;
       o[3] += f[w] * x.w;
     }
+    const int d = EV * part + c;
     if (sh.ranges == 1) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
       for (int n = 0; n < 4; ++n) o[n] *= inv;
       store_out<BF, 4>(a, token, head, d, o);
     } else {
-      *reinterpret_cast<float2*>(part + 2 + d) = make_float2(o[0], o[1]);
-      *reinterpret_cast<float2*>(part + 4 + d) = make_float2(o[2], o[3]);
+      *reinterpret_cast<float2*>(out + 2 + d) = make_float2(o[0], o[1]);
+      *reinterpret_cast<float2*>(out + 4 + d) = make_float2(o[2], o[3]);
     }
   }
-  if ((threadIdx.x & 15) == 0) {
+  if (part == 0 && rj < rows) {
     if (sh.ranges > 1) {
-      part[0] = top;
-      part[1] = sum;
+      out[0] = top;
+      out[1] = sum;
     } else if (a.lse) {
       a.lse[at] = sum == 0.0f ? -INFINITY : (top - H::kShift + __builtin_amdgcn_logf(sum)) * kLn2;
     }
@@ -797,8 +876,11 @@ int check_scales(const SpkPagedCache& c, const SpkPagedScales* s, const char* wh
 }
 
 template <int D, bool BF>
-void launch_attn(const AttnMx4& a, const Plan& r, hipStream_t s) {
-  if (r.shares) hipLaunchKernelGGL((mx4_rows_kernel<D, BF>), dim3(r.shares), dim3(256), 0, s, a);
+void launch_attn(const AttnMx4& a, const Plan& r, bool bytes, hipStream_t s) {
+  if (r.shares && bytes)
+    hipLaunchKernelGGL((mx4_rows_kernel<D, BF, true>), dim3(r.shares), dim3(256), 0, s, a);
+  else if (r.shares)
+    hipLaunchKernelGGL((mx4_rows_kernel<D, BF, D == 64>), dim3(r.shares), dim3(256), 0, s, a);
   if (r.tiles) hipLaunchKernelGGL((mx4_tiles_kernel<D, BF>), dim3(r.splits, a.kv_heads, r.tiles), dim3(512), 0, s, a);
   if (!r.join) return;
   hipLaunchKernelGGL((paged_join_kernel<D, BF>), dim3((unsigned)((r.join_rows + 3) / 4)), dim3(256), 0, s, a);
@@ -839,7 +921,7 @@ extern "C" int spk_mrope_append_mx4(const SpkMropeArgs* p, const SpkPagedScales*
 extern "C" size_t spk_paged_attention_mx4_workspace_size(const SpkPagedAttnArgs* p) {
   Cache c;
   if (check_attn(p, "spk_paged_attention_mx4", &c, false) || p->cache.num_seqs == 0 || p->cache.total_tokens == 0) return 0;
-  return spk_paged::workspace_bound(*p);
+  return spk_paged::workspace_bound_mx4(*p);
 }
 
 extern "C" size_t spk_paged_attention_mx4_workspace_need(const SpkPagedAttnArgs* p) {
@@ -861,11 +943,14 @@ extern "C" int spk_paged_attention_mx4(const SpkPagedAttnArgs* p, const SpkPaged
   a.vscale = scales->v_scales;
   hipStream_t s = spk::to_hip(stream);
   const bool bf = c.dtype == SPK_BF16;
+  // a position's scales are whole dwords
+  const bool bytes = (a.sc.page_stride | a.sc.token_stride | a.sc.head_stride) % 4 || !spk::aligned(a.kscale, 4) ||
+                     !spk::aligned(a.vscale, 4);
   if (c.head_dim == 64)
-    bf ? launch_attn<64, true>(a, r, s) : launch_attn<64, false>(a, r, s);
+    bf ? launch_attn<64, true>(a, r, bytes, s) : launch_attn<64, false>(a, r, bytes, s);
   else if (c.head_dim == 128)
-    bf ? launch_attn<128, true>(a, r, s) : launch_attn<128, false>(a, r, s);
+    bf ? launch_attn<128, true>(a, r, bytes, s) : launch_attn<128, false>(a, r, bytes, s);
   else
-    bf ? launch_attn<256, true>(a, r, s) : launch_attn<256, false>(a, r, s);
+    bf ? launch_attn<256, true>(a, r, bytes, s) : launch_attn<256, false>(a, r, bytes, s);
   return spk::check_launch(who);
 }
