@@ -686,7 +686,7 @@ int spk_mx4_dequantize(const SpkMx4* m, int64_t rows, int32_t cols, int32_t dtyp
  * in_dim values.  With 16-bit rows a weight enters rounded to their type (as
  * spk_mx4_dequantize; bf16 holds every one), with x4 exactly.  residual
  * (nullable) may be out; out overlaps no other input.  in_dim % 32 == 0; rows
- * and out_dim any. */
+ * and out_dim any (up to 2^30 each, 2^39 results). */
 typedef struct SpkMx4MatmulArgs {
   int32_t dtype;               /* SPK_F16 or SPK_BF16: x, residual and out */
   int32_t rows, out_dim, in_dim;

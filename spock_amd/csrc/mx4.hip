@@ -138,88 +138,134 @@ __device__ __forceinline__ uint16_t narrow(float f) {
   return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-// Up to 16 MT rows of x: a workgroup takes 16 NT rows of w and all of their depth, 128
-// at a time, every NW-th step to a wave; the waves' sums meet in LDS, in their order.
-// A lane of the 16x16 products' A operand holds one block of a row of w, 32 codes
+// Few rows of x, 16 to a workgroup (XR = 4: up to 4): a wave takes 16 NT rows of w and every
+// KW-th step of 128 values of their depth, and the KW waves' sums meet in LDS, in their
+// order.  A lane of the 16x16 products' A operand holds one block of a row of w, 32 codes
 // under one scale, as four contraction steps of 8 (rows in 16 bits) or as they
 // are (rows in 4 bits, whose scales the instruction applies).
-template <bool X4, bool BF, int MT, int NT, int NW>
-__global__ __launch_bounds__(64 * NW) void mx4_few_rows_kernel(Mm a) {
-  __shared__ float sums[NW][NT * 16][MT * 16 + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+//
+// In that order neighbouring lanes read different rows, and a load takes 64 cycles of the
+// address pipe, one for each line that four lanes touch (57 measured, 16 where four lanes
+// share a line): one row times 248320 x 1024 took 36 us that way, whatever the tile.  So
+// codes, scales and x go straight into the wave's own LDS, row by row, two steps ahead,
+// their pieces exchanged so that rows read side by side are in different banks.
+// SB: bytes of a load of scales (4: a step's scales of a row are an aligned dword).
+template <bool X4, bool BF, int XR, int NT, int KW, int SB>
+__global__ __launch_bounds__(KW > 4 ? 64 * KW : 256) void mx4_few_rows_kernel(Mm a) {
+  constexpr int W = KW > 4 ? KW : 4, TILES = W / KW;  // waves, and groups of them that share rows of w
+  constexpr int XL = X4 ? 1 : XR / 4;                 // loads of x
+  constexpr int NS = 4 / SB;
+  constexpr int P = NT + XL + NS * (X4 ? 2 : 1);      // loads of a step
+  constexpr int SIZE = 64 * (NT + XL) + 16 * NS * (X4 ? 2 : 1);  // 16-byte pieces of a step
+  constexpr int SUMS = 16 * (16 * NT + 1) / 4;        // of a wave's sums
+  constexpr int FIRST = W * (SIZE > SUMS ? SIZE : SUMS);
+  // an array to each step: a load into one is then known not to touch the others
+  __shared__ __align__(16) uint4 sa[FIRST], sb[W * SIZE], sc[W * SIZE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
-  const uint8_t *wc[NT], *ws[NT];
+  const int kw = wave % KW;
+  const int n0 = (blockIdx.x * TILES + wave / KW) * 16 * NT, m0 = blockIdx.y * 16;
+  const int blocks = a.depth / 32, steps = (blocks + 3) / 4;
+
+  const int wpiece = lane % 4 ^ (lane >> 3 & 3);  // of row lane / 4 in its place
+  const uint8_t *wp[NT], *wsp, *xp[XL], *xsp = nullptr;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = min(n0 + 16 * t + ln, a.cols - 1);
-    wc[t] = a.wc + n * a.wct;
-    ws[t] = a.ws + n * a.wst;
-  }
-  const uint16_t* x[MT];
-  const uint8_t *xc[MT], *xs[MT];
+  for (int t = 0; t < NT; ++t) wp[t] = a.wc + min(n0 + 16 * t + lane / 4, a.cols - 1) * a.wct + 16 * wpiece;
+  wsp = a.ws + min(n0 + lane % (16 * NT), a.cols - 1) * a.wst;
+  int xpiece[XL];
+  if constexpr (X4) {
+    xpiece[0] = wpiece;
+    xp[0] = a.xc + min(m0 + lane / 4, a.rows - 1) * a.xct + 16 * wpiece;
+    xsp = a.xs + min(m0 + lane % 16, a.rows - 1) * a.xst;
+  } else {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int64_t m = min(m0 + 16 * t + ln, a.rows - 1);
-    if constexpr (X4) {
-      xc[t] = a.xc + m * a.xct;
-      xs[t] = a.xs + m * a.xst;
-    } else {
-      x[t] = a.x + m * a.xt;
+    for (int i = 0; i < XL; ++i) {
+      const int row = 4 * i + lane / 16;
+      xpiece[i] = lane % 16 ^ (row & 7);
+      xp[i] = reinterpret_cast<const uint8_t*>(a.x + min(m0 + row, a.rows - 1) * a.xt) + 16 * xpiece[i];
     }
   }
-  floatx4 acc[NT][MT];
+  auto load = [&](int st, uint4* to) __attribute__((always_inline)) {
+    st = min(st, steps - 1);  // past the end the last one again, which nobody uses
+    const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
+    uint4* w = to + SIZE * wave;
+    uint4 *x = w + 64 * NT, *s = x + 64 * XL;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
+      spk_mx4::load_lds<16>(SB == 4 || 4 * st + wpiece < blocks ? wp[t] + 64 * (int64_t)st : zero, w + 64 * t);
 #pragma unroll
-    for (int u = 0; u < MT; ++u) acc[t][u] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = 128 * wave; k < a.depth; k += 128 * NW) {
-    const int b = k / 32 + g;  // this lane's block
-    const bool there = 32 * b < a.depth;
-    uint4 w[NT];
-    uint32_t s[NT];
+    for (int i = 0; i < XL; ++i)
+      spk_mx4::load_lds<16>(SB == 4 || 4 * st + (X4 ? xpiece[i] : xpiece[i] / 4) < blocks ? xp[i] + (X4 ? 64 : 256) * (int64_t)st : zero, x + 64 * i);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      w[t] = *(there ? reinterpret_cast<const uint4*>(wc[t] + 16 * b) : kZero);
-      s[t] = *(there ? ws[t] + b : reinterpret_cast<const uint8_t*>(kZero));
+    for (int b = 0; b < NS; ++b) {
+      spk_mx4::load_lds<SB>(SB == 4 || 4 * st + b < blocks ? wsp + 4 * (int64_t)st + b : zero, s + 16 * b);
+      if constexpr (X4) spk_mx4::load_lds<SB>(SB == 4 || 4 * st + b < blocks ? xsp + 4 * (int64_t)st + b : zero, s + 16 * (NS + b));
     }
+  };
+  // Where this lane's operands lie, in bytes.  (As one number each: of an address made of many
+  // parts the compiler no longer knows the array, and waits for all loads before it reads.)
+  const int mine = 16 * SIZE * wave, wat = mine + 16 * (4 * ln + (g ^ (ln >> 1 & 3)));
+  const int xrow = ln & (XR - 1);
+  const int xat = mine + 1024 * NT + 16 * (X4 ? 4 * ln + (g ^ (ln >> 1 & 3)) : 16 * xrow + (4 * g ^ (xrow & 7)));
+  const int sat = mine + 1024 * (NT + XL) + (SB == 4 ? 4 * ln + g : 256 * g + 4 * ln);
+  floatx4 acc[NT];
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
+  for (int t = 0; t < NT; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto step = [&](int st, const uint4* at, uint4* to) __attribute__((always_inline)) {
+    load(st + 2 * KW, to);
+    spk_mx4::arrived<2 * P>();
+    if (st < steps) {
+      const auto* p = reinterpret_cast<const uint8_t*>(at);
+      uint4 w[NT], x[4];
+      uint32_t s[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        w[t] = *reinterpret_cast<const uint4*>(p + wat + 1024 * t);
+        s[t] = p[sat + 64 * t];
+      }
       if constexpr (X4) {
-        const uint4 v = *(there ? reinterpret_cast<const uint4*>(xc[u] + 16 * b) : kZero);
-        const uint32_t vs = *(there ? xs[u] + b : reinterpret_cast<const uint8_t*>(kZero));
+        x[0] = *reinterpret_cast<const uint4*>(p + xat);
+        const uint32_t xs = p[sat + 256 * NS];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(four_bits(w[t]), four_bits(v), acc[t][u], 4, 4, 0,
-                                                                       (int)s[t], 0, (int)vs);
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(four_bits(w[t]), four_bits(x[0]), acc[t], 4, 4, 0, (int)s[t], 0,
+                                                                    (int)xs);
       } else {
-        const uint4* p = there ? reinterpret_cast<const uint4*>(x[u] + 32 * b) : kZero;
-        uint4 v[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = p[c];
+        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const uint4*>(p + (xat ^ 16 * e));
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            acc[t][u] = mfma16<BF>(spk_mx4::expand<BF>((&w[t].x)[c], spk_mx4::scale_of(s[t])), v[c], acc[t][u]);
+          for (int t = 0; t < NT; ++t)
+            acc[t] = mfma16<BF>(spk_mx4::expand<BF>((&w[t].x)[e], spk_mx4::scale_of(s[t])), x[e], acc[t]);
       }
     }
+  };
+  load(kw, sa);
+  load(kw + KW, sb);
+  for (int st = kw; st < steps; st += 3 * KW) {
+    step(st, sa, sc);
+    step(st + KW, sb, sa);
+    step(st + 2 * KW, sc, sb);
   }
+  spk_mx4::arrived<0>();  // loads past the end still write LDS
+  __syncthreads();
+  auto sums = reinterpret_cast<float(*)[16][16 * NT + 1]>(sa);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int u = 0; u < MT; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[wave][16 * t + 4 * g + i][16 * u + ln] = acc[t][u][i];
+    for (int i = 0; i < 4; ++i) sums[wave][ln][16 * t + 4 * g + i] = acc[t][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < 256 * NT * MT; i += 64 * NW) {
-    const int n = i % (16 * NT), m = i / (16 * NT);
-    if (m0 + m >= a.rows || n0 + n >= a.cols) continue;
-    float sum = sums[0][n][m];
+  // neighbouring threads have neighbouring columns
+  for (int i = threadIdx.x; i < 256 * NT * TILES; i += 64 * W) {
+    const int m = i / (16 * NT * TILES), c = i - m * (16 * NT * TILES), n = blockIdx.x * 16 * NT * TILES + c;
+    if (m0 + m >= a.rows || n >= a.cols) continue;
+    const int first = c / (16 * NT) * KW, at = c % (16 * NT);
+    float sum = sums[first][m][at];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) sum += sums[w][n][m];
-    if (a.res) sum += widen<BF>(a.res[(m0 + m) * a.rt + n0 + n]);
-    a.out[(m0 + m) * a.ot + n0 + n] = narrow<BF>(sum);
+    for (int w = 1; w < KW; ++w) sum += sums[first + w][m][at];
+    if (a.res) sum += widen<BF>(a.res[(m0 + m) * a.rt + n]);
+    a.out[(m0 + m) * a.ot + n] = narrow<BF>(sum);
   }
 }
 
@@ -260,20 +306,6 @@ __device__ __forceinline__ void store_tile(const Mm& a, int vec, int m, int n, c
         }
       }
   }
-}
-
-// A wave's load straight into LDS, side by side at `to`: B bytes of a lane (of one byte
-// a dword is written).
-template <int B, typename T>
-__device__ __forceinline__ void load_lds(const uint8_t* from, T* to) {
-  const auto g = (const __attribute__((address_space(1))) void*)from;
-  const auto l = (__attribute__((address_space(3))) void*)to;
-  if constexpr (B == 16)
-    __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
-  else if constexpr (B == 4)
-    __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
-  else
-    __builtin_amdgcn_global_load_lds(g, l, 1, 0, 0);
 }
 
 // All loads but the newest N of this wave have arrived, its LDS reads are done, and so are
@@ -343,11 +375,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles16_kernel(Mm a, int 
     const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
 #pragma unroll
     for (int i = 0; i < PX; ++i)
-      load_lds<16>(!TAIL || 2 * st + px / 4 < blocks ? xp[i] + 128 * (int64_t)st : zero, x + 64 * (i * NW + wave));
+      spk_mx4::load_lds<16>(!TAIL || 2 * st + px / 4 < blocks ? xp[i] + 128 * (int64_t)st : zero, x + 64 * (i * NW + wave));
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
-      load_lds<16>(!TAIL || 2 * st + pw < blocks ? wp[i] + 32 * (int64_t)st : zero, w + 64 * (i * NW + wave));
-      load_lds<1>(!TAIL || 2 * st + lane % 2 < blocks ? sp[i] + 2 * (int64_t)st : zero, s + 64 * (i * NW + wave));
+      spk_mx4::load_lds<16>(!TAIL || 2 * st + pw < blocks ? wp[i] + 32 * (int64_t)st : zero, w + 64 * (i * NW + wave));
+      spk_mx4::load_lds<1>(!TAIL || 2 * st + lane % 2 < blocks ? sp[i] + 2 * (int64_t)st : zero, s + 64 * (i * NW + wave));
     }
   };
   floatx16 acc[TN][TM];
@@ -441,18 +473,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles4_kernel(Mm a, int v
     const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
 #pragma unroll
     for (int i = 0; i < PX; ++i)
-      load_lds<16>(!TAIL || 4 * st + piece < blocks ? xp[i] + 64 * (int64_t)st : zero, x + 64 * (i * NW + wave));
+      spk_mx4::load_lds<16>(!TAIL || 4 * st + piece < blocks ? xp[i] + 64 * (int64_t)st : zero, x + 64 * (i * NW + wave));
 #pragma unroll
     for (int i = 0; i < PW; ++i)
-      load_lds<16>(!TAIL || 4 * st + piece < blocks ? wp[i] + 64 * (int64_t)st : zero, w + 64 * (i * NW + wave));
+      spk_mx4::load_lds<16>(!TAIL || 4 * st + piece < blocks ? wp[i] + 64 * (int64_t)st : zero, w + 64 * (i * NW + wave));
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
       if constexpr (TAIL) {
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-          load_lds<1>(4 * st + b < blocks ? sp[i] + 4 * (int64_t)st + b : zero, s + b * (BM + BN) + 64 * (i * NW + wave));
+          spk_mx4::load_lds<1>(4 * st + b < blocks ? sp[i] + 4 * (int64_t)st + b : zero, s + b * (BM + BN) + 64 * (i * NW + wave));
       } else {
-        load_lds<4>(sp[i] + 4 * (int64_t)st, s + 64 * (i * NW + wave));
+        spk_mx4::load_lds<4>(sp[i] + 4 * (int64_t)st, s + 64 * (i * NW + wave));
       }
     }
   };
@@ -587,18 +619,53 @@ void launch_tiles(const Mm& a, int vec, hipStream_t s) {
   }
 }
 
+template <bool X4, bool BF, int XR, int NT, int KW>
+void launch_few(const Mm& a, hipStream_t s) {
+  constexpr int W = KW > 4 ? KW : 4, N = 16 * NT * W / KW;
+  const dim3 grid((a.cols + N - 1) / N, (a.rows + 15) / 16), block(64 * W);
+  const bool dwords = a.depth % 128 == 0 && a.wst % 4 == 0 && spk::aligned(a.ws, 4) && (!X4 || (a.xst % 4 == 0 && spk::aligned(a.xs, 4)));
+  if (dwords)
+    hipLaunchKernelGGL((mx4_few_rows_kernel<X4, BF, XR, NT, KW, 4>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((mx4_few_rows_kernel<X4, BF, XR, NT, KW, 1>), grid, block, 0, s, a);
+}
+
+// Tiles of 16 x 16 of the result.
+int64_t small_tiles(const Mm& a) { return (int64_t)((a.cols + 15) / 16) * ((a.rows + 15) / 16); }
+
+int64_t big_tiles(const Mm& a) { return (int64_t)((a.cols + 255) / 256) * ((a.rows + 255) / 256); }
+
+// As many columns to a wave as leave some 800 waves, each with a quarter of the depth until
+// there are enough without (1 row, us with (4, 1), (4, 4), (2, 4), (1, 4) of NT and KW: 1024 x 3584
+// -, 5.7, 4.6, 4.1; 14336 x 4096 -, 8.2, 8.7, 10.9; 32768 x 4096 24.1, 14.6, -, -; 248320 x 1024
+// 29.1, 32.4, -, -).
+template <bool X4, bool BF, int XR>
+void launch_few_rows(const Mm& a, hipStream_t s) {
+  const int64_t tiles = small_tiles(a);
+  if (tiles >= 8192)
+    launch_few<X4, BF, XR, 4, 1>(a, s);
+  else if (tiles >= 800)
+    launch_few<X4, BF, XR, 4, 4>(a, s);
+  else if (tiles >= 400)
+    launch_few<X4, BF, XR, 2, 4>(a, s);
+  else
+    launch_few<X4, BF, XR, 1, 4>(a, s);
+}
+
 template <bool X4, bool BF>
 void launch_matmul(const Mm& a, hipStream_t s) {
   const int vec = spk::aligned(a.out, 8) && a.ot % 4 == 0 && (!a.res || (spk::aligned(a.res, 8) && a.rt % 4 == 0));
-  const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.cols + 255) / 256);
-  if (a.rows <= 64) {
-    const dim3 grid((a.cols + 31) / 32, (a.rows + 63) / 64);
-    hipLaunchKernelGGL((mx4_few_rows_kernel<X4, BF, 4, 2, 4>), grid, dim3(256), 0, s, a);
-  } else if (big >= 128) {
+  // A tile of 16 x 16 and 128 of depth takes some 0.2 ns in the one kernel, tiles of 128 x 128
+  // that are fewer than the chip holds 1 us (rows in 4 bits 0.4): 100 rows times 14336 x 4096
+  // (6272 tiles) 44 and 33 us, 200 times 4096 x 4096 (3328) 25 and 33.  Tiles of 256 x 256 pay
+  // once most of the chip has one: 2000 times 4096 x 4096 (128 tiles) 102 us and 84 with the
+  // smaller, rows in 4 bits 40 and 44; 2000 times 7168 x 1024 (224 tiles) 38 and 54.
+  if (a.rows <= 16 || small_tiles(a) < (X4 ? 2200 : 5000))
+    a.rows <= 4 && !X4 ? launch_few_rows<X4, BF, 4>(a, s) : launch_few_rows<X4, BF, 16>(a, s);
+  else if (big_tiles(a) >= (X4 ? 128 : 200))
     launch_tiles<X4, BF, 2, 4, 4, 2>(a, vec, s);
-  } else {
+  else
     launch_tiles<X4, BF, 2, 2, 2, 2>(a, vec, s);
-  }
 }
 
 }  // namespace
@@ -646,6 +713,8 @@ extern "C" int spk_mx4_matmul(const SpkMx4MatmulArgs* p, spk_stream_t stream) {
     return spk::fail(SPK_ERR_SHAPE, "%s: rows %d out_dim %d in_dim %d (a positive multiple of 32)", who, p->rows, p->out_dim,
                      p->in_dim);
   if (p->rows == 0 || p->out_dim == 0) return SPK_OK;
+  if (p->rows > 1 << 30 || p->out_dim > 1 << 30 || (int64_t)((p->rows + 255) / 256) * ((p->out_dim + 255) / 256) >= 1 << 23)
+    return spk::fail(SPK_ERR_SHAPE, "%s: rows %d out_dim %d (up to 2^30 each and 2^39 results)", who, p->rows, p->out_dim);
   if (const int rc = check_mx4(p->w, p->out_dim, p->in_dim, who, "w")) return rc;
   if (p->x) {
     if (!spk::aligned(p->x, 16) || p->x_stride % 8)

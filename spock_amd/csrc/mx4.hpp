@@ -86,4 +86,27 @@ __device__ __forceinline__ uint32_t scale_byte16(uint32_t most) {
   return most >= 0x7c00u ? kNone : scale_byte(__float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)most)));
 }
 
+// A wave's load straight into LDS, side by side at `to`: B bytes of a lane (of one byte
+// a dword is written).
+template <int B, typename T>
+__device__ __forceinline__ void load_lds(const void* from, T* to) {
+  const auto g = (const __attribute__((address_space(1))) void*)from;
+  const auto l = (__attribute__((address_space(3))) void*)to;
+  if constexpr (B == 16)
+    __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else if constexpr (B == 4)
+    __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
+  else
+    __builtin_amdgcn_global_load_lds(g, l, 1, 0, 0);
+}
+
+// All loads of this wave but the newest N have arrived.  (As a builtin, which the compiler
+// takes into account: told in assembly it waits for all of them before it reads what they wrote.)
+template <int N>
+__device__ __forceinline__ void arrived() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
+  asm volatile("" ::: "memory");
+}
+
 }  // namespace spk_mx4

@@ -190,29 +190,6 @@ struct AttnMx4 : Attn {
   Scales sc;
 };
 
-// A wave's load straight into LDS, side by side at `to`: B bytes of a lane (of one byte
-// a dword is written).
-template <int B, typename T>
-__device__ __forceinline__ void load_lds(const void* from, T* to) {
-  const auto g = (const __attribute__((address_space(1))) void*)from;
-  const auto l = (__attribute__((address_space(3))) void*)to;
-  if constexpr (B == 16)
-    __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
-  else if constexpr (B == 4)
-    __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
-  else
-    __builtin_amdgcn_global_load_lds(g, l, 1, 0, 0);
-}
-
-// All loads of this wave but the newest N have arrived.  (As a builtin, which the compiler
-// takes into account: told in assembly it waits for all of them before it reads what they wrote.)
-template <int N>
-__device__ __forceinline__ void arrived() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
-  asm volatile("" ::: "memory");
-}
-
 // Few rows per sequence and KV head: spk_paged_attention's form for them (16 rows of
 // a sequence and a range of its keys to a workgroup, every fourth step of 32 keys
 // to a wave, scores transposed, the waves' states joined in LDS), from 4 bits.
@@ -278,7 +255,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
   // the lower lanes ask for the pages of the keys from k0 on
   auto ask = [&](int k0, int32_t* ids) __attribute__((always_inline)) {
     if (lane < 32)
-      load_lds<4>(table + spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + lane, lo), end - 1)), ids + 32 * wave);
+      spk_mx4::load_lds<4>(table + spk_paged::divide(a.c.div, (uint32_t)min(max(k0 + lane, lo), end - 1)), ids + 32 * wave);
   };
   // what row r of a step's keys and of its values in LDS holds
   const int kfirst = lane / CP, kpiece = lane % CP ^ (CP == 8 ? kfirst & 7 : CP == 4 ? kfirst >> 1 & 3 : 0);
@@ -294,11 +271,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int64_t k = __shfl(off.codes, RL * i + kfirst), v = __shfl(off.codes, value_key(RL * i + kfirst));
-      load_lds<16>(kcode + k + 16 * kpiece, x + 64 * i);
-      load_lds<16>(vcode + v + 16 * (lane % CP), x + KW + 64 * i);
+      spk_mx4::load_lds<16>(kcode + k + 16 * kpiece, x + 64 * i);
+      spk_mx4::load_lds<16>(vcode + v + 16 * (lane % CP), x + KW + 64 * i);
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i) load_lds<SB>(scales + off.scales + SB * i, x + 2 * KW + 16 * i);
+    for (int i = 0; i < NS; ++i) spk_mx4::load_lds<SB>(scales + off.scales + SB * i, x + 2 * KW + 16 * i);
     return (uint32_t)__ballot(there);
   };
   const int r = min(r0 + ln, rows - 1);  // this lane's row
@@ -329,7 +306,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
   auto step = [&](int k0, const uint4* at, uint32_t has, int32_t* ids, uint4* to, uint32_t& next) __attribute__((always_inline)) {
     next = load(k0 + 128 * (N - 1), ids, to);
     ask(k0 + 128 * (2 * N - 1), ids);
-    arrived<(N - 1) * P>();
+    spk_mx4::arrived<(N - 1) * P>();
     if (k0 >= end) return;
     const auto* x = reinterpret_cast<const uint8_t*>(at);
     const bool full = has == 0xffffffffu && k0 >= lo_all && k0 + 32 <= hi_all;
@@ -473,7 +450,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
     ask(k0, ia);
     ask(k0 + 128, ib);
     if constexpr (N == 3) ask(k0 + 256, ic);
-    arrived<0>();
+    spk_mx4::arrived<0>();
     if constexpr (N == 3) {
       ha = load(k0, ia, sa);
       ask(k0 + 384, ia);
@@ -494,7 +471,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
       }
     }
   }
-  arrived<0>();  // loads past the end still write LDS
+  spk_mx4::arrived<0>();  // loads past the end still write LDS
 
   // join the waves, 4 dimensions of each 16th of a row at a time
   l += spk::lane_xor16(l);
@@ -558,7 +535,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
   }
 }
 
-// LDS reads, DMA-free waits: all LDS work of this wave is done, and the workgroup meets.
+// All LDS work of this wave is done, and the workgroup meets.
 __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0) alone

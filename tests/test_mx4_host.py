@@ -44,6 +44,7 @@ BAD = [(lambda: dict(dtype=0), -5), (lambda: dict(dtype=3), -5), (lambda: dict(i
        (lambda: dict(x_stride=65), -4), (lambda: dict(x_stride=56), -2), (lambda: dict(x=None, x4=_four(codes=None)), -1),
        (lambda: dict(x=None, x4=_four(code_stride=16)), -2), (lambda: dict(out=None), -1), (lambda: dict(out=513), -4),
        (lambda: dict(out_stride=4), -2), (lambda: dict(residual=512, residual_stride=4), -2),
+       (lambda: dict(rows=2 ** 30 + 1), -2), (lambda: dict(out_dim=2 ** 30 + 1), -2), (lambda: dict(rows=2 ** 20, out_dim=2 ** 19), -2),
        (lambda: dict(residual=512, residual_stride=6), -5), (lambda: dict(residual=513, residual_stride=5), -4)]
 
 
