@@ -297,14 +297,16 @@ def _on(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape=None) -> N
 
 
 def _flat(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape) -> None:
-    _on(what, name, t, dev, dtype, shape)
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+        _on(what, name, t, dev, dtype, shape)
     if not t.is_contiguous():
         raise _lib.SpockError(f"{what}: {name} must be contiguous")
 
 
 def _rows(what: str, name: str, t: torch.Tensor, dev: int, dtype, shape):
     """Token and head strides of a [tokens][heads][dim] view: any, and 0 where there is one."""
-    _on(what, name, t, dev, dtype, shape)
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+        _on(what, name, t, dev, dtype, shape)
     token, head, last = t.stride()
     if last != 1:
         raise _lib.SpockError(f"{what}: the last dimension of {name} must be contiguous")
@@ -400,7 +402,9 @@ def _mrope_args(what: str, cache: SpkPagedCache, q, k, v, positions, rope, pair_
         raise _lib.SpockError(f"{what}: pairing must be one of {sorted(_PAIRINGS)}, got {pairing!r}")
     if out is None:
         out = q.new_empty(shape)
-    outs = _rows(what, "out", out, dev, dtype, shape)
+        outs = heads * D, D
+    else:
+        outs = _rows(what, "out", out, dev, dtype, shape)
     a = SpkMropeArgs(cache, heads, rot, _PAIRINGS[pairing], num_axes, axes, positions.data_ptr(), positions.stride(0),
                      rope.data_ptr(), rows, eps, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
                      v.data_ptr(), vs[0], vs[1], _ptr(q_norm_weight), _ptr(k_norm_weight), out.data_ptr(), outs[0], outs[1])
@@ -433,16 +437,19 @@ def _attention_args(what: str, cache: SpkPagedCache, q, max_query_len, max_conte
                     workspace, need_of):
     """(SpkPagedAttnArgs, out, lse, workspace) of an attention over `cache`, checked."""
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    _, heads, D = shape
     qs = _rows(what, "q", q, dev, dtype, shape)
     gs = (0, 0) if gate is None else _rows(what, "gate", gate, dev, dtype, shape)
     if out is None:
         out = q.new_empty(shape)
-    outs = _rows(what, "out", out, dev, dtype, shape)
+        outs = heads * D, D
+    else:
+        outs = _rows(what, "out", out, dev, dtype, shape)
     if lse is not None:
         _flat(what, "lse", lse, dev, torch.float32, shape[:2])
     elif return_lse:
         lse = q.new_empty(shape[:2], dtype=torch.float32)
-    a = SpkPagedAttnArgs(cache, shape[1], max_query_len, max_context_len, window, scale, q.data_ptr(), qs[0], qs[1],
+    a = SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window, scale, q.data_ptr(), qs[0], qs[1],
                          _ptr(gate), gs[0], gs[1], out.data_ptr(), outs[0], outs[1], _ptr(lse), None, 0)
     need = need_of(C.byref(a))
     if need:
@@ -577,27 +584,32 @@ class Mx4(NamedTuple):
 
 
 def _mx4_rows(what: str, name: str, m: Mx4, dev: int):
-    """(SpkMx4, rows, values of a row) of 4-bit rows: two dimensions with any stride between rows, others contiguous."""
+    """(SpkMx4, leading shape, rows, values of a row) of 4-bit rows: two dimensions with any stride between rows, others
+    contiguous."""
     if not isinstance(m, Mx4):
         raise _lib.SpockError(f"{what}: {name} must be an Mx4, got {type(m).__name__}")
     codes, scales = m
-    if codes.dim() < 1 or codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1] or \
-            codes.shape[-1] != 16 * scales.shape[-1]:
+    *lead, half = codes.shape if codes.dim() else (-1,)
+    if (*lead, half // 16) != scales.shape or half % 16:
         raise _lib.SpockError(f"{what}: {name} must have codes [..., n / 2] and scales [..., n / 32], "
                               f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
-    for t in m:
-        _on(what, name, t, dev, torch.uint8)
-    rows, cols = codes.shape[:-1].numel(), 2 * codes.shape[-1]
+    _on(what, name, codes, dev, torch.uint8)
+    _on(what, name, scales, dev, torch.uint8)
+    rows = 1
+    for n in lead:
+        rows *= n
     return SpkMx4(codes.data_ptr(), _row_stride(what, name, codes), scales.data_ptr(),
-                  _row_stride(what, name, scales)), rows, cols
+                  _row_stride(what, name, scales)), lead, rows, 2 * half
 
 
 def _row_stride(what: str, name: str, t: torch.Tensor) -> int:
     """Elements between the rows of [..., n]: any in two dimensions, else those of a contiguous tensor."""
     if t.dim() == 2:
-        if t.shape[1] > 1 and t.stride(1) != 1:
+        stride, last = t.stride()
+        if last != 1 and t.shape[1] > 1:
             raise _lib.SpockError(f"{what}: {name} must have contiguous rows, got strides {t.stride()}")
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        rows, n = t.shape
+        return stride if rows > 1 else n
     if not t.is_contiguous():
         raise _lib.SpockError(f"{what}: {name} must be two-dimensional or contiguous, got strides {t.stride()}")
     return t.shape[-1]
@@ -607,18 +619,18 @@ def mx4_quantize(x: torch.Tensor, out: Optional[Mx4] = None) -> Mx4:
     """Rows of x [..., n] (float32, float16 or bfloat16, n a multiple of 32) in 4 bits (spk_mx4_quantize)."""
     what = "mx4_quantize"
     dev = _device(what, x)
-    if x.dim() < 1 or x.shape[-1] % 32 or x.dtype not in _ROWS:
+    dtype = _ROWS.get(x.dtype)
+    *lead, n = x.shape if x.dim() else (-1,)
+    if n % 32 or dtype is None:
         raise _lib.SpockError(f"{what}: x must be [..., a multiple of 32] float16, bfloat16 or float32, "
                               f"got {tuple(x.shape)} {x.dtype}")
-    n = x.shape[-1]
     stride = _row_stride(what, "x", x)
     if out is None:
-        out = Mx4(x.new_empty((*x.shape[:-1], n // 2), dtype=torch.uint8),
-                  x.new_empty((*x.shape[:-1], n // 32), dtype=torch.uint8))
-    m, rows, cols = _mx4_rows(what, "out", out, dev)
-    if out.codes.shape[:-1] != x.shape[:-1] or cols != n:
-        raise _lib.SpockError(f"{what}: out holds {tuple(out.codes.shape[:-1])} rows of {cols} values, x is {tuple(x.shape)}")
-    _launch(dev, what, lib().spk_mx4_quantize, x.data_ptr(), _ROWS[x.dtype], stride, rows, cols, C.byref(m))
+        out = Mx4(x.new_empty((*lead, n // 2), dtype=torch.uint8), x.new_empty((*lead, n // 32), dtype=torch.uint8))
+    m, rows_of, rows, cols = _mx4_rows(what, "out", out, dev)
+    if rows_of != lead or cols != n:
+        raise _lib.SpockError(f"{what}: out holds {tuple(rows_of)} rows of {cols} values, x is {tuple(x.shape)}")
+    _launch(dev, what, lib().spk_mx4_quantize, x.data_ptr(), dtype, stride, rows, cols, C.byref(m))
     return out
 
 
@@ -628,8 +640,8 @@ def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.bfloat16, out: Optional[to
     if not isinstance(m, Mx4):
         raise _lib.SpockError(f"{what}: expected an Mx4, got {type(m).__name__}")
     dev = _device(what, m.codes)
-    a, rows, cols = _mx4_rows(what, "m", m, dev)
-    shape = (*m.codes.shape[:-1], cols)
+    a, lead, rows, cols = _mx4_rows(what, "m", m, dev)
+    shape = (*lead, cols)
     if out is None:
         if dtype not in _ROWS:
             raise _lib.SpockError(f"{what}: dtype must be float16, bfloat16 or float32, got {dtype}")
@@ -663,37 +675,40 @@ def mx4_matmul(x, w: Mx4, residual: Optional[torch.Tensor] = None, dtype: Option
     what = "mx4_matmul"
     four = isinstance(x, Mx4)
     dev = _device(what, x.codes if four else x)
-    a = SpkMx4MatmulArgs()
-    a.w, n, k = _mx4_rows(what, "w", w, dev)
-    if w.codes.dim() != 2:
+    mw, shape, n, k = _mx4_rows(what, "w", w, dev)
+    if len(shape) != 1:
         raise _lib.SpockError(f"{what}: w must be [out][in], got codes {tuple(w.codes.shape)}")
+    x_at, x_stride, x4 = None, 0, SpkMx4()
     if four:
-        a.x4, rows, depth = _mx4_rows(what, "x", x, dev)
-        lead = x.codes.shape[:-1]
+        x4, lead, rows, depth = _mx4_rows(what, "x", x, dev)
         if dtype is None:
             dtype = residual.dtype if residual is not None else out.dtype if out is not None else torch.bfloat16
     else:
         if x.dim() < 1 or dtype not in (None, x.dtype):
             raise _lib.SpockError(f"{what}: x is {tuple(x.shape)} {x.dtype}, the result {dtype}")
-        lead, depth, dtype = x.shape[:-1], x.shape[-1], x.dtype
-        rows = lead.numel()
-        a.x, a.x_stride = x.data_ptr(), _row_stride(what, "x", x)
-    if dtype not in _HALF:
+        *lead, depth = x.shape
+        dtype, rows = x.dtype, 1
+        for size in lead:
+            rows *= size
+        x_at, x_stride = x.data_ptr(), _row_stride(what, "x", x)
+    kind = _HALF.get(dtype)
+    if kind is None:
         raise _lib.SpockError(f"{what}: rows and result must be float16 or bfloat16, got {dtype}")
     if depth != k:
         raise _lib.SpockError(f"{what}: x has rows of {depth} values, w of {k}")
     shape = (*lead, n)
+    res, res_stride = None, 0
     if residual is not None:
         _on(what, "residual", residual, dev, dtype, shape)
-        a.residual, a.residual_stride = residual.data_ptr(), _row_stride(what, "residual", residual)
+        res, res_stride = residual.data_ptr(), _row_stride(what, "residual", residual)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=w.codes.device)
+        out, stride = w.codes.new_empty(shape, dtype=dtype), n
     else:
         _on(what, "out", out, dev, dtype, shape)
-    a.out, a.out_stride = out.data_ptr(), _row_stride(what, "out", out)
-    a.dtype, a.rows, a.out_dim, a.in_dim = _HALF[dtype], rows, n, k
+        stride = _row_stride(what, "out", out)
     if rows and n:  # of no rows there is no address
-        _call(lib().spk_mx4_matmul, a, dev, what)
+        _call(lib().spk_mx4_matmul, SpkMx4MatmulArgs(kind, rows, n, k, x_at, x_stride, x4, mw, res, res_stride, out.data_ptr(),
+                                                     stride), dev, what)
     return out
 
 
@@ -706,6 +721,19 @@ def mx4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, device="
     return pool(), pool()
 
 
+def _pool_strides(what: str, name: str, k: torch.Tensor, v: torch.Tensor, dev: int, shape):
+    """The strides of two pools of this shape, which have to be the same."""
+    _on(what, name, k, dev, torch.uint8, shape)
+    _on(what, name, v, dev, torch.uint8, shape)
+    a, b = k.stride(), v.stride()
+    if 1 in shape:  # a stride of one element is not read
+        a, b = ([n if size > 1 else 0 for n, size in zip(t, shape)] for t in (a, b))
+    if a != b or (a[3] != 1 and shape[3] > 1):
+        raise _lib.SpockError(f"{what}: the {name} of k_cache and v_cache need equal strides and a contiguous last dimension, "
+                              f"got {k.stride()} and {v.stride()}")
+    return a
+
+
 def _paged_cache_mx4(what: str, q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, block_table, cu_seqlens, context_lens):
     dev, dtype = _device(what, q), q.dtype
     if not isinstance(k_cache, Mx4) or not isinstance(v_cache, Mx4):
@@ -715,21 +743,14 @@ def _paged_cache_mx4(what: str, q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, blo
                               f"got {tuple(q.shape)} and {tuple(k_cache.codes.shape)}")
     if dtype not in _HALF:
         raise _lib.SpockError(f"{what}: q must be float16 or bfloat16, got {dtype}")
-    pages, page_size, kv_heads, half = k_cache.codes.shape
+    codes, scales = k_cache
+    shape = codes.shape
+    pages, page_size, kv_heads, half = shape
     tokens, _, dim = q.shape
     if dim != 2 * half or dim % 32:
         raise _lib.SpockError(f"{what}: q has head_dim {dim}, the cache {2 * half}")
-    strides = []
-    for name, n, pair in (("codes", half, (k_cache.codes, v_cache.codes)), ("scales", dim // 32, (k_cache.scales, v_cache.scales))):
-        shape = (pages, page_size, kv_heads, n)
-        for t in pair:
-            _on(what, name, t, dev, torch.uint8, shape)
-        # a stride of one element is not read
-        k, v = ([s if size > 1 else 0 for s, size in zip(t.stride(), shape)] for t in pair)
-        if k != v or (n > 1 and k[3] != 1):
-            raise _lib.SpockError(f"{what}: the {name} of k_cache and v_cache need equal strides and a contiguous last dimension, "
-                                  f"got {pair[0].stride()} and {pair[1].stride()}")
-        strides.append(k)
+    c = _pool_strides(what, "codes", codes, v_cache.codes, dev, shape)
+    s = _pool_strides(what, "scales", scales, v_cache.scales, dev, (pages, page_size, kv_heads, dim // 32))
     seqs = context_lens.numel()
     _on(what, "block_table", block_table, dev, torch.int32)
     _flat(what, "cu_seqlens", cu_seqlens, dev, torch.int32, (seqs + 1,))
@@ -737,11 +758,10 @@ def _paged_cache_mx4(what: str, q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, blo
     if block_table.dim() != 2 or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise _lib.SpockError(f"{what}: block_table must be [{seqs}][max_pages] with contiguous rows, "
                               f"got {tuple(block_table.shape)}")
-    c, s = strides
     cache = SpkPagedCache(_HALF[dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, tokens,
-                          k_cache.codes.data_ptr(), v_cache.codes.data_ptr(), c[0], c[1], c[2],
+                          codes.data_ptr(), v_cache.codes.data_ptr(), c[0], c[1], c[2],
                           block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), context_lens.data_ptr())
-    return cache, SpkPagedScales(k_cache.scales.data_ptr(), v_cache.scales.data_ptr(), s[0], s[1], s[2])
+    return cache, SpkPagedScales(scales.data_ptr(), v_cache.scales.data_ptr(), s[0], s[1], s[2])
 
 
 def mrope_append_mx4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, rope: torch.Tensor,
