@@ -7,6 +7,7 @@ hand-written gfx950 kernel behind include/spock_hip.h.
 from __future__ import annotations
 
 import ctypes as C
+from math import prod
 from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
@@ -595,20 +596,17 @@ def _mx4_rows(what: str, name: str, m: Mx4, dev: int):
                               f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
     _on(what, name, codes, dev, torch.uint8)
     _on(what, name, scales, dev, torch.uint8)
-    rows = 1
-    for n in lead:
-        rows *= n
     return SpkMx4(codes.data_ptr(), _row_stride(what, name, codes), scales.data_ptr(),
-                  _row_stride(what, name, scales)), lead, rows, 2 * half
+                  _row_stride(what, name, scales)), lead, prod(lead), 2 * half
 
 
 def _row_stride(what: str, name: str, t: torch.Tensor) -> int:
     """Elements between the rows of [..., n]: any in two dimensions, else those of a contiguous tensor."""
     if t.dim() == 2:
         stride, last = t.stride()
-        if last != 1 and t.shape[1] > 1:
-            raise _lib.SpockError(f"{what}: {name} must have contiguous rows, got strides {t.stride()}")
         rows, n = t.shape
+        if last != 1 and n > 1:
+            raise _lib.SpockError(f"{what}: {name} must have contiguous rows, got strides {t.stride()}")
         return stride if rows > 1 else n
     if not t.is_contiguous():
         raise _lib.SpockError(f"{what}: {name} must be two-dimensional or contiguous, got strides {t.stride()}")
@@ -627,10 +625,13 @@ def mx4_quantize(x: torch.Tensor, out: Optional[Mx4] = None) -> Mx4:
     stride = _row_stride(what, "x", x)
     if out is None:
         out = Mx4(x.new_empty((*lead, n // 2), dtype=torch.uint8), x.new_empty((*lead, n // 32), dtype=torch.uint8))
-    m, rows_of, rows, cols = _mx4_rows(what, "out", out, dev)
-    if rows_of != lead or cols != n:
-        raise _lib.SpockError(f"{what}: out holds {tuple(rows_of)} rows of {cols} values, x is {tuple(x.shape)}")
-    _launch(dev, what, lib().spk_mx4_quantize, x.data_ptr(), dtype, stride, rows, cols, C.byref(m))
+        m = SpkMx4(out.codes.data_ptr(), n // 2, out.scales.data_ptr(), n // 32)
+        rows = prod(lead)
+    else:
+        m, rows_of, rows, cols = _mx4_rows(what, "out", out, dev)
+        if rows_of != lead or cols != n:
+            raise _lib.SpockError(f"{what}: out holds {tuple(rows_of)} rows of {cols} values, x is {tuple(x.shape)}")
+    _launch(dev, what, lib().spk_mx4_quantize, x.data_ptr(), dtype, stride, rows, n, C.byref(m))
     return out
 
 
@@ -687,9 +688,7 @@ def mx4_matmul(x, w: Mx4, residual: Optional[torch.Tensor] = None, dtype: Option
         if x.dim() < 1 or dtype not in (None, x.dtype):
             raise _lib.SpockError(f"{what}: x is {tuple(x.shape)} {x.dtype}, the result {dtype}")
         *lead, depth = x.shape
-        dtype, rows = x.dtype, 1
-        for size in lead:
-            rows *= size
+        dtype, rows = x.dtype, prod(lead)
         x_at, x_stride = x.data_ptr(), _row_stride(what, "x", x)
     kind = _HALF.get(dtype)
     if kind is None:
