@@ -334,53 +334,94 @@ __device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int* t
 // their use.  The tile is formed transposed (w is the A operand), so that a lane's
 // outputs lie side by side in a row of out.  All that is loaded goes to LDS, also
 // the scales: a load to registers among the others would make the compiler wait for all.
-// TAIL: the depth ends inside a stage; what lies past it is zero in x and w.
+//
+// What is read of a row at a time are whole lines, 128 bytes to 8 lanes: a line of which 64 or
+// 32 bytes are taken is fetched again for the rest, and the loads were the bound
+// (8192 x 8192 x 8192 in 4 bits with 64 bytes a time: 406 us, without products 397; so
+// 344, 3.2 PFLOP/s, products alone 207, and the loads, all of whose lines an XCD's workgroups
+// wait for together, still bound it; 2001 x 14336 x 4096 in 16 bits 200 us, 1.2 PFLOP/s).
+// Pieces of 16 bytes lie in LDS exchanged within their line by the row's number (p ^ row % 8),
+// so that 8 rows read side by side are in different banks.
+// What lies past the depth is zero in x and w.
+//
+// The wave's rows of a matrix: L lanes to a row, which take B bytes each of a line of it.
+// (A pointer to each load's rows took 30 registers more than there are.)
+template <int B, int L>
+struct Lines {
+  const uint8_t* at;  // of this lane in the first 64 / L rows
+  int64_t stride;     // of 64 / L rows
+  int left;           // rows from this lane's on
 
-// Rows in 16 bits: a stage is 64 values, 128 bytes of a row of x and 32 of w.  Pieces of 16
-// bytes are exchanged within a row so that 8 rows read side by side are in different
-// banks: of x by the row's number (p ^ row % 8), of w in every other four rows.  Of w a lane
-// needs one block, whose 4 dwords of codes are 4 products' operands.
-template <bool BF, int WM, int WN, int TM, int TN, bool TAIL>
+  __device__ __forceinline__ Lines(const uint8_t* rows, int64_t row_stride, int first, int end, int bytes) {
+    const int row = (threadIdx.x & 63) / L;
+    at = rows + (first + row) * row_stride + bytes;
+    stride = 64 / L * row_stride;
+    left = end - first - row;
+  }
+  // The i-th 64 / L rows, `bytes` further; zeros where `within` is false or there are no more rows.
+  __device__ __forceinline__ void load(int i, int64_t bytes, bool within, void* to) const {
+    const uint8_t* here = at;
+    asm("" : "+v"(here));  // the sum is formed each time, and takes no registers in between
+    spk_mx4::load_lds<B>(within && 64 / L * i < left ? here + (i * stride + bytes) : reinterpret_cast<const uint8_t*>(kZero), to);
+  }
+};
+
+// The scales of a wave's RW rows, a group of stages of 256 values (8 blocks) at a time: 16 bytes
+// to each of L lanes of a row (SB = 16), or a byte to a dword where rows of scales are not
+// of aligned 16 bytes (SB = 1).  (4 bytes of a row's line at each stage: 40 us of 380.)
+template <int SB, int L, int RW>
+struct Scales {
+  static constexpr int kGroup = SB == 16 ? 2 * L : 1, kLanes = SB == 16 ? L : 8;
+  static constexpr int kLoads = RW * kLanes / 64, kWords = SB == 16 ? 4 * L : 8;  // dwords of a row
+  Lines<SB, kLanes> lines;
+
+  __device__ __forceinline__ Scales(const uint8_t* rows, int64_t row_stride, int first, int end)
+      : lines(rows, row_stride, first, end, SB * ((int)threadIdx.x % kLanes)) {}
+  static __device__ __forceinline__ int half(int st) { return st / kGroup & 1; }
+  // the group of stage st to the wave's place in its half
+  __device__ __forceinline__ void load(int st, int blocks, uint32_t* to) const {
+    const int first = st / kGroup * (8 * kGroup);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) lines.load(i, first, first + SB * ((int)threadIdx.x % kLanes) < blocks, to + (SB == 16 ? 256 : 64) * i);
+  }
+  // blocks 4 n + h and 4 n + 2 + h of row r in bytes 0 and 2 (SB = 16), else block 2 c + h
+  static __device__ __forceinline__ uint32_t of(const uint32_t* s, int r, int st, int c, int h) {
+    return SB == 16 ? s[kWords * r + 2 * (st % kGroup) + c / 2] >> (8 * h) : s[8 * r + 2 * c + h];
+  }
+};
+
+// Rows in 16 bits.  64 values of x are a stage, 256 of w one: a lane's 16 bytes are a
+// block, whose 4 dwords of codes are 4 products' operands.
+template <bool BF, int WM, int WN, int TM, int TN, int SB>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles16_kernel(Mm a, int vec) {
   constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN;
-  constexpr int PX = BM / (8 * NW), PW = BN / (32 * NW), PS = BN / (32 * NW);  // loads of a wave and stage
-  constexpr int P = PX + PW + PS;
-  static_assert(BM % (8 * NW) == 0 && BN % (32 * NW) == 0, "whole loads");
-  // x, w and the scales of three stages, an array to each: a load into one is then known
-  // not to touch the others (the compiler tells eight apart)
-  __shared__ __align__(16) uint4 sa[BM * 8 + BN * 2 + BN / 2], sb[BM * 8 + BN * 2 + BN / 2], sc[BM * 8 + BN * 2 + BN / 2];
+  constexpr int PX = BM / (8 * NW), PW = BN / (8 * NW);  // loads of a wave
+  static_assert(BM == 32 * NW && BN == 32 * NW, "a wave loads 32 rows of x and of w");
+  using S = Scales<SB, 2, 32>;
+  // an array to each stage: a load into one is then known not to touch the others
+  __shared__ __align__(16) uint4 xa[BM * 8], xb[BM * 8], wa[BN * 8], wb[BN * 8];
+  __shared__ __align__(16) uint32_t sc[2 * BN * S::kWords];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   int tm, tn;
   tile_at(blockIdx.x, (a.rows + BM - 1) / BM, (a.cols + BN - 1) / BN, &tm, &tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  const int blocks = a.depth / 32, stages = (blocks + 1) / 2;
+  const int blocks = a.depth / 32, stages = (blocks + 7) / 8;
 
-  const int px = lane % 8 ^ lane / 8, pw = lane % 2 ^ (lane >> 3 & 1);
-  const uint8_t *xp[PX], *wp[PW], *sp[PS];
+  const int piece = lane % 8 ^ lane / 8;
+  const Lines<16, 8> xl(reinterpret_cast<const uint8_t*>(a.x), 2 * a.xt, m0 + 32 * wave, a.rows, 16 * piece);
+  const Lines<16, 8> wl(a.wc, a.wct, n0 + 32 * wave, a.cols, 16 * piece);
+  const S scales(a.ws, a.wst, n0 + 32 * wave, a.cols);
+  auto load_x = [&](int st, uint4* x) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < PX; ++i)
-    xp[i] = reinterpret_cast<const uint8_t*>(a.x + min(m0 + 8 * (i * NW + wave) + lane / 8, a.rows - 1) * a.xt) + 16 * px;
-#pragma unroll
-  for (int i = 0; i < PW; ++i) {
-    const int n = min(n0 + 32 * (i * NW + wave) + lane / 2, a.cols - 1);
-    wp[i] = a.wc + n * a.wct + 16 * pw;
-    sp[i] = a.ws + n * a.wst + lane % 2;
-  }
-  auto load = [&](int st, uint4* x) __attribute__((always_inline)) {
-    uint4* w = x + BM * 8;
-    uint32_t* s = reinterpret_cast<uint32_t*>(w + BN * 2);
-    st = min(st, stages - 1);  // past the end the last one again, which nobody reads
-    const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
-#pragma unroll
-    for (int i = 0; i < PX; ++i)
-      spk_mx4::load_lds<16>(!TAIL || 2 * st + px / 4 < blocks ? xp[i] + 128 * (int64_t)st : zero, x + 64 * (i * NW + wave));
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      spk_mx4::load_lds<16>(!TAIL || 2 * st + pw < blocks ? wp[i] + 32 * (int64_t)st : zero, w + 64 * (i * NW + wave));
-      spk_mx4::load_lds<1>(!TAIL || 2 * st + lane % 2 < blocks ? sp[i] + 2 * (int64_t)st : zero, s + 64 * (i * NW + wave));
-    }
+    for (int i = 0; i < PX; ++i) xl.load(i, 128 * (int64_t)st, 2 * st + piece / 4 < blocks, x + 64 * (PX * wave + i));
+  };
+  auto load_w = [&](int st, int i, uint4* w) __attribute__((always_inline)) {
+    wl.load(i, 128 * (int64_t)st, 8 * st + piece < blocks, w + 64 * (PW * wave + i));
+  };
+  auto load_s = [&](int st) __attribute__((always_inline)) {
+    scales.load(st, blocks, sc + (S::half(st) * BN + 32 * wave) * S::kWords);
   };
   floatx16 acc[TN][TM];
 #pragma unroll
@@ -389,20 +430,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles16_kernel(Mm a, int 
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
-  const int xbase = (32 * wm * TM + ln) * 8, nbase = 32 * wn * TN + ln;
-  const int flip = ln & 7, wat = 2 * nbase + (h ^ (ln >> 2 & 1)), sat = 2 * nbase + h;
-  auto step = [&](int st, const uint4* x, uint4* to) __attribute__((always_inline)) {
-    const uint4* w = x + BM * 8;
-    const uint32_t* s = reinterpret_cast<const uint32_t*>(w + BN * 2);
-    load(st + 2, to);
-    __builtin_amdgcn_sched_barrier(0);
+  const int xbase = (32 * wm * TM + ln) * 8, nbase = 32 * wn * TN + ln, flip = ln & 7;
+  // Quarter q of stage st of w, with the stage of x at `x`; the next ones to xn and wnext.
+  auto step = [&](int st, int q, const uint4* x, uint4* xn, const uint4* w, uint4* wnext) __attribute__((always_inline)) {
     uint4 codes[TN], v[2][TM];
     float scale[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      codes[j] = w[wat + 64 * j];
-      scale[j] = spk_mx4::scale_of(s[sat + 64 * j]);
+      const uint32_t* s = sc + S::half(st) * BN * S::kWords;
+      scale[j] = spk_mx4::scale_of(S::of(s, nbase + 32 * j, st, q, h) >> (SB == 16 ? 16 * (q & 1) : 0) & 255);
+      codes[j] = w[8 * nbase + 256 * j + ((2 * q + h) ^ flip)];
     }
+    __builtin_amdgcn_sched_barrier(0);  // the scales, whose halves the compiler does not tell apart, before loads of them
+    if (q == 0 && (st + 1) % S::kGroup == 0) load_s(st + 1);
+    load_w(st + 1, q, wnext);
+    load_x(4 * st + q + 1, xn);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < TM; ++i) v[0][i] = x[xbase + 256 * i + (4 * h ^ flip)];
 #pragma unroll
@@ -419,74 +462,68 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles16_kernel(Mm a, int 
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[j][i] = mfma32<BF>(f[j], v[c & 1][i], acc[j][i]);
     }
-    meet_after<P>();  // all but what this step asked for
+    meet_after<0>();
   };
-  load(0, sa);
-  load(1, sb);
-  meet_after<P>();
+  auto stage = [&](int st, const uint4* w, uint4* wnext) __attribute__((always_inline)) {
+    step(st, 0, xa, xb, w, wnext);
+    step(st, 1, xb, xa, w, wnext);
+    step(st, 2, xa, xb, w, wnext);
+    step(st, 3, xb, xa, w, wnext);
+  };
+  load_s(0);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) load_w(0, c, wa);
+  load_x(0, xa);
+  meet_after<0>();
   int st = 0;
-  for (; st + 3 <= stages; st += 3) {
-    step(st, sa, sc);
-    step(st + 1, sb, sa);
-    step(st + 2, sc, sb);
+  for (; st + 2 <= stages; st += 2) {
+    stage(st, wa, wb);
+    stage(st + 1, wb, wa);
   }
-  if (st < stages) step(st, sa, sc);
-  if (st + 1 < stages) step(st + 1, sb, sa);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
+  if (st < stages) stage(st, wa, wb);
   store_tile<BF, TM, TN>(a, vec, m0 + 32 * wm * TM + ln, n0 + 32 * wn * TN + 4 * h, acc);
 }
 
-// Rows in 4 bits: a stage is 128 values, 64 bytes of a row of x and of w (pieces exchanged by
-// half of the row's number) and their four scales, which the products apply.  Without
-// TAIL a row's four scales are an aligned dword, with it they are bytes apart.
-template <bool BF, int WM, int WN, int TM, int TN, bool TAIL>
+// Rows in 4 bits: a stage is 256 values of x and of w and their eight scales, which
+// the products apply.
+template <bool BF, int WM, int WN, int TM, int TN, int SB>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles4_kernel(Mm a, int vec) {
-  constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, B = TAIL ? 4 : 1;
-  constexpr int PX = BM / (16 * NW), PW = BN / (16 * NW), PS = (BM + BN) / (64 * NW);  // loads of a wave and stage
-  constexpr int P = PX + PW + PS * B;
-  static_assert(BM % (16 * NW) == 0 && BN % (16 * NW) == 0 && (BM + BN) % (64 * NW) == 0, "whole loads");
-  constexpr int N = (BM + BN) * 4 + (BM + BN) * B / 4;
-  __shared__ __align__(16) uint4 sa[N], sb[N], sc[N], sd[N];
+  constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, R = BM + BN;
+  static_assert(BM == 32 * NW && BN == 32 * NW, "a wave loads 64 rows, all of x or all of w");
+  using S = Scales<SB, 1, 64>;
+  __shared__ __align__(16) uint4 sa[R * 8], sb[R * 8];
+  __shared__ __align__(16) uint32_t sc[2 * R * S::kWords], unused[SB == 16 ? 64 * NW : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   int tm, tn;
   tile_at(blockIdx.x, (a.rows + BM - 1) / BM, (a.cols + BN - 1) / BN, &tm, &tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  const int blocks = a.depth / 32, stages = (blocks + 3) / 4;
+  const int blocks = a.depth / 32, stages = (blocks + 7) / 8;
 
-  const int piece = lane % 4 ^ (lane / 8 & 3);
-  const uint8_t *xp[PX], *wp[PW], *sp[PS];
+  // rows of x, then of w
+  const int piece = lane % 8 ^ lane / 8;
+  const bool x_wave = wave < NW / 2;
+  const int row = x_wave ? m0 + 64 * wave : n0 + 64 * wave - BM, end = x_wave ? a.rows : a.cols;
+  const Lines<16, 8> lines(x_wave ? a.xc : a.wc, x_wave ? a.xct : a.wct, row, end, 16 * piece);
+  const S scales(x_wave ? a.xs : a.ws, x_wave ? a.xst : a.wst, row, end);
+  auto load = [&](int st, uint4* to) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < PX; ++i) xp[i] = a.xc + min(m0 + 16 * (i * NW + wave) + lane / 4, a.rows - 1) * a.xct + 16 * piece;
-#pragma unroll
-  for (int i = 0; i < PW; ++i) wp[i] = a.wc + min(n0 + 16 * (i * NW + wave) + lane / 4, a.cols - 1) * a.wct + 16 * piece;
-#pragma unroll
-  for (int i = 0; i < PS; ++i) {  // rows of x, then of w
-    const int row = 64 * (i * NW + wave) + lane;
-    sp[i] = row < BM ? a.xs + min(m0 + row, a.rows - 1) * a.xst : a.ws + min(n0 + row - BM, a.cols - 1) * a.wst;
-  }
-  auto load = [&](int st, uint4* x) __attribute__((always_inline)) {
-    uint4* w = x + BM * 4;
-    uint32_t* s = reinterpret_cast<uint32_t*>(w + BN * 4);
-    st = min(st, stages - 1);
-    const uint8_t* zero = reinterpret_cast<const uint8_t*>(kZero);
-#pragma unroll
-    for (int i = 0; i < PX; ++i)
-      spk_mx4::load_lds<16>(!TAIL || 4 * st + piece < blocks ? xp[i] + 64 * (int64_t)st : zero, x + 64 * (i * NW + wave));
-#pragma unroll
-    for (int i = 0; i < PW; ++i)
-      spk_mx4::load_lds<16>(!TAIL || 4 * st + piece < blocks ? wp[i] + 64 * (int64_t)st : zero, w + 64 * (i * NW + wave));
-#pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      if constexpr (TAIL) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          spk_mx4::load_lds<1>(4 * st + b < blocks ? sp[i] + 4 * (int64_t)st + b : zero, s + b * (BM + BN) + 64 * (i * NW + wave));
-      } else {
-        spk_mx4::load_lds<4>(sp[i] + 4 * (int64_t)st, s + 64 * (i * NW + wave));
-      }
-    }
+    for (int i = 0; i < 8; ++i) lines.load(i, 128 * (int64_t)st, 8 * st + piece < blocks, to + 64 * (8 * wave + i));
+  };
+  auto load_s = [&](int st) __attribute__((always_inline)) {
+    scales.load(st, blocks, sc + (S::half(st) * R + 64 * wave) * S::kWords);
+  };
+  // A line that comes from memory keeps all of an XCD's workgroups waiting for it that share it:
+  // each asks two stages ahead for a part of those it has in common with its neighbours,
+  // of which a dword comes that nobody uses (8192 x 8192 x 8192: 361 us without, 344).
+  const bool ofx = lane < 32;
+  const int arow = ofx ? min(m0 + BM / 4 * (tn % 4) + 8 * wave + lane / 4, a.rows - 1)
+                       : min(n0 + BN / 4 * (tm % 4) + 8 * wave + lane / 4 - 8, a.cols - 1);
+  const uint8_t* ap = ofx ? a.xc + arow * a.xct : a.wc + arow * a.wct;
+  auto ahead = [&](int st) __attribute__((always_inline)) {
+    if constexpr (SB == 16)  // with SB = 1 there is no room for it
+      spk_mx4::load_lds<4>(8 * (st + 2) < blocks ? ap + 128 * (int64_t)(st + 2) : reinterpret_cast<const uint8_t*>(kZero), unused + 64 * wave);
   };
   floatx16 acc[TN][TM];
 #pragma unroll
@@ -495,64 +532,57 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_tiles4_kernel(Mm a, int v
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.0f;
-  const int mbase = 32 * wm * TM + ln, nbase = 32 * wn * TN + ln, flip = ln >> 1 & 3;
+  const int mbase = 32 * wm * TM + ln, nbase = BM + 32 * wn * TN + ln, flip = ln & 7;
   auto step = [&](int st, const uint4* x, uint4* to) __attribute__((always_inline)) {
-    const uint4* w = x + BM * 4;
-    const uint32_t* s = reinterpret_cast<const uint32_t*>(w + BN * 4);
-    load(st + 3, to);
-    __builtin_amdgcn_sched_barrier(0);
-    // the scales of this half's blocks: bytes 0 and 2, or two dwords
-    uint32_t xsc[TM][2], wsc[TN][2];
-    auto scales = [&](uint32_t (&to)[2], int row) __attribute__((always_inline)) {
-      if constexpr (TAIL) {
-        to[0] = s[row + h * (BM + BN)];
-        to[1] = s[row + (2 + h) * (BM + BN)];
-      } else {
-        to[0] = to[1] = s[row] >> (8 * h);
-      }
-    };
+    const uint32_t* s = sc + S::half(st) * R * S::kWords;
+    uint32_t xsc[4][TM], wsc[4][TN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) scales(xsc[i], mbase + 32 * i);
+    for (int c = 0; c < 4; c += SB == 16 ? 2 : 1) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) scales(wsc[j], BM + nbase + 32 * j);
-    uint4 f[2][TN], v[2][TM];
+      for (int i = 0; i < TM; ++i) xsc[c][i] = S::of(s, mbase + 32 * i, st, c, h);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j) f[b][j] = w[4 * nbase + 128 * j + ((2 * b + h) ^ flip)];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) v[b][i] = x[4 * mbase + 128 * i + ((2 * b + h) ^ flip)];
+      for (int j = 0; j < TN; ++j) wsc[c][j] = S::of(s, nbase + 32 * j, st, c, h);
     }
+    __builtin_amdgcn_sched_barrier(0);  // the scales, whose halves the compiler does not tell apart, before loads of them
+    if ((st + 1) % S::kGroup == 0) load_s(st + 1);
+    uint4 f[2][TN], v[2][TM];
+    auto operands = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+      for (int j = 0; j < TN; ++j) f[c & 1][j] = x[8 * nbase + 256 * j + ((2 * c + h) ^ flip)];
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(four_bits(f[0][j]), four_bits(v[0][i]), acc[j][i], 4, 4, 0,
-                                                                    (int)wsc[j][0], 0, (int)xsc[i][0]);
-    constexpr int second = TAIL ? 0 : 2;  // byte of the second scale
+      for (int i = 0; i < TM; ++i) v[c & 1][i] = x[8 * mbase + 256 * i + ((2 * c + h) ^ flip)];
+    };
+    load(st + 1, to);
+    __builtin_amdgcn_sched_barrier(0);
+    operands(0);
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int c = 0; c < 4; ++c) {
+      if (c < 3) operands(c + 1);
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-        acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(four_bits(f[1][j]), four_bits(v[1][i]), acc[j][i], 4, 4, second,
-                                                                    (int)wsc[j][1], second, (int)xsc[i][1]);
-    meet_after<2 * P>();
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          if (SB == 16 && c % 2)
+            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(four_bits(f[c & 1][j]), four_bits(v[c & 1][i]), acc[j][i], 4, 4,
+                                                                        2, (int)wsc[c & 2][j], 2, (int)xsc[c & 2][i]);
+          else
+            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(four_bits(f[c & 1][j]), four_bits(v[c & 1][i]), acc[j][i], 4, 4,
+                                                                        0, (int)wsc[c][j], 0, (int)xsc[c][i]);
+        }
+    }
+    ahead(st);
+    meet_after<SB == 16>();  // all but that
   };
+  load_s(0);
   load(0, sa);
-  load(1, sb);
-  load(2, sc);
-  meet_after<2 * P>();
+  meet_after<0>();
   int st = 0;
-  for (; st + 4 <= stages; st += 4) {
-    step(st, sa, sd);
+  for (; st + 2 <= stages; st += 2) {
+    step(st, sa, sb);
     step(st + 1, sb, sa);
-    step(st + 2, sc, sb);
-    step(st + 3, sd, sc);
   }
-  if (st < stages) step(st, sa, sd);
-  if (st + 1 < stages) step(st + 1, sb, sa);
-  if (st + 2 < stages) step(st + 2, sc, sb);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the end still write LDS
+  if (st < stages) step(st, sa, sb);
+  spk_mx4::arrived<0>();
   store_tile<BF, TM, TN>(a, vec, m0 + 32 * wm * TM + ln, n0 + 32 * wn * TN + 4 * h, acc);
 }
 
@@ -606,16 +636,17 @@ template <bool X4, bool BF, int WM, int WN, int TM, int TN>
 void launch_tiles(const Mm& a, int vec, hipStream_t s) {
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
   const dim3 grid(((a.rows + BM - 1) / BM) * ((a.cols + BN - 1) / BN)), block(64 * WM * WN);
+  const auto whole = [&](const uint8_t* scales, int64_t stride) { return a.depth % 512 == 0 && stride % 16 == 0 && spk::aligned(scales, 16); };
+  const bool wide = whole(a.ws, a.wst) && (!X4 || whole(a.xs, a.xst));
   if constexpr (X4) {
-    const bool dwords = a.depth % 128 == 0 && a.xst % 4 == 0 && a.wst % 4 == 0 && spk::aligned(a.xs, 4) && spk::aligned(a.ws, 4);
-    if (dwords)
-      hipLaunchKernelGGL((mx4_tiles4_kernel<BF, WM, WN, TM, TN, false>), grid, block, 0, s, a, vec);
+    if (wide)
+      hipLaunchKernelGGL((mx4_tiles4_kernel<BF, WM, WN, TM, TN, 16>), grid, block, 0, s, a, vec);
     else
-      hipLaunchKernelGGL((mx4_tiles4_kernel<BF, WM, WN, TM, TN, true>), grid, block, 0, s, a, vec);
-  } else if (a.depth % 64 == 0) {
-    hipLaunchKernelGGL((mx4_tiles16_kernel<BF, WM, WN, TM, TN, false>), grid, block, 0, s, a, vec);
+      hipLaunchKernelGGL((mx4_tiles4_kernel<BF, WM, WN, TM, TN, 1>), grid, block, 0, s, a, vec);
+  } else if (wide) {
+    hipLaunchKernelGGL((mx4_tiles16_kernel<BF, WM, WN, TM, TN, 16>), grid, block, 0, s, a, vec);
   } else {
-    hipLaunchKernelGGL((mx4_tiles16_kernel<BF, WM, WN, TM, TN, true>), grid, block, 0, s, a, vec);
+    hipLaunchKernelGGL((mx4_tiles16_kernel<BF, WM, WN, TM, TN, 1>), grid, block, 0, s, a, vec);
   }
 }
 
