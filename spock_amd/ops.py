@@ -642,16 +642,18 @@ def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.bfloat16, out: Optional[to
         raise _lib.SpockError(f"{what}: expected an Mx4, got {type(m).__name__}")
     dev = _device(what, m.codes)
     a, lead, rows, cols = _mx4_rows(what, "m", m, dev)
-    shape = (*lead, cols)
     if out is None:
-        if dtype not in _ROWS:
+        kind = _ROWS.get(dtype)
+        if kind is None:
             raise _lib.SpockError(f"{what}: dtype must be float16, bfloat16 or float32, got {dtype}")
-        out = m.codes.new_empty(shape, dtype=dtype)
-    elif out.dtype not in _ROWS:
-        raise _lib.SpockError(f"{what}: out must be float16, bfloat16 or float32, got {out.dtype}")
-    _on(what, "out", out, dev, out.dtype, shape)
-    _launch(dev, what, lib().spk_mx4_dequantize, C.byref(a), rows, cols, _ROWS[out.dtype], out.data_ptr(),
-            _row_stride(what, "out", out))
+        out, stride = m.codes.new_empty((*lead, cols), dtype=dtype), cols
+    else:
+        kind = _ROWS.get(out.dtype)
+        if kind is None:
+            raise _lib.SpockError(f"{what}: out must be float16, bfloat16 or float32, got {out.dtype}")
+        _on(what, "out", out, dev, out.dtype, (*lead, cols))
+        stride = _row_stride(what, "out", out)
+    _launch(dev, what, lib().spk_mx4_dequantize, C.byref(a), rows, cols, kind, out.data_ptr(), stride)
     return out
 
 
