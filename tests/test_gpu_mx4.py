@@ -214,6 +214,33 @@ def test_matmul_strides_and_in_place(dev, rows, four):
     assert bool((hold[:, :7] == 3).all()) and bool((hold[:, 106:] == 3).all())
 
 
+@pytest.mark.parametrize("rows,out", [(5, 1100), (1300, 1100)])
+@pytest.mark.parametrize("four", [False, True], ids=["x16", "x4"])
+def test_matmul_rows_far_apart(dev, four, rows, out):
+    """Rows 4 MB apart, more than 2^32 bytes in all: the same bits as side by side."""
+    from spock_amd import ops
+    gen, apart, depth = torch.Generator().manual_seed(rows), 2 ** 22, 544
+
+    def far(t):
+        size = t.element_size()
+        hold = torch.empty(t.shape[0] * apart // size, dtype=t.dtype, device=dev).as_strided(t.shape, (apart // size, 1))
+        return hold.copy_(t)
+
+    x = _rows(gen, rows, depth, torch.bfloat16, spread=0.5).to(dev)
+    w = ops.mx4_quantize(_rows(gen, out, depth, torch.float32, spread=0.5).to(dev))
+    near = ops.mx4_quantize(x) if four else x
+    want = ops.mx4_matmul(near, w)
+    got = far(torch.zeros_like(want))
+    spread = ops.Mx4(*map(far, near)) if four else far(near)
+    ops.mx4_matmul(spread, ops.Mx4(*map(far, w)), out=got)
+    assert torch.equal(got, want)
+    if four:
+        assert torch.equal(ops.mx4_dequantize(spread), ops.mx4_dequantize(near))
+        again = ops.Mx4(*(far(torch.zeros_like(t)) for t in near))
+        ops.mx4_quantize(far(x), out=again)
+        assert torch.equal(again.codes, near.codes) and torch.equal(again.scales, near.scales)
+
+
 @pytest.mark.parametrize("rows", [2, 70, 300])
 @pytest.mark.parametrize("four", [False, True], ids=["x16", "x4"])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])

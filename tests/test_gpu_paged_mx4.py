@@ -115,6 +115,37 @@ def test_scales_at_odd_bytes(dev, heads, kv, dim, lens):
     _check(out.cpu(), lse.cpu(), _reference(q, k, v, table, cu, ctx), torch.tensor(rows))
 
 
+@pytest.mark.parametrize("lens", [[(1, 500), (1, 90)], [(150, 520), (1, 33)]], ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (4, 2, 256)])
+def test_pages_far_apart(dev, heads, kv, dim, lens):
+    """Pages 2^27 bytes apart, more than 2^32 in all: stored and read as in a compact pool, bit for bit."""
+    from spock_amd import ops
+    print(f"[mx4 far pages {heads}/{kv}x{dim} {lens}]", flush=True)
+    gen = torch.Generator().manual_seed(dim)
+    cu, ctx, table, pages = _tables(lens, 16, dim)
+    assert pages > 33
+
+    def far(t):
+        inner = t[0].contiguous().stride()
+        hold = torch.empty(pages * 2 ** 27, dtype=torch.uint8, device=dev).as_strided(t.shape, (2 ** 27, *inner))
+        return hold.copy_(t)
+
+    k, v = (_on(dev, _pool(gen, pages, 16, kv, dim), "tokens") for _ in range(2))
+    fk, fv = (ops.Mx4(*map(far, m)) for m in (k, v))
+    q, nk, nv = (_normal(gen, cu[-1], n, dim, dtype=torch.float16).to(dev) for n in (heads, kv, kv))
+    table, cu_d, ctx_d = table.to(dev), _i32(cu, dev), _i32(ctx, dev)
+    positions = torch.arange(cu[-1], dtype=torch.int32, device=dev)[None]
+    angle = torch.rand(cu[-1], dim // 2, generator=gen) * 6
+    rope = torch.stack([angle.cos(), angle.sin()], -1).flatten(1).to(dev)
+    outs = []
+    for ck, cv in ((k, v), (fk, fv)):
+        turned = ops.mrope_append_mx4(q, nk, nv, positions, rope, [0] * (dim // 2), ck, cv, table, cu_d, ctx_d)
+        outs.append(ops.paged_attention_mx4(turned, ck, cv, table, cu_d, ctx_d, max(n for n, _ in lens), max(ctx)))
+    assert torch.equal(*outs)
+    for near, there in zip((*k, *v), (*fk, *fv)):
+        assert torch.equal(near, there)
+
+
 @pytest.mark.parametrize("byte", [255, 254, 141])
 @pytest.mark.parametrize("lens", [[(1, 37), (1, 300), (1, 5)], [(9, 300), (6, 6), (20, 45)], [(150, 200)]], ids=str)
 @pytest.mark.parametrize("dtype,dim", [("f16", 256), ("bf16", 128), ("f16", 64)])
