@@ -81,6 +81,18 @@ def test_attention(dev, dtype, heads, kv, dim, lens):
     _check(*_attend(dev, q, k, v, table, cu, ctx, window=window, gate=gate, order=order), ref)
 
 
+# rows on either side of where a sequence has many: 128, 256 and 512 for heads of 64, 128 and 256
+@pytest.mark.parametrize("lens", [[(64, 200), (65, 200)], [(128, 300), (1, 40), (129, 140)], [(256, 300)], [(257, 300), (256, 256), (3, 9)]], ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (2, 1, 128), (4, 2, 256)])
+def test_attention_where_rows_become_many(dev, heads, kv, dim, lens):
+    print(f"[mx4 attention many {heads}/{kv}x{dim} {lens}]", flush=True)
+    gen = torch.Generator().manual_seed(dim + len(lens))
+    cu, ctx, table, pages = _tables(lens, 16, dim)
+    k, v = (_pool(gen, pages, 16, kv, dim) for _ in range(2))
+    q = _normal(gen, cu[-1], heads, dim, dtype=torch.bfloat16, std=2.0)
+    _check(*_attend(dev, q, k, v, table, cu, ctx), _reference(q, k, v, table, cu, ctx))
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 32, 100, 5000])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attention_windows(dev, dtype, window):
@@ -93,7 +105,7 @@ def test_attention_windows(dev, dtype, window):
     _check(*_attend(dev, q, k, v, table, cu, ctx, window=window), _reference(q, k, v, table, cu, ctx, window=window))
 
 
-@pytest.mark.parametrize("lens", [[(1, 300), (1, 1), (0, 5), (7, 90)], [(150, 200)]], ids=str)
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 1), (0, 5), (7, 90)], [(150, 200)], [(300, 350)]], ids=str)
 @pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128), (6, 3, 256)])
 def test_scales_at_odd_bytes(dev, heads, kv, dim, lens):
     """Pools whose rows of scales begin at odd addresses and lie odd numbers of bytes apart."""
@@ -115,7 +127,7 @@ def test_scales_at_odd_bytes(dev, heads, kv, dim, lens):
     _check(out.cpu(), lse.cpu(), _reference(q, k, v, table, cu, ctx), torch.tensor(rows))
 
 
-@pytest.mark.parametrize("lens", [[(1, 500), (1, 90)], [(150, 520), (1, 33)]], ids=str)
+@pytest.mark.parametrize("lens", [[(1, 500), (1, 90)], [(150, 520), (1, 33)], [(300, 520), (1, 33)]], ids=str)
 @pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (4, 2, 256)])
 def test_pages_far_apart(dev, heads, kv, dim, lens):
     """Pages 2^27 bytes apart, more than 2^32 in all: stored and read as in a compact pool, bit for bit."""
@@ -147,7 +159,7 @@ def test_pages_far_apart(dev, heads, kv, dim, lens):
 
 
 @pytest.mark.parametrize("byte", [255, 254, 141])
-@pytest.mark.parametrize("lens", [[(1, 37), (1, 300), (1, 5)], [(9, 300), (6, 6), (20, 45)], [(150, 200)]], ids=str)
+@pytest.mark.parametrize("lens", [[(1, 37), (1, 300), (1, 5)], [(9, 300), (6, 6), (20, 45)], [(150, 200)], [(530, 560)]], ids=str)
 @pytest.mark.parametrize("dtype,dim", [("f16", 256), ("bf16", 128), ("f16", 64)])
 def test_what_a_row_does_not_see_cannot_reach_it(dev, dtype, dim, lens, byte):
     """Blocks that are no numbers, or larger than the type, in slots without a token, and in keys and values of tokens after
@@ -180,7 +192,7 @@ def test_what_a_row_does_not_see_cannot_reach_it(dev, dtype, dim, lens, byte):
         _check(*_attend(dev, q, kk, vv, table, cu, ctx, window=window), _reference(q, kk, vv, table, cu, ctx, window=window))
 
 
-@pytest.mark.parametrize("lens", [[(1, 300)], [(9, 300), (2, 70)], [(150, 200), (1, 90)]], ids=str)
+@pytest.mark.parametrize("lens", [[(1, 300)], [(9, 300), (2, 70)], [(150, 200), (1, 90)], [(530, 560), (1, 90)]], ids=str)
 def test_bad_pages_and_bounds(dev, lens):
     """Pages outside the pool stand for no page; lengths beyond the table and bounds that are too low or too high change
     nothing but the rounding."""
