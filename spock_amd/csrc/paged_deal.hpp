@@ -236,18 +236,22 @@ SPK_HD bool find_tile(const Deal& a, int at, int last, int lane, int* seq, int* 
 // The host's plan.
 // ---------------------------------------------------------------------------
 
-// Rows of a sequence that are not many.  Over a cache in 4 bits pieces of 16 rows carry further: 8
-// sequences of 160 rows, heads of 256, 51 us and 76 as tiles of 256 rows, of 480 rows 115 and 129; 16 of
-// 192, heads of 128, 200 and 271, of 480 421 and 245; 256 rows, heads of 64, 77 and 60.
+// Rows of a sequence that are not many, next to sequences of many rows and by themselves.  Over a
+// cache in 4 bits pieces of 16 rows carry further: 8 sequences of 160 rows, heads of 256, 51 us
+// and 76 as tiles of 256 rows, of 480 rows 115 and 129; 16 of 192, heads of 128, 200 and 271, of 480 421
+// and 245; 256 rows, heads of 64, 77 and 60.  But next to many rows the pieces that they might
+// be take their time in the launch and in the join (2048 tokens and 31 single ones, heads of 128: 344 us, 397).
+constexpr int kFew = 128;
+
 template <bool FOUR>
-int few_rows(const SpkPagedAttnArgs& p) {
-  return FOUR ? 2 * p.cache.head_dim : 128;
+int few_alone(const SpkPagedAttnArgs& p) {
+  return FOUR ? 2 * p.cache.head_dim : kFew;
 }
 constexpr int64_t kMostGroups = 16777215;  // workgroups of 256 in a launch: below 2^32 threads
 
 // How a call's rows and keys are dealt to the kernels.
 struct Plan {
-  int few, many, shares, share_rows, tiles, splits, chunk;
+  int many, shares, share_rows, tiles, splits, chunk;
   bool join, join_few;
   int64_t join_rows;
   int64_t longest, steps;  // rows of a sequence, and steps of 128 keys, by the bounds
@@ -283,10 +287,8 @@ Plan plan_with(const SpkPagedAttnArgs& p) {
   // whatever it has; one that has none to the others
   // Many are more than 128, two pieces of 64 (16 sequences at 4000 keys, heads of
   // 128: 128 rows 68 us, 83 as many; 192 rows 88 as many, 118 in three pieces).
-  const int few = few_rows<FOUR>(p);
-  r.few = few;
-  const bool any_many = longest > few;
-  r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : few + 1;
+  const bool any_many = longest > few_alone<FOUR>(p);
+  r.many = !any_many ? INT32_MAX : c.num_seqs == 1 ? 1 : kFew + 1;
   // pieces of 16 rows where none has more (16 rows: 35 us, 38 in pieces of 64;
   // 36 rows: 42 in one of 64, 68 in three of 16)
   r.share_rows = FOUR || longest <= 16 ? 16 : 64;
@@ -298,7 +300,7 @@ Plan plan_with(const SpkPagedAttnArgs& p) {
   // sequences of few rows: all of them, unless the one there is has many.
   // Next to many rows a sequence of few is 128 rows at most; else the bound may be low.
   const int64_t some = all / r.share_rows + c.num_seqs;
-  const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(few / r.share_rows * (int64_t)c.num_seqs, some) : 0);
+  const int64_t pieces = c.num_kv_heads * (!any_many ? some : c.num_seqs > 1 ? std::min<int64_t>(kFew / r.share_rows * (int64_t)c.num_seqs, some) : 0);
   r.shares = (int)(FOUR ? shares_mx4(p, pieces, steps) : shares_of(pieces, steps));
 
   // sequences of many rows: one workgroup to a CU.  A tile's keys are split into
@@ -306,7 +308,7 @@ Plan plan_with(const SpkPagedAttnArgs& p) {
   // steps in each; a range's share of the join costs as much as some 4 steps
   // (2048 tokens at 16384 keys, 64 workgroups: 347 us in 3 ranges, 322 in the 4 that
   // fill the chip; six prompts in 500 workgroups: 184 us, 210 in 2 ranges each).
-  const int64_t seqs = std::min<int64_t>(c.num_seqs, all / (few + 1) + 1);
+  const int64_t seqs = std::min<int64_t>(c.num_seqs, all / (kFew + 1) + 1);
   r.tiles = any_many ? (int)std::min<int64_t>((all + 255 * seqs) / 256, INT32_MAX) : 0;
   const int64_t groups = std::max<int64_t>(1, (int64_t)r.tiles * c.num_kv_heads);
   int64_t per = steps, least = (groups + 255) / 256 * steps;
@@ -318,7 +320,7 @@ Plan plan_with(const SpkPagedAttnArgs& p) {
   r.splits = r.tiles ? (int)((steps + per - 1) / per) : 1;
   r.join = r.splits > 1 || (r.shares && steps > 1);
   // rows to join: all tokens', or of each sequence those that few can be
-  const int64_t every = (int64_t)c.total_tokens * p.num_q_heads, of_few = (int64_t)c.num_seqs * c.num_kv_heads * few;
+  const int64_t every = (int64_t)c.total_tokens * p.num_q_heads, of_few = (int64_t)c.num_seqs * c.num_kv_heads * kFew;
   r.join_few = any_many && r.splits == 1 && of_few < every;
   r.join_rows = r.join_few ? of_few : every;
   return r;
@@ -365,7 +367,7 @@ size_t bound_with(const SpkPagedAttnArgs& p) {
   int64_t parts = shared(16);
   if (!FOUR && r.longest > 16) parts = std::max(parts, shared(64));
   int64_t split = 0;
-  if (r.longest > r.few && r.steps >= 8)
+  if (r.tiles && r.steps >= 8)
     split = std::min(131072 + 256 * std::min<int64_t>(512, (all + 255) / 256 * c.num_kv_heads), rows * (r.steps / 4));
   return up(parts * part_bytes(p)) + up(rows * 2 * sizeof(int32_t)) + split * part_bytes(p);
 }

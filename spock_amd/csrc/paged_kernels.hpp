@@ -597,7 +597,7 @@ int fill_attn(const SpkPagedAttnArgs* p, const char* who, Plan (*plan_of)(const 
   a->oh = p->out_head_stride;
   static_cast<spk_paged::Deal&>(*a) = spk_paged::deal_of(*p, r, a->c);
   a->heads = p->num_q_heads;
-  a->few = r.join_few ? r.few : 0;
+  a->few = r.join_few ? spk_paged::kFew : 0;
   const float scale = p->scale != 0.0f ? p->scale : 1.0f / std::sqrt((float)c.head_dim);
   a->scale_log2 = scale * 1.44269504088896341f;
   return SPK_OK;
