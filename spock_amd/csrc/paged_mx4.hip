@@ -57,9 +57,9 @@ struct MropeMx4 : Mrope {
 // Memory bounds it where there are many tokens, the chain of loads (lengths, page, angles)
 // where there are few: 32768 tokens of 16 + 4 + 4 heads of 128 in bf16 115 us, 4.0 TB/s (133
 // with the 140 registers and three waves to a SIMD that the compiler takes by itself, 151 with each
-// head's loads where they are used), 64 tokens 11 us.
+// head's loads where they are used), 64 tokens 11 us.  (Pairs side by side in fp16 do not fit.)
 template <int D, bool BF, bool ADJ>
-__global__ __launch_bounds__(256, 4) void mrope_append_mx4_kernel(MropeMx4 a) {
+__global__ __launch_bounds__(256, ADJ && !BF ? 3 : 4) void mrope_append_mx4_kernel(MropeMx4 a) {
   constexpr int L = D / 16, RG = 64 / L;  // lanes of a head, heads at a time
   __shared__ int chunk_top[4][RG][D / 8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
