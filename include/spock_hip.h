@@ -719,8 +719,9 @@ int spk_mrope_append_mx4(const SpkMropeArgs* args, const SpkPagedScales* scales,
  * gives them in dtype; a block whose scale passes 2^13 (fp16) or 2^125 (bf16)
  * counts as NaN, as one of byte 255 does: a row that sees such a value has NaN in
  * that block's dimensions, one that sees such a key is NaN, and no other row is
- * touched.  Weights are rounded to dtype before the product with V.  Where the
- * bounds allow no sequence more than 2 head_dim rows, all take the form of few rows. */
+ * touched.  Before the product with V weights are two 16-bit parts (value and
+ * remainder) for any number of rows.  Where the bounds allow no sequence more than
+ * 2 head_dim rows, all take the form of few rows. */
 size_t spk_paged_attention_mx4_workspace_size(const SpkPagedAttnArgs* args);
 size_t spk_paged_attention_mx4_workspace_need(const SpkPagedAttnArgs* args);
 int spk_paged_attention_mx4(const SpkPagedAttnArgs* args, const SpkPagedScales* scales, spk_stream_t stream);

@@ -207,6 +207,16 @@ struct AttnMx4 : Attn {
   Scales sc;
 };
 
+// Two weights as what they are in the 16-bit type and what that leaves of them, both to
+// nearest: some 22 bits together in fp16, 16 in bf16.  (A cached value is finite, or its block is
+// no number: there is no infinity whose sign the smaller part could turn.)
+template <bool BF>
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t* most, uint32_t* rest) {
+  *most = Half<BF>::pack(a, b);
+  const float2_t x = Half<BF>::unpack(*most);
+  *rest = Half<BF>::pack(a - x.x, b - x.y);
+}
+
 // Few rows per sequence and KV head: spk_paged_attention's form for them (16 rows of
 // a sequence and a range of its keys to a workgroup, every fourth step of 32 keys
 // to a wave, scores transposed, the waves' states joined in LDS), from 4 bits.
@@ -225,9 +235,10 @@ struct AttnMx4 : Attn {
 // 8; the queries' dimensions are dealt the same way.  Of the values it holds D / 16
 // dimensions of its 8 keys.  Codes become 16-bit values with their scale in the conversion:
 // exact but for what the type cannot hold.  A weight enters the second product
-// rounded to 16 bits: the cache's own rounding is a hundred times as much.
-// Memory bounds long contexts (64 sequences, heads of 128: 139 us, 4.4 TB/s with the join's),
-// the way to the first keys short ones (1500 keys: 14 us).
+// in two parts (`two_parts`): the products of the second one take 2 us of 39 with drafted
+// tokens (16 sequences of 36 rows, heads of 256) and nothing where memory bounds it.
+// Memory bounds long contexts (64 sequences, heads of 128: 144 us, 3.9 TB/s with the join's),
+// the way to the first keys short ones (1500 keys: 15 us).
 // BYTES: the scales' rows are not aligned to 4 bytes (or have 2), and are loaded by the byte.
 template <int D, bool BF, bool BYTES>
 __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void mx4_rows_kernel(AttnMx4 a) {
@@ -405,7 +416,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
       w[i] = exp2_fast(__builtin_fmaf(w[i], a.scale_log2, H::kShift - base));
       l += w[i];
     }
-    const uint4 p = make_uint4(H::pack(w[0], w[1]), H::pack(w[2], w[3]), H::pack(w[4], w[5]), H::pack(w[6], w[7]));
+    uint4 p0, p1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) two_parts<BF>(w[2 * i], w[2 * i + 1], &(&p0.x)[i], &(&p1.x)[i]);
     // a block of values that is no number must not meet the zero weight of a row that
     // does not see it: it counts as zeros here, and is added row by row below
     uint32_t odd_keys = 0, zeros = 0;
@@ -445,7 +458,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 3 : 2) - BYTES) void
         for (int i = 0; i < 4; ++i)
           (&f.x)[i] = __builtin_amdgcn_perm((&v[2 * i + 1].x)[(e & 7) >> 1], (&v[2 * i].x)[(e & 7) >> 1],
                                             e & 1 ? 0x07060302u : 0x05040100u);
-        acc[e] = H::mfma16(f, p, acc[e]);
+        acc[e] = H::mfma16(f, p0, acc[e]);
+        acc[e] = H::mfma16(f, p1, acc[e]);
       }
     }
     while (odd_keys) {
@@ -572,23 +586,27 @@ __device__ __forceinline__ void meet() {
 // bytes exchanged by the row's number, so that neither 8 keys' pieces side by side (the
 // scores' operand) nor 4 values' halves of 32 dimensions (the transposing load's) share
 // banks.  The transposing load makes of 4 keys' values the output's operand.
-// The matrix instructions and the LDS reads that feed them bound it: 2048 tokens at 16384 keys,
-// 8 heads of 256, 292 us, 880 TFLOP/s.
+// A weight enters the product with V in two parts here too, for half as many matrix instructions
+// more: rounded to one part 2048 tokens at 16384 keys, 8 heads of 256, take 285 us and two
+// prompts of heads of 64 91, in two parts 372 and 106.  But the error is then the plain form's, where one
+// part has a third more (fp16 2.8e-4 for 2.1e-4, bf16 2.2e-3 for 1.7e-3), and the same for all numbers of rows.
+// The matrix instructions and the LDS reads that feed them bound it: those 372 us are 690 TFLOP/s of
+// the attention's own operations, 1040 with the second parts.
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
   using H = Half<BF>;
   constexpr int KT = 8192 / D;             // keys of a tile
   constexpr int KS = D / 16;               // contraction steps of the scores
-  constexpr int QR = D == 256 ? 10 : KS;   // of the queries' pieces in registers, the rest in LDS
+  constexpr int QR = D == 256 ? 8 : KS;   // of the queries' pieces in registers, the rest in LDS
   constexpr int DT = D / 32;               // output tiles
   constexpr int CH = D / 8;                // 16-byte pieces of a row
   constexpr int TK = D / 16;               // threads of a key
   constexpr int WK = 64 / TK;              // keys of a wave's threads
   constexpr int NB = D == 256 ? 1 : 2;     // blocks of 32 keys at a time
   // LDS reads ahead of the product that uses them, and of the queries' 16 pieces those in
-  // registers, as the registers allow: 2048 tokens at 16384 keys, heads of 256, take 292 us with
-  // (1, 10), 295 with (1, 8), 297 with (2, 6), 325 with (0, 12) and 337 with (0, 10).  Heads of 128: 4
-  // and 6 ahead 173 and 177 us (six prompts).
+  // registers, as the registers allow: 2048 tokens at 16384 keys, heads of 256, take 372 us with
+  // (1, 8) and 374 with (1, 6); (1, 10) would keep 40 bytes of a lane on the private stack.  (Before weights had two
+  // parts (0, 12) took 325 for 292, and with heads of 128 6 reads ahead 177 for 173, six prompts.)
   constexpr int AHEAD = D == 256 ? 1 : 4;
   __shared__ __align__(16) uint4 ks[2][1024], vs[2][1024];
   __shared__ __align__(16) uint4 qs[KS > QR ? (KS - QR) * 512 : 1];
@@ -753,7 +771,7 @@ __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
         for (int t = 0; t < DT; ++t) acc[t] *= f;
       }
       // the weights of 16 keys while the product of the 16 before them runs
-      uint4 p4[2 * NB];
+      uint4 p0[2 * NB], p1[2 * NB];
       auto weigh = [&](int i, int e0, int e1) __attribute__((always_inline)) {
         floatx16& x = s[i >> 1];
 #pragma unroll
@@ -763,8 +781,8 @@ __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
         }
         if (e1 == 8) {
           const int f = 8 * (i & 1);
-          p4[i] = make_uint4(H::pack(x[f], x[f + 1]), H::pack(x[f + 2], x[f + 3]), H::pack(x[f + 4], x[f + 5]),
-                             H::pack(x[f + 6], x[f + 7]));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) two_parts<BF>(x[f + 2 * n], x[f + 2 * n + 1], &(&p0[i].x)[n], &(&p1[i].x)[n]);
         }
       };
       weigh(0, 0, 8);
@@ -778,7 +796,8 @@ __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
           },
           [&](int c, uint4 v) {
             const int i = c / DT, t = c % DT;
-            acc[t] = H::mfma32(v, p4[i], acc[t]);
+            acc[t] = H::mfma32(v, p0[i], acc[t]);
+            acc[t] = H::mfma32(v, p1[i], acc[t]);
             if (i + 1 < 2 * NB) weigh(i + 1, 8 * t / DT, 8 * (t + 1) / DT);
           });
       if (some) {

@@ -93,6 +93,47 @@ def test_attention_where_rows_become_many(dev, heads, kv, dim, lens):
     _check(*_attend(dev, q, k, v, table, cu, ctx), _reference(q, k, v, table, cu, ctx))
 
 
+# pieces of 16 rows, and tiles of 256 of sequences of many rows
+@pytest.mark.parametrize("lens", [[(1, 400), (9, 90)], [(290, 310), (5, 40)]], ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (2, 1, 128), (4, 2, 256)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_weights_keep_their_bits(dev, dtype, heads, kv, dim, lens):
+    """A weight enters the product with V in two parts, each half a step off at most: what is lost of it is the square of one
+    rounding, which shows where values of both signs cancel.  paged_ref's bound with that in the place of one rounding of
+    softmax . |V|, which is the same attention over |V|."""
+    print(f"[mx4 attention weights {dtype} {heads}/{kv}x{dim} {lens}]", flush=True)
+    t, gen = DT[dtype], torch.Generator().manual_seed(dim + len(lens))
+    cu, ctx, table, pages = _tables(lens, 16, dim)
+    k, v = (_pool(gen, pages, 16, kv, dim) for _ in range(2))
+    q = _normal(gen, cu[-1], heads, dim, dtype=t, std=2.0)
+    want, lse, bound = _reference(q, k, v, table, cu, ctx)
+    size = _reference(q, k, (v[0] & 0x77, v[1]), table, cu, ctx)[0]
+    half = R.HALF[t]
+    bound -= (half - half * half) * size
+    _check(*_attend(dev, q, k, v, table, cu, ctx), (want, lse, bound))
+
+
+@pytest.mark.parametrize("lens", [[(1, 400), (9, 90)], [(290, 310), (5, 40)]], ids=str)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (2, 1, 128), (4, 2, 256)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_weights_keep_their_bits_of_exact_scores(dev, dtype, heads, kv, dim, lens):
+    """As above where the scores leave no room for one rounding in fp16 either: a query has one element, so that a product
+    with a key is exact.  Left of a weight's error are, in 2^-24, the scale's own (4 of the score's size), the sum
+    with the maximum (2 of it, and 7 for fp16's shift) and exp2 (8): 8 of the scores' size and 16, and as much in the sum."""
+    print(f"[mx4 attention exact scores {dtype} {heads}/{kv}x{dim} {lens}]", flush=True)
+    t, gen = DT[dtype], torch.Generator().manual_seed(3 * dim + len(lens))
+    cu, ctx, table, pages = _tables(lens, 16, dim)
+    k, v = (_pool(gen, pages, 16, kv, dim) for _ in range(2))
+    q = torch.zeros(cu[-1], heads, dim).scatter_(2, torch.randint(0, dim, (cu[-1], heads, 1), generator=gen), 16.0 if dim == 64 else 32.0).to(t)
+    want, lse, _ = _reference(q, k, v, table, cu, ctx)
+    size = _reference(q, k, (v[0] & 0x77, v[1]), table, cu, ctx)[0]
+    half, most = R.HALF[t], float(M.values(*k).abs().max()) * 32 / math.sqrt(dim)
+    rel = half * half + 2 * (8 * most + 16) * 2.0 ** -24 + 2 * max(ctx) * 2.0 ** -24
+    assert rel < half / 4
+    bound = rel * size + max(ctx) * 2.0 ** -32 * float(M.values(*v).abs().max()) + half * want.abs() * (1 + half)
+    _check(*_attend(dev, q, k, v, table, cu, ctx), (want, lse, bound))
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 32, 100, 5000])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attention_windows(dev, dtype, window):
