@@ -268,9 +268,13 @@ inline int64_t shares_of(int64_t pieces, int64_t steps) {
 // Over a cache in 4 bits: whole rounds of the workgroups that the chip holds at once (3 to a
 // CU, heads of 256 2), 2 to a piece: 64 sequences over 8 KV heads with 1, 2, 3 and 4 to a piece
 // take 150, 139, 136 and 140 us; one of 130,001 keys with 2 and 3 workgroups to a CU 50 and 41.
+// Of more pieces than a round holds one round more than theirs carries what is split: with 2 to
+// a piece all are (heads of 128, 32 over 8, with that round and with 2 to a piece: 512 sequences of 64
+// tokens at 4096 keys 5.7 ms and 7.4, and half the workspace; 1024 single tokens at 100 to 1500 385 us
+// and 569; 256 at 300 to 16000 482 and 498; two and four rounds more are never faster).
 inline int64_t shares_mx4(const SpkPagedAttnArgs& p, int64_t pieces, int64_t steps) {
   const int64_t round = p.cache.head_dim == 256 ? 512 : 768;
-  const int64_t n = (2 * pieces + round - 1) / round * round;
+  const int64_t n = std::min((2 * pieces + round - 1) / round, (pieces + round - 1) / round + 1) * round;
   return std::min<int64_t>(std::min<int64_t>(n, pieces * (steps + 1)), INT32_MAX);
 }
 
