@@ -326,6 +326,19 @@ def _device(what: str, t: torch.Tensor) -> int:
     return t.get_device()
 
 
+def _fits(what: str, **sizes: int) -> None:
+    """Sizes that go to the library in 32 bits, in which ctypes puts larger ones without a word."""
+    if any(n >> 31 for n in sizes.values()):
+        raise _lib.SpockError(f"{what}: sizes must be below 2^31 and not negative, got "
+                              + ", ".join(f"{name} {n}" for name, n in sizes.items()))
+
+
+def _bounds(*bounds: int):
+    """Bounds and windows as 32 bits have them: of 2^31 and more they are the largest, which bounds no less; below 0 they are -1,
+    which is refused."""
+    return tuple(min(max(n, -1), 2 ** 31 - 1) for n in bounds)
+
+
 def _paged_cache(what: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                  cu_seqlens: torch.Tensor, context_lens: torch.Tensor) -> SpkPagedCache:
     dev, dtype = _device(what, q), q.dtype
@@ -336,7 +349,7 @@ def _paged_cache(what: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise _lib.SpockError(f"{what}: q must be float16 or bfloat16, got {dtype}")
     shape = k_cache.shape
     pages, page_size, kv_heads, dim = shape
-    tokens, _, q_dim = q.shape
+    tokens, heads, q_dim = q.shape
     if q_dim != dim:
         raise _lib.SpockError(f"{what}: q has head_dim {q_dim}, the cache {dim}")
     _on(what, "k_cache", k_cache, dev, dtype)
@@ -354,6 +367,9 @@ def _paged_cache(what: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if block_table.dim() != 2 or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise _lib.SpockError(f"{what}: block_table must be [{seqs}][max_pages] with contiguous rows, "
                               f"got {tuple(block_table.shape)}")
+    if (pages | page_size | kv_heads | tokens | heads | seqs | block_table.shape[1]) >> 31:
+        _fits(what, pages=pages, page_size=page_size, kv_heads=kv_heads, tokens=tokens, heads=heads, sequences=seqs,
+              max_pages=block_table.shape[1])
     return SpkPagedCache(_HALF[dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, tokens,
                          k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2],
                          block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), context_lens.data_ptr())
@@ -386,6 +402,8 @@ def _mrope_args(what: str, cache: SpkPagedCache, q, k, v, positions, rope, pair_
         raise _lib.SpockError(f"{what}: pair_axis must be a sequence of axis numbers, got {pair_axis!r}") from None
     rot = 2 * len(axes)
     rows = rope.shape[0]
+    if rows >> 31:
+        _fits(what, rope_rows=rows)
     _flat(what, "rope", rope, dev, torch.float32, (rows, rot))
     num_axes = positions.shape[0]
     _on(what, "positions", positions, dev, torch.int32, (num_axes, T))
@@ -439,6 +457,8 @@ def _attention_args(what: str, cache: SpkPagedCache, q, max_query_len, max_conte
     """(SpkPagedAttnArgs, out, lse, workspace) of an attention over `cache`, checked."""
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
     _, heads, D = shape
+    if (max_query_len | max_context_len | window) >> 31:
+        max_query_len, max_context_len, window = _bounds(max_query_len, max_context_len, window)
     qs = _rows(what, "q", q, dev, dtype, shape)
     gs = (0, 0) if gate is None else _rows(what, "gate", gate, dev, dtype, shape)
     if out is None:
@@ -486,6 +506,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
 def _attention_sizes(tokens, heads, kv_heads, head_dim, page_size, max_pages, num_seqs, max_query_len, max_context_len, window):
     """SpkPagedAttnArgs of these sizes, without buffers."""
+    _fits("workspace", tokens=tokens, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page_size=page_size, max_pages=max_pages,
+          num_seqs=num_seqs)
+    max_query_len, max_context_len, window = _bounds(max_query_len, max_context_len, window)
     cache = SpkPagedCache(_lib.SPK_F16, kv_heads, head_dim, page_size, 1, max_pages, num_seqs, tokens, 16, 16, 0, 0, 0,
                           16, max_pages, 16, 16)
     return SpkPagedAttnArgs(cache, heads, max_query_len, max_context_len, window)
@@ -622,6 +645,8 @@ def mx4_quantize(x: torch.Tensor, out: Optional[Mx4] = None) -> Mx4:
     if n % 32 or dtype is None:
         raise _lib.SpockError(f"{what}: x must be [..., a multiple of 32] float16, bfloat16 or float32, "
                               f"got {tuple(x.shape)} {x.dtype}")
+    if n >> 31:
+        _fits(what, row=n)
     stride = _row_stride(what, "x", x)
     if out is None:
         out = Mx4(x.new_empty((*lead, n // 2), dtype=torch.uint8), x.new_empty((*lead, n // 32), dtype=torch.uint8))
@@ -642,6 +667,8 @@ def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.bfloat16, out: Optional[to
         raise _lib.SpockError(f"{what}: expected an Mx4, got {type(m).__name__}")
     dev = _device(what, m.codes)
     a, lead, rows, cols = _mx4_rows(what, "m", m, dev)
+    if cols >> 31:
+        _fits(what, row=cols)
     if out is None:
         kind = _ROWS.get(dtype)
         if kind is None:
@@ -697,6 +724,8 @@ def mx4_matmul(x, w: Mx4, residual: Optional[torch.Tensor] = None, dtype: Option
         raise _lib.SpockError(f"{what}: rows and result must be float16 or bfloat16, got {dtype}")
     if depth != k:
         raise _lib.SpockError(f"{what}: x has rows of {depth} values, w of {k}")
+    if (rows | n | k) >> 31:
+        _fits(what, rows=rows, out=n, values=k)
     shape = (*lead, n)
     res, res_stride = None, 0
     if residual is not None:
@@ -747,7 +776,7 @@ def _paged_cache_mx4(what: str, q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, blo
     codes, scales = k_cache
     shape = codes.shape
     pages, page_size, kv_heads, half = shape
-    tokens, _, dim = q.shape
+    tokens, heads, dim = q.shape
     if dim != 2 * half or dim % 32:
         raise _lib.SpockError(f"{what}: q has head_dim {dim}, the cache {2 * half}")
     c = _pool_strides(what, "codes", codes, v_cache.codes, dev, shape)
@@ -759,6 +788,9 @@ def _paged_cache_mx4(what: str, q: torch.Tensor, k_cache: Mx4, v_cache: Mx4, blo
     if block_table.dim() != 2 or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise _lib.SpockError(f"{what}: block_table must be [{seqs}][max_pages] with contiguous rows, "
                               f"got {tuple(block_table.shape)}")
+    if (pages | page_size | kv_heads | tokens | heads | seqs | block_table.shape[1]) >> 31:
+        _fits(what, pages=pages, page_size=page_size, kv_heads=kv_heads, tokens=tokens, heads=heads, sequences=seqs,
+              max_pages=block_table.shape[1])
     cache = SpkPagedCache(_HALF[dtype], kv_heads, dim, page_size, pages, block_table.shape[1], seqs, tokens,
                           codes.data_ptr(), v_cache.codes.data_ptr(), c[0], c[1], c[2],
                           block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), context_lens.data_ptr())
