@@ -636,10 +636,36 @@ def _row_stride(what: str, name: str, t: torch.Tensor) -> int:
     return t.shape[-1]
 
 
+def _memory_order(t: torch.Tensor):
+    """The order of [..., n]'s dimensions in memory, as permute() takes it, where it is another than their own; else None."""
+    if t.dim() < 3 or t.is_contiguous():
+        return None
+    order = sorted(range(t.dim() - 1), key=lambda i: -t.stride(i))
+    return None if order == sorted(order) else (*order, t.dim() - 1)
+
+
+def _permuted(t, order):
+    """A tensor, or an Mx4's two, with dimensions in that order."""
+    if isinstance(t, Mx4):
+        return Mx4(_permuted(t.codes, order), _permuted(t.scales, order))
+    return t.permute(order) if isinstance(t, torch.Tensor) and t.dim() == len(order) else t
+
+
+def _back(order):
+    return sorted(range(len(order)), key=order.__getitem__)
+
+
 def mx4_quantize(x: torch.Tensor, out: Optional[Mx4] = None) -> Mx4:
-    """Rows of x [..., n] (float32, float16 or bfloat16, n a multiple of 32) in 4 bits (spk_mx4_quantize)."""
+    """Rows of x [..., n] (float32, float16 or bfloat16, n a multiple of 32) in 4 bits (spk_mx4_quantize).
+
+    x of more than two dimensions lies in memory without gaps, in any order of those before the last (a pool of
+    mx4_cache has the tokens inside the heads), and `out` in the same order."""
     what = "mx4_quantize"
     dev = _device(what, x)
+    order = _memory_order(x)
+    if order:
+        m = mx4_quantize(_permuted(x, order), _permuted(out, order))
+        return _permuted(m, _back(order)) if out is None else out
     dtype = _ROWS.get(x.dtype)
     *lead, n = x.shape if x.dim() else (-1,)
     if n % 32 or dtype is None:
@@ -661,11 +687,16 @@ def mx4_quantize(x: torch.Tensor, out: Optional[Mx4] = None) -> Mx4:
 
 
 def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The values of 4-bit rows, [..., n] in dtype (of `out` where it is given; spk_mx4_dequantize)."""
+    """The values of 4-bit rows, [..., n] in dtype (of `out` where it is given; spk_mx4_dequantize).  Rows of more than two
+    dimensions and `out` lie in memory as in mx4_quantize; a fresh result has the order of m."""
     what = "mx4_dequantize"
     if not isinstance(m, Mx4):
         raise _lib.SpockError(f"{what}: expected an Mx4, got {type(m).__name__}")
     dev = _device(what, m.codes)
+    order = _memory_order(m.codes)
+    if order:
+        y = mx4_dequantize(_permuted(m, order), dtype, _permuted(out, order))
+        return _permuted(y, _back(order)) if out is None else out
     a, lead, rows, cols = _mx4_rows(what, "m", m, dev)
     if cols >> 31:
         _fits(what, row=cols)

@@ -111,6 +111,36 @@ def test_strides_shapes_and_streams(dev):
             bad()
 
 
+@pytest.mark.parametrize("shape", [(5, 16, 2, 64), (3, 7, 1, 128), (1, 20, 3, 32), (4, 1, 1, 256)], ids=str)
+def test_pools_as_rows(dev, shape):
+    """What mx4_cache makes, whose memory has another order than its dimensions, is quantised into and read back as it is."""
+    from spock_amd import ops
+    from spock_amd._lib import SpockError
+    gen = torch.Generator().manual_seed(shape[1])
+    pool, other = ops.mx4_cache(*shape, dev)
+    x = _rows(gen, math.prod(shape[:3]), shape[3], torch.bfloat16).view(shape)
+    codes, scales = M.quantize(x)
+    there = torch.empty(shape[0], shape[2], shape[1], shape[3], dtype=x.dtype, device=dev).transpose(1, 2).copy_(x)
+    assert ops.mx4_quantize(there, out=pool) is pool
+    fresh = ops.mx4_quantize(there)
+    for m in (pool, fresh):
+        assert m.codes.shape == codes.shape and torch.equal(m.codes.cpu(), codes) and torch.equal(m.scales.cpu(), scales)
+    for t in DT.values():
+        have = ops.mx4_dequantize(pool, t)
+        assert have.shape == x.shape and torch.equal(have.cpu().double(), M.values(codes, scales, t))
+    hold = torch.zeros_like(there)
+    assert ops.mx4_dequantize(pool, out=hold) is hold and torch.equal(hold.cpu().double(), M.values(codes, scales, x.dtype))
+    some = ops.mx4_dequantize(ops.Mx4(*(t[1:] for t in pool)))
+    assert torch.equal(some.cpu().double(), M.values(codes, scales, torch.bfloat16)[1:])
+    assert torch.equal(other.codes, torch.zeros_like(other.codes))
+    if shape[1] > 1 and shape[2] > 1:  # another order, gaps
+        for bad in (lambda: ops.mx4_quantize(x.to(dev), out=pool), lambda: ops.mx4_dequantize(pool, out=x.to(dev)),
+                    lambda: ops.mx4_dequantize(ops.Mx4(*(t[:, 1:] for t in pool))),
+                    lambda: ops.mx4_dequantize(ops.Mx4(pool.codes, pool.scales.contiguous()))):
+            with pytest.raises(SpockError):
+                bad()
+
+
 def _product(x, w, residual, dtype, four):
     """(result, bound) in 64 bits; x, w as values."""
     y = x @ w.T
