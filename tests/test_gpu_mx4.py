@@ -4,6 +4,7 @@
 Bars: codes, scales and values are exact.  A product is one rounding of its result (2^-11 fp16, 2^-8 bf16,
 relative), after in_dim + 4 fp32 roundings at most (products of the operands are exact, each sum is rounded once and
 the waves' sums and the residual add four more), each 2^-24 of sum |x| |w| (+ |residual|)."""
+import functools
 import math
 
 import pytest
@@ -218,6 +219,76 @@ def test_matmul_many_rows(dev, dtype, four, rows, out, depth):
     _check(hold[:, 4:4 + out], want.cpu(), bound.cpu())
     assert bool(torch.isnan(hold[:, 4 + out - 2]).all()) and not bool(torch.isnan(hold[:, 4:4 + out - 2]).any())
     assert bool((hold[:, :4] == 3).all()) and bool((hold[:, 4 + out:] == 3).all())
+
+
+# what a program calls for one row and a few, with weights of every size: each form of the kernel for few rows with scales by
+# the dword (depths of whole steps of 128) and by the byte
+FEW = [(rows, out, depth) for out in (131200, 13000, 6500, 1100) for rows in (1, 4, 16) for depth in (256, 160)] + \
+    [(33, 2200, 384), (33, 2200, 96), (40, 6000, 128), (40, 6000, 96), (20, 150, 512)]
+# tiles with scales of aligned 16 bytes, in several groups of stages, the last not whole
+LONG = [(1302, 1026, 2560), (1302, 1026, 512), (3590, 3603, 2560), (3590, 3603, 512)]
+
+
+def _form(four, rows, out, depth, aligned=True):
+    """Which kernel a product takes, as its rule in csrc/mx4.hip has it."""
+    tiles, big = -(-out // 16) * -(-rows // 16), -(-out // 256) * -(-rows // 256)
+    if rows <= 16 or tiles < (2200 if four else 5000):
+        form = (4, 1) if tiles >= 8192 else (4, 4) if tiles >= 800 else (2, 4) if tiles >= 400 else (1, 4)
+        return ("few", 4 if rows <= 4 and not four else 16, *form, 4 if depth % 128 == 0 and aligned else 1)
+    return ("tiles", 256 if big >= (128 if four else 200) else 128, 16 if depth % 512 == 0 and aligned else 1)
+
+
+@functools.lru_cache(maxsize=1)
+def _weights(out, depth):
+    """Codes of all kinds and scales from 2^-6 to 1, and their values."""
+    gen = torch.Generator().manual_seed(out + depth)
+    codes = torch.randint(0, 256, (out, depth // 2), generator=gen, dtype=torch.uint8)
+    scales = torch.randint(121, 128, (out, depth // 32), generator=gen).to(torch.uint8)
+    return codes, scales, M.values(codes, scales)
+
+
+@pytest.mark.parametrize("rows,out,depth", FEW + LONG)
+@pytest.mark.parametrize("four", [False, True], ids=["x16", "x4"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_matmul_forms(dev, dtype, four, rows, out, depth):
+    from spock_amd import ops
+    print(f"[mx4 matmul form {dtype} {'x4' if four else 'x16'} {rows}x{out}x{depth}]", flush=True)
+    t, gen = DT[dtype], torch.Generator().manual_seed(rows)
+    codes, scales, wv = _weights(out, depth)
+    if four:
+        m = torch.randint(0, 256, (rows, depth // 2), generator=gen, dtype=torch.uint8), \
+            torch.randint(124, 128, (rows, depth // 32), generator=gen).to(torch.uint8)
+        xv, mine = M.values(*m), ops.Mx4(*(v.to(dev) for v in m))
+    else:
+        x = torch.randn(rows, depth, generator=gen).to(t)
+        xv, mine = x.double(), x.to(dev)
+    res = torch.randn(rows, out, generator=gen).to(t).to(dev) if rows % 3 else None
+    got = ops.mx4_matmul(mine, ops.Mx4(codes.to(dev), scales.to(dev)), residual=res, dtype=t)
+    _check(got, *(v.cpu() for v in _product(xv.to(dev), wv.to(dev), res, t, four)))
+
+
+@pytest.mark.parametrize("rows,out", [(4, 70), (40, 70), (1300, 1030)])
+def test_matmul_weights_past_fp16(dev, rows, out):
+    """Rows in fp16: a weight enters as mx4_dequantize gives it there, rounded to fp16's steps where its scale is below
+    2^-23, infinite where it passes 65504, whatever its scale."""
+    from spock_amd import ops
+    print(f"[mx4 matmul past fp16 {rows}x{out}]", flush=True)
+    gen, depth = torch.Generator().manual_seed(rows), 128
+    codes = torch.randint(0, 256, (out, depth // 2), generator=gen, dtype=torch.uint8)
+    scales = torch.randint(127 - 27, 127 - 22, (out, depth // 32), generator=gen).to(torch.uint8)
+    scales[::3] = torch.randint(127 + 13, 127 + 17, scales[::3].shape, generator=gen).to(torch.uint8)
+    codes[::6] &= 0x99  # magnitudes of 0 and 0.5: finite up to scales of 2^16
+    x = torch.randn(rows, depth, generator=gen).to(torch.float16)
+    x[:, ::2] *= 2.0 ** -9
+    x[0, 5] = 0.0  # times an infinity: NaN
+    wv = M.values(codes, scales, torch.float16)
+    assert bool(torch.isinf(wv).any()) and bool(torch.isfinite(wv[::6]).all()) and bool((M.values(codes, scales)[1::3] != wv[1::3]).any())
+    got = ops.mx4_matmul(x.to(dev), ops.Mx4(codes.to(dev), scales.to(dev))).cpu()
+    want, bound = _product(x.double(), wv, None, torch.float16, False)
+    low, want16 = want.abs() + bound, want.to(torch.float16)
+    near = torch.isfinite(want) & (low > 65504)  # next to fp16's end, where the sum's own error decides
+    _check(torch.where(near, want16, got), torch.where(near | (want.abs() > 65504), want16.double(), want), bound, floor=2.0 ** -25)
+    assert bool((torch.isnan(got) == torch.isnan(want)).all())
 
 
 @pytest.mark.parametrize("four", [False, True], ids=["x16", "x4"])

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import mx4_ref as M
+import test_gpu_mx4 as G
 
 
 def test_the_reference_is_the_format():
@@ -137,3 +138,12 @@ def test_python_refusals():
                  lambda: ops.mx4_matmul(x, m), lambda: ops.mx4_matmul(m, m)):
         with pytest.raises(SpockError):
             call()
+
+
+def test_every_form_of_the_product_is_tested():
+    """Each kernel that the rule of spk_mx4_matmul chooses among has a shape in the tests on the GPU."""
+    for four in (False, True):
+        have = {G._form(four, *x) for x in G.FEW + G.LONG + G.SHAPES} | {G._form(four, *x, x[0] % 2 == 0) for x in G.MANY}
+        want = {("few", xr, *form, sb) for xr in ((16,) if four else (4, 16)) for form in ((4, 1), (4, 4), (2, 4), (1, 4)) for sb in (4, 1)}
+        want |= {("tiles", size, sb) for size in (128, 256) for sb in (16, 1)}
+        assert have == want, want - have
