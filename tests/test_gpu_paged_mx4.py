@@ -360,6 +360,34 @@ def test_append_not_numbers(dev, dtype):
     assert bool(torch.isfinite(ops.mx4_dequantize(ops.Mx4(*(x.transpose(1, 2).contiguous() for x in mine[0])), t)).all())
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_append_past_the_type(dev, dtype):
+    """Keys that a norm's weight takes past what the type's scales hold, in bf16 also past fp32: the largest code of the largest
+    scale, with their signs, and the block's others against that scale."""
+    from spock_amd import ops
+    t, gen = DT[dtype], torch.Generator().manual_seed(6)
+    cu, ctx, table, pages = _tables([(9, 9)], 16, 6)
+    q, k, v, positions, rope, axis = _step(gen, [(9, 9)], 4, 2, 128, 64, 1, t, spare=0)
+    kw = torch.zeros(128).to(t)
+    kw[[3, 100]] = 60000.0 if dtype == "f16" else 3.2e38  # one that rotates with 35, and one that does not
+    k[:, :, 100] = torch.where(torch.arange(18).view(9, 2) % 3 == 0, -6.0, 5.0).to(t)
+    k[5, 1, 100] = 0.6  # at the type's end, not past it
+    zero = torch.full((pages, 16, 2, 128), math.nan, dtype=torch.float64)
+    rows = R.mrope_append(q, k, v, positions, rope, axis, zero, zero, table, cu, ctx, None, kw)[1][int(table[0, 0]), :9]
+    most = 6 * 2.0 ** M.MOST[t]
+    assert float(rows.abs().max()) > (2 * most if dtype == "f16" else 2.0 ** 129) and bool((rows[:, :, 96:].abs() > most).any(-1).any())
+    codes, scales = M.quantize(rows, M.MOST[t])
+    assert int(scales.max()) == M.MOST[t] + 127
+    mine = ops.mx4_cache(pages, 16, 2, 128, dev)
+    ops.mrope_append_mx4(q.to(dev), k.to(dev), v.to(dev), positions.to(dev), rope.to(dev), axis, *mine, table.to(dev), _i32(cu, dev),
+                         _i32(ctx, dev), k_norm_weight=kw.to(dev))
+    have = [x.cpu()[int(table[0, 0]), :9] for x in mine[0]]
+    assert torch.equal(have[1], scales)
+    assert torch.equal(M.values(*have), M.values(codes, scales))
+    cut = M.values(codes, scales).abs() == most
+    assert bool(cut[:, :, 100].sum() >= 17) and torch.equal(M.values(*have)[cut].sign(), rows[cut].sign())
+
+
 def test_python_refusals(dev):
     from spock_amd import ops
     from spock_amd._lib import SpockError
