@@ -692,14 +692,16 @@ void launch_few_rows(const Mm& a, hipStream_t s) {
 template <bool X4, bool BF>
 void launch_matmul(const Mm& a, hipStream_t s) {
   const int vec = spk::aligned(a.out, 8) && a.ot % 4 == 0 && (!a.res || (spk::aligned(a.res, 8) && a.rt % 4 == 0));
-  // A tile of 16 x 16 and 128 of depth takes some 0.2 ns in the one kernel, tiles of 128 x 128
-  // that are fewer than the chip holds 1 us (rows in 4 bits 0.4): 100 rows times 14336 x 4096
-  // (6272 tiles) 44 and 33 us, 200 times 4096 x 4096 (3328) 25 and 33.  Tiles of 256 x 256 pay
-  // once most of the chip has one: 2000 times 4096 x 4096 (128 tiles) 102 us and 84 with the
-  // smaller, rows in 4 bits 40 and 44; 2000 times 7168 x 1024 (224 tiles) 38 and 54.
+  // Few rows, us with the kernel for them and with tiles of 128 x 128 (which take about the same time
+  // until the chip is full): 300 times 4096 x 4096 (4864 small tiles) 33 and 39, 400 (6400) 45 and
+  // 40; 64 times 14336 x 4096 (3584) 29 and 39, 100 (6272) 46 and 40.  Rows in 4 bits: 100 times
+  // 4096 x 4096 (1792) 12 and 15, 200 (3328) 19 and 16; 64 times 14336 x 4096 23 and 17.
+  // Tiles of 256 x 256 pay once most of the chip has one (us with them and with tiles of 128 x 128): 2000
+  // times 4096 x 4096 (128 tiles) 91 and 69, 2700 (176) 100 and 100, 3300 (208) 104 and 122; rows in 4
+  // bits 42 and 31, 47 and 47, 48 and 54; 2000 times 7168 x 1024 (224) 38 and 40, 22.7 and 23.4.
   if (a.rows <= 16 || small_tiles(a) < (X4 ? 2200 : 5000))
     a.rows <= 4 && !X4 ? launch_few_rows<X4, BF, 4>(a, s) : launch_few_rows<X4, BF, 16>(a, s);
-  else if (big_tiles(a) >= (X4 ? 128 : 200))
+  else if (big_tiles(a) >= 200)
     launch_tiles<X4, BF, 2, 4, 4, 2>(a, vec, s);
   else
     launch_tiles<X4, BF, 2, 2, 2, 2>(a, vec, s);

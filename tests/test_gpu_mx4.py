@@ -235,7 +235,7 @@ def _form(four, rows, out, depth, aligned=True):
     if rows <= 16 or tiles < (2200 if four else 5000):
         form = (4, 1) if tiles >= 8192 else (4, 4) if tiles >= 800 else (2, 4) if tiles >= 400 else (1, 4)
         return ("few", 4 if rows <= 4 and not four else 16, *form, 4 if depth % 128 == 0 and aligned else 1)
-    return ("tiles", 256 if big >= (128 if four else 200) else 128, 16 if depth % 512 == 0 and aligned else 1)
+    return ("tiles", 256 if big >= 200 else 128, 16 if depth % 512 == 0 and aligned else 1)
 
 
 @functools.lru_cache(maxsize=1)
