@@ -237,10 +237,12 @@ SPK_HD bool find_tile(const Deal& a, int at, int last, int lane, int* seq, int* 
 // ---------------------------------------------------------------------------
 
 // Rows of a sequence that are not many, next to sequences of many rows and by themselves.  Over a
-// cache in 4 bits pieces of 16 rows carry further: 8 sequences of 160 rows, heads of 256, 51 us
-// and 76 as tiles of 256 rows, of 480 rows 115 and 129; 16 of 192, heads of 128, 200 and 271, of 480 421
-// and 245; 256 rows, heads of 64, 77 and 60.  But next to many rows the pieces that they might
-// be take their time in the launch and in the join (2048 tokens and 31 single ones, heads of 128: 344 us, 397).
+// cache in 4 bits pieces of 16 rows carry further, to some 2 head_dim rows: at 4000 keys 8 sequences
+// of 160 rows, heads of 256, take 44 us and 64 as tiles of 256 rows, of 400 rows 97 and 89, of 480 100
+// and 99; 16 of 192, heads of 128, 160 and 168, of 240 184 and 170, of 480 323 and 242; 16 of 256,
+// heads of 64, 71 and 77.  But next to many rows the pieces that they might be take their time in
+// the launch and in the join: one sequence of 2048 tokens and 31 single ones, heads of 128, take 249 us
+// with up to 128 rows in pieces there and 266 with 256.
 constexpr int kFew = 128;
 
 template <bool FOUR>

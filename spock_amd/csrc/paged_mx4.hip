@@ -583,15 +583,20 @@ __device__ __forceinline__ void meet() {
 // A thread holds 16 codes of a key and 16 of a value, a half of a block, loaded into
 // registers three tiles ahead, and turns them into 16-bit values in LDS one tile before they
 // are used: once for 256 rows.  Keys and values lie in LDS alike, rows of pieces of 16
-// bytes exchanged by the row's number, so that neither 8 keys' pieces side by side (the
-// scores' operand) nor 4 values' halves of 32 dimensions (the transposing load's) share
-// banks.  The transposing load makes of 4 keys' values the output's operand.
+// bytes exchanged by the row's number: 8 keys' pieces side by side (the scores' operand) and 4
+// values' halves of 32 dimensions (the transposing load's) lie in 128 bytes of banks without
+// sharing any.  That is half of the 64 banks: the other rows that a cycle of 256 bytes
+// could read have the same ones.  Counted are 2.5 conflict cycles for each LDS instruction
+// (2048 tokens at 16384 keys: 39.9 million in 177 million busy CU cycles), which that arithmetic gives: 4 for a key
+// read, 2 for a transposing one, some 8 for a store, none for the queries' pieces.
+// The transposing load makes of 4 keys' values the output's operand.
 // A weight enters the product with V in two parts here too, for half as many matrix instructions
 // more: rounded to one part 2048 tokens at 16384 keys, 8 heads of 256, take 285 us and two
-// prompts of heads of 64 91, in two parts 372 and 106.  But the error is then the plain form's, where one
-// part has a third more (fp16 2.8e-4 for 2.1e-4, bf16 2.2e-3 for 1.7e-3), and the same for all numbers of rows.
-// The matrix instructions and the LDS reads that feed them bound it: those 372 us are 690 TFLOP/s of
-// the attention's own operations, 1040 with the second parts.
+// prompts of heads of 64 91, in two parts 370 and 106.  But the error is then the plain form's (2-norm
+// against 64 bits: fp16 2.1e-4, bf16 1.7e-3), where one part has a third more, and the same for all
+// numbers of rows.
+// The matrix instructions, busy for 53% of the time, and the LDS reads that feed them bound it: those
+// 370 us are 700 TFLOP/s of the attention's own operations, 1050 with the second parts.
 template <int D, bool BF>
 __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
   using H = Half<BF>;
@@ -604,9 +609,9 @@ __global__ __launch_bounds__(512, 2) void mx4_tiles_kernel(AttnMx4 a) {
   constexpr int WK = 64 / TK;              // keys of a wave's threads
   constexpr int NB = D == 256 ? 1 : 2;     // blocks of 32 keys at a time
   // LDS reads ahead of the product that uses them, and of the queries' 16 pieces those in
-  // registers, as the registers allow: 2048 tokens at 16384 keys, heads of 256, take 372 us with
-  // (1, 8) and 374 with (1, 6); (1, 10) would keep 40 bytes of a lane on the private stack.  (Before weights had two
-  // parts (0, 12) took 325 for 292, and with heads of 128 6 reads ahead 177 for 173, six prompts.)
+  // registers, as the registers allow: 2048 tokens at 16384 keys, heads of 256, take 368 us with
+  // (1, 8), 370 with (1, 6) and (2, 6), 385 with (0, 10); (1, 10) would keep 40 bytes of a lane on the
+  // private stack.  Heads of 128 (six prompts): 175 us 4 and 6 ahead, 178 2 ahead.
   constexpr int AHEAD = D == 256 ? 1 : 4;
   __shared__ __align__(16) uint4 ks[2][1024], vs[2][1024];
   __shared__ __align__(16) uint4 qs[KS > QR ? (KS - QR) * 512 : 1];
